@@ -52,6 +52,7 @@ extern "C" {
 typedef struct TritLm TritLm;
 typedef struct TritLmPrefix TritLmPrefix;
 typedef struct TritDense TritDense;
+typedef struct TritKv TritKv;
 
 /* A tensor-parallel group's id (NCCL's unique id as 256 hex characters
  * and a NUL, into out of cap >= 257 bytes), made once on one rank and
@@ -293,6 +294,20 @@ int trit_lm_last_timing(const TritLm *lm, double *prefill_ms, double *decode_ms,
  * (Dense::table -> Weights::Q8, gemm.rs:383-409). NULL on failure. */
 TritDense *trit_dense_q8_0(const void *blocks, size_t n, size_t k, int table, int device);
 
+/* A layer from ggml Q4_0 blocks of an `n x k` row-major matrix (18 bytes a
+ * block of 32 weights: an f16 scale d and 32 codes c of 4 bits, code i in the
+ * low half of byte i and code 16 + i in its high half; the weight is
+ * d (c - 8)), kept in 4 bits on the GPU. k is a multiple of 32. table = 0:
+ * rows of x are rounded to int8 codes in groups of 32 with f16-rounded
+ * scales, as in a Q8_0 layer; table = 1: f32 rows as they are. Sums are f32,
+ * in another order than a Q8_0 layer's. A call of more than 32 rows with
+ * table = 0 (n a multiple of 32, k of 128) runs on the int8 tensor cores from
+ * an int8 copy of the weights that the first such call makes (n x k bytes
+ * more). The other calls use no scratch memory: they may overlap, and may be
+ * captured. NULL on failure. (The reference expands Q4_0 tensors when it
+ * loads them, src/cpu/ggml_quants.rs:1-6.) */
+TritDense *trit_dense_q4_0(const void *blocks, size_t n, size_t k, int table, int device);
+
 /* out (rows x n) = x (rows x k) times the layer, both in host memory.
  * Returns 0, or -1. (Dense::forward, gemm.rs:500-542.) */
 int trit_dense_forward(TritDense *layer, const float *x, size_t rows, float *out);
@@ -325,6 +340,99 @@ void trit_dense_free(TritDense *layer);
  * does not wait. */
 int trit_dense_q8_0_forward_static(const void *codes, const void *scales, size_t n, size_t k, const float *x,
                                    size_t rows, float *out, void *cuda_stream);
+
+/* ---- a key/value cache held in 8 bits ----
+ *
+ * The paged cache of an attention layer stack, for callers that run their
+ * own decoder or encoder (trit_lm_load's "kv": "q8" uses the same kernels).
+ * A sequence is a list of positions; `page_tokens` consecutive positions make
+ * a page. Keys and values are rounded to f16 on arrival (beyond +-65504 to
+ * that, NaN to 0). A page that is not full yet stays f16 (one buffer a
+ * sequence); when its last position arrives, the page's keys of each layer
+ * and kv head, and its values, become int8 codes with one f32 scale,
+ *   scale = max|x| / 127,  code = the whole number nearest x / scale
+ * (ties to even), and count as code * scale from then on. What the cache
+ * holds depends on the values only, not on how many calls brought them.
+ * No counterpart in the reference, whose cache is f32 (layers.rs:343-504).
+ *
+ * A step of a decoder: trit_cuda_kv_extend once, then for every layer
+ * trit_cuda_kv_append and trit_cuda_kv_attend, all with the same sequences
+ * and counts. Device pointers throughout; rows of several sequences are
+ * packed, sequence after sequence. `stream` is a cudaStream_t (NULL: the
+ * default stream); calls queue their work there and do not wait. Work on
+ * different streams is put in the order of the calls. `type` is 0 for f32, 1
+ * for f16, 2 for bf16. Strides are elements between rows (0: packed).
+ *
+ * In a stream capture only trit_cuda_kv_attend and trit_cuda_kv_read are
+ * taken; a replay reads the positions that the sequences had when it was
+ * captured, and the caller orders it after the calls it depends on. The
+ * graph owns the memory it works in. The sequences must stay as they were:
+ * a replay after a trit_cuda_kv_release, trit_cuda_kv_compact or
+ * trit_cuda_kv_extend of them reads what now lies there.
+ *
+ * A call that fails on its arguments changes nothing. */
+
+/* A cache. `options_json` is an object: "layers" (1), "kv_heads" and "pages"
+ * (needed; "pages" counts full pages, each of every layer), "head_dim" (128;
+ * 64 or 128), "page_tokens" (64; 16, 32, 64 or 128), "sequences" (64: how many
+ * may be open at once), "max_tokens" (4096: positions a sequence), "device"
+ * (0). NULL on failure. */
+TritKv *trit_cuda_kv_new(const char *options_json);
+
+/* Frees a cache and its device memory. NULL is a no-op. */
+void trit_cuda_kv_free(TritKv *kv);
+
+/* n new sequences without positions, their ids into out. Returns 0, or -1. */
+int trit_cuda_kv_open(TritKv *kv, size_t n, int32_t *out);
+
+/* n new sequences, out[i] starting as the first tokens[i] positions of
+ * seqs[i] (tokens NULL: all of them). Full pages are shared until their last
+ * holder is released (they never change); only the open page is copied. A cut
+ * inside a full page keeps that page's values as f16. Returns 0, or -1. */
+int trit_cuda_kv_fork(TritKv *kv, const int32_t *seqs, const int64_t *tokens, size_t n, int32_t *out, void *stream);
+
+/* n new sequences equal to seqs[i], on pages of their own. Returns 0, or -1. */
+int trit_cuda_kv_copy(TritKv *kv, const int32_t *seqs, size_t n, int32_t *out, void *stream);
+
+/* The sequences go, and with them the pages that no other holds. Returns 0,
+ * or -1. */
+int trit_cuda_kv_release(TritKv *kv, const int32_t *seqs, size_t n);
+
+/* counts[i] more positions for seqs[i] (each named once), to be appended in
+ * every layer. Returns 0, or -1 (and then no sequence has grown). */
+int trit_cuda_kv_extend(TritKv *kv, const int32_t *seqs, const int64_t *counts, size_t n, void *stream);
+
+/* The keys and values of the last counts[i] positions of seqs[i] in one
+ * layer: rows of kv_heads x head_dim values. Every position is appended once
+ * in every layer, in order. Returns 0, or -1. */
+int trit_cuda_kv_append(TritKv *kv, int32_t layer, const int32_t *seqs, const int64_t *counts, size_t n, const void *k,
+                        size_t k_stride, const void *v, size_t v_stride, int type, void *stream);
+
+/* Attention of counts[i] query rows of heads x head_dim values against
+ * seqs[i]: softmax(scale q k) v, query head h on kv head
+ * h / (heads / kv_heads). causal = 1: the rows stand at the sequence's last
+ * counts[i] positions, each seeing the positions up to its own; causal = 0:
+ * every row sees all positions (an encoder's states). Zeros where there is
+ * none. `out` may be `q`, with the same stride. Returns 0, or -1. */
+int trit_cuda_kv_attend(TritKv *kv, int32_t layer, const int32_t *seqs, const int64_t *counts, size_t n, const void *q,
+                        size_t q_stride, int32_t heads, int type, float scale, int causal, void *out,
+                        size_t out_stride, void *stream);
+
+/* What the cache holds of positions firsts[i] .. firsts[i] + counts[i] of
+ * seqs[i] in one layer, packed rows of kv_heads x head_dim values; k or v may
+ * be NULL. Returns 0, or -1. */
+int trit_cuda_kv_read(TritKv *kv, int32_t layer, const int32_t *seqs, const int64_t *firsts, const int64_t *counts,
+                      size_t n, void *k, void *v, int type, void *stream);
+
+/* Moves the pages in use to the front of the pool. Returns the number of
+ * pages moved, or -1. */
+int64_t trit_cuda_kv_compact(TritKv *kv, void *stream);
+
+/* A sequence's positions, or -1. */
+int64_t trit_cuda_kv_length(const TritKv *kv, int32_t seq);
+
+/* Full pages in use and in all. Returns 0, or -1. */
+int trit_cuda_kv_pages(const TritKv *kv, int64_t *used, int64_t *total);
 
 #ifdef __cplusplus
 }

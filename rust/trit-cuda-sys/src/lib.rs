@@ -37,6 +37,10 @@ pub mod ffi {
     pub struct TritDense {
         _p: [u8; 0],
     }
+    #[repr(C)]
+    pub struct TritKv {
+        _p: [u8; 0],
+    }
 
     #[link(name = "trit_cuda")]
     extern "C" {
@@ -108,10 +112,41 @@ pub mod ffi {
         ) -> c_int;
         pub fn trit_dense_q8_0(blocks: *const c_void, n: usize, k: usize, table: c_int, device: c_int)
             -> *mut TritDense;
+        pub fn trit_dense_q4_0(blocks: *const c_void, n: usize, k: usize, table: c_int, device: c_int)
+            -> *mut TritDense;
         pub fn trit_dense_forward(layer: *mut TritDense, x: *const f32, rows: usize, out: *mut f32) -> c_int;
         pub fn trit_dense_forward_device(
             layer: *mut TritDense, x: *const f32, rows: usize, out: *mut f32, cuda_stream: *mut c_void,
         ) -> c_int;
+        pub fn trit_cuda_kv_new(options_json: *const c_char) -> *mut TritKv;
+        pub fn trit_cuda_kv_free(kv: *mut TritKv);
+        pub fn trit_cuda_kv_open(kv: *mut TritKv, n: usize, out: *mut i32) -> c_int;
+        pub fn trit_cuda_kv_fork(
+            kv: *mut TritKv, seqs: *const i32, tokens: *const i64, n: usize, out: *mut i32, stream: *mut c_void,
+        ) -> c_int;
+        pub fn trit_cuda_kv_copy(
+            kv: *mut TritKv, seqs: *const i32, n: usize, out: *mut i32, stream: *mut c_void,
+        ) -> c_int;
+        pub fn trit_cuda_kv_release(kv: *mut TritKv, seqs: *const i32, n: usize) -> c_int;
+        pub fn trit_cuda_kv_extend(
+            kv: *mut TritKv, seqs: *const i32, counts: *const i64, n: usize, stream: *mut c_void,
+        ) -> c_int;
+        pub fn trit_cuda_kv_append(
+            kv: *mut TritKv, layer: i32, seqs: *const i32, counts: *const i64, n: usize, k: *const c_void,
+            k_stride: usize, v: *const c_void, v_stride: usize, kind: c_int, stream: *mut c_void,
+        ) -> c_int;
+        pub fn trit_cuda_kv_attend(
+            kv: *mut TritKv, layer: i32, seqs: *const i32, counts: *const i64, n: usize, q: *const c_void,
+            q_stride: usize, heads: i32, kind: c_int, scale: f32, causal: c_int, out: *mut c_void,
+            out_stride: usize, stream: *mut c_void,
+        ) -> c_int;
+        pub fn trit_cuda_kv_read(
+            kv: *mut TritKv, layer: i32, seqs: *const i32, firsts: *const i64, counts: *const i64, n: usize,
+            k: *mut c_void, v: *mut c_void, kind: c_int, stream: *mut c_void,
+        ) -> c_int;
+        pub fn trit_cuda_kv_compact(kv: *mut TritKv, stream: *mut c_void) -> i64;
+        pub fn trit_cuda_kv_length(kv: *const TritKv, seq: i32) -> i64;
+        pub fn trit_cuda_kv_pages(kv: *const TritKv, used: *mut i64, total: *mut i64) -> c_int;
         pub fn trit_dense_free(layer: *mut TritDense);
         pub fn trit_dense_q8_0_forward_static(
             codes: *const c_void, scales: *const c_void, n: usize, k: usize, x: *const f32, rows: usize,

@@ -10,6 +10,7 @@
 
 #include "../../include/trit_cuda.h"
 #include "engine.h"
+#include "kv8.h"
 #include "nccl_link.h"
 
 struct TritLm {
@@ -22,6 +23,9 @@ struct TritLmPrefix {
 struct TritDense {
   std::unique_ptr<trit::DenseOp> op;
   std::mutex mu;
+};
+struct TritKv {
+  std::unique_ptr<trit::KvCache> kv;
 };
 
 namespace {
@@ -56,6 +60,17 @@ int64_t copy_out(const std::vector<int>& toks, int32_t* out, size_t cap) {
   size_t n = std::min(cap, toks.size());
   for (size_t i = 0; i < n; ++i) out[i] = toks[i];
   return (int64_t)toks.size();
+}
+
+// A call on a cache: under its mutex, failures as everywhere.
+template <class T, class F>
+T on_kv(const TritKv* kv, T failed, F body) {
+  return guard<T>(failed, [&]() {
+    need(kv, "kv");
+    trit::KvCache& c = *const_cast<TritKv*>(kv)->kv;
+    std::lock_guard<std::mutex> lock(c.mutex());
+    return body(c);
+  });
 }
 
 }  // namespace
@@ -338,6 +353,15 @@ TritDense* trit_dense_q8_0(const void* blocks, size_t n, size_t k, int table, in
   });
 }
 
+TritDense* trit_dense_q4_0(const void* blocks, size_t n, size_t k, int table, int device) {
+  return guard<TritDense*>(nullptr, [&]() {
+    need(blocks, "blocks");
+    auto h = std::make_unique<TritDense>();
+    h->op = trit::dense_q4_0(blocks, n, k, device, table != 0);
+    return h.release();
+  });
+}
+
 int trit_dense_forward(TritDense* layer, const float* x, size_t rows, float* out) {
   return guard<int>(-1, [&]() {
     need(layer, "layer");
@@ -380,5 +404,122 @@ int trit_dense_forward_device(TritDense* layer, const float* x, size_t rows, flo
 }
 
 void trit_dense_free(TritDense* layer) { delete layer; }
+
+TritKv* trit_cuda_kv_new(const char* options_json) {
+  return guard<TritKv*>(nullptr, [&]() {
+    trit::KvOptions o = trit::KvOptions::parse(options_json);
+    auto h = std::make_unique<TritKv>();
+    h->kv = std::make_unique<trit::KvCache>(o);
+    return h.release();
+  });
+}
+
+void trit_cuda_kv_free(TritKv* kv) { delete kv; }
+
+int trit_cuda_kv_open(TritKv* kv, size_t n, int32_t* out) {
+  return on_kv(kv, -1, [&](trit::KvCache& c) {
+    if (n) need(out, "out");
+    c.open(n, out);
+    return 0;
+  });
+}
+
+int trit_cuda_kv_fork(TritKv* kv, const int32_t* seqs, const int64_t* tokens, size_t n, int32_t* out, void* stream) {
+  return on_kv(kv, -1, [&](trit::KvCache& c) {
+    if (n) {
+      need(seqs, "seqs");
+      need(out, "out");
+    }
+    c.fork(seqs, tokens, n, out, (cudaStream_t)stream);
+    return 0;
+  });
+}
+
+int trit_cuda_kv_copy(TritKv* kv, const int32_t* seqs, size_t n, int32_t* out, void* stream) {
+  return on_kv(kv, -1, [&](trit::KvCache& c) {
+    if (n) {
+      need(seqs, "seqs");
+      need(out, "out");
+    }
+    c.copy(seqs, n, out, (cudaStream_t)stream);
+    return 0;
+  });
+}
+
+int trit_cuda_kv_release(TritKv* kv, const int32_t* seqs, size_t n) {
+  return on_kv(kv, -1, [&](trit::KvCache& c) {
+    if (n) need(seqs, "seqs");
+    c.release(seqs, n);
+    return 0;
+  });
+}
+
+int trit_cuda_kv_extend(TritKv* kv, const int32_t* seqs, const int64_t* counts, size_t n, void* stream) {
+  return on_kv(kv, -1, [&](trit::KvCache& c) {
+    if (n) {
+      need(seqs, "seqs");
+      need(counts, "counts");
+    }
+    c.extend(seqs, counts, n, (cudaStream_t)stream);
+    return 0;
+  });
+}
+
+int trit_cuda_kv_append(TritKv* kv, int32_t layer, const int32_t* seqs, const int64_t* counts, size_t n, const void* k,
+                        size_t k_stride, const void* v, size_t v_stride, int type, void* stream) {
+  return on_kv(kv, -1, [&](trit::KvCache& c) {
+    if (n) {
+      need(seqs, "seqs");
+      need(counts, "counts");
+    }
+    c.append(layer, seqs, counts, n, k, k_stride, v, v_stride, type, (cudaStream_t)stream);
+    return 0;
+  });
+}
+
+int trit_cuda_kv_attend(TritKv* kv, int32_t layer, const int32_t* seqs, const int64_t* counts, size_t n, const void* q,
+                        size_t q_stride, int32_t heads, int type, float scale, int causal, void* out,
+                        size_t out_stride, void* stream) {
+  return on_kv(kv, -1, [&](trit::KvCache& c) {
+    if (n) {
+      need(seqs, "seqs");
+      need(counts, "counts");
+    }
+    c.attend(layer, seqs, counts, n, q, q_stride, heads, type, scale, causal != 0, out, out_stride,
+             (cudaStream_t)stream);
+    return 0;
+  });
+}
+
+int trit_cuda_kv_read(TritKv* kv, int32_t layer, const int32_t* seqs, const int64_t* firsts, const int64_t* counts,
+                      size_t n, void* k, void* v, int type, void* stream) {
+  return on_kv(kv, -1, [&](trit::KvCache& c) {
+    if (n) {
+      need(seqs, "seqs");
+      need(firsts, "firsts");
+      need(counts, "counts");
+    }
+    c.read(layer, seqs, firsts, counts, n, k, v, type, (cudaStream_t)stream);
+    return 0;
+  });
+}
+
+int64_t trit_cuda_kv_compact(TritKv* kv, void* stream) {
+  return on_kv<int64_t>(kv, -1, [&](trit::KvCache& c) { return c.compact((cudaStream_t)stream); });
+}
+
+int64_t trit_cuda_kv_length(const TritKv* kv, int32_t seq) {
+  return on_kv<int64_t>(kv, -1, [&](trit::KvCache& c) { return c.length(seq); });
+}
+
+int trit_cuda_kv_pages(const TritKv* kv, int64_t* used, int64_t* total) {
+  return on_kv(kv, -1, [&](trit::KvCache& c) {
+    need(used, "used");
+    need(total, "total");
+    *used = c.pages_used();
+    *total = c.options().pages;
+    return 0;
+  });
+}
 
 }  // extern "C"

@@ -1774,7 +1774,7 @@ void Lm::generate_batch(size_t S, const int* const* prompts, const size_t* lens,
 // ------------------------------------------------------------ DenseOp ----
 DenseOp::~DenseOp() {
   cudaSetDevice(device);
-  void* bufs[] = {mem, xq, xs, xdev, ydev, best_val, best_idx, token, tc_status};
+  void* bufs[] = {mem, xq, xs, xdev, ydev, best_val, best_idx, token, tc_status, wide_codes, wide_scales};
   for (void* b : bufs)
     if (b) cudaFree(b);
   if (stream) cudaStreamDestroy(stream);
@@ -1823,7 +1823,76 @@ std::unique_ptr<DenseOp> dense_q8_0(const void* blocks, size_t n, size_t k, int 
   return op;
 }
 
+std::unique_ptr<DenseOp> dense_q4_0(const void* blocks, size_t n, size_t k, int device, bool table) {
+  if (n == 0 || k == 0 || k % 32) throw Error("Q4_0 rows are whole blocks of 32");
+  if (n > INT32_MAX || k > INT32_MAX) throw Error("a layer has at most 2^31 - 1 rows and columns");
+  auto op = std::make_unique<DenseOp>();
+  op->device = device;
+  op->table = table;
+  op->q4 = true;
+  TRIT_CUDA(cudaSetDevice(device));
+  TRIT_CUDA(cudaStreamCreateWithFlags(&op->stream, cudaStreamNonBlocking));
+  op->tab.n = op->mat.n = op->w4.n = (int)n;
+  op->tab.k = op->mat.k = op->w4.k = (int)k;
+  op->w4.chunks = (int)((k + 127) / 128);
+  const size_t cells = (n + 15) / 16 * 16 * op->w4.chunks;  // 128 values of a row, the padding's too
+  const size_t so = (cells * 64 + 255) / 256 * 256;
+  TRIT_CUDA(cudaMalloc(&op->mem, so + cells * 8));
+  op->w4.codes = op->mem;
+  op->w4.scales = (char*)op->mem + so;
+  void* raw = nullptr;
+  TRIT_CUDA(cudaMalloc(&raw, n * (k / 32) * 18));
+  cudaError_t e = cudaMemcpy(raw, blocks, n * (k / 32) * 18, cudaMemcpyHostToDevice);
+  if (e == cudaSuccess) e = launch_q4_pack(raw, op->w4, op->mem, (char*)op->mem + so, op->stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(op->stream);
+  cudaFree(raw);
+  TRIT_CUDA(e);
+  int major = 0;
+  TRIT_CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device));
+  op->tc_ok = !table && major == 10 && n % 32 == 0 && k % 128 == 0;
+  return op;
+}
+
+// Up to 16 rows the 4-bit kernel, which reads the weights once a pass. From
+// kWideRows rows of 8-bit activations on, the int8 tensor-core product of the
+// same codes and scales: its weights are expanded once and kept.
+void DenseOp::forward_q4(const float* x, size_t m, float* y, cudaStream_t s) {
+  constexpr size_t kWideRows = 33;
+  if (m < kWideRows || !tc_ok) {
+    TRIT_CUDA(launch_q4(w4, x, (int)m, !table, y, s));
+    return;
+  }
+  if (!wide_codes) {
+    const size_t n = w4.n, k = w4.k;
+    TRIT_CUDA(cudaMalloc(&wide_scales, n * (k / 32) * 2));
+    TRIT_CUDA(cudaMalloc(&tc_status, 4));
+    TRIT_CUDA(cudaMemset(tc_status, 0, 4));
+    TRIT_CUDA(cudaMalloc(&wide_codes, n * k));
+    TRIT_CUDA(launch_q4_expand(w4, wide_codes, wide_scales, stream));
+    TRIT_CUDA(cudaStreamSynchronize(stream));
+    mat.kind = kQ8_0; mat.agroup = 32; mat.half = 1;
+    mat.codes = wide_codes;
+    mat.scales = wide_scales;
+    TRIT_CUDA(make_tc_weight_map(&tc_w, mat, mat.codes));
+  }
+  if (m > rows_cap) {
+    if (xq) TRIT_CUDA(cudaFree(xq));
+    if (xs) TRIT_CUDA(cudaFree(xs));
+    xq = nullptr; xs = nullptr; rows_cap = 0;
+    TRIT_CUDA(cudaMalloc(&xq, (m + 63) / 64 * 64 * (size_t)mat.k));
+    TRIT_CUDA(cudaMalloc(&xs, m * (size_t)(mat.k / 32) * 4));
+    rows_cap = m;
+    TRIT_CUDA(make_tc_frame_map(&tc_x, xq, (m + 63) / 64 * 64, (size_t)mat.k));
+  }
+  TRIT_CUDA(launch_norm_quant(x, (int)m, mat.k, nullptr, 0.0f, mat.agroup, mat.half, xq, xs, s));
+  TRIT_CUDA(launch_gemm_tc(tc_w, tc_x, mat, xs, (int)m, kEpOut, y, mat.n, 1.0f, tc_status, s));
+}
+
 void DenseOp::forward_device(const float* x, size_t m, float* y, cudaStream_t s) {
+  if (q4) {
+    forward_q4(x, m, y, s);
+    return;
+  }
   if (m > rows_cap) {
     if (xq) cudaFree(xq);
     if (xs) cudaFree(xs);

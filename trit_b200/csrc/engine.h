@@ -299,11 +299,19 @@ struct DenseOp {
   int sm_count = 148;
   TcMap tc_w{}, tc_x{};
   int* tc_status = nullptr;
+  // 4-bit weights (dense_q4_0): their packed form, and the int8 form that a
+  // product of many rows expands them to (`mat`), held from the first one on.
+  bool q4 = false;
+  DQ4 w4{};
+  int8_t* wide_codes = nullptr;
+  void* wide_scales = nullptr;
   ~DenseOp();
+  void forward_q4(const float* x, size_t m, float* y, cudaStream_t s);
   void forward_device(const float* x, size_t m, float* y, cudaStream_t s);
 };
 
 std::unique_ptr<DenseOp> dense_q8_0(const void* blocks, size_t n, size_t k, int device, bool table);
+std::unique_ptr<DenseOp> dense_q4_0(const void* blocks, size_t n, size_t k, int device, bool table);
 
 // The text trit_cuda_last_error() returns on this thread ("" clears it).
 void set_last_error(const std::string& text);

@@ -102,6 +102,13 @@ cudaError_t launch_silu_quant(const float* g, int m, int units, int group, int h
 // Ternary 2-bit words [n][k/16] -> int8 codes c - 1 in {-1, 0, 1}, [n][k].
 cudaError_t launch_expand_ternary(const DMat& W, int8_t* out, cudaStream_t s);
 
+// Products with 4-bit weights (dense_q4.cu): y (m x n) = x (m x k) times the
+// layer, with x as it is or rounded to 8-bit codes in groups of 32 first;
+// the packing of Q4_0 blocks, and their expansion to Q8_0 codes and scales.
+cudaError_t launch_q4(const DQ4& W, const float* x, int m, bool quantize, float* y, cudaStream_t s);
+cudaError_t launch_q4_pack(const void* blocks, const DQ4& W, void* codes, void* scales, cudaStream_t s);
+cudaError_t launch_q4_expand(const DQ4& W, int8_t* codes, void* scales, cudaStream_t s);
+
 // The persistent batch-1 decode (decode.cu).
 constexpr int kEventSlots = 32;  // event stamps a layer (TRIT_PHASE_TRACE=3)
 struct DecodeArgs {

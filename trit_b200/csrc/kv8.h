@@ -1,0 +1,171 @@
+// The paged key/value cache held in 8 bits: its device layout, the kernels'
+// launchers (kv8.cu) and the host side that hands out pages and sequences
+// (kv_cache.cpp).
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <mutex>
+#include <queue>
+#include <string>
+#include <vector>
+
+namespace trit {
+
+enum KvType : int { kKvF32 = 0, kKvF16 = 1, kKvBF16 = 2 };
+
+// Device memory of a cache. A (page, layer, which, head) block is page * hd
+// codes, each stored as code + 128:
+//   keys    [token][hd]
+//   values  [token / 2][hd][token % 2]  (the two keys that share a register
+//           of the value product lie side by side)
+// with one f32 scale a block. A sequence's open page (the positions behind
+// its last full page) is f16 in the same order, in the sequence's own buffer.
+struct KvView {
+  uint8_t* codes = nullptr;   // [pages][layers][2][kv_heads][page * hd]
+  float* scales = nullptr;    // [pages][layers][2][kv_heads]
+  __half* open = nullptr;     // [sequences][layers][2][kv_heads][page * hd]
+  int* table = nullptr;       // [sequences][pages_per_seq] physical page numbers
+  int layers = 0, kv_heads = 0, hd = 0, page = 0;
+  int pages_per_seq = 0;
+};
+
+// Consecutive rows of one sequence: rows row0 .. row0 + count of the call's
+// tensors are its positions first .. first + count; `len` positions are in
+// the cache. tile0: attention tiles of the runs before.
+struct KvRun {
+  int seq, first, row0, count, len, tile0;
+};
+// Runs travel as a kernel parameter: a call needs no copy to the device and
+// leaves nothing behind that a later call could overwrite.
+constexpr int kKvRuns = 128;
+struct KvRuns {
+  int n = 0;
+  // Rows of a decode step instead of runs: row r is position row_pos[r] of
+  // sequence row_seq[r], which then has row_pos[r] + 1 positions.
+  const int* row_seq = nullptr;
+  const int* row_pos = nullptr;
+  KvRun run[kKvRuns];
+};
+
+struct KvAttendArgs {
+  const void* q = nullptr;
+  void* out = nullptr;
+  size_t q_stride = 0, out_stride = 0;  // elements between rows
+  int type = kKvF32;
+  int heads = 0;
+  int layer = 0;
+  int causal = 1;
+  float scale = 1.0f;
+  int max_len = 0;  // the longest run's positions
+};
+
+// Writes the runs' rows of one layer; pages that fill up become codes.
+cudaError_t launch_kv_append(const KvView& kv, const KvRuns& runs, int layer, const void* k, size_t k_stride,
+                             const void* v, size_t v_stride, int type, int max_count, cudaStream_t s);
+// How launch_kv_attend will run: tiles, splits of the positions, and the
+// f32 workspace that the splits meet in (0 without splits).
+struct KvAttendPlan {
+  int tiles = 0, splits = 1, cols = 0, chunks = 0;
+  size_t workspace = 0;  // bytes
+};
+KvAttendPlan plan_kv_attend(const KvView& kv, KvRuns& runs, const KvAttendArgs& a);
+cudaError_t launch_kv_attend(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& plan,
+                             float* workspace, cudaStream_t s);
+// Positions first .. first + count of each run as values, rows of
+// [kv_heads][hd] from row0 on.
+cudaError_t launch_kv_read(const KvView& kv, const KvRuns& runs, int layer, void* k, void* v, int type, int max_count,
+                           cudaStream_t s);
+// Sequence moves: run i makes sequence `seq` start as `count` positions of
+// sequence `first`: the open page's values (dequantized where the cut lies
+// inside a full page) and, with copy_table, the table entries of its full
+// pages.
+cudaError_t launch_kv_fork(const KvView& kv, const KvRuns& runs, bool copy_table, cudaStream_t s);
+// table[index[i]] = page[i]; up to kKvRuns * 3 entries ride in a parameter.
+struct KvEntries {
+  int n = 0;
+  int index[kKvRuns * 3], page[kKvRuns * 3];
+};
+cudaError_t launch_kv_table(const KvView& kv, const KvEntries& e, cudaStream_t s);
+// Page moves[2i] -> moves[2i + 1] (device pairs; no page is both read and
+// written).
+cudaError_t launch_kv_move(const KvView& kv, const int* moves, int n, cudaStream_t s);
+// Entries of the first pages_used[...] of every table row follow the moves.
+cudaError_t launch_kv_remap(const KvView& kv, const int* moves, int n, int* remap, int pages, int sequences,
+                            cudaStream_t s);
+
+struct KvOptions {
+  int device = 0, layers = 1, kv_heads = 0, hd = 128, page = 64, pages = 0, sequences = 64, max_tokens = 4096;
+  static KvOptions parse(const char* json);
+};
+
+// The host side of one cache: which sequence holds which pages. Calls on it
+// take turns (the caller holds mutex()); work on different streams is put in
+// order with events.
+class KvCache {
+ public:
+  explicit KvCache(const KvOptions& o);
+  ~KvCache();
+  KvCache(const KvCache&) = delete;
+  KvCache& operator=(const KvCache&) = delete;
+
+  std::mutex& mutex() { return mu_; }
+  const KvOptions& options() const { return opt_; }
+  const KvView& view() const { return view_; }
+
+  void open(size_t n, int* out);
+  void fork(const int* seqs, const int64_t* tokens, size_t n, int* out, cudaStream_t s);
+  void copy(const int* seqs, size_t n, int* out, cudaStream_t s);
+  void release(const int* seqs, size_t n);
+  void extend(const int* seqs, const int64_t* counts, size_t n, cudaStream_t s);
+  void append(int layer, const int* seqs, const int64_t* counts, size_t n, const void* k, size_t k_stride,
+              const void* v, size_t v_stride, int type, cudaStream_t s);
+  void attend(int layer, const int* seqs, const int64_t* counts, size_t n, const void* q, size_t q_stride, int heads,
+              int type, float scale, bool causal, void* out, size_t out_stride, cudaStream_t s);
+  void read(int layer, const int* seqs, const int64_t* firsts, const int64_t* counts, size_t n, void* k, void* v,
+            int type, cudaStream_t s);
+  int64_t compact(cudaStream_t s);
+  int64_t length(int seq) const;
+  int pages_used() const { return opt_.pages - (int)free_pages_.size(); }
+
+  // For a decoder that runs the kernels itself: the positions of a
+  // sequence are all in the cache, or will be when its stream gets there.
+  void mark_filled(int seq);
+
+ private:
+  struct Seq {
+    bool live = false;
+    int64_t len = 0;
+    std::vector<int> pages;       // one entry for every page begun (len positions)
+    std::vector<int64_t> filled;  // positions appended, by layer
+  };
+  using MinHeap = std::priority_queue<int, std::vector<int>, std::greater<int>>;
+
+  void release_memory();
+  Seq& seq(int id);
+  const Seq& seq(int id) const;
+  int new_seq();
+  void drop_pages(Seq& q);
+  void check_layer(int layer) const;
+  // Orders stream s behind everything this cache queued on other streams.
+  void enter(cudaStream_t s, const char* what, bool may_capture = false);
+  void leave(cudaStream_t s);
+  void set_entries(const std::vector<std::pair<int, int>>& entries, cudaStream_t s);
+
+  KvOptions opt_;
+  KvView view_;
+  std::mutex mu_;
+  std::vector<Seq> seqs_;
+  MinHeap free_seqs_, free_pages_;
+  std::vector<int> refs_;  // sequences that hold each page
+  float* workspace_ = nullptr;
+  size_t workspace_bytes_ = 0;
+  int *moves_ = nullptr, *remap_ = nullptr;
+  cudaEvent_t order_ = nullptr;
+  unsigned long long last_stream_ = 0;
+  bool used_ = false, capturing_ = false;
+};
+
+}  // namespace trit

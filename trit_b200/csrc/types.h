@@ -32,6 +32,15 @@ struct DTable {
   const void* scales = nullptr;
 };
 
+// 4-bit weights with an f16 scale per 32 values (ggml Q4_0), in the order
+// that k_q4 reads (dense_q4.cu): tiles of 16 rows, chunks of 128 values.
+struct DQ4 {
+  int n = 0, k = 0;
+  int chunks = 0;  // ceil(k / 128)
+  const void* codes = nullptr;
+  const void* scales = nullptr;
+};
+
 struct DLayer {
   const float* norm_attn = nullptr;
   const float* q_norm = nullptr;  // null: no qk norm (llama, mistral, granite)

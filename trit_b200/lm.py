@@ -84,6 +84,24 @@ def library() -> ctypes.CDLL:
                                                        _i32p, _size]),
         "trit_lm_bidirectional_tokens": (ctypes.c_int64, [ctypes.c_void_p, _f32p, _size, _size, _i32p]),
         "trit_dense_q8_0": (ctypes.c_void_p, [ctypes.c_void_p, _size, _size, ctypes.c_int, ctypes.c_int]),
+        "trit_dense_q4_0": (ctypes.c_void_p, [ctypes.c_void_p, _size, _size, ctypes.c_int, ctypes.c_int]),
+        "trit_cuda_kv_new": (ctypes.c_void_p, [ctypes.c_char_p]),
+        "trit_cuda_kv_free": (None, [ctypes.c_void_p]),
+        "trit_cuda_kv_open": (ctypes.c_int, [ctypes.c_void_p, _size, _i32p]),
+        "trit_cuda_kv_fork": (ctypes.c_int, [ctypes.c_void_p, _i32p, _i64p, _size, _i32p, ctypes.c_void_p]),
+        "trit_cuda_kv_copy": (ctypes.c_int, [ctypes.c_void_p, _i32p, _size, _i32p, ctypes.c_void_p]),
+        "trit_cuda_kv_release": (ctypes.c_int, [ctypes.c_void_p, _i32p, _size]),
+        "trit_cuda_kv_extend": (ctypes.c_int, [ctypes.c_void_p, _i32p, _i64p, _size, ctypes.c_void_p]),
+        "trit_cuda_kv_append": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, _i32p, _i64p, _size, ctypes.c_void_p,
+                                               _size, ctypes.c_void_p, _size, ctypes.c_int, ctypes.c_void_p]),
+        "trit_cuda_kv_attend": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, _i32p, _i64p, _size, ctypes.c_void_p,
+                                               _size, ctypes.c_int32, ctypes.c_int, ctypes.c_float, ctypes.c_int,
+                                               ctypes.c_void_p, _size, ctypes.c_void_p]),
+        "trit_cuda_kv_read": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, _i32p, _i64p, _i64p, _size,
+                                             ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
+        "trit_cuda_kv_compact": (ctypes.c_int64, [ctypes.c_void_p, ctypes.c_void_p]),
+        "trit_cuda_kv_length": (ctypes.c_int64, [ctypes.c_void_p, ctypes.c_int32]),
+        "trit_cuda_kv_pages": (ctypes.c_int, [ctypes.c_void_p, _i64p, _i64p]),
         "trit_dense_forward": (ctypes.c_int, [ctypes.c_void_p, _f32p, _size, _f32p]),
         "trit_dense_forward_device": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, _size, ctypes.c_void_p,
                                                      ctypes.c_void_p]),
@@ -347,7 +365,7 @@ class CausalLm:
 
 
 class Dense:
-    """One product layer from ggml Q8_0 blocks (Dense, src/cpu/gemm.rs:14-24)."""
+    """One product layer from ggml Q8_0 blocks (Dense, src/cpu/gemm.rs:14-24), or from Q4_0 blocks."""
 
     def __init__(self, handle: int, n: int, k: int, table: bool):
         self._handle, self.n, self.k, self.table = handle, n, k, table
@@ -358,6 +376,18 @@ class Dense:
         if b.size != n * (k // 32) * 34:
             raise TritError(f"{b.size} bytes are not the Q8_0 blocks of a {n}x{k} matrix")
         h = library().trit_dense_q8_0(b.ctypes.data, n, k, 1 if table else 0, device)
+        if not h:
+            raise _error()
+        return cls(h, n, k, table)
+
+    @classmethod
+    def q4_0(cls, blocks: np.ndarray, n: int, k: int, table: bool = False, device: int = 0) -> "Dense":
+        """A layer that keeps Q4_0 blocks in 4 bits (trit_dense_q4_0): with table=False rows of x are rounded to
+        int8 in groups of 32, with table=True they are f32."""
+        b = np.ascontiguousarray(blocks, dtype=np.uint8)
+        if b.size != n * (k // 32) * 18:
+            raise TritError(f"{b.size} bytes are not the Q4_0 blocks of a {n}x{k} matrix")
+        h = library().trit_dense_q4_0(b.ctypes.data, n, k, 1 if table else 0, device)
         if not h:
             raise _error()
         return cls(h, n, k, table)
@@ -381,6 +411,143 @@ class Dense:
 
     def __del__(self):
         self.close()
+
+
+_KV_TYPES = {"f32": 0, "f16": 1, "bf16": 2}
+
+
+def _counts(values, n: int) -> np.ndarray:
+    a = np.ascontiguousarray(values, dtype=np.int64).reshape(-1)
+    if a.size != n:
+        raise TritError(f"{a.size} counts for {n} sequences")
+    return a
+
+
+class KvCache:
+    """A paged key/value cache held in 8 bits with a scale for each page and
+    head (trit_cuda_kv_*, include/trit_cuda.h). Tensors are device pointers;
+    rows of several sequences are packed one sequence after another; `dtype` is
+    "f32", "f16" or "bf16"; `stream` is a cudaStream_t handle (None: the
+    default stream). A decoder step is extend() once, then append() and
+    attend() for every layer."""
+
+    def __init__(self, kv_heads: int, pages: int, **options):
+        """Options are the keys of trit_cuda_kv_new (layers, head_dim,
+        page_tokens, sequences, max_tokens, device)."""
+        self._handle = None
+        text = json.dumps(dict(options, kv_heads=kv_heads, pages=pages)).encode()
+        self._handle = library().trit_cuda_kv_new(text)
+        if not self._handle:
+            raise _error()
+
+    def close(self) -> None:
+        if getattr(self, "_handle", None):
+            library().trit_cuda_kv_free(self._handle)
+            self._handle = None
+
+    def __del__(self):
+        self.close()
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    @staticmethod
+    def _type(dtype: str) -> int:
+        if dtype not in _KV_TYPES:
+            raise TritError(f"dtype {dtype!r} is not one of {', '.join(_KV_TYPES)}")
+        return _KV_TYPES[dtype]
+
+    def open(self, n: int = 1) -> list[int]:
+        """n new sequences without positions."""
+        out = np.zeros(max(n, 1), dtype=np.int32)
+        if library().trit_cuda_kv_open(self._handle, n, _ptr(out, _i32p)) != 0:
+            raise _error()
+        return out[:n].tolist()
+
+    def fork(self, seqs: Sequence[int], tokens: Sequence[int] | None = None, stream: int | None = None) -> list[int]:
+        """New sequences that start as the first tokens[i] positions of
+        seqs[i] (None: all); their full pages are shared."""
+        ids = _ids(seqs)
+        out = np.zeros(max(ids.size, 1), dtype=np.int32)
+        cut = _ptr(_counts(tokens, ids.size), _i64p) if tokens is not None else None
+        if library().trit_cuda_kv_fork(self._handle, _ptr(ids, _i32p), cut, ids.size, _ptr(out, _i32p), stream) != 0:
+            raise _error()
+        return out[:ids.size].tolist()
+
+    def copy(self, seqs: Sequence[int], stream: int | None = None) -> list[int]:
+        """New sequences equal to seqs, on pages of their own."""
+        ids = _ids(seqs)
+        out = np.zeros(max(ids.size, 1), dtype=np.int32)
+        if library().trit_cuda_kv_copy(self._handle, _ptr(ids, _i32p), ids.size, _ptr(out, _i32p), stream) != 0:
+            raise _error()
+        return out[:ids.size].tolist()
+
+    def release(self, seqs: Sequence[int]) -> None:
+        ids = _ids(seqs)
+        if library().trit_cuda_kv_release(self._handle, _ptr(ids, _i32p), ids.size) != 0:
+            raise _error()
+
+    def extend(self, seqs: Sequence[int], counts: Sequence[int], stream: int | None = None) -> None:
+        """counts[i] more positions for seqs[i], to be appended in every layer."""
+        ids = _ids(seqs)
+        n = _counts(counts, ids.size)
+        if library().trit_cuda_kv_extend(self._handle, _ptr(ids, _i32p), _ptr(n, _i64p), ids.size, stream) != 0:
+            raise _error()
+
+    def append(self, layer: int, seqs: Sequence[int], counts: Sequence[int], k_ptr: int, v_ptr: int,
+               dtype: str = "f32", k_stride: int = 0, v_stride: int = 0, stream: int | None = None) -> None:
+        """The keys and values of the last counts[i] positions of seqs[i]:
+        rows of kv_heads x head_dim values (strides in elements, 0: packed)."""
+        ids = _ids(seqs)
+        n = _counts(counts, ids.size)
+        if library().trit_cuda_kv_append(self._handle, layer, _ptr(ids, _i32p), _ptr(n, _i64p), ids.size, k_ptr,
+                                         k_stride, v_ptr, v_stride, self._type(dtype), stream) != 0:
+            raise _error()
+
+    def attend(self, layer: int, seqs: Sequence[int], counts: Sequence[int], q_ptr: int, out_ptr: int, heads: int,
+               scale: float, dtype: str = "f32", causal: bool = True, q_stride: int = 0, out_stride: int = 0,
+               stream: int | None = None) -> None:
+        """Attention of counts[i] rows of heads x head_dim values against
+        seqs[i]; causal rows stand at its last positions."""
+        ids = _ids(seqs)
+        n = _counts(counts, ids.size)
+        if library().trit_cuda_kv_attend(self._handle, layer, _ptr(ids, _i32p), _ptr(n, _i64p), ids.size, q_ptr,
+                                         q_stride, heads, self._type(dtype), scale, 1 if causal else 0, out_ptr,
+                                         out_stride, stream) != 0:
+            raise _error()
+
+    def read(self, layer: int, seqs: Sequence[int], firsts: Sequence[int], counts: Sequence[int], k_ptr: int | None,
+             v_ptr: int | None, dtype: str = "f32", stream: int | None = None) -> None:
+        """What the cache holds of positions firsts[i] .. firsts[i] + counts[i]
+        of seqs[i], as packed rows."""
+        ids = _ids(seqs)
+        f, n = _counts(firsts, ids.size), _counts(counts, ids.size)
+        if library().trit_cuda_kv_read(self._handle, layer, _ptr(ids, _i32p), _ptr(f, _i64p), _ptr(n, _i64p), ids.size,
+                                       k_ptr, v_ptr, self._type(dtype), stream) != 0:
+            raise _error()
+
+    def compact(self, stream: int | None = None) -> int:
+        """Moves the pages in use to the front of the pool; how many moved."""
+        n = library().trit_cuda_kv_compact(self._handle, stream)
+        if n < 0:
+            raise _error()
+        return int(n)
+
+    def length(self, seq: int) -> int:
+        n = library().trit_cuda_kv_length(self._handle, seq)
+        if n < 0:
+            raise _error()
+        return int(n)
+
+    def pages(self) -> tuple[int, int]:
+        """Full pages: (in use, in all)."""
+        used, total = ctypes.c_int64(), ctypes.c_int64()
+        if library().trit_cuda_kv_pages(self._handle, ctypes.byref(used), ctypes.byref(total)) != 0:
+            raise _error()
+        return used.value, total.value
 
 
 def tp_id() -> str:
