@@ -88,8 +88,13 @@ void trit_cuda_free_text(char *text);
  * every key is optional and an unknown key fails (as trit_load_json,
  * include/trit.h:76-87):
  *   "device":       CUDA device index (0)
- *   "kv":           "f16" (default) or "f32": the element type of the paged
- *                   KV cache; "f32" holds what the reference holds
+ *   "kv":           "f16" (default), "f32" or "q8": the element type of the
+ *                   paged KV cache; "f32" holds what the reference holds;
+ *                   "q8" holds 8-bit codes with a scale a page and kv head
+ *                   (see trit_cuda_kv_new), about half the memory and bytes
+ *                   of "f16": logits drift (a value by about 1 %), decoding
+ *                   runs layered, pages of 16, 32, 64 or 128 positions, at
+ *                   most 16 prefixes at once
  *   "max_context":  positions per stream (4096)
  *   "max_streams":  stream slots for trit_lm_generate_batch (1)
  *   "page_tokens":  positions per KV page (64)

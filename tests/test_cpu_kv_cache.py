@@ -48,3 +48,14 @@ def test_q4_0_arguments():
         Dense.q4_0(np.zeros(4 * 1 * 18, np.uint8), 4, 48)
     with pytest.raises(TritError, match="whole blocks of 32"):
         Dense.q4_0(np.zeros(0, np.uint8), 0, 32)
+
+
+@pytest.mark.parametrize("options, words", [
+    (b'{"kv": "q4"}', 'kv is "f16", "f32" or "q8"'),
+    (b'{"kv": "q8", "page_tokens": 48}', "page_tokens is 16, 32, 64 or 128"),
+    (b'{"kv": "q8", "exact": false, "tc_attention": true}', "tc_attention"),
+])
+def test_bad_cache_options_of_a_model(options, words):
+    lib = lm.library()
+    assert lib.trit_lm_load(b"/nonexistent/model", options) is None
+    assert words in lib.trit_cuda_last_error().decode()

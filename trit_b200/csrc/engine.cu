@@ -1,6 +1,7 @@
 // Loading a decoder into device memory and running CausalLm's generation
 // flows (src/models/parts/causal_lm.rs:141-302) on one GPU.
 #include "engine.h"
+#include "kv8.h"
 #include "nccl_link.h"
 
 #include <sys/stat.h>
@@ -17,6 +18,10 @@
 #include <thread>
 
 namespace trit {
+
+// Prefixes that a model with an 8-bit cache keeps at once (each has an open
+// page of its own).
+constexpr int kQ8Prefixes = 16;
 
 void CudaCheck::ok(cudaError_t e, const char* what) {
   if (e != cudaSuccess) throw Error(std::string("CUDA: ") + cudaGetErrorString(e) + " (" + what + ")");
@@ -38,8 +43,10 @@ Options Options::parse(const char* text, bool lenient) {
     };
     if (k == "device") o.device = count(0, 63);
     else if (k == "kv") {
-      if (v.kind != Json::String || (v.str != "f16" && v.str != "f32")) throw Error("options: kv is \"f16\" or \"f32\"");
+      if (v.kind != Json::String || (v.str != "f16" && v.str != "f32" && v.str != "q8"))
+        throw Error("options: kv is \"f16\", \"f32\" or \"q8\"");
       o.kv_f16 = v.str == "f16";
+      o.kv_q8 = v.str == "q8";
     } else if (k == "max_context") o.max_context = count(1, 1 << 20);
     else if (k == "max_streams") o.max_streams = count(1, 4096);
     else if (k == "page_tokens") o.page_tokens = count(1, 4096);
@@ -87,6 +94,9 @@ Options Options::parse(const char* text, bool lenient) {
     }
   }
   if (o.tc_attention && o.exact) throw Error("options: tc_attention needs \"exact\": false (it is not the reference's arithmetic)");
+  if (o.kv_q8 && o.tc_attention) throw Error("options: tc_attention reads an f16 cache (kv is \"q8\")");
+  if (o.kv_q8 && o.page_tokens != 16 && o.page_tokens != 32 && o.page_tokens != 64 && o.page_tokens != 128)
+    throw Error("options: page_tokens is 16, 32, 64 or 128 with kv \"q8\"");
   return o;
 }
 
@@ -101,11 +111,22 @@ PrefixState::~PrefixState() {
 void Lm::release_prefix(PrefixState* p) {
   prefix_free_.insert(prefix_free_.end(), p->pages.begin(), p->pages.end());
   p->pages.clear();
+  if (kv8_ && p->seq >= 0) kv8_->release(&p->seq, 1);
+  p->seq = -1;
   p->owner = nullptr;
   prefixes_.erase(p);
 }
 
 void Lm::map_slot(int slot, const PrefixState* prefix) {
+  if (kv8_) {
+    // The whole context is set aside at once (the pool holds it for every
+    // slot), so that no later step needs the host.
+    kv8_->reset(slot);
+    if (prefix && prefix->seq >= 0) kv8_->fork_into(prefix->seq, (int64_t)prefix->tokens.size(), slot, stream_);
+    const int64_t rest = opt_.max_context - kv8_->length(slot);
+    kv8_->extend(&slot, &rest, 1, stream_);
+    return;
+  }
   const int pps = cache_.pages_per_stream;
   int* row = table_host_.data() + (size_t)slot * pps;
   bool changed = false;
@@ -355,6 +376,7 @@ Lm::Lm(const std::string& dir, const Options& o) : opt_(o) {
       comm_ = nccl_join(id, opt_.tp_size, opt_.tp_rank, opt_.device, opt_.tp_timeout_s);
       if (opt_.decode == "persistent") opt_.decode = "layered";  // the persistent kernel runs a whole model
     }
+    if (opt_.kv_q8) opt_.decode = "layered";  // the persistent kernel reads f16 and f32 caches
     load(dir);
     alloc_buffers();
     setup_tensor_cores();
@@ -462,6 +484,7 @@ void Lm::release() {
   for (auto& e : ev_)
     if (e) cudaEventDestroy(e);
   if (stream_) cudaStreamDestroy(stream_);
+  kv8_.reset();
   arena_ = pool_ = nullptr;
   d_layers_ = nullptr;
   page_table_ = nullptr;
@@ -635,7 +658,7 @@ std::string Lm::status() const {
   std::snprintf(buf, sizeof buf,
                 "\"arena_bytes\": %zu, \"device\": %d, \"kv\": \"%s\", \"decode\": \"%s\", \"exact\": %s, "
                 "\"prefix_pages\": [%d, %d], \"max_streams\": %d, \"max_context\": %d",
-                arena_bytes_, opt_.device, opt_.kv_f16 ? "f16" : "f32", opt_.decode.c_str(),
+                arena_bytes_, opt_.device, opt_.kv_q8 ? "q8" : opt_.kv_f16 ? "f16" : "f32", opt_.decode.c_str(),
                 opt_.exact ? "true" : "false", prefix_pages_used(), prefix_pages_total(), opt_.max_streams,
                 opt_.max_context);
   return "{\"source\": " + quote(source_) + ", \"weights_from\": " + quote(weights_from_) +
@@ -746,10 +769,26 @@ void Lm::alloc_buffers() {
   size_t pages = (size_t)opt_.max_streams * cache_.pages_per_stream;
   prefix_pages_total_ = opt_.prefix_pages >= 0 ? opt_.prefix_pages : cache_.pages_per_stream;
   pool_pages_ = (size_t)pages + prefix_pages_total_;
-  TRIT_CUDA(cudaMalloc(&pool_, pool_pages_ * page_bytes_));
-  // Zeroed: positions past a stream's end are read (and masked) by the
-  // tensor-core prompt attention, which must see finite values there.
-  TRIT_CUDA(cudaMemset(pool_, 0, pool_pages_ * page_bytes_));
+  if (opt_.kv_q8) {
+    // Slots are sequences 0 .. max_streams - 1, then up to kQ8Prefixes.
+    KvOptions o;
+    o.device = opt_.device;
+    o.layers = cfg_.layers;
+    o.kv_heads = cfg_.kv_heads;
+    o.hd = hd;
+    o.page = opt_.page_tokens;
+    o.pages = (int)std::max<size_t>(1, pool_pages_);
+    o.sequences = opt_.max_streams + kQ8Prefixes;
+    o.max_tokens = opt_.max_context;
+    kv8_ = std::make_unique<KvCache>(o);
+    std::vector<int> slots(opt_.max_streams);
+    kv8_->open(slots.size(), slots.data());
+  } else {
+    TRIT_CUDA(cudaMalloc(&pool_, pool_pages_ * page_bytes_));
+    // Zeroed: positions past a stream's end are read (and masked) by the
+    // tensor-core prompt attention, which must see finite values there.
+    TRIT_CUDA(cudaMemset(pool_, 0, pool_pages_ * page_bytes_));
+  }
   cache_.pool = pool_;
   table_host_.resize(pages);
   for (size_t i = 0; i < pages; ++i) table_host_[i] = (int)i;
@@ -849,7 +888,8 @@ void Lm::reduce_into_x(int m) {
   timing_.gpu_launches += 1;
 }
 
-void Lm::hidden(int m, int max_tk, const std::vector<std::pair<int, int>>* runs) {
+void Lm::hidden(int m, int max_tk, const std::vector<std::pair<int, int>>* runs, const int* host_stream,
+                const int* host_pos) {
   const int d = cfg_.d, qd = cfg_.heads * cfg_.hd, kvd = cfg_.kv_heads * cfg_.hd;
   cudaStream_t s = stream_;
   // Prompt tiles: a run of one stream's rows is cut into tiles whose rows
@@ -857,7 +897,7 @@ void Lm::hidden(int m, int max_tk, const std::vector<std::pair<int, int>>* runs)
   // the tensor-core kernel when "exact" is off).
   int ntiles = 0, rows_max = 0;
   const bool tc_attention = attention_tc_ && runs && causal_;
-  if (runs && causal_ && !runs->empty()) {
+  if (runs && causal_ && !runs->empty() && !kv8_) {
     const int R = tc_attention ? attention_tc_rows(cfg_) : attention_tile_rows(cfg_, (max_tk + 3) / 4 * 4, cache_.f16);
     for (const auto& run : *runs)
       for (int r = 0; r < run.second; r += R) {
@@ -909,7 +949,9 @@ void Lm::hidden(int m, int max_tk, const std::vector<std::pair<int, int>>* runs)
     TRIT_CUDA(launch_qk_rope_append(qkv_, m, cfg_, L.q_norm, L.k_norm, rope_, opt_.max_context, cache_, row_stream_,
                                     row_pos_, l, s));
     clock_.mark("attention", s);
-    if (ntiles && tc_attention)
+    if (kv8_)
+      attention_q8(l, m, max_tk, runs, host_stream, host_pos);
+    else if (ntiles && tc_attention)
       TRIT_CUDA(launch_attention_tc(kv_map_, qkv_, (const int2*)tiles_dev_, ntiles, cfg_, cache_, row_stream_, row_pos_,
                                     l, att_, tc_status_, s));
     else if (ntiles)
@@ -947,6 +989,52 @@ void Lm::hidden(int m, int max_tk, const std::vector<std::pair<int, int>>* runs)
     clock_.mark(nullptr, s);
   }
   timing_.gpu_launches += cfg_.layers * 10 + (cfg_.embedding_multiplier != 1.0f ? 1 : 0);
+}
+
+// Attention of the m rows in qkv_ over the 8-bit cache: their keys and
+// values are appended (a page that fills up is quantized), then read. Prompt
+// rows come as runs of consecutive positions, decode rows with their
+// sequence and position on the device.
+void Lm::attention_q8(int layer, int m, int max_tk, const std::vector<std::pair<int, int>>* runs,
+                      const int* host_stream, const int* host_pos) {
+  const int hd = cfg_.hd, qd = cfg_.heads * hd, kvd = cfg_.kv_heads * hd, ld = qd + 2 * kvd;
+  const KvView& kv = kv8_->view();
+  KvAttendArgs a;
+  a.q = qkv_;
+  a.out = att_;
+  a.q_stride = ld;
+  a.out_stride = qd;
+  a.heads = cfg_.heads;
+  a.layer = layer;
+  a.causal = causal_ ? 1 : 0;
+  a.scale = 1.0f / std::sqrt((float)hd);
+  a.max_len = max_tk;
+  KvRuns r;
+  auto go = [&](int most) {
+    TRIT_CUDA(launch_kv_append(kv, r, layer, qkv_ + qd, ld, qkv_ + qd + kvd, ld, kKvF32, most, stream_));
+    const KvAttendPlan plan = plan_kv_attend(kv, r, a);
+    TRIT_CUDA(launch_kv_attend(kv, r, a, plan, kv8_->workspace(), stream_));
+    timing_.gpu_launches += 1;
+  };
+  if (!causal_) {
+    r.run[r.n++] = KvRun{0, 0, 0, m, m, 0};
+    go(m);
+  } else if (!runs) {
+    r.n = m;
+    r.row_seq = row_stream_;
+    r.row_pos = row_pos_;
+    go(1);
+  } else {
+    int most = 0;
+    for (size_t i = 0; i < runs->size(); ++i) {
+      const int row = (*runs)[i].first, count = (*runs)[i].second;
+      r.run[r.n++] = KvRun{host_stream[row], host_pos[row], row, count, host_pos[row] + count, 0};
+      most = std::max(most, count);
+      if (r.n < kKvRuns && i + 1 < runs->size()) continue;
+      go(most);
+      r.n = most = 0;
+    }
+  }
 }
 
 // CausalLm::set_ffn_scales (causal_lm.rs:305-307): the normed MLP input of
@@ -1210,7 +1298,7 @@ void Lm::run_prompt(size_t m, int slot, int first, const std::function<void(size
     fill(c0, c0 + mc);
     const int top = first + (int)c0 + mc;
     const std::vector<std::pair<int, int>> runs = {{0, mc}};  // one stream
-    hidden(mc, top, &runs);
+    hidden(mc, top, &runs, host, host + rows_cap_);
     last_rows_ = mc;
   }
 }
@@ -1578,7 +1666,12 @@ std::unique_ptr<PrefixState> Lm::prefix(const int* ids, size_t n) {
     int* staged = stage_ids(ids, n, nullptr, 0);
     map_slot(0, p.get());
     run_prompt(n, 0, 0, [&](size_t c0, size_t c1) { embed_rows(staged, c0, c1, x_); });
-    if (n % opt_.page_tokens) {
+    if (kv8_) {
+      const int slot = 0;
+      const int64_t tokens = (int64_t)n;
+      kv8_->settle(slot, tokens);
+      kv8_->fork(&slot, &tokens, 1, &p->seq, stream_);
+    } else if (n % opt_.page_tokens) {
       TRIT_CUDA(cudaMalloc(&p->partial, page_bytes_));
       const char* own = (const char*)pool_ + full * page_bytes_;  // slot 0, logical page `full`
       TRIT_CUDA(cudaMemcpyAsync(p->partial, own, page_bytes_, cudaMemcpyDeviceToDevice, stream_));
@@ -1679,7 +1772,7 @@ void Lm::generate_batch(size_t S, const int* const* prompts, const size_t* lens,
       runs.emplace_back(r, e - r);
       r = e;
     }
-    hidden(mc, top, &runs);
+    hidden(mc, top, &runs, hs, hp);
     timing_.gpu_launches += 1;
     for (auto& e : ends)
       TRIT_CUDA(cudaMemcpyAsync(batch_last_ + (size_t)e.second * d, x_ + (size_t)e.first * d, (size_t)d * 4,

@@ -20,6 +20,7 @@ namespace trit {
 struct Options {
   int device = 0;
   bool kv_f16 = true;            // the paged KV cache in f16 (f32: the reference's cache)
+  bool kv_q8 = false;            // the paged KV cache in 8 bits (kv8.h; needs the layered kernels)
   int max_context = 4096;        // positions per stream
   int max_streams = 1;           // stream slots for generate_batch
   int page_tokens = 64;          // positions per KV page
@@ -67,6 +68,7 @@ struct CudaCheck {
 };
 #define TRIT_CUDA(x) ::trit::CudaCheck::ok((x), #x)
 
+class KvCache;
 class Lm;
 
 // A prompt start that many calls share (Prefix, causal_lm.rs:118-122,
@@ -78,6 +80,7 @@ struct PrefixState {
   std::vector<int> tokens;
   std::vector<int> pages;
   void* partial = nullptr;
+  int seq = -1;         // with an 8-bit cache: the sequence that keeps it instead
   Lm* owner = nullptr;  // gets the pages back; null once the model is gone
   ~PrefixState();
 };
@@ -169,7 +172,11 @@ class Lm {
   // (prompt chunks), or null for one row per attention block.
   // `runs`: prompt rows as runs of consecutive positions of one stream
   // (first row, rows), cut into attention tiles here; null for decode rows.
-  void hidden(int m, int max_tk, const std::vector<std::pair<int, int>>* runs = nullptr);
+  // host_stream, host_pos: the rows' streams and positions (prompts only).
+  void hidden(int m, int max_tk, const std::vector<std::pair<int, int>>* runs = nullptr,
+              const int* host_stream = nullptr, const int* host_pos = nullptr);
+  void attention_q8(int layer, int m, int max_tk, const std::vector<std::pair<int, int>>* runs, const int* host_stream,
+                    const int* host_pos);
   void setup_tensor_cores();
   // The final norm, the output table and the best token of nb rows at x
   // (row stride ldx) into tokens; with tensor parallelism the ranks' best
@@ -216,6 +223,9 @@ class Lm {
   // cache
   DCache cache_{};
   void* pool_ = nullptr;
+  // The cache in 8 bits ("kv": "q8"), in place of the pool: slot s is its
+  // sequence s, prefixes are sequences behind the slots'.
+  std::unique_ptr<KvCache> kv8_;
   size_t page_bytes_ = 0;
   int* page_table_ = nullptr;
   std::vector<int> table_host_;       // the page table as the device holds it

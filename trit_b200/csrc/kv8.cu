@@ -713,7 +713,9 @@ KvAttendPlan plan_kv_attend(const KvView& kv, KvRuns& runs, const KvAttendArgs& 
   const int want = 2 * 3 * current_sm_count(), blocks = std::max(1, p.tiles * kv.kv_heads);
   const int most_splits = std::max(1, a.max_len / (16 * 4 * kAttendWarps));
   p.splits = std::max(1, std::min(std::min((want + blocks - 1) / blocks, most_splits), 1024));
-  if (p.splits > 1) p.workspace = (size_t)p.tiles * kv.kv_heads * p.splits * p.cols * (kv.hd + 2) * 4;
+  const size_t one = (size_t)p.tiles * kv.kv_heads * p.cols * (kv.hd + 2) * 4;
+  if (p.splits > 1) p.splits = std::max<int>(1, (int)std::min<size_t>(p.splits, kKvWorkspace / std::max<size_t>(one, 1)));
+  if (p.splits > 1) p.workspace = one * p.splits;
   return p;
 }
 

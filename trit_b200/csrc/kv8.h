@@ -71,6 +71,8 @@ struct KvAttendPlan {
   int tiles = 0, splits = 1, cols = 0, chunks = 0;
   size_t workspace = 0;  // bytes
 };
+// No plan asks for more.
+constexpr size_t kKvWorkspace = 32u << 20;
 KvAttendPlan plan_kv_attend(const KvView& kv, KvRuns& runs, const KvAttendArgs& a);
 cudaError_t launch_kv_attend(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& plan,
                              float* workspace, cudaStream_t s);
@@ -130,9 +132,15 @@ class KvCache {
   int64_t length(int seq) const;
   int pages_used() const { return opt_.pages - (int)free_pages_.size(); }
 
-  // For a decoder that runs the kernels itself: the positions of a
-  // sequence are all in the cache, or will be when its stream gets there.
-  void mark_filled(int seq);
+  // For a decoder that runs the kernels itself on its one stream (Lm): a
+  // sequence without positions again; the first `tokens` positions of
+  // `parent` for such a sequence; a sequence of which `tokens` positions were
+  // written and the rest only set aside.
+  void reset(int seq);
+  void fork_into(int parent, int64_t tokens, int child, cudaStream_t s);
+  void settle(int seq, int64_t tokens);
+  // Memory for the joins of any one attention call.
+  float* workspace() const { return workspace_; }
 
  private:
   struct Seq {
@@ -147,6 +155,8 @@ class KvCache {
   Seq& seq(int id);
   const Seq& seq(int id) const;
   int new_seq();
+  void share(Seq& child, const Seq& parent, int64_t tokens);
+  void check_filled(int id) const;
   void drop_pages(Seq& q);
   void check_layer(int layer) const;
   // Orders stream s behind everything this cache queued on other streams.
@@ -161,7 +171,6 @@ class KvCache {
   MinHeap free_seqs_, free_pages_;
   std::vector<int> refs_;  // sequences that hold each page
   float* workspace_ = nullptr;
-  size_t workspace_bytes_ = 0;
   int *moves_ = nullptr, *remap_ = nullptr;
   cudaEvent_t order_ = nullptr;
   unsigned long long last_stream_ = 0;

@@ -56,6 +56,7 @@ KvCache::KvCache(const KvOptions& o) : opt_(o) {
     TRIT_CUDA(cudaMalloc(&view_.table, table));
     TRIT_CUDA(cudaMalloc(&moves_, (size_t)o.pages * 8));
     TRIT_CUDA(cudaMalloc(&remap_, (size_t)o.pages * 4));
+    TRIT_CUDA(cudaMalloc(&workspace_, kKvWorkspace));
     // The attention reads whole steps of 16 positions of an open page, also
     // those behind its end: they must hold numbers from the start.
     TRIT_CUDA(cudaMemset(view_.open, 0, open));
@@ -97,6 +98,19 @@ int KvCache::new_seq() {
   q.pages.clear();
   q.filled.assign(opt_.layers, 0);
   return id;
+}
+
+void KvCache::share(Seq& c, const Seq& p, int64_t tokens) {
+  c.len = tokens;
+  c.pages.assign(p.pages.begin(), p.pages.begin() + tokens / opt_.page);
+  c.filled.assign(opt_.layers, tokens);
+  for (int pg : c.pages) ++refs_[pg];
+}
+
+void KvCache::check_filled(int id) const {
+  const Seq& q = seq(id);
+  for (int64_t f : q.filled)
+    if (f != q.len) throw Error("sequence " + std::to_string(id) + " has positions that were not appended yet");
 }
 
 void KvCache::drop_pages(Seq& q) {
@@ -159,8 +173,7 @@ void KvCache::fork(const int* ids, const int64_t* tokens, size_t n, int* out, cu
     const Seq& p = seq(ids[i]);
     if (tokens && (tokens[i] < 0 || tokens[i] > p.len))
       throw Error("a fork at " + std::to_string(tokens[i]) + " of a sequence of " + std::to_string(p.len) + " positions");
-    for (int64_t f : p.filled)
-      if (f != p.len) throw Error("sequence " + std::to_string(ids[i]) + " has positions that were not appended yet");
+    check_filled(ids[i]);
   }
   if (!n) return;
   enter(s, "fork");
@@ -170,10 +183,7 @@ void KvCache::fork(const int* ids, const int64_t* tokens, size_t n, int* out, cu
     out[i] = id;
     Seq& c = seqs_[id];
     const Seq& p = seqs_[ids[i]];
-    c.len = tokens ? tokens[i] : p.len;
-    c.pages.assign(p.pages.begin(), p.pages.begin() + c.len / opt_.page);
-    c.filled.assign(opt_.layers, c.len);
-    for (int pg : c.pages) ++refs_[pg];
+    share(c, p, tokens ? tokens[i] : p.len);
     runs.run[runs.n++] = KvRun{id, ids[i], 0, (int)c.len, (int)p.len, 0};
     if (runs.n == kKvRuns || i + 1 == n) {
       TRIT_CUDA(launch_kv_fork(view_, runs, true, s));
@@ -187,8 +197,7 @@ void KvCache::copy(const int* ids, size_t n, int* out, cudaStream_t s) {
   size_t pages = 0;
   for (size_t i = 0; i < n; ++i) {
     const Seq& p = seq(ids[i]);
-    for (int64_t f : p.filled)
-      if (f != p.len) throw Error("sequence " + std::to_string(ids[i]) + " has positions that were not appended yet");
+    check_filled(ids[i]);
     pages += p.pages.size();
   }
   if (n > free_seqs_.size())
@@ -394,13 +403,6 @@ void KvCache::attend(int layer, const int* ids, const int64_t* counts, size_t n,
       // A captured call's workspace belongs to its graph: two graphs of one
       // cache, or a graph and a call, may then run at once.
       if (plan.workspace) TRIT_CUDA(cudaMallocAsync(&ws, plan.workspace, s));
-    } else if (plan.workspace > workspace_bytes_) {
-      if (workspace_) TRIT_CUDA(cudaFree(workspace_));
-      workspace_ = nullptr;
-      workspace_bytes_ = 0;
-      TRIT_CUDA(cudaMalloc(&workspace_, plan.workspace));
-      workspace_bytes_ = plan.workspace;
-      ws = workspace_;
     }
     TRIT_CUDA(launch_kv_attend(view_, runs, a, plan, ws, s));
     if (capturing_ && plan.workspace) TRIT_CUDA(cudaFreeAsync(ws, s));
@@ -478,9 +480,35 @@ int64_t KvCache::compact(cudaStream_t s) {
   return n;
 }
 
-void KvCache::mark_filled(int id) {
+void KvCache::reset(int id) {
   Seq& q = seq(id);
-  q.filled.assign(opt_.layers, q.len);
+  drop_pages(q);
+  q.len = 0;
+  q.filled.assign(opt_.layers, 0);
+}
+
+void KvCache::fork_into(int parent, int64_t tokens, int child, cudaStream_t s) {
+  Seq& c = seq(child);
+  const Seq& p = seq(parent);
+  check_filled(parent);
+  if (c.len || tokens < 0 || tokens > p.len) throw Error("internal: a fork into a sequence with positions");
+  enter(s, "fork");
+  share(c, p, tokens);
+  KvRuns runs;
+  runs.run[runs.n++] = KvRun{child, parent, 0, (int)tokens, (int)p.len, 0};
+  TRIT_CUDA(launch_kv_fork(view_, runs, true, s));
+  leave(s);
+}
+
+void KvCache::settle(int id, int64_t tokens) {
+  Seq& q = seq(id);
+  if (tokens < 0 || tokens > q.len) throw Error("internal: a sequence settled past its positions");
+  while ((int64_t)q.pages.size() > tokens / opt_.page) {
+    if (--refs_[q.pages.back()] == 0) free_pages_.push(q.pages.back());
+    q.pages.pop_back();
+  }
+  q.len = tokens;
+  q.filled.assign(opt_.layers, tokens);
 }
 
 }  // namespace trit

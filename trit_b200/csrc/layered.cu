@@ -377,7 +377,8 @@ __global__ void __launch_bounds__(256) k_qk_rope_append(float* qkv, int m, DConf
         for (int i = 0; i < 4; ++i) v[i] = __fmul_rn(v[i], cfg.q_scale);
       }
     }
-    if (is_q) {
+    if (is_q || !cache.pool) {
+      // Without a pool (the 8-bit cache) keys stay in the row too.
 #pragma unroll
       for (int i = 0; i < 4; ++i) head[lane * 4 + i] = v[i];
     } else {
