@@ -55,21 +55,105 @@ __device__ __forceinline__ int nearest_code(float x, float scale, float inv) {
   return x < 0.0f ? -c : c;
 }
 
+// 8 values at p (any alignment of the type; `vec`: 16-byte aligned).
+__device__ __forceinline__ void kv_load8(const void* p, size_t i, int type, bool vec, float (&v)[8]) {
+  if (!vec) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = kv_load(p, i + j, type);
+  } else if (type == kKvF32) {
+    const float4 a = *(const float4*)((const float*)p + i), b = *(const float4*)((const float*)p + i + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+    const uint4 a = *(const uint4*)((const __half*)p + i);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (type == kKvF16) {
+        const float2 f = __half22float2(*(const __half2*)&w[j]);
+        v[2 * j] = f.x;
+        v[2 * j + 1] = f.y;
+      } else {
+        v[2 * j] = __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+      }
+    }
+  }
+}
+__device__ __forceinline__ void kv_store8(void* p, size_t i, int type, bool vec, const float (&v)[8]) {
+  if (!vec) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) kv_store(p, i + j, type, v[j]);
+  } else if (type == kKvF32) {
+    *(float4*)((float*)p + i) = make_float4(v[0], v[1], v[2], v[3]);
+    *(float4*)((float*)p + i + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (type == kKvF16) {
+        const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+        w[j] = *(const uint32_t*)&h;
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+        w[j] = *(const uint32_t*)&h;
+      }
+    }
+    *(uint4*)((__half*)p + i) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+__device__ __forceinline__ void halves8(uint4 h, float (&v)[8]) {
+  const uint32_t w[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = __half22float2(*(const __half2*)&w[j]);
+    v[2 * j] = f.x;
+    v[2 * j + 1] = f.y;
+  }
+}
+
+// Codes + 128 of 8 values, packed in order. x * inv is within 4e-5 of
+// x / scale (two roundings of a number below 128), so rounding it is exact
+// unless it lands within 1e-4 of a border; those go through nearest_code.
+// Adding 1.5 * 2^23 rounds, and leaves the code in the low bits.
+__device__ __forceinline__ uint2 codes8(const float (&v)[8], float scale, float inv) {
+  uint32_t c[8];
+  float far = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float y = __fmul_rn(v[j], inv), r = __fadd_rn(y, 12582912.0f + 128.0f);
+    c[j] = __float_as_uint(r);
+    far = fmaxf(far, fabsf(__fsub_rn(y, __fsub_rn(r, 12582912.0f + 128.0f))));
+  }
+  if (far > 0.4999f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c[j] = (uint32_t)(nearest_code(v[j], scale, inv) + 128);
+  }
+  uint2 w;
+  w.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+  w.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
+  return w;
+}
+
 // ------------------------------------------------------------- append ----
 // One block writes one page's share of a run, for one (keys or values, kv
 // head). Block 0 takes the run's first page, which may begin in the open
 // buffer, and then the last, partial page, which ends there: the same block,
-// so that the second does not overwrite what the first still reads.
+// so that the second does not overwrite what the first still reads. The
+// page's share passes through shared memory as f16, eight values a thread
+// and turn, while its largest value is found.
 // Bound by bytes: rows in (2 or 4 bytes a value), codes out.
 constexpr int kAppendThreads = 256;
 
+template <int HD>
 __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const __grid_constant__ KvView kv,
                                                               const __grid_constant__ KvRuns runs, int layer,
                                                               const void* k, size_t k_stride, const void* v,
-                                                              size_t v_stride, int type, int run0) {
-  extern __shared__ __align__(16) __half held[];  // [page][hd], token-major
+                                                              size_t v_stride, int type, int vec, int run0) {
+  constexpr int U = HD / 8;  // 8-value units of a position
+  extern __shared__ __align__(16) uint4 held[];  // [page][U] f16
   __shared__ float warp_top[kAppendThreads / 32];
-  const int which = blockIdx.y & 1, head = blockIdx.y >> 1, hd = kv.hd, P = kv.page;
+  const int which = blockIdx.y & 1, head = blockIdx.y >> 1, P = kv.page;
   KvRun run;
   const int ri = run0 + blockIdx.z;
   if (runs.row_seq) {
@@ -85,31 +169,42 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const __grid_const
   const int first_page = run.first / P, last_page = (end - 1) / P;
   const void* src = which ? v : k;
   const size_t stride = which ? v_stride : k_stride;
-  __half* open = kv.open + kv_block(kv, run.seq, layer, which, head) * (size_t)(P * hd);
+  __half* open = kv.open + kv_block(kv, run.seq, layer, which, head) * (size_t)(P * HD);
   int page = first_page + blockIdx.x;
   if (page > last_page) return;
   if (blockIdx.x > 0 && (page + 1) * P > end) return;  // the partial last page is block 0's
   for (;;) {
-    const int a = max(run.first, page * P), b = min(end, (page + 1) * P);  // positions from this call
-    const bool full = (page + 1) * P <= end;
+    const int a = max(run.first - page * P, 0), b = min(end - page * P, P);  // the call's positions in the page
+    const bool full = b == P;
     float top = 0.0f;
-    // The page's earlier positions from the open buffer (a full page needs
-    // them), the call's from its rows.
-    const int t0 = full ? 0 : a - page * P, t1 = b - page * P;
-    for (int i = threadIdx.x; i < (t1 - t0) * hd; i += kAppendThreads) {
-      const int t = t0 + i / hd, d = i % hd, pos = page * P + t;
-      __half x;
-      const int at = which ? ((t >> 1) * hd + d) * 2 + (t & 1) : t * hd + d;
-      if (pos < a) {
-        x = open[at];
+    for (int i = threadIdx.x + (full ? 0 : a * U); i < b * U; i += kAppendThreads) {
+      const int t = i / U, u = i % U;
+      uint4 h;
+      if (t < a) {
+        // Of this page's earlier positions, which a full page needs.
+        if (which) {
+          const uint4 x = *(const uint4*)(open + ((t >> 1) * HD + 8 * u) * 2),
+                      y = *(const uint4*)(open + ((t >> 1) * HD + 8 * u) * 2 + 8);
+          const uint32_t sel = (t & 1) ? 0x7632 : 0x5410;
+          h = make_uint4(__byte_perm(x.x, x.y, sel), __byte_perm(x.z, x.w, sel), __byte_perm(y.x, y.y, sel),
+                         __byte_perm(y.z, y.w, sel));
+        } else {
+          h = *(const uint4*)(open + t * HD + 8 * u);
+        }
       } else {
-        x = to_cache_f16(kv_load(src, (size_t)(run.row0 + pos - run.first) * stride + (size_t)head * hd + d, type));
-        if (!full) open[at] = x;
+        float f[8];
+        kv_load8(src, (size_t)(run.row0 + page * P + t - run.first) * stride + (size_t)head * HD + 8 * u, type, vec, f);
+        __half x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = to_cache_f16(f[j]);
+        h = *(const uint4*)x;
       }
-      if (full) {
-        held[t * hd + d] = x;
-        top = fmaxf(top, fabsf(__half2float(x)));
-      }
+      held[i] = h;
+      const uint32_t w[4] = {h.x, h.y, h.z, h.w};
+      __half2 m = __habs2(*(const __half2*)&w[0]);
+#pragma unroll
+      for (int j = 1; j < 4; ++j) m = __hmax2(m, __habs2(*(const __half2*)&w[j]));
+      top = fmaxf(top, fmaxf(__low2float(m), __high2float(m)));
     }
     if (full) {
 #pragma unroll
@@ -122,24 +217,45 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const __grid_const
       const int phys = kv.table[(size_t)run.seq * kv.pages_per_seq + page];
       const size_t block = kv_block(kv, phys, layer, which, head);
       if (threadIdx.x == 0) kv.scales[block] = scale;
-      uint8_t* out = kv.codes + block * (size_t)(P * hd);
-      for (int i = threadIdx.x * 4; i < P * hd; i += kAppendThreads * 4) {
-        uint32_t w = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int at = i + j;
-          int t, d;
-          if (which) {
-            t = at / (2 * hd) * 2 + (at & 1);
-            d = at % (2 * hd) / 2;
-          } else {
-            t = at / hd;
-            d = at % hd;
-          }
-          const int c = scale > 0.0f ? nearest_code(__half2float(held[t * hd + d]), scale, inv) : 0;
-          w |= (uint32_t)(c + 128) << (8 * j);
+      uint4* out = (uint4*)(kv.codes + block * (size_t)(P * HD));
+      for (int i = threadIdx.x; i < P * HD / 16; i += kAppendThreads) {
+        // 16 codes: two units of a key, or one unit of two values.
+        float x[8], y[8];
+        if (which) {
+          const int t = i / U * 2, u = i % U;
+          halves8(held[t * U + u], x);
+          halves8(held[(t + 1) * U + u], y);
+        } else {
+          halves8(held[2 * i], x);
+          halves8(held[2 * i + 1], y);
         }
-        *(uint32_t*)(out + i) = w;
+        const uint2 cx = codes8(x, scale, inv), cy = codes8(y, scale, inv);
+        out[i] = which ? make_uint4(__byte_perm(cx.x, cy.x, 0x5140), __byte_perm(cx.x, cy.x, 0x7362),
+                                    __byte_perm(cx.y, cy.y, 0x5140), __byte_perm(cx.y, cy.y, 0x7362))
+                       : make_uint4(cx.x, cx.y, cy.x, cy.y);
+      }
+    } else if (!which) {
+      // A thread's own units, straight on.
+      for (int i = threadIdx.x + a * U; i < b * U; i += kAppendThreads) ((uint4*)open)[i] = held[i];
+    } else {
+      __syncthreads();
+      // Values lie in pairs of positions; a pair that this call brings half
+      // of keeps its other half.
+      for (int i = threadIdx.x + (a >> 1) * U; i < ((b + 1) >> 1) * U; i += kAppendThreads) {
+        const int t = i / U * 2, u = i % U;
+        __half* to = open + ((t >> 1) * HD + 8 * u) * 2;
+        if (t >= a && t + 1 < b) {
+          const uint4 x = held[t * U + u], y = held[(t + 1) * U + u];
+          ((uint4*)to)[0] = make_uint4(__byte_perm(x.x, y.x, 0x5410), __byte_perm(x.x, y.x, 0x7632),
+                                       __byte_perm(x.y, y.y, 0x5410), __byte_perm(x.y, y.y, 0x7632));
+          ((uint4*)to)[1] = make_uint4(__byte_perm(x.z, y.z, 0x5410), __byte_perm(x.z, y.z, 0x7632),
+                                       __byte_perm(x.w, y.w, 0x5410), __byte_perm(x.w, y.w, 0x7632));
+        } else {
+          const int mine = t >= a ? t : t + 1;
+          const __half* x = (const __half*)&held[mine * U + u];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) to[2 * j + (mine & 1)] = x[j];
+        }
       }
     }
     if (blockIdx.x > 0 || page == last_page || end % P == 0) return;
@@ -612,16 +728,68 @@ __device__ __forceinline__ float kv_value(const KvView& kv, int seq, int len, in
   return __fmul_rn((float)((int)kv.codes[block * bytes + at] - 128), kv.scales[block]);
 }
 
+// A unit is 8 values of a pair of positions: the 16 codes that lie together.
+template <int HD>
 __global__ void __launch_bounds__(256) k_kv_read(const __grid_constant__ KvView kv, const __grid_constant__ KvRuns runs,
-                                                 int layer, void* k, void* v, int type) {
+                                                 int layer, void* k, void* v, int type, int vec) {
+  constexpr int U = HD / 8;
   const KvRun& run = runs.run[blockIdx.z];
-  const int which = blockIdx.y & 1, head = blockIdx.y >> 1;
+  const int which = blockIdx.y & 1, head = blockIdx.y >> 1, P = kv.page;
   void* dst = which ? v : k;
   if (!dst) return;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < (size_t)run.count * kv.hd; i += (size_t)gridDim.x * 256) {
-    const int row = (int)(i / kv.hd), d = (int)(i % kv.hd);
-    kv_store(dst, ((size_t)(run.row0 + row) * kv.kv_heads + head) * kv.hd + d, type,
-             kv_value(kv, run.seq, run.len, run.first + row, layer, which, head, d));
+  const int p0 = run.first >> 1, p1 = (run.first + run.count + 1) >> 1;  // pairs
+  const size_t bytes = (size_t)P * HD;
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < (p1 - p0) * U; i += gridDim.x * 256) {
+    const int pos = (p0 + i / U) * 2, u = i % U, page = pos / P, t = pos % P;
+    float x[2][8];
+    if ((page + 1) * P > run.len) {
+      const __half* open = kv.open + kv_block(kv, run.seq, layer, which, head) * bytes;
+      if (which) {
+        const uint4* h = (const uint4*)(open + ((t >> 1) * HD + 8 * u) * 2);
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          float f[8];
+          halves8(h[z], f);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[0][4 * z + j] = f[2 * j];
+            x[1][4 * z + j] = f[2 * j + 1];
+          }
+        }
+      } else {
+        halves8(*(const uint4*)(open + t * HD + 8 * u), x[0]);
+        halves8(*(const uint4*)(open + (t + 1) * HD + 8 * u), x[1]);
+      }
+    } else {
+      const size_t block = kv_block(kv, kv.table[(size_t)run.seq * kv.pages_per_seq + page], layer, which, head);
+      const uint8_t* c = kv.codes + block * bytes;
+      const float scale = kv.scales[block];
+      uint32_t w[2][2];
+      if (which) {
+        const uint4 q = *(const uint4*)(c + ((t >> 1) * HD + 8 * u) * 2);
+        w[0][0] = __byte_perm(q.x, q.y, 0x6420);
+        w[1][0] = __byte_perm(q.x, q.y, 0x7531);
+        w[0][1] = __byte_perm(q.z, q.w, 0x6420);
+        w[1][1] = __byte_perm(q.z, q.w, 0x7531);
+      } else {
+        const uint2 q0 = *(const uint2*)(c + t * HD + 8 * u), q1 = *(const uint2*)(c + (t + 1) * HD + 8 * u);
+        w[0][0] = q0.x;
+        w[0][1] = q0.y;
+        w[1][0] = q1.x;
+        w[1][1] = q1.y;
+      }
+#pragma unroll
+      for (int z = 0; z < 2; ++z)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          x[z][j] = __fmul_rn((float)((int)(w[z][j >> 2] >> (8 * (j & 3)) & 255u) - 128), scale);
+    }
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      const int row = pos + z - run.first;
+      if (row >= 0 && row < run.count)
+        kv_store8(dst, ((size_t)(run.row0 + row) * kv.kv_heads + head) * HD + 8 * u, type, vec, x[z]);
+    }
   }
 }
 
@@ -652,7 +820,16 @@ __global__ void __launch_bounds__(256) k_kv_move(const __grid_constant__ KvView 
   const size_t blocks = (size_t)kv.layers * 2 * kv.kv_heads, n = blocks * kv.page * kv.hd / 16;
   const uint4* a = (const uint4*)(kv.codes + (size_t)src * n * 16);
   uint4* b = (uint4*)(kv.codes + (size_t)dst * n * 16);
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) b[i] = a[i];
+  // Eight loads a thread in flight; n is a multiple of 64.
+  for (size_t i0 = (size_t)blockIdx.x * 2048; i0 < n; i0 += (size_t)gridDim.x * 2048) {
+    uint4 x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i0 + j * 256 + threadIdx.x < n) x[j] = load16(a + i0 + j * 256 + threadIdx.x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i0 + j * 256 + threadIdx.x < n) b[i0 + j * 256 + threadIdx.x] = x[j];
+  }
   if (blockIdx.x == 0)
     for (size_t i = threadIdx.x; i < blocks; i += 256) kv.scales[dst * blocks + i] = kv.scales[src * blocks + i];
 }
@@ -685,9 +862,16 @@ cudaError_t launch_kv_append(const KvView& kv, const KvRuns& runs, int layer, co
   if (runs.n <= 0 || max_count <= 0) return cudaSuccess;
   // A run of c rows touches at most (c - 2) / page + 2 pages.
   const int pages = max_count == 1 ? 1 : (max_count - 2) / kv.page + 2;
-  for (int r0 = 0; r0 < runs.n; r0 += 65535)
-    k_kv_append<<<dim3(pages, 2 * kv.kv_heads, std::min(runs.n - r0, 65535)), kAppendThreads,
-                  (size_t)kv.page * kv.hd * 2, s>>>(kv, runs, layer, k, k_stride, v, v_stride, type, r0);
+  const size_t size = type == kKvF32 ? 4 : 2;
+  const int vec = ((uintptr_t)k | (uintptr_t)v | k_stride * size | v_stride * size) % 16 == 0;
+  for (int r0 = 0; r0 < runs.n; r0 += 65535) {
+    const dim3 grid(pages, 2 * kv.kv_heads, std::min(runs.n - r0, 65535));
+    const size_t smem = (size_t)kv.page * kv.hd * 2;
+    if (kv.hd == 128)
+      k_kv_append<128><<<grid, kAppendThreads, smem, s>>>(kv, runs, layer, k, k_stride, v, v_stride, type, vec, r0);
+    else
+      k_kv_append<64><<<grid, kAppendThreads, smem, s>>>(kv, runs, layer, k, k_stride, v, v_stride, type, vec, r0);
+  }
   return cudaGetLastError();
 }
 
@@ -741,8 +925,11 @@ cudaError_t launch_kv_attend(const KvView& kv, const KvRuns& runs, const KvAtten
 cudaError_t launch_kv_read(const KvView& kv, const KvRuns& runs, int layer, void* k, void* v, int type, int max_count,
                            cudaStream_t s) {
   if (runs.n <= 0 || max_count <= 0) return cudaSuccess;
-  const int x = (int)std::min<size_t>(((size_t)max_count * kv.hd + 1023) / 1024, 1024);
-  k_kv_read<<<dim3(x, 2 * kv.kv_heads, runs.n), 256, 0, s>>>(kv, runs, layer, k, v, type);
+  const int x = (int)std::min<size_t>((((size_t)max_count / 2 + 1) * (kv.hd / 8) + 255) / 256, 1024);
+  const int vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0;
+  const dim3 grid(x, 2 * kv.kv_heads, runs.n);
+  if (kv.hd == 128) k_kv_read<128><<<grid, 256, 0, s>>>(kv, runs, layer, k, v, type, vec);
+  else k_kv_read<64><<<grid, 256, 0, s>>>(kv, runs, layer, k, v, type, vec);
   return cudaGetLastError();
 }
 
@@ -760,7 +947,7 @@ cudaError_t launch_kv_table(const KvView& kv, const KvEntries& e, cudaStream_t s
 
 cudaError_t launch_kv_move(const KvView& kv, const int* moves, int n, cudaStream_t s) {
   const size_t vec = (size_t)kv.layers * 2 * kv.kv_heads * kv.page * kv.hd / 16;
-  const int x = (int)std::max<size_t>(1, std::min<size_t>((vec + 1023) / 1024, 64));
+  const int x = (int)std::max<size_t>(1, std::min<size_t>((vec + 2047) / 2048, 64));
   for (int i = 0; i < n; i += 65535) k_kv_move<<<dim3(x, std::min(n - i, 65535)), 256, 0, s>>>(kv, moves + 2 * i);
   return cudaGetLastError();
 }
