@@ -1017,7 +1017,7 @@ void Lm::attention_q8(int layer, int m, int max_tk, const std::vector<std::pair<
     timing_.gpu_launches += 1;
   };
   if (!causal_) {
-    r.run[r.n++] = KvRun{0, 0, 0, m, m, 0};
+    r.run[r.n++] = KvRun{0, 0, 0, m, m};
     go(m);
   } else if (!runs) {
     r.n = m;
@@ -1028,7 +1028,7 @@ void Lm::attention_q8(int layer, int m, int max_tk, const std::vector<std::pair<
     int most = 0;
     for (size_t i = 0; i < runs->size(); ++i) {
       const int row = (*runs)[i].first, count = (*runs)[i].second;
-      r.run[r.n++] = KvRun{host_stream[row], host_pos[row], row, count, host_pos[row] + count, 0};
+      r.run[r.n++] = KvRun{host_stream[row], host_pos[row], row, count, host_pos[row] + count};
       most = std::max(most, count);
       if (r.n < kKvRuns && i + 1 < runs->size()) continue;
       go(most);

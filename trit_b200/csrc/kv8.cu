@@ -315,6 +315,12 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
   const __half2 h = __hsub2(*(const __half2*)&x, __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
   return *(const uint32_t*)&h;
 }
+// 2^x to 2 units in the last place (0 below 2^-126).
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *(const uint32_t*)&h;
@@ -327,41 +333,149 @@ __device__ __forceinline__ uint4 load16(const void* p) {
   return v;
 }
 
-template <int HD, bool SPLIT, int NT>
-__global__ void __launch_bounds__(kAttendWarps * 32) k_kv_attend(const __grid_constant__ KvView kv,
-                                                                 const __grid_constant__ KvRuns runs,
-                                                                 const __grid_constant__ KvAttendArgs a, int chunks,
-                                                                 int splits, float* part) {
-  constexpr int CL = NT * (SPLIT ? 4 : 8);   // columns a block
-  constexpr int LT = SPLIT ? 1 : 2;          // columns a thread holds in an n-tile
-  constexpr int KB = HD / 64;                // 64-wide blocks of a key
-  constexpr int MT = HD / 16;                // 16-row tiles of the values
-  __shared__ float s_o[kAttendWarps][CL][HD];
-  __shared__ float s_m[kAttendWarps][CL], s_l[kAttendWarps][CL];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, j = lane & 3;
-  const int head = blockIdx.y, g = a.heads / kv.kv_heads, P = kv.page;
+__device__ __forceinline__ void copy16(void* smem, const void* global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(smem)), "l"(global)
+               : "memory");
+}
 
-  KvRun run;
-  int chunk;
+template <int HD, int NT>
+struct AttendShape {
+  static constexpr int UNIT = HD * 32;  // bytes of 16 positions' codes, or of their f16 keys (or values)
+  static constexpr int STAGES = HD == 128 && NT == 1 ? 4 : 6;
+  static constexpr int BLOCKS = HD == 128 && NT == 2 ? 2 : 3;  // an SM (registers)
+  static constexpr int SMEM = kAttendWarps * STAGES * UNIT;
+};
+
+// The run and its place among the blocks of a kv head.
+__device__ __forceinline__ void find_run(const KvRuns& runs, int block, int chunks, int splits, KvRun& run, int& chunk,
+                                         int& split) {
   if (runs.row_seq) {
-    const int row = blockIdx.x / chunks;
-    chunk = blockIdx.x % chunks;
+    const int row = block / (chunks * splits);
     run.seq = runs.row_seq[row];
     run.first = runs.row_pos[row];
     run.row0 = row;
     run.count = 1;
     run.len = run.first + 1;
+    run.block0 = row * chunks * splits;
+    run.splits = splits;
   } else {
     int lo = 0, hi = runs.n - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
-      if (runs.run[mid].tile0 <= (int)blockIdx.x) lo = mid;
+      if (runs.run[mid].block0 <= block) lo = mid;
       else hi = mid - 1;
     }
     run = runs.run[lo];
-    chunk = blockIdx.x - run.tile0;
   }
+  const int at = block - run.block0;
+  chunk = at / run.splits;
+  split = at % run.splits;
+}
+
+template <int HD, bool SPLIT, int NT>
+__global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS)
+    k_kv_attend(const __grid_constant__ KvView kv, const __grid_constant__ KvRuns runs,
+                const __grid_constant__ KvAttendArgs a, int chunks, int splits, int vec, void* workspace) {
+  using Shape = AttendShape<HD, NT>;
+  constexpr int CL = NT * (SPLIT ? 4 : 8);   // columns a block
+  constexpr int LT = SPLIT ? 1 : 2;          // columns a thread holds in an n-tile
+  constexpr int KB = HD / 64;                // 64-wide blocks of a key
+  constexpr int MT = HD / 16;                // 16-row tiles of the values
+  constexpr int STAGES = Shape::STAGES;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float s_m[kAttendWarps][CL], s_l[kAttendWarps][CL];
+  __shared__ int s_last;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, j = lane & 3;
+  const int head = blockIdx.y, g = a.heads / kv.kv_heads, P = kv.page;
+
+  KvRun run;
+  int chunk, split;
+  find_run(runs, blockIdx.x, chunks, splits, run, chunk, split);
   const int cols = run.count * g, c0 = chunk * CL;
+  // The last column sees most: positions [0, kend).
+  const int last_row = (min(cols, c0 + CL) - 1) / g;
+  const int kend = a.causal ? min(run.len, run.first + last_row + 1) : run.len;
+
+  // This warp's share, in steps of 16 positions; a step of codes is one unit
+  // of loads, a step of the open page two (its keys, then its values).
+  const int steps = (kend + 15) / 16, shares = run.splits * kAttendWarps;
+  const int per = (steps + shares - 1) / shares;
+  const int s0 = min(steps, (split * kAttendWarps + warp) * per), s1 = min(steps, s0 + per);
+  const int full = run.len / P * P / 16;  // steps that lie in full pages
+  const int f1 = max(s0, min(s1, full)), ncode = f1 - s0, units = ncode + 2 * (s1 - f1);
+
+  const int page_steps = kv.page_shift - 4;  // log2 of a page's steps
+  const int* table = kv.table + (size_t)run.seq * kv.pages_per_seq;
+  const size_t bytes = (size_t)P * HD;
+  const size_t head_scale = ((size_t)a.layer * 2) * kv.kv_heads + head;  // of a page's blocks
+  const uint32_t page_blocks = (uint32_t)kv.layers * 2 * kv.kv_heads, page_bytes = page_blocks * (uint32_t)bytes;
+  const int last_page = ncode ? (f1 - 1) >> page_steps : 0;
+  // Lane i keeps the page number of page fbase + i for the loads, and the
+  // scales of page base + i (with the values' logarithm and inverse) for the
+  // sums.
+  int fbase = s0 >> page_steps, base = fbase, pid = 0;
+  float ksc = 0.0f, vlog = kZeroScaleLog2, vinv = 2147483648.0f;
+  auto scales = [&](int page) {
+    const float* sc = kv.scales + (size_t)page * page_blocks + head_scale;
+    const float vs = sc[kv.kv_heads];
+    ksc = sc[0];
+    vlog = vs > 0.0f ? __log2f(vs) : kZeroScaleLog2;
+    vinv = vs > 0.0f ? __fdividef(1.0f, vs) : 2147483648.0f;
+  };
+  if (ncode && fbase + lane <= last_page) pid = table[fbase + lane];
+  uint8_t* mine = smem + (size_t)warp * STAGES * Shape::UNIT + lane * 16;
+  const uint8_t* codes_k = kv.codes + head_scale * bytes + r * HD + 16 * j;
+  const uint8_t* codes_v = kv.codes + (head_scale + kv.kv_heads) * bytes + j * (2 * HD) + 16 * r;
+  // Every lane copies the bytes that it will itself take as operands, so
+  // only its own wait stands between.
+  int slot_in = 0, slot_out = 0, ahead = 0;  // ahead: units fetched
+  auto fetch = [&]() {
+    const int unit = ahead++;
+    if (unit < units) {
+      uint8_t* to = mine + slot_in * Shape::UNIT;
+      slot_in = slot_in == STAGES - 1 ? 0 : slot_in + 1;
+      if (unit < ncode) {
+        const int step = s0 + unit;
+        int pg = (step >> page_steps) - fbase;
+        if (pg == 32) {
+          fbase += 32;
+          pg = 0;
+          if (fbase + lane <= last_page) pid = table[fbase + lane];
+        }
+        const uint32_t page = (uint32_t)__shfl_sync(0xffffffffu, pid, pg);
+        const size_t at = (size_t)page * page_bytes + (uint32_t)(step & ((1 << page_steps) - 1)) * (16 * HD);
+        const uint8_t *kp = codes_k + at, *vp = codes_v + at;
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+          copy16(to + (2 * b) * 512, kp + 64 * b);
+          copy16(to + (2 * b + 1) * 512, kp + 64 * b + 8 * HD);
+          copy16(to + (2 * KB + 2 * b) * 512, vp + 128 * b);
+          copy16(to + (2 * KB + 2 * b + 1) * 512, vp + 128 * b + 4 * 2 * HD);
+        }
+      } else {
+        const int tok = (f1 - full + (unit - ncode) / 2) * 16, which = (unit - ncode) & 1;
+        const __half* x = kv.open + kv_block(kv, run.seq, a.layer, which, head) * bytes;
+        x += which ? (size_t)(tok / 2 + j) * (2 * HD) + 16 * r : (size_t)(tok + r) * HD + 16 * j;
+        const int half = which ? 4 * 2 * HD : 8 * HD, wide = which ? 128 : 64;
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+          copy16(to + (4 * b) * 512, x + wide * b);
+          copy16(to + (4 * b + 1) * 512, x + wide * b + 8);
+          copy16(to + (4 * b + 2) * 512, x + wide * b + half);
+          copy16(to + (4 * b + 3) * 512, x + wide * b + half + 8);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto next = [&]() {  // the unit that is consumed next
+    const uint4* in = (const uint4*)(mine + slot_out * Shape::UNIT);
+    slot_out = slot_out == STAGES - 1 ? 0 : slot_out + 1;
+    return in;
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 2; ++i) fetch();
+  if (ncode && fbase + lane <= last_page) scales(pid);
 
   // The query columns' operand: thread (r, j) holds column r of every n-tile,
   // values 64 b + 16 j + 4 s + {0..3} of step (b, s).
@@ -372,15 +486,19 @@ __global__ void __launch_bounds__(kAttendWarps * 32) k_kv_attend(const __grid_co
     const int c = c0 + (SPLIT ? t * 4 + (r >> 1) : t * 8 + r);
     const bool live = c < cols;
     const size_t at = live ? (size_t)(run.row0 + c / g) * a.q_stride + (size_t)(head * g + c % g) * HD : 0;
-    float v[KB * 16];
+    float v[KB * 2][8];
     float top = 0.0f;
 #pragma unroll
-    for (int b = 0; b < KB; ++b)
+    for (int b = 0; b < KB * 2; ++b) {
+      if (live) {
+        kv_load8(a.q, at + (b >> 1) * 64 + j * 16 + (b & 1) * 8, a.type, vec, v[b]);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        v[b * 16 + i] = live ? kv_load(a.q, at + b * 64 + j * 16 + i, a.type) : 0.0f;
-        top = fmaxf(top, fabsf(v[b * 16 + i]));
+        for (int i = 0; i < 8; ++i) v[b][i] = 0.0f;
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[b][i]));
+    }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     int e = 0;
@@ -393,7 +511,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32) k_kv_attend(const __grid_co
         float x[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x[i] = v[b * 16 + 4 * s + i] * down;
+          x[i] = v[2 * b + (s >> 1)][4 * (s & 1) + i] * down;
           if (SPLIT && (r & 1)) x[i] -= __half2float(__float2half_rn(x[i]));
         }
         qf[t][b][s][0] = pack_f16(x[0], x[1]);
@@ -405,23 +523,13 @@ __global__ void __launch_bounds__(kAttendWarps * 32) k_kv_attend(const __grid_co
   }
   // The positions a softmax column sees: [0, limit).
   int limit[NT][LT];
-  int kend = 0;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int i = 0; i < LT; ++i) {
       const int c = c0 + (SPLIT ? t * 4 + j : t * 8 + 2 * j + i);
       limit[t][i] = c >= cols ? 0 : a.causal ? min(run.len, run.first + c / g + 1) : run.len;
-      kend = max(kend, limit[t][i]);
     }
-#pragma unroll
-  for (int o = 1; o < 4; o <<= 1) kend = max(kend, __shfl_xor_sync(0xffffffffu, kend, o));
-
-  // This warp's share, in steps of 16 positions.
-  const int steps = (kend + 15) / 16, shares = splits * kAttendWarps;
-  const int per = (steps + shares - 1) / shares;
-  const int s0 = min(steps, ((int)blockIdx.z * kAttendWarps + warp) * per), s1 = min(steps, s0 + per);
-  const int full = run.len / P * P / 16;  // steps that lie in full pages
 
   float o[NT][MT][4], m[NT][LT], l[NT][LT];
 #pragma unroll
@@ -437,32 +545,35 @@ __global__ void __launch_bounds__(kAttendWarps * 32) k_kv_attend(const __grid_co
     }
   }
 
-  // Scores of 16 positions to P^T and the running sums. s[t]: positions
-  // key0 + r and key0 + r + 8 of the thread's columns.
-  auto softmax = [&](float (&s)[NT][4], int key0, float key_scale, float log2_value_scale, float inv_value_scale,
-                     uint32_t (&p)[NT][2]) {
-    float x[NT][LT][2];
+  // Scores of two steps of 16 positions to P^T and the running sums. s[z][t]:
+  // positions key0[z] + r and key0[z] + r + 8 of the thread's columns.
+  auto softmax = [&](float (&s)[2][NT][4], const int (&key0)[2], const float (&ks)[2], const float (&lv)[2],
+                     const float (&iv)[2], uint32_t (&p)[2][NT][2]) {
+    float x[2][NT][LT][2];
     bool raise = false;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int z = 0; z < 2; ++z)
 #pragma unroll
-      for (int i = 0; i < LT; ++i) {
-        const float f = factor[t][i] * key_scale;
-        const float d0 = SPLIT ? s[t][0] + s[t][1] : s[t][i], d1 = SPLIT ? s[t][2] + s[t][3] : s[t][2 + i];
-        x[t][i][0] = key0 + r < limit[t][i] ? fmaf(d0, f, log2_value_scale) : -INFINITY;
-        x[t][i][1] = key0 + r + 8 < limit[t][i] ? fmaf(d1, f, log2_value_scale) : -INFINITY;
-        raise |= fmaxf(x[t][i][0], x[t][i][1]) > m[t][i] + kRaise;
-      }
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < LT; ++i) {
+          const float f = factor[t][i] * ks[z];
+          const float d0 = SPLIT ? s[z][t][0] + s[z][t][1] : s[z][t][i];
+          const float d1 = SPLIT ? s[z][t][2] + s[z][t][3] : s[z][t][2 + i];
+          x[z][t][i][0] = key0[z] + r < limit[t][i] ? fmaf(d0, f, lv[z]) : -INFINITY;
+          x[z][t][i][1] = key0[z] + r + 8 < limit[t][i] ? fmaf(d1, f, lv[z]) : -INFINITY;
+          raise |= fmaxf(x[z][t][i][0], x[z][t][i][1]) > m[t][i] + kRaise;
+        }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int i = 0; i < LT; ++i) {
-          float top = fmaxf(x[t][i][0], x[t][i][1]);
+          float top = fmaxf(fmaxf(x[0][t][i][0], x[0][t][i][1]), fmaxf(x[1][t][i][0], x[1][t][i][1]));
 #pragma unroll
           for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
           if (top > m[t][i] + kRaise) {
-            const float to = top - kBelow, alpha = exp2f(m[t][i] - to);
+            const float to = top - kBelow, alpha = exp2_fast(m[t][i] - to);
             m[t][i] = to;
             l[t][i] *= alpha;
 #pragma unroll
@@ -479,158 +590,137 @@ __global__ void __launch_bounds__(kAttendWarps * 32) k_kv_attend(const __grid_co
         }
     }
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float e[LT][2];
+    for (int z = 0; z < 2; ++z)
 #pragma unroll
-      for (int i = 0; i < LT; ++i) {
-        e[i][0] = exp2f(x[t][i][0] - m[t][i]);
-        e[i][1] = exp2f(x[t][i][1] - m[t][i]);
-        l[t][i] = fmaf(e[i][0] + e[i][1], inv_value_scale, l[t][i]);
-      }
+      for (int t = 0; t < NT; ++t) {
+        float e[LT][2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t w;
-        if (SPLIT) {
-          const float hi = __half2float(__float2half_rn(e[0][h]));
-          w = pack_f16(hi, e[0][h] - hi);
-        } else {
-          w = pack_f16(e[0][h], e[LT - 1][h]);
+        for (int i = 0; i < LT; ++i) {
+          e[i][0] = exp2_fast(x[z][t][i][0] - m[t][i]);
+          e[i][1] = exp2_fast(x[z][t][i][1] - m[t][i]);
+          l[t][i] = fmaf(e[i][0] + e[i][1], iv[z], l[t][i]);
         }
-        p[t][h] = transpose8(w);
-      }
-    }
-  };
-
-  const int steps_page = P / 16;
-  const size_t table0 = (size_t)run.seq * kv.pages_per_seq;
-  const size_t bytes = (size_t)P * HD;
-  const int f1 = min(s1, full);
-  if (s0 < f1) {
-    // Lane i keeps the page number and scales of page base + i.
-    int base = s0 / steps_page, pid = 0;
-    float ksc = 0.0f, vsc = 0.0f;
-    const int last = (f1 - 1) / steps_page;
-    auto refill = [&]() {
-      const int pg = base + lane;
-      if (pg <= last) {
-        pid = kv.table[table0 + pg];
-        const size_t block = kv_block(kv, pid, a.layer, 0, head);
-        ksc = kv.scales[block];
-        vsc = kv.scales[block + kv.kv_heads];
-      }
-    };
-    refill();
-    uint4 kn[KB][2], vn[KB][2];  // the next step's codes
-    float ksn, vsn;
-    auto fetch = [&](int step) {
-      int pg = step / steps_page - base;
-      if (pg == 32) {
-        base += 32;
-        pg = 0;
-        refill();
-      }
-      const int page = __shfl_sync(0xffffffffu, pid, pg);
-      ksn = __shfl_sync(0xffffffffu, ksc, pg);
-      vsn = __shfl_sync(0xffffffffu, vsc, pg);
-      const int tok = step % steps_page * 16;
-      const uint8_t* kp = kv.codes + kv_block(kv, page, a.layer, 0, head) * bytes + (size_t)(tok + r) * HD + 16 * j;
-      const uint8_t* vp =
-          kv.codes + kv_block(kv, page, a.layer, 1, head) * bytes + (size_t)(tok / 2 + j) * (2 * HD) + 16 * r;
-#pragma unroll
-      for (int b = 0; b < KB; ++b) {
-        kn[b][0] = load16(kp + 64 * b);
-        kn[b][1] = load16(kp + 64 * b + 8 * HD);
-        vn[b][0] = load16(vp + 128 * b);
-        vn[b][1] = load16(vp + 128 * b + 4 * 2 * HD);
-      }
-    };
-    fetch(s0);
-    for (int step = s0; step < f1; ++step) {
-      uint4 kc[KB][2], vc[KB][2];
-#pragma unroll
-      for (int b = 0; b < KB; ++b)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          kc[b][h] = kn[b][h];
-          vc[b][h] = vn[b][h];
+          uint32_t w;
+          if (SPLIT) {
+            const float hi = __half2float(__float2half_rn(e[0][h]));
+            w = pack_f16(hi, e[0][h] - hi);
+          } else {
+            w = pack_f16(e[0][h], e[LT - 1][h]);
+          }
+          p[z][t][h] = transpose8(w);
         }
-      const float ks = ksn, vs = vsn;
-      if (step + 1 < f1) fetch(step + 1);
-      float s[NT][4];
+      }
+  };
+
+  uint32_t p[2][NT][2];
+  float s[2][NT][4];
+  auto clear = [&]() {
+#pragma unroll
+    for (int z = 0; z < 2; ++z)
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) s[t][x] = 0.0f;
+        for (int x = 0; x < 4; ++x) s[z][t][x] = 0.0f;
+  };
+  // Steps of codes, two at a time (two chains of products in flight).
+  int unit = 0;
+  for (; unit < ncode; unit += 2) {
+    const bool two = unit + 1 < ncode;
+    fetch();
+    fetch();
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    float ks[2], lv[2], iv[2];
+    int key0[2];
+    const uint4* in[2];
 #pragma unroll
-      for (int b = 0; b < KB; ++b) {
-        const uint32_t w0[4] = {kc[b][0].x, kc[b][0].y, kc[b][0].z, kc[b][0].w};
-        const uint32_t w1[4] = {kc[b][1].x, kc[b][1].y, kc[b][1].z, kc[b][1].w};
+    for (int z = 0; z < 2; ++z) {
+      const int step = s0 + unit + z;
+      if (z == 0 || two) {
+        int pg = (step >> page_steps) - base;
+        if (pg == 32) {
+          base += 32;
+          pg = 0;
+          if (base + lane <= last_page) scales(table[base + lane]);
+        }
+        ks[z] = __shfl_sync(0xffffffffu, ksc, pg);
+        lv[z] = __shfl_sync(0xffffffffu, vlog, pg);
+        iv[z] = __shfl_sync(0xffffffffu, vinv, pg);
+        key0[z] = step * 16;
+        in[z] = next();
+      } else {
+        ks[z] = lv[z] = iv[z] = 0.0f;
+        key0[z] = 0x3fffffff;  // past every limit
+        in[z] = in[0];
+      }
+    }
+    clear();
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        const uint4 k0 = in[z][(2 * b) * 32], k1 = in[z][(2 * b + 1) * 32];
+        const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const uint32_t a0 = codes_lo(w0[q]), a1 = codes_lo(w1[q]), a2 = codes_hi(w0[q]), a3 = codes_hi(w1[q]);
 #pragma unroll
-          for (int t = 0; t < NT; ++t) mma16816(s[t], a0, a1, a2, a3, qf[t][b][q][0], qf[t][b][q][1]);
+          for (int t = 0; t < NT; ++t) mma16816(s[z][t], a0, a1, a2, a3, qf[t][b][q][0], qf[t][b][q][1]);
         }
       }
-      uint32_t p[NT][2];
-      const bool some = vs > 0.0f;
-      softmax(s, step * 16, ks, some ? __log2f(vs) : kZeroScaleLog2, some ? 1.0f / vs : 2147483648.0f, p);
+    softmax(s, key0, ks, lv, iv, p);
+#pragma unroll
+    for (int z = 0; z < 2; ++z)
 #pragma unroll
       for (int b = 0; b < KB; ++b) {
-        const uint32_t w0[4] = {vc[b][0].x, vc[b][0].y, vc[b][0].z, vc[b][0].w};
-        const uint32_t w1[4] = {vc[b][1].x, vc[b][1].y, vc[b][1].z, vc[b][1].w};
+        const uint4 v0 = in[z][(2 * KB + 2 * b) * 32], v1 = in[z][(2 * KB + 2 * b + 1) * 32];
+        const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const uint32_t a0 = codes_lo(w0[q]), a1 = codes_hi(w0[q]), a2 = codes_lo(w1[q]), a3 = codes_hi(w1[q]);
 #pragma unroll
-          for (int t = 0; t < NT; ++t) mma16816(o[t][4 * b + q], a0, a1, a2, a3, p[t][0], p[t][1]);
+          for (int t = 0; t < NT; ++t) mma16816(o[t][4 * b + q], a0, a1, a2, a3, p[z][t][0], p[z][t][1]);
         }
       }
-    }
   }
-  // The open page's positions, f16.
-  const __half* ko = kv.open + kv_block(kv, run.seq, a.layer, 0, head) * bytes;
-  const __half* vo = kv.open + kv_block(kv, run.seq, a.layer, 1, head) * bytes;
-  for (int step = max(s0, full); step < s1; ++step) {
-    const int tok = (step - full) * 16;
-    float s[NT][4];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) s[t][x] = 0.0f;
-#pragma unroll
-    for (int b = 0; b < KB; ++b) {
-      const __half* k0 = ko + (size_t)(tok + r) * HD + 64 * b + 16 * j;
-      uint32_t w0[8], w1[8];
-      *(uint4*)w0 = *(const uint4*)k0;
-      *(uint4*)(w0 + 4) = *(const uint4*)(k0 + 8);
-      *(uint4*)w1 = *(const uint4*)(k0 + 8 * HD);
-      *(uint4*)(w1 + 4) = *(const uint4*)(k0 + 8 * HD + 8);
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-          mma16816(s[t], w0[2 * q], w1[2 * q], w0[2 * q + 1], w1[2 * q + 1], qf[t][b][q][0], qf[t][b][q][1]);
+  // The open page, f16: a unit of keys, then one of values.
+  for (unit = ncode; unit < units; ++unit) {
+    const bool keys = ((unit - ncode) & 1) == 0;
+    if (keys) {
+      while (ahead < min(units, unit + STAGES)) fetch();
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      clear();
     }
-    uint32_t p[NT][2];
-    softmax(s, step * 16, 1.0f, 0.0f, 1.0f, p);
+    const uint4* in = next();
 #pragma unroll
-    for (int b = 0; b < KB; ++b) {
-      const __half* v0 = vo + (size_t)(tok / 2 + j) * (2 * HD) + 128 * b + 16 * r;
-      uint32_t w0[8], w1[8];
-      *(uint4*)w0 = *(const uint4*)v0;
-      *(uint4*)(w0 + 4) = *(const uint4*)(v0 + 8);
-      *(uint4*)w1 = *(const uint4*)(v0 + 4 * 2 * HD);
-      *(uint4*)(w1 + 4) = *(const uint4*)(v0 + 4 * 2 * HD + 8);
+    for (int b = 0; b < KB; ++b)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
+      for (int z = 0; z < 2; ++z) {
+        const uint4 x0 = in[(4 * b + z) * 32], x1 = in[(4 * b + 2 + z) * 32];
+        const uint32_t w0[4] = {x0.x, x0.y, x0.z, x0.w}, w1[4] = {x1.x, x1.y, x1.z, x1.w};
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-          mma16816(o[t][4 * b + q], w0[2 * q], w0[2 * q + 1], w1[2 * q], w1[2 * q + 1], p[t][0], p[t][1]);
+        for (int y = 0; y < 2; ++y) {
+          const int q = 2 * z + y;
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            if (keys) mma16816(s[0][t], w0[2 * y], w1[2 * y], w0[2 * y + 1], w1[2 * y + 1], qf[t][b][q][0], qf[t][b][q][1]);
+            else mma16816(o[t][4 * b + q], w0[2 * y], w0[2 * y + 1], w1[2 * y], w1[2 * y + 1], p[0][t][0], p[0][t][1]);
+          }
+        }
+      }
+    if (keys) {
+      const int key0[2] = {(f1 + (unit - ncode) / 2) * 16, 0x3fffffff};
+      const float one[2] = {1.0f, 1.0f}, none[2] = {0.0f, 0.0f};
+      softmax(s, key0, one, none, one, p);
     }
   }
 
-  // The warps' sums meet in shared memory.
+  // The warps' sums meet in shared memory, where their loads were.
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  float* s_o = (float*)smem;  // [warps][CL][HD]
+  static_assert(Shape::SMEM >= kAttendWarps * CL * HD * 4, "the sums fit where the loads were");
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -643,14 +733,18 @@ __global__ void __launch_bounds__(kAttendWarps * 32) k_kv_attend(const __grid_co
         s_m[warp][c] = m[t][i];
         s_l[warp][c] = sum;
       }
+      float* to = s_o + ((size_t)warp * CL + c) * HD;
 #pragma unroll
       for (int k = 0; k < MT; ++k) {
         const int d = KB == 1 ? 8 * r + 2 * k : 64 * (k >> 2) + 8 * r + 2 * (k & 3);
-        s_o[warp][c][d] = SPLIT ? o[t][k][0] + o[t][k][1] : o[t][k][i];
-        s_o[warp][c][d + 1] = SPLIT ? o[t][k][2] + o[t][k][3] : o[t][k][2 + i];
+        *(float2*)(to + d) = SPLIT ? make_float2(o[t][k][0] + o[t][k][1], o[t][k][2] + o[t][k][3])
+                                   : make_float2(o[t][k][i], o[t][k][2 + i]);
       }
     }
   __syncthreads();
+  const int nsplit = run.splits;
+  // Partial results: [kv head][block][column][HD + 2] behind the counters.
+  float* part = (float*)workspace + kKvCounters + ((size_t)head * gridDim.x + blockIdx.x) * CL * (HD + 2);
   for (int x = threadIdx.x; x < CL * HD; x += kAttendWarps * 32) {
     const int lc = x / HD, d = x % HD, c = c0 + lc;
     if (c >= cols) break;
@@ -662,58 +756,49 @@ __global__ void __launch_bounds__(kAttendWarps * 32) k_kv_attend(const __grid_co
     for (int w = 0; w < kAttendWarps; ++w) {
       const float f = exp2f(s_m[w][lc] - top);
       sum = fmaf(f, s_l[w][lc], sum);
-      val = fmaf(f, s_o[w][lc][d], val);
+      val = fmaf(f, s_o[((size_t)w * CL + lc) * HD + d], val);
     }
-    if (splits == 1) {
+    if (nsplit == 1) {
       const size_t at = (size_t)(run.row0 + c / g) * a.out_stride + (size_t)(head * g + c % g) * HD + d;
       kv_store(a.out, at, a.type, sum == 0.0f ? 0.0f : val / sum);
     } else {
-      // [tile][kv head][split][column][hd + 2]
-      float* to = part + ((((size_t)blockIdx.x * gridDim.y + head) * splits + blockIdx.z) * CL + lc) * (HD + 2);
-      to[d] = val;
+      part[lc * (HD + 2) + d] = val;
       if (d == 0) {
-        to[HD] = top;
-        to[HD + 1] = sum;
+        part[lc * (HD + 2) + HD] = top;
+        part[lc * (HD + 2) + HD + 1] = sum;
       }
     }
   }
-}
-
-// Joins the splits of a (tile, kv head): one thread a value.
-__global__ void __launch_bounds__(128) k_kv_join(const __grid_constant__ KvView kv, const __grid_constant__ KvRuns runs,
-                                                 const __grid_constant__ KvAttendArgs a, int chunks, int splits, int CL,
-                                                 const float* part) {
-  const int head = blockIdx.y, g = a.heads / kv.kv_heads, hd = kv.hd;
-  int row0, count, chunk;
-  if (runs.row_seq) {
-    row0 = blockIdx.x / chunks;
-    chunk = blockIdx.x % chunks;
-    count = 1;
-  } else {
-    int lo = 0, hi = runs.n - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (runs.run[mid].tile0 <= (int)blockIdx.x) lo = mid;
-      else hi = mid - 1;
+  if (nsplit == 1) return;
+  // The block that comes last of a tile's shares joins them, in their order
+  // (so the result does not depend on which it is). The counter wraps back
+  // to zero.
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    unsigned* counter = (unsigned*)workspace + ((size_t)head * gridDim.x + blockIdx.x - split) % kKvCounters;
+    s_last = atomicInc(counter, nsplit - 1) == (unsigned)nsplit - 1;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  const float* first = part - (size_t)split * CL * (HD + 2);
+  for (int x = threadIdx.x; x < CL * HD; x += kAttendWarps * 32) {
+    const int lc = x / HD, d = x % HD, c = c0 + lc;
+    if (c >= cols) break;
+    float top = kMInit, sum = 0.0f, val = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < nsplit; ++i) {
+      const float* q = first + ((size_t)i * CL + lc) * (HD + 2);
+      const float qm = __ldcg(q + HD), ql = __ldcg(q + HD + 1), qv = __ldcg(q + d);
+      const float to = fmaxf(top, qm), fa = exp2f(top - to), fb = exp2f(qm - to);
+      sum = fmaf(sum, fa, ql * fb);
+      val = fmaf(val, fa, qv * fb);
+      top = to;
     }
-    row0 = runs.run[lo].row0;
-    count = runs.run[lo].count;
-    chunk = blockIdx.x - runs.run[lo].tile0;
+    kv_store(a.out, (size_t)(run.row0 + c / g) * a.out_stride + (size_t)(head * g + c % g) * HD + d, a.type,
+             sum == 0.0f ? 0.0f : val / sum);
   }
-  const int x = blockIdx.z * 128 + threadIdx.x, lc = x / hd, d = x % hd, c = chunk * CL + lc;
-  if (lc >= CL || c >= count * g) return;
-  const float* p = part + (((size_t)blockIdx.x * gridDim.y + head) * splits * CL + lc) * (hd + 2);
-  const size_t step = (size_t)CL * (hd + 2);
-  float top = kMInit;
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, p[s * step + hd]);
-  float sum = 0.0f, val = 0.0f;
-  for (int s = 0; s < splits; ++s) {
-    const float f = exp2f(p[s * step + hd] - top);
-    sum = fmaf(f, p[s * step + hd + 1], sum);
-    val = fmaf(f, p[s * step + d], val);
-  }
-  kv_store(a.out, (size_t)(row0 + c / g) * a.out_stride + (size_t)(head * g + c % g) * hd + d, a.type,
-           sum == 0.0f ? 0.0f : val / sum);
 }
 
 // ---------------------------------------------------------- read, fork ----
@@ -848,10 +933,19 @@ __global__ void k_kv_remap(int* table, const int* remap, size_t entries) {
 }
 
 template <int HD, bool SPLIT, int NT>
-cudaError_t attend(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& p, float* ws,
+cudaError_t attend(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& p, int vec, void* ws,
                    cudaStream_t s) {
+  constexpr int smem = AttendShape<HD, NT>::SMEM;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  static DeviceOnce once;
+  e = once.run(dev, [] {
+    return cudaFuncSetAttribute(k_kv_attend<HD, SPLIT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  });
+  if (e != cudaSuccess) return e;
   k_kv_attend<HD, SPLIT, NT>
-      <<<dim3(p.tiles, kv.kv_heads, p.splits), kAttendWarps * 32, 0, s>>>(kv, runs, a, p.chunks, p.splits, ws);
+      <<<dim3(p.blocks, kv.kv_heads), kAttendWarps * 32, smem, s>>>(kv, runs, a, p.chunks, p.splits, vec, ws);
   return cudaGetLastError();
 }
 
@@ -875,51 +969,91 @@ cudaError_t launch_kv_append(const KvView& kv, const KvRuns& runs, int layer, co
   return cudaGetLastError();
 }
 
+// One or two n-tiles of columns a block, two when the columns need them (a
+// block reads its positions once for all of its columns).
+//
+// Positions are cut into shares of `c` steps a block, for one to four rounds
+// of blocks over the GPU: fewer rounds waste less on starting up, more even
+// out lengths that differ. The cost of a round is its longest share and about
+// four steps of start (measured: a block's first codes arrive after 2 us, a
+// step takes 0.5).
 KvAttendPlan plan_kv_attend(const KvView& kv, KvRuns& runs, const KvAttendArgs& a) {
   KvAttendPlan p;
   const int g = a.heads / kv.kv_heads, unit = a.type == kKvF32 ? 4 : 8;
   int most = 1;
   for (int i = 0; i < runs.n && !runs.row_seq; ++i) most = std::max(most, runs.run[i].count);
-  // One or two n-tiles of columns a block: two when the columns need them
-  // (a block reads its positions once for all of its columns).
   p.cols = (size_t)most * g > (size_t)unit ? 2 * unit : unit;
+  const int slots = current_sm_count() * (kv.hd == 128 && p.cols > unit ? 2 : 3);
+  // Tiles and steps of the runs (of the longest row for a decode step, whose
+  // positions only the device knows).
+  double tiles = 0, work = 0;
+  int longest = 1;
+  p.chunks = (g + p.cols - 1) / p.cols;
   if (runs.row_seq) {
-    p.chunks = (g + p.cols - 1) / p.cols;
-    p.tiles = runs.n * p.chunks;
+    tiles = (double)runs.n * p.chunks;
+    longest = (a.max_len + 15) / 16;
+    work = tiles * longest;
   } else {
     for (int i = 0; i < runs.n; ++i) {
-      runs.run[i].tile0 = p.tiles;
-      p.tiles += (int)(((size_t)runs.run[i].count * g + p.cols - 1) / p.cols);
+      const double t = (double)(((size_t)runs.run[i].count * g + p.cols - 1) / p.cols);
+      const int steps = (runs.run[i].len + 15) / 16;
+      tiles += t;
+      work += t * steps;
+      longest = std::max(longest, steps);
     }
   }
-  // Splits of the positions until the blocks fill the GPU twice over, each
-  // warp keeping at least four steps of 16 positions.
-  const int want = 2 * 3 * current_sm_count(), blocks = std::max(1, p.tiles * kv.kv_heads);
-  const int most_splits = std::max(1, a.max_len / (16 * 4 * kAttendWarps));
-  p.splits = std::max(1, std::min(std::min((want + blocks - 1) / blocks, most_splits), 1024));
-  const size_t one = (size_t)p.tiles * kv.kv_heads * p.cols * (kv.hd + 2) * 4;
-  if (p.splits > 1) p.splits = std::max<int>(1, (int)std::min<size_t>(p.splits, kKvWorkspace / std::max<size_t>(one, 1)));
-  if (p.splits > 1) p.workspace = one * p.splits;
+  tiles *= kv.kv_heads;
+  work *= kv.kv_heads;
+  int share = longest;
+  if (tiles < 4.0 * slots && tiles <= kKvCounters) {
+    double best = (double)((int)((tiles + slots - 1) / slots)) * (longest + 4);
+    for (int rounds = 1; rounds <= 4; ++rounds) {
+      // sum ceil(steps / c) over the tiles is about work / c + tiles / 2.
+      const double room = (double)rounds * slots - 0.5 * tiles;
+      if (room <= 0) continue;
+      const int c = std::max(16, (int)(work / room) + 1);
+      if (c < longest && rounds * (c + 4.0) < best) {
+        best = rounds * (c + 4.0);
+        share = c;
+      }
+    }
+  }
+  const size_t bytes = (size_t)kv.kv_heads * p.cols * (kv.hd + 2) * 4;
+  for (;; share = std::min(longest, 2 * share)) {
+    p.blocks = 0;
+    p.joins = false;
+    if (runs.row_seq) {
+      p.splits = (longest + share - 1) / share;
+      p.blocks = runs.n * p.chunks * p.splits;
+      p.joins = p.splits > 1;
+    } else {
+      for (int i = 0; i < runs.n; ++i) {
+        KvRun& r = runs.run[i];
+        r.block0 = p.blocks;
+        r.splits = std::max(1, ((r.len + 15) / 16 + share - 1) / share);
+        p.joins |= r.splits > 1;
+        p.blocks += (int)(((size_t)r.count * g + p.cols - 1) / p.cols) * r.splits;
+      }
+    }
+    p.workspace = kKvCounters * 4 + p.blocks * bytes;
+    if (!p.joins || ((size_t)p.blocks * kv.kv_heads <= kKvCounters && p.workspace <= kKvWorkspace)) break;
+  }
   return p;
 }
 
-cudaError_t launch_kv_attend(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& p,
-                             float* ws, cudaStream_t s) {
-  if (p.tiles <= 0) return cudaSuccess;
-  if (p.splits > 1 && !ws) return cudaErrorInvalidValue;
+cudaError_t launch_kv_attend(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& p, void* ws,
+                             cudaStream_t s) {
+  if (p.blocks <= 0) return cudaSuccess;
+  if (p.joins && !ws) return cudaErrorInvalidValue;
+  const size_t size = a.type == kKvF32 ? 4 : 2;
+  const int vec = ((uintptr_t)a.q | a.q_stride * size) % 16 == 0;
   const bool two = p.cols == (a.type == kKvF32 ? 8 : 16);
-  cudaError_t e;
   if (kv.hd == 128) {
-    if (a.type == kKvF32) e = two ? attend<128, true, 2>(kv, runs, a, p, ws, s) : attend<128, true, 1>(kv, runs, a, p, ws, s);
-    else e = two ? attend<128, false, 2>(kv, runs, a, p, ws, s) : attend<128, false, 1>(kv, runs, a, p, ws, s);
-  } else {
-    if (a.type == kKvF32) e = two ? attend<64, true, 2>(kv, runs, a, p, ws, s) : attend<64, true, 1>(kv, runs, a, p, ws, s);
-    else e = two ? attend<64, false, 2>(kv, runs, a, p, ws, s) : attend<64, false, 1>(kv, runs, a, p, ws, s);
+    if (a.type == kKvF32) return two ? attend<128, true, 2>(kv, runs, a, p, vec, ws, s) : attend<128, true, 1>(kv, runs, a, p, vec, ws, s);
+    return two ? attend<128, false, 2>(kv, runs, a, p, vec, ws, s) : attend<128, false, 1>(kv, runs, a, p, vec, ws, s);
   }
-  if (e != cudaSuccess || p.splits == 1) return e;
-  k_kv_join<<<dim3(p.tiles, kv.kv_heads, (p.cols * kv.hd + 127) / 128), 128, 0, s>>>(kv, runs, a, p.chunks, p.splits,
-                                                                                   p.cols, ws);
-  return cudaGetLastError();
+  if (a.type == kKvF32) return two ? attend<64, true, 2>(kv, runs, a, p, vec, ws, s) : attend<64, true, 1>(kv, runs, a, p, vec, ws, s);
+  return two ? attend<64, false, 2>(kv, runs, a, p, vec, ws, s) : attend<64, false, 1>(kv, runs, a, p, vec, ws, s);
 }
 
 cudaError_t launch_kv_read(const KvView& kv, const KvRuns& runs, int layer, void* k, void* v, int type, int max_count,

@@ -29,18 +29,20 @@ struct KvView {
   __half* open = nullptr;     // [sequences][layers][2][kv_heads][page * hd]
   int* table = nullptr;       // [sequences][pages_per_seq] physical page numbers
   int layers = 0, kv_heads = 0, hd = 0, page = 0;
+  int page_shift = 0;  // page = 1 << page_shift
   int pages_per_seq = 0;
 };
 
 // Consecutive rows of one sequence: rows row0 .. row0 + count of the call's
 // tensors are its positions first .. first + count; `len` positions are in
-// the cache. tile0: attention tiles of the runs before.
+// the cache. block0, splits: the attention's blocks of the runs before, and the
+// shares that this run's positions are cut into.
 struct KvRun {
-  int seq, first, row0, count, len, tile0;
+  int seq, first, row0, count, len, block0 = 0, splits = 1;
 };
 // Runs travel as a kernel parameter: a call needs no copy to the device and
 // leaves nothing behind that a later call could overwrite.
-constexpr int kKvRuns = 128;
+constexpr int kKvRuns = 120;  // 28 bytes each, in a parameter space of 4 KB
 struct KvRuns {
   int n = 0;
   // Rows of a decode step instead of runs: row r is position row_pos[r] of
@@ -65,17 +67,20 @@ struct KvAttendArgs {
 // Writes the runs' rows of one layer; pages that fill up become codes.
 cudaError_t launch_kv_append(const KvView& kv, const KvRuns& runs, int layer, const void* k, size_t k_stride,
                              const void* v, size_t v_stride, int type, int max_count, cudaStream_t s);
-// How launch_kv_attend will run: tiles, splits of the positions, and the
-// f32 workspace that the splits meet in (0 without splits).
+// How launch_kv_attend will run: blocks for each kv head, query columns a
+// block, and whether shares of the positions meet in the workspace. `chunks`
+// and `splits` are for rows of a decode step (the same for each).
 struct KvAttendPlan {
-  int tiles = 0, splits = 1, cols = 0, chunks = 0;
-  size_t workspace = 0;  // bytes
+  int blocks = 0, cols = 0, chunks = 1, splits = 1;
+  bool joins = false;
+  size_t workspace = 0;  // bytes, with joins
 };
-// No plan asks for more.
-constexpr size_t kKvWorkspace = 32u << 20;
+// The workspace: f32 partial results behind one counter a tile, which is
+// zero between calls. No plan needs more.
+constexpr size_t kKvCounters = 8192, kKvWorkspace = 32u << 20;
 KvAttendPlan plan_kv_attend(const KvView& kv, KvRuns& runs, const KvAttendArgs& a);
 cudaError_t launch_kv_attend(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& plan,
-                             float* workspace, cudaStream_t s);
+                             void* workspace, cudaStream_t s);
 // Positions first .. first + count of each run as values, rows of
 // [kv_heads][hd] from row0 on.
 cudaError_t launch_kv_read(const KvView& kv, const KvRuns& runs, int layer, void* k, void* v, int type, int max_count,
@@ -140,7 +145,7 @@ class KvCache {
   void fork_into(int parent, int64_t tokens, int child, cudaStream_t s);
   void settle(int seq, int64_t tokens);
   // Memory for the joins of any one attention call.
-  float* workspace() const { return workspace_; }
+  void* workspace() const { return workspace_; }
 
  private:
   struct Seq {
@@ -170,7 +175,7 @@ class KvCache {
   std::vector<Seq> seqs_;
   MinHeap free_seqs_, free_pages_;
   std::vector<int> refs_;  // sequences that hold each page
-  float* workspace_ = nullptr;
+  void* workspace_ = nullptr;
   int *moves_ = nullptr, *remap_ = nullptr;
   cudaEvent_t order_ = nullptr;
   unsigned long long last_stream_ = 0;

@@ -36,7 +36,8 @@ KvOptions KvOptions::parse(const char* text) {
   if (o.hd != 64 && o.hd != 128) throw Error("options: head_dim is 64 or 128");
   if (o.page != 16 && o.page != 32 && o.page != 64 && o.page != 128)
     throw Error("options: page_tokens is 16, 32, 64 or 128");
-  if ((size_t)o.layers * 2 * o.kv_heads > 65535u * 32u) throw Error("options: layers * kv_heads is too large");
+  if ((size_t)o.layers * 2 * o.kv_heads * o.page * o.hd >> 32)
+    throw Error("options: a page of all layers and heads holds 4 GB or more");
   return o;
 }
 
@@ -46,6 +47,7 @@ KvCache::KvCache(const KvOptions& o) : opt_(o) {
   view_.kv_heads = o.kv_heads;
   view_.hd = o.hd;
   view_.page = o.page;
+  while ((1 << view_.page_shift) < o.page) ++view_.page_shift;
   view_.pages_per_seq = std::max(1, o.max_tokens / o.page);
   const size_t blocks = (size_t)o.layers * 2 * o.kv_heads, block = (size_t)o.page * o.hd;
   const size_t open = (size_t)o.sequences * blocks * block * 2, table = (size_t)o.sequences * view_.pages_per_seq * 4;
@@ -60,6 +62,7 @@ KvCache::KvCache(const KvOptions& o) : opt_(o) {
     // The attention reads whole steps of 16 positions of an open page, also
     // those behind its end: they must hold numbers from the start.
     TRIT_CUDA(cudaMemset(view_.open, 0, open));
+    TRIT_CUDA(cudaMemset(workspace_, 0, kKvCounters * 4));
     TRIT_CUDA(cudaMemset(view_.table, 0, table));
     TRIT_CUDA(cudaDeviceSynchronize());
     TRIT_CUDA(cudaEventCreateWithFlags(&order_, cudaEventDisableTiming));
@@ -184,7 +187,7 @@ void KvCache::fork(const int* ids, const int64_t* tokens, size_t n, int* out, cu
     Seq& c = seqs_[id];
     const Seq& p = seqs_[ids[i]];
     share(c, p, tokens ? tokens[i] : p.len);
-    runs.run[runs.n++] = KvRun{id, ids[i], 0, (int)c.len, (int)p.len, 0};
+    runs.run[runs.n++] = KvRun{id, ids[i], 0, (int)c.len, (int)p.len};
     if (runs.n == kKvRuns || i + 1 == n) {
       TRIT_CUDA(launch_kv_fork(view_, runs, true, s));
       runs.n = 0;
@@ -228,7 +231,7 @@ void KvCache::copy(const int* ids, size_t n, int* out, cudaStream_t s) {
       moves.push_back(pg);
       entries.emplace_back(id * view_.pages_per_seq + (int)k, pg);
     }
-    runs.run[runs.n++] = KvRun{id, ids[i], 0, (int)c.len, (int)p.len, 0};
+    runs.run[runs.n++] = KvRun{id, ids[i], 0, (int)c.len, (int)p.len};
     if (runs.n == kKvRuns || i + 1 == n) {
       TRIT_CUDA(launch_kv_fork(view_, runs, false, s));
       runs.n = 0;
@@ -337,7 +340,7 @@ void KvCache::append(int layer, const int* ids, const int64_t* counts, size_t n,
   for (size_t i = 0; i < n; ++i) {
     Seq& q = seqs_[ids[i]];
     if (counts[i]) {
-      runs.run[runs.n++] = KvRun{ids[i], (int)(q.len - counts[i]), row, (int)counts[i], (int)q.len, 0};
+      runs.run[runs.n++] = KvRun{ids[i], (int)(q.len - counts[i]), row, (int)counts[i], (int)q.len};
       most = std::max(most, (int)counts[i]);
       row += (int)counts[i];
       q.filled[layer] = q.len;
@@ -392,20 +395,21 @@ void KvCache::attend(int layer, const int* ids, const int64_t* counts, size_t n,
   for (size_t i = 0; i < n; ++i) {
     const Seq& p = seqs_[ids[i]];
     if (counts[i]) {
-      runs.run[runs.n++] = KvRun{ids[i], (int)(p.len - counts[i]), row, (int)counts[i], (int)p.len, 0};
+      runs.run[runs.n++] = KvRun{ids[i], (int)(p.len - counts[i]), row, (int)counts[i], (int)p.len};
       a.max_len = std::max(a.max_len, (int)p.len);
       row += (int)counts[i];
     }
     if (runs.n < kKvRuns && i + 1 < n) continue;
     const KvAttendPlan plan = plan_kv_attend(view_, runs, a);
-    float* ws = workspace_;
-    if (capturing_) {
+    void* ws = workspace_;
+    if (capturing_ && plan.joins) {
       // A captured call's workspace belongs to its graph: two graphs of one
       // cache, or a graph and a call, may then run at once.
-      if (plan.workspace) TRIT_CUDA(cudaMallocAsync(&ws, plan.workspace, s));
+      TRIT_CUDA(cudaMallocAsync(&ws, plan.workspace, s));
+      TRIT_CUDA(cudaMemsetAsync(ws, 0, kKvCounters * 4, s));
     }
     TRIT_CUDA(launch_kv_attend(view_, runs, a, plan, ws, s));
-    if (capturing_ && plan.workspace) TRIT_CUDA(cudaFreeAsync(ws, s));
+    if (capturing_ && plan.joins) TRIT_CUDA(cudaFreeAsync(ws, s));
     runs.n = 0;
     a.max_len = 0;
   }
@@ -434,7 +438,7 @@ void KvCache::read(int layer, const int* ids, const int64_t* firsts, const int64
   for (size_t i = 0; i < n; ++i) {
     if (counts[i]) {
       runs.run[runs.n++] = KvRun{ids[i], (int)firsts[i], row, (int)counts[i],
-                                  (int)seqs_[ids[i]].filled[layer], 0};
+                                  (int)seqs_[ids[i]].filled[layer]};
       most = std::max(most, (int)counts[i]);
       row += (int)counts[i];
     }
@@ -495,7 +499,7 @@ void KvCache::fork_into(int parent, int64_t tokens, int child, cudaStream_t s) {
   enter(s, "fork");
   share(c, p, tokens);
   KvRuns runs;
-  runs.run[runs.n++] = KvRun{child, parent, 0, (int)tokens, (int)p.len, 0};
+  runs.run[runs.n++] = KvRun{child, parent, 0, (int)tokens, (int)p.len};
   TRIT_CUDA(launch_kv_fork(view_, runs, true, s));
   leave(s);
 }

@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import json
 import os
+from array import array
 from typing import Iterable, Sequence
 
 import numpy as np
@@ -87,21 +88,21 @@ def library() -> ctypes.CDLL:
         "trit_dense_q4_0": (ctypes.c_void_p, [ctypes.c_void_p, _size, _size, ctypes.c_int, ctypes.c_int]),
         "trit_cuda_kv_new": (ctypes.c_void_p, [ctypes.c_char_p]),
         "trit_cuda_kv_free": (None, [ctypes.c_void_p]),
-        "trit_cuda_kv_open": (ctypes.c_int, [ctypes.c_void_p, _size, _i32p]),
-        "trit_cuda_kv_fork": (ctypes.c_int, [ctypes.c_void_p, _i32p, _i64p, _size, _i32p, ctypes.c_void_p]),
-        "trit_cuda_kv_copy": (ctypes.c_int, [ctypes.c_void_p, _i32p, _size, _i32p, ctypes.c_void_p]),
-        "trit_cuda_kv_release": (ctypes.c_int, [ctypes.c_void_p, _i32p, _size]),
-        "trit_cuda_kv_extend": (ctypes.c_int, [ctypes.c_void_p, _i32p, _i64p, _size, ctypes.c_void_p]),
-        "trit_cuda_kv_append": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, _i32p, _i64p, _size, ctypes.c_void_p,
+        "trit_cuda_kv_open": (ctypes.c_int, [ctypes.c_void_p, _size, ctypes.c_void_p]),
+        "trit_cuda_kv_fork": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, _size, ctypes.c_void_p, ctypes.c_void_p]),
+        "trit_cuda_kv_copy": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, _size, ctypes.c_void_p, ctypes.c_void_p]),
+        "trit_cuda_kv_release": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, _size]),
+        "trit_cuda_kv_extend": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, _size, ctypes.c_void_p]),
+        "trit_cuda_kv_append": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, _size, ctypes.c_void_p,
                                                _size, ctypes.c_void_p, _size, ctypes.c_int, ctypes.c_void_p]),
-        "trit_cuda_kv_attend": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, _i32p, _i64p, _size, ctypes.c_void_p,
+        "trit_cuda_kv_attend": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, _size, ctypes.c_void_p,
                                                _size, ctypes.c_int32, ctypes.c_int, ctypes.c_float, ctypes.c_int,
                                                ctypes.c_void_p, _size, ctypes.c_void_p]),
-        "trit_cuda_kv_read": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, _i32p, _i64p, _i64p, _size,
+        "trit_cuda_kv_read": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, _size,
                                              ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
         "trit_cuda_kv_compact": (ctypes.c_int64, [ctypes.c_void_p, ctypes.c_void_p]),
         "trit_cuda_kv_length": (ctypes.c_int64, [ctypes.c_void_p, ctypes.c_int32]),
-        "trit_cuda_kv_pages": (ctypes.c_int, [ctypes.c_void_p, _i64p, _i64p]),
+        "trit_cuda_kv_pages": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
         "trit_dense_forward": (ctypes.c_int, [ctypes.c_void_p, _f32p, _size, _f32p]),
         "trit_dense_forward_device": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, _size, ctypes.c_void_p,
                                                      ctypes.c_void_p]),
@@ -416,11 +417,16 @@ class Dense:
 _KV_TYPES = {"f32": 0, "f16": 1, "bf16": 2}
 
 
-def _counts(values, n: int) -> np.ndarray:
-    a = np.ascontiguousarray(values, dtype=np.int64).reshape(-1)
-    if a.size != n:
-        raise TritError(f"{a.size} counts for {n} sequences")
-    return a
+def _words(values: Iterable[int], kind: str = "i", n: int | None = None) -> tuple[array, int]:
+    """An array of C ints ("i") or 64-bit ints ("q") and its address: a step's
+    few numbers, for which numpy would cost more than the call."""
+    try:
+        a = array(kind, values)
+    except (TypeError, OverflowError) as e:
+        raise TritError(f"sequences and counts are whole numbers: {e}") from None
+    if n is not None and len(a) != n:
+        raise TritError(f"{len(a)} counts for {n} sequences")
+    return a, a.buffer_info()[0]
 
 
 class KvCache:
@@ -436,13 +442,15 @@ class KvCache:
         page_tokens, sequences, max_tokens, device)."""
         self._handle = None
         text = json.dumps(dict(options, kv_heads=kv_heads, pages=pages)).encode()
-        self._handle = library().trit_cuda_kv_new(text)
+        lib = library()
+        self._handle = lib.trit_cuda_kv_new(text)
         if not self._handle:
             raise _error()
+        self._free = lib.trit_cuda_kv_free
 
     def close(self) -> None:
         if getattr(self, "_handle", None):
-            library().trit_cuda_kv_free(self._handle)
+            self._free(self._handle)
             self._handle = None
 
     def __del__(self):
@@ -462,49 +470,51 @@ class KvCache:
 
     def open(self, n: int = 1) -> list[int]:
         """n new sequences without positions."""
-        out = np.zeros(max(n, 1), dtype=np.int32)
-        if library().trit_cuda_kv_open(self._handle, n, _ptr(out, _i32p)) != 0:
+        out, to = _words(bytes(4 * max(n, 0)))
+        if library().trit_cuda_kv_open(self._handle, n, to) != 0:
             raise _error()
-        return out[:n].tolist()
+        return out.tolist()
 
     def fork(self, seqs: Sequence[int], tokens: Sequence[int] | None = None, stream: int | None = None) -> list[int]:
         """New sequences that start as the first tokens[i] positions of
         seqs[i] (None: all); their full pages are shared."""
-        ids = _ids(seqs)
-        out = np.zeros(max(ids.size, 1), dtype=np.int32)
-        cut = _ptr(_counts(tokens, ids.size), _i64p) if tokens is not None else None
-        if library().trit_cuda_kv_fork(self._handle, _ptr(ids, _i32p), cut, ids.size, _ptr(out, _i32p), stream) != 0:
+        ids, at = _words(seqs)
+        n = len(ids)
+        cut, cut_at = _words(tokens, "q", n) if tokens is not None else (None, None)
+        out, to = _words(bytes(4 * n))
+        if library().trit_cuda_kv_fork(self._handle, at, cut_at, n, to, stream) != 0:
             raise _error()
-        return out[:ids.size].tolist()
+        return out.tolist()
 
     def copy(self, seqs: Sequence[int], stream: int | None = None) -> list[int]:
         """New sequences equal to seqs, on pages of their own."""
-        ids = _ids(seqs)
-        out = np.zeros(max(ids.size, 1), dtype=np.int32)
-        if library().trit_cuda_kv_copy(self._handle, _ptr(ids, _i32p), ids.size, _ptr(out, _i32p), stream) != 0:
+        ids, at = _words(seqs)
+        out, to = _words(bytes(4 * len(ids)))
+        if library().trit_cuda_kv_copy(self._handle, at, len(ids), to, stream) != 0:
             raise _error()
-        return out[:ids.size].tolist()
+        return out.tolist()
 
     def release(self, seqs: Sequence[int]) -> None:
-        ids = _ids(seqs)
-        if library().trit_cuda_kv_release(self._handle, _ptr(ids, _i32p), ids.size) != 0:
+        """The sequences go, with the pages that no other holds."""
+        ids, at = _words(seqs)
+        if library().trit_cuda_kv_release(self._handle, at, len(ids)) != 0:
             raise _error()
 
     def extend(self, seqs: Sequence[int], counts: Sequence[int], stream: int | None = None) -> None:
         """counts[i] more positions for seqs[i], to be appended in every layer."""
-        ids = _ids(seqs)
-        n = _counts(counts, ids.size)
-        if library().trit_cuda_kv_extend(self._handle, _ptr(ids, _i32p), _ptr(n, _i64p), ids.size, stream) != 0:
+        ids, at = _words(seqs)
+        n, n_at = _words(counts, "q", len(ids))
+        if library().trit_cuda_kv_extend(self._handle, at, n_at, len(ids), stream) != 0:
             raise _error()
 
     def append(self, layer: int, seqs: Sequence[int], counts: Sequence[int], k_ptr: int, v_ptr: int,
                dtype: str = "f32", k_stride: int = 0, v_stride: int = 0, stream: int | None = None) -> None:
         """The keys and values of the last counts[i] positions of seqs[i]:
         rows of kv_heads x head_dim values (strides in elements, 0: packed)."""
-        ids = _ids(seqs)
-        n = _counts(counts, ids.size)
-        if library().trit_cuda_kv_append(self._handle, layer, _ptr(ids, _i32p), _ptr(n, _i64p), ids.size, k_ptr,
-                                         k_stride, v_ptr, v_stride, self._type(dtype), stream) != 0:
+        ids, at = _words(seqs)
+        n, n_at = _words(counts, "q", len(ids))
+        if library().trit_cuda_kv_append(self._handle, layer, at, n_at, len(ids), k_ptr, k_stride, v_ptr, v_stride,
+                                         self._type(dtype), stream) != 0:
             raise _error()
 
     def attend(self, layer: int, seqs: Sequence[int], counts: Sequence[int], q_ptr: int, out_ptr: int, heads: int,
@@ -512,21 +522,22 @@ class KvCache:
                stream: int | None = None) -> None:
         """Attention of counts[i] rows of heads x head_dim values against
         seqs[i]; causal rows stand at its last positions."""
-        ids = _ids(seqs)
-        n = _counts(counts, ids.size)
-        if library().trit_cuda_kv_attend(self._handle, layer, _ptr(ids, _i32p), _ptr(n, _i64p), ids.size, q_ptr,
-                                         q_stride, heads, self._type(dtype), scale, 1 if causal else 0, out_ptr,
-                                         out_stride, stream) != 0:
+        ids, at = _words(seqs)
+        n, n_at = _words(counts, "q", len(ids))
+        if library().trit_cuda_kv_attend(self._handle, layer, at, n_at, len(ids), q_ptr, q_stride, heads,
+                                         self._type(dtype), scale, 1 if causal else 0, out_ptr, out_stride,
+                                         stream) != 0:
             raise _error()
 
     def read(self, layer: int, seqs: Sequence[int], firsts: Sequence[int], counts: Sequence[int], k_ptr: int | None,
              v_ptr: int | None, dtype: str = "f32", stream: int | None = None) -> None:
         """What the cache holds of positions firsts[i] .. firsts[i] + counts[i]
         of seqs[i], as packed rows."""
-        ids = _ids(seqs)
-        f, n = _counts(firsts, ids.size), _counts(counts, ids.size)
-        if library().trit_cuda_kv_read(self._handle, layer, _ptr(ids, _i32p), _ptr(f, _i64p), _ptr(n, _i64p), ids.size,
-                                       k_ptr, v_ptr, self._type(dtype), stream) != 0:
+        ids, at = _words(seqs)
+        f, f_at = _words(firsts, "q", len(ids))
+        n, n_at = _words(counts, "q", len(ids))
+        if library().trit_cuda_kv_read(self._handle, layer, at, f_at, n_at, len(ids), k_ptr, v_ptr, self._type(dtype),
+                                       stream) != 0:
             raise _error()
 
     def compact(self, stream: int | None = None) -> int:
@@ -537,6 +548,7 @@ class KvCache:
         return int(n)
 
     def length(self, seq: int) -> int:
+        """The positions of a sequence."""
         n = library().trit_cuda_kv_length(self._handle, seq)
         if n < 0:
             raise _error()
@@ -545,7 +557,7 @@ class KvCache:
     def pages(self) -> tuple[int, int]:
         """Full pages: (in use, in all)."""
         used, total = ctypes.c_int64(), ctypes.c_int64()
-        if library().trit_cuda_kv_pages(self._handle, ctypes.byref(used), ctypes.byref(total)) != 0:
+        if library().trit_cuda_kv_pages(self._handle, ctypes.addressof(used), ctypes.addressof(total)) != 0:
             raise _error()
         return used.value, total.value
 
