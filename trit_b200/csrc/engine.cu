@@ -1009,31 +1009,44 @@ void Lm::attention_q8(int layer, int m, int max_tk, const std::vector<std::pair<
   a.causal = causal_ ? 1 : 0;
   a.scale = 1.0f / std::sqrt((float)hd);
   a.max_len = max_tk;
+  const int group = cfg_.heads / cfg_.kv_heads;
   KvRuns r;
-  auto go = [&](int most) {
+  // Runs of one call are of one kind: few rows each, or many.
+  auto go = [&](int most, bool prompt) {
     TRIT_CUDA(launch_kv_append(kv, r, layer, qkv_ + qd, ld, qkv_ + qd + kvd, ld, kKvF32, most, stream_));
-    const KvAttendPlan plan = plan_kv_attend(kv, r, a);
-    TRIT_CUDA(launch_kv_attend(kv, r, a, plan, kv8_->workspace(), stream_));
+    if (prompt) {
+      const KvAttendPlan plan = plan_kv_prompt(kv, r, a);
+      TRIT_CUDA(launch_kv_prompt(kv, r, a, plan, kv8_->workspace(), kv8_->status(), stream_));
+    } else {
+      const KvAttendPlan plan = plan_kv_attend(kv, r, a);
+      TRIT_CUDA(launch_kv_attend(kv, r, a, plan, kv8_->workspace(), stream_));
+    }
     timing_.gpu_launches += 1;
+    r.n = 0;
   };
   if (!causal_) {
     r.run[r.n++] = KvRun{0, 0, 0, m, m};
-    go(m);
+    go(m, kv_prompt_run(m, group));
   } else if (!runs) {
     r.n = m;
     r.row_seq = row_stream_;
     r.row_pos = row_pos_;
-    go(1);
+    go(1, false);
   } else {
     int most = 0;
-    for (size_t i = 0; i < runs->size(); ++i) {
-      const int row = (*runs)[i].first, count = (*runs)[i].second;
+    bool prompt = false;
+    for (const auto& run : *runs) {
+      const int row = run.first, count = run.second;
+      const bool many = kv_prompt_run(count, group);
+      if (r.n && (many != prompt || r.n == kKvRuns)) {
+        go(most, prompt);
+        most = 0;
+      }
+      prompt = many;
       r.run[r.n++] = KvRun{host_stream[row], host_pos[row], row, count, host_pos[row] + count};
       most = std::max(most, count);
-      if (r.n < kKvRuns && i + 1 < runs->size()) continue;
-      go(most);
-      r.n = most = 0;
     }
+    if (r.n) go(most, prompt);
   }
 }
 
@@ -1271,6 +1284,7 @@ void Lm::setup_tensor_cores() {
 
 // Throws if a tensor-core product gave up waiting (its status word).
 void Lm::check_tc_status() {
+  if (kv8_ && kv8_->take_failure()) throw Error("the attention of the 8-bit cache gave up waiting for its pipeline");
   if (!tc_ready_) return;
   int st = 0;
   TRIT_CUDA(cudaMemcpy(&st, tc_status_, 4, cudaMemcpyDeviceToHost));

@@ -7,38 +7,13 @@
 // each (layer, keys or values, kv head) block of the page gets one f32 scale
 // max|x| / 127 and codes nearest x / scale. Codes depend on the positions'
 // values alone, not on how many calls brought them.
-#include "kv8.h"
-
-#include <cuda_bf16.h>
-
 #include <algorithm>
 
 #include "kernels.h"
+#include "kv8.cuh"
 
 namespace trit {
 namespace {
-
-constexpr float kF16Max = 65504.0f;
-constexpr float kMInit = -1e30f;  // "no key yet": finite, so that differences stay numbers
-
-__host__ __device__ __forceinline__ size_t kv_block(const KvView& kv, int page_or_seq, int layer, int which, int head) {
-  return (((size_t)page_or_seq * kv.layers + layer) * 2 + which) * kv.kv_heads + head;
-}
-
-__device__ __forceinline__ float kv_load(const void* p, size_t i, int type) {
-  if (type == kKvF32) return ((const float*)p)[i];
-  if (type == kKvF16) return __half2float(((const __half*)p)[i]);
-  return __bfloat162float(((const __nv_bfloat16*)p)[i]);
-}
-__device__ __forceinline__ void kv_store(void* p, size_t i, int type, float v) {
-  if (type == kKvF32) ((float*)p)[i] = v;
-  else if (type == kKvF16) ((__half*)p)[i] = __float2half_rn(v);
-  else ((__nv_bfloat16*)p)[i] = __float2bfloat16_rn(v);
-}
-__device__ __forceinline__ __half to_cache_f16(float v) {
-  if (v != v) v = 0.0f;
-  return __float2half_rn(fminf(fmaxf(v, -kF16Max), kF16Max));
-}
 
 // The whole number nearest x / scale, ties to even, decided exactly: the
 // estimate is at most one off, and fma gives the sign of x - (q +- 1/2)
@@ -53,63 +28,6 @@ __device__ __forceinline__ int nearest_code(float x, float scale, float inv) {
   else if (down < 0.0f || (down == 0.0f && odd)) q -= 1.0f;
   const int c = (int)q;
   return x < 0.0f ? -c : c;
-}
-
-// 8 values at p (any alignment of the type; `vec`: 16-byte aligned).
-__device__ __forceinline__ void kv_load8(const void* p, size_t i, int type, bool vec, float (&v)[8]) {
-  if (!vec) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = kv_load(p, i + j, type);
-  } else if (type == kKvF32) {
-    const float4 a = *(const float4*)((const float*)p + i), b = *(const float4*)((const float*)p + i + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-    const uint4 a = *(const uint4*)((const __half*)p + i);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (type == kKvF16) {
-        const float2 f = __half22float2(*(const __half2*)&w[j]);
-        v[2 * j] = f.x;
-        v[2 * j + 1] = f.y;
-      } else {
-        v[2 * j] = __uint_as_float(w[j] << 16);
-        v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-      }
-    }
-  }
-}
-__device__ __forceinline__ void kv_store8(void* p, size_t i, int type, bool vec, const float (&v)[8]) {
-  if (!vec) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) kv_store(p, i + j, type, v[j]);
-  } else if (type == kKvF32) {
-    *(float4*)((float*)p + i) = make_float4(v[0], v[1], v[2], v[3]);
-    *(float4*)((float*)p + i + 4) = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (type == kKvF16) {
-        const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-        w[j] = *(const uint32_t*)&h;
-      } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-        w[j] = *(const uint32_t*)&h;
-      }
-    }
-    *(uint4*)((__half*)p + i) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-}
-__device__ __forceinline__ void halves8(uint4 h, float (&v)[8]) {
-  const uint32_t w[4] = {h.x, h.y, h.z, h.w};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 f = __half22float2(*(const __half2*)&w[j]);
-    v[2 * j] = f.x;
-    v[2 * j + 1] = f.y;
-  }
 }
 
 // Codes + 128 of 8 values, packed in order. x * inv is within 4e-5 of
@@ -288,9 +206,6 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const __grid_const
 //
 // Bound by the codes' bytes: 2 hd bytes a position and kv head.
 constexpr int kAttendWarps = 4;
-constexpr float kRaise = 14.0f, kBelow = 7.0f;
-constexpr float kZeroScaleLog2 = -31.0f;  // below every f16 page's scale (6e-8 / 127)
-
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   asm volatile(
@@ -303,27 +218,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
-}
-// Two codes (bytes 0, 1 or 2, 3 of w, each code + 128) as exact f16.
-__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
-  const uint32_t x = __byte_perm(w, 0x64646464u, 0x4140);
-  const __half2 h = __hsub2(*(const __half2*)&x, __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
-  return *(const uint32_t*)&h;
-}
-__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
-  const uint32_t x = __byte_perm(w, 0x64646464u, 0x4342);
-  const __half2 h = __hsub2(*(const __half2*)&x, __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
-  return *(const uint32_t*)&h;
-}
-// 2^x to 2 units in the last place (0 below 2^-126).
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *(const uint32_t*)&h;
 }
 __device__ __forceinline__ uint4 load16(const void* p) {
   uint4 v;
@@ -345,32 +239,6 @@ struct AttendShape {
   static constexpr int BLOCKS = HD == 128 && NT == 2 ? 2 : 3;  // an SM (registers)
   static constexpr int SMEM = kAttendWarps * STAGES * UNIT;
 };
-
-// The run and its place among the blocks of a kv head.
-__device__ __forceinline__ void find_run(const KvRuns& runs, int block, int chunks, int splits, KvRun& run, int& chunk,
-                                         int& split) {
-  if (runs.row_seq) {
-    const int row = block / (chunks * splits);
-    run.seq = runs.row_seq[row];
-    run.first = runs.row_pos[row];
-    run.row0 = row;
-    run.count = 1;
-    run.len = run.first + 1;
-    run.block0 = row * chunks * splits;
-    run.splits = splits;
-  } else {
-    int lo = 0, hi = runs.n - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (runs.run[mid].block0 <= block) lo = mid;
-      else hi = mid - 1;
-    }
-    run = runs.run[lo];
-  }
-  const int at = block - run.block0;
-  chunk = at / run.splits;
-  split = at % run.splits;
-}
 
 template <int HD, bool SPLIT, int NT>
 __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS)

@@ -81,6 +81,15 @@ constexpr size_t kKvCounters = 8192, kKvWorkspace = 32u << 20;
 KvAttendPlan plan_kv_attend(const KvView& kv, KvRuns& runs, const KvAttendArgs& a);
 cudaError_t launch_kv_attend(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& plan,
                              void* workspace, cudaStream_t s);
+// Attention of runs with many query rows (kv8_prompt.cu). *status is set
+// when a wait inside the kernel ran out.
+KvAttendPlan plan_kv_prompt(const KvView& kv, KvRuns& runs, const KvAttendArgs& a);
+cudaError_t launch_kv_prompt(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& plan,
+                             void* workspace, int* status, cudaStream_t s);
+// Whether a run's rows are worth the kernel of many rows: it takes a
+// tile of 128 query columns at the cost of one, the other kernel reads the
+// positions again for every 4 to 16 columns.
+inline bool kv_prompt_run(int count, int group) { return (size_t)count * group > 32; }
 // Positions first .. first + count of each run as values, rows of
 // [kv_heads][hd] from row0 on.
 cudaError_t launch_kv_read(const KvView& kv, const KvRuns& runs, int layer, void* k, void* v, int type, int max_count,
@@ -144,6 +153,10 @@ class KvCache {
   void reset(int seq);
   void fork_into(int parent, int64_t tokens, int child, cudaStream_t s);
   void settle(int seq, int64_t tokens);
+  // Whether an attention kernel gave up waiting since the last call, and the
+  // word that says so (host memory that kernels write).
+  bool take_failure();
+  int* status() const { return status_; }
   // Memory for the joins of any one attention call.
   void* workspace() const { return workspace_; }
 
@@ -167,6 +180,7 @@ class KvCache {
   // Orders stream s behind everything this cache queued on other streams.
   void enter(cudaStream_t s, const char* what, bool may_capture = false);
   void leave(cudaStream_t s);
+  void attend_runs(KvRuns& runs, KvAttendArgs& a, bool prompt, cudaStream_t s);
   void set_entries(const std::vector<std::pair<int, int>>& entries, cudaStream_t s);
 
   KvOptions opt_;
@@ -176,7 +190,7 @@ class KvCache {
   MinHeap free_seqs_, free_pages_;
   std::vector<int> refs_;  // sequences that hold each page
   void* workspace_ = nullptr;
-  int *moves_ = nullptr, *remap_ = nullptr;
+  int *moves_ = nullptr, *remap_ = nullptr, *status_ = nullptr;
   cudaEvent_t order_ = nullptr;
   unsigned long long last_stream_ = 0;
   bool used_ = false, capturing_ = false;

@@ -59,6 +59,8 @@ KvCache::KvCache(const KvOptions& o) : opt_(o) {
     TRIT_CUDA(cudaMalloc(&moves_, (size_t)o.pages * 8));
     TRIT_CUDA(cudaMalloc(&remap_, (size_t)o.pages * 4));
     TRIT_CUDA(cudaMalloc(&workspace_, kKvWorkspace));
+    TRIT_CUDA(cudaHostAlloc(&status_, 4, cudaHostAllocDefault));
+    *status_ = 0;
     // The attention reads whole steps of 16 positions of an open page, also
     // those behind its end: they must hold numbers from the start.
     TRIT_CUDA(cudaMemset(view_.open, 0, open));
@@ -83,6 +85,7 @@ void KvCache::release_memory() {
   void* bufs[] = {view_.codes, view_.scales, view_.open, view_.table, moves_, remap_, workspace_};
   for (void* b : bufs)
     if (b) cudaFree(b);
+  if (status_) cudaFreeHost(status_);
   if (order_) cudaEventDestroy(order_);
 }
 
@@ -129,6 +132,7 @@ void KvCache::check_layer(int layer) const {
 
 void KvCache::enter(cudaStream_t s, const char* what, bool may_capture) {
   TRIT_CUDA(cudaSetDevice(opt_.device));
+  if (take_failure()) throw Error("an attention call before this one gave up waiting for its pipeline");
   cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
   TRIT_CUDA(cudaStreamIsCapturing(s, &st));
   capturing_ = st != cudaStreamCaptureStatusNone;
@@ -390,30 +394,44 @@ void KvCache::attend(int layer, const int* ids, const int64_t* counts, size_t n,
   a.layer = layer;
   a.causal = causal ? 1 : 0;
   a.scale = scale;
-  KvRuns runs;
+  const int group = heads / opt_.kv_heads;
+  KvRuns few, many;
   int row = 0;
   for (size_t i = 0; i < n; ++i) {
     const Seq& p = seqs_[ids[i]];
-    if (counts[i]) {
-      runs.run[runs.n++] = KvRun{ids[i], (int)(p.len - counts[i]), row, (int)counts[i], (int)p.len};
-      a.max_len = std::max(a.max_len, (int)p.len);
-      row += (int)counts[i];
-    }
-    if (runs.n < kKvRuns && i + 1 < n) continue;
-    const KvAttendPlan plan = plan_kv_attend(view_, runs, a);
-    void* ws = workspace_;
-    if (capturing_ && plan.joins) {
-      // A captured call's workspace belongs to its graph: two graphs of one
-      // cache, or a graph and a call, may then run at once.
-      TRIT_CUDA(cudaMallocAsync(&ws, plan.workspace, s));
-      TRIT_CUDA(cudaMemsetAsync(ws, 0, kKvCounters * 4, s));
-    }
-    TRIT_CUDA(launch_kv_attend(view_, runs, a, plan, ws, s));
-    if (capturing_ && plan.joins) TRIT_CUDA(cudaFreeAsync(ws, s));
-    runs.n = 0;
-    a.max_len = 0;
+    if (!counts[i]) continue;
+    KvRuns& to = kv_prompt_run((int)counts[i], group) ? many : few;
+    to.run[to.n++] = KvRun{ids[i], (int)(p.len - counts[i]), row, (int)counts[i], (int)p.len};
+    row += (int)counts[i];
+    if (to.n == kKvRuns) attend_runs(to, a, &to == &many, s);
   }
+  attend_runs(few, a, false, s);
+  attend_runs(many, a, true, s);
   leave(s);
+}
+
+void KvCache::attend_runs(KvRuns& runs, KvAttendArgs& a, bool prompt, cudaStream_t s) {
+  if (!runs.n) return;
+  a.max_len = 0;
+  for (int i = 0; i < runs.n; ++i) a.max_len = std::max(a.max_len, runs.run[i].len);
+  const KvAttendPlan plan = prompt ? plan_kv_prompt(view_, runs, a) : plan_kv_attend(view_, runs, a);
+  void* ws = workspace_;
+  if (capturing_ && plan.joins) {
+    // A captured call's workspace belongs to its graph: two graphs of one
+    // cache, or a graph and a call, may then run at once.
+    TRIT_CUDA(cudaMallocAsync(&ws, plan.workspace, s));
+    TRIT_CUDA(cudaMemsetAsync(ws, 0, kKvCounters * 4, s));
+  }
+  if (prompt) TRIT_CUDA(launch_kv_prompt(view_, runs, a, plan, ws, status_, s));
+  else TRIT_CUDA(launch_kv_attend(view_, runs, a, plan, ws, s));
+  if (capturing_ && plan.joins) TRIT_CUDA(cudaFreeAsync(ws, s));
+  runs.n = 0;
+}
+
+bool KvCache::take_failure() {
+  const bool failed = *(volatile int*)status_ != 0;
+  *(volatile int*)status_ = 0;
+  return failed;
 }
 
 void KvCache::read(int layer, const int* ids, const int64_t* firsts, const int64_t* counts, size_t n, void* k, void* v,
