@@ -1,28 +1,30 @@
 // Attention of many query rows over the 8-bit cache on the fifth-generation
-// tensor cores. A block takes 128 query columns (a column is one query row of
-// one head of the kv head's group) and walks the positions 128 at a time:
+// tensor cores. A block takes one or two tiles of 128 query columns (a column
+// is one query row of one head of the kv head's group) and walks the positions
+// 128 at a time:
 //   S = Q K^T    tcgen05.mma kind::f16, M 128 columns, N 128 positions
 //   O += P V     M 128 columns, N the head's values, K 128 positions
 // Roles:
-//   warps 0-3   widen the codes of a tile to f16 (exact: a byte permute and a
-//               subtraction for two codes) into swizzled shared memory, keys
-//               and values each in two buffers; the open page's f16 is
-//               copied. Codes are loaded half a tile ahead in registers.
-//   warps 4-11  softmax: a thread owns one query column and half of a tile's
-//               positions (and half of O's values); the two threads of a
-//               column agree on the tile's largest score.
-//   warp 12     owns TMEM and issues the products.
-// P goes to TMEM, where the second product takes it as its first operand, so
-// shared memory carries only K, V and Q.
+//   warps 0-3   widen the codes of a step to f16 (exact: a byte permute and a
+//               subtraction for two codes) into swizzled shared memory; the
+//               open page's f16 is copied. Codes are loaded half a step ahead
+//               in registers, page numbers a step ahead.
+//   warps 4-    softmax, four warps a tile: a thread owns one query column
+//               (one TMEM lane). Two passes over its scores in TMEM: the
+//               largest, then P, which takes the place of the scores there
+//               and is the second product's first operand.
+//   last warp   owns TMEM and issues the products, for two tiles in turn: while
+//               one tile's run, the other's softmax does.
 //
 // f32 rows take two products each (Q and P as f16 value and remainder, 22
 // bits, summed in one accumulator), f16 and bf16 rows one (a row scaled by a
 // power of two; P rounded to 2^-11, below the output's rounding). Scales are
 // applied as in k_kv_attend: the key scale to S, the value scale in the
 // exponent of P. Bound by the tensor cores: 4 * 128 * 128 * hd operations a
-// tile, twice that for f32 rows.
+// tile and step, twice that for f32 rows.
 #include <algorithm>
 
+#include "device.cuh"
 #include "kernels.h"
 #include "kv8.cuh"
 #include "tc.cuh"
@@ -30,19 +32,26 @@
 namespace trit {
 namespace {
 
-constexpr int kTile = 128;  // query columns, and positions a step
-constexpr int kConvThreads = 128, kSoftThreads = 256;
-constexpr int kPromptThreads = kConvThreads + kSoftThreads + 32;
-// TMEM columns: S (two buffers), O, P (value, remainder).
-constexpr uint32_t kColO = 256, kColP = 384, kColPLow = 448;
+constexpr int kTile = 128;  // query columns of a tile, and positions a step
+constexpr int kConvThreads = 128;
+
+// QT: query tiles a block. V is in one buffer where two do not fit.
+template <int HD, bool LOW, int QT>
+struct PromptShape {
+  static constexpr int TILE = kTile * HD * 2;  // bytes of an f16 tile
+  static constexpr int BLOCKS = QT == 1 && !(LOW && HD == 128) ? 2 : 1;  // an SM
+  static constexpr int KS = QT == 1 && HD == 128 ? 1 : 2, VS = (QT == 1 || LOW) && HD == 128 ? 1 : 2;
+  static constexpr int THREADS = kConvThreads + QT * 128 + 32;
+  static constexpr uint32_t COL_O = QT * kTile;  // TMEM columns: S (then P) of each tile, O of each
+  static constexpr uint32_t COLS = QT == 2 ? 512 : 256;
+};
 
 struct PromptSmem {
-  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], sfree[2], qfull, pfull, ofull, pair[4], drain;
-  // Of a tile's groups of 16 positions: key scale, log2 and inverse of the
-  // value scale. Four tiles deep: a buffer is written again only when S of
-  // the tile two later is made, which waits for the softmax of this one.
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], qfull, done;
+  // Of a step's groups of 16 positions: key scale, log2 and inverse of the
+  // value scale. Four steps deep: a buffer is written again when the keys
+  // of the step two later are in use, which the softmax of this one precedes.
   float scales[4][8][4];
-  float top[2][2][kTile];  // by parity, half and column
   uint32_t tmem;
   int abort, last;
 };
@@ -75,24 +84,107 @@ __device__ __forceinline__ int tile_at(int r, int c) {
   return (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-template <int HD, bool LOW>
-constexpr int prompt_smem() {
-  return 1024 + (LOW ? 2 : 1) * kTile * HD * 2 + 4 * kTile * HD * 2 + (int)sizeof(PromptSmem);
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
 }
 
-template <int HD, bool LOW>
-__global__ void __launch_bounds__(kPromptThreads, 1)
+// The largest score of a row of S (128 TMEM columns from s_col), each group
+// of 16 with its scales; positions from `limit` on do not count.
+template <bool MASK>
+__device__ __forceinline__ float tile_top(uint32_t s_col, const float (*scales)[4], float factor, int key0, int limit) {
+  float top = kMInit;
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    uint32_t r[2][32];
+    tmem_ld<32>(s_col + 64 * b, r[0]);
+    tmem_ld<32>(s_col + 64 * b + 32, r[1]);
+    tmem_wait_ld();
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const uint32_t* x = r[h >> 1] + 16 * (h & 1);
+      const float2 sc = *(const float2*)scales[4 * b + h];
+      float y[4];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        float v = __uint_as_float(x[k]);
+        if (MASK && key0 + 64 * b + 16 * h + k >= limit) v = -INFINITY;
+        y[k & 3] = k < 4 ? v : fmaxf(y[k & 3], v);
+      }
+      const float v = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
+      top = fmaxf(top, MASK && v == -INFINITY ? v : fmaf(v, factor * sc.x, sc.y));
+    }
+  }
+  return top;
+}
+
+// S to P in its place: 2^(t - m) as f16 (and its remainder: 16 columns of
+// each in turn), and their sums over the value scales.
+template <bool MASK, bool LOW>
+__device__ __forceinline__ void tile_weights(uint32_t s_col, const float (*scales)[4], float factor, float m, int key0,
+                                             int limit, float2& sum) {
+  uint32_t r[2][32];
+  tmem_ld<32>(s_col, r[0]);
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    tmem_wait_ld();
+    if (b < 3) tmem_ld<32>(s_col + 32 * b + 32, r[(b + 1) & 1]);
+    const uint32_t* x = r[b & 1];
+    uint32_t out[32];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float4 sc = *(const float4*)scales[2 * b + h];
+      const float f = factor * sc.x, d = sc.y - m;
+      const float2 f2 = make_float2(f, f), d2 = make_float2(d, d), i2 = make_float2(sc.z, sc.z);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        float2 e = fma2(make_float2(__uint_as_float(x[16 * h + 2 * k]), __uint_as_float(x[16 * h + 2 * k + 1])), f2, d2);
+        if (MASK) {
+          const int key = key0 + 32 * b + 16 * h + 2 * k;
+          if (key >= limit) e.x = -INFINITY;
+          if (key + 1 >= limit) e.y = -INFINITY;
+        }
+        e.x = exp2_fast(e.x);
+        e.y = exp2_fast(e.y);
+        sum = fma2(e, i2, sum);
+        const __half2 p = __floats2half2_rn(e.x, e.y);
+        out[8 * h + k] = *(const uint32_t*)&p;
+        if (LOW) {
+          const float2 low = sub2(e, __half22float2(p));
+          out[16 + 8 * h + k] = pack_f16(low.x, low.y);
+        }
+      }
+    }
+    if (LOW) tmem_st32(s_col + 32 * b, out);
+    else tmem_st16(s_col + 16 * b, out);
+  }
+}
+
+template <int HD, bool LOW, int QT>
+constexpr int prompt_smem() {
+  using Shape = PromptShape<HD, LOW, QT>;
+  return 1024 + (QT * (LOW ? 2 : 1) + Shape::KS + Shape::VS) * Shape::TILE + (int)sizeof(PromptSmem);
+}
+
+template <int HD, bool LOW, int QT>
+__global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape<HD, LOW, QT>::BLOCKS)
     k_kv_prompt(const __grid_constant__ KvView kv, const __grid_constant__ KvRuns runs,
                 const __grid_constant__ KvAttendArgs a, int vec, int vec_out, void* workspace, int* status) {
-  constexpr int TILE = kTile * HD * 2;  // bytes of an f16 tile
-  constexpr int UH = HD / 2;            // values of O a softmax thread holds
+  using Shape = PromptShape<HD, LOW, QT>;
+  constexpr int TILE = Shape::TILE, KS = Shape::KS, VS = Shape::VS, QB = (LOW ? 2 : 1) * TILE;
+  constexpr int COLS = QT * kTile;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t* q_s = base;
-  uint8_t* k_s = q_s + (LOW ? 2 : 1) * TILE;  // [2]
-  uint8_t* v_s = k_s + 2 * TILE;              // [2]
-  PromptSmem* S = (PromptSmem*)(v_s + 2 * TILE);
+  uint8_t* q_s = base;                  // [QT][value, remainder]
+  uint8_t* k_s = q_s + QT * QB;         // [KS]
+  uint8_t* v_s = k_s + KS * TILE;       // [VS]
+  PromptSmem* S = (PromptSmem*)(v_s + VS * TILE);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int MMA_WARP = 4 + 4 * QT;
   const int head = blockIdx.y, g = a.heads / kv.kv_heads, P = kv.page;
 
   KvRun run;
@@ -100,13 +192,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   // The last tiles of a causal prompt see most: they start first.
   const int block = gridDim.x - 1 - blockIdx.x;
   find_run(runs, block, 1, 1, run, chunk, split);
-  const int cols = run.count * g, c0 = chunk * kTile;
-  const int last_row = (min(cols, c0 + kTile) - 1) / g;
+  const int cols = run.count * g, c0 = chunk * COLS;
+  const int groups = QT == 2 && c0 + kTile < cols ? 2 : 1;  // tiles with columns
+  const int last_row = (min(cols, c0 + COLS) - 1) / g;
   const int kend = a.causal ? min(run.len, run.first + last_row + 1) : run.len;
   const int tiles = (kend + kTile - 1) / kTile, per = (tiles + run.splits - 1) / run.splits;
   const int t0 = min(tiles, split * per), nt = min(tiles, t0 + per) - t0;
   const int full = run.len & ~(P - 1);  // positions in full pages
-  const size_t bytes = (size_t)P * HD;
   volatile int* abort = &S->abort;
 
   if (threadIdx.x == 0) {
@@ -116,18 +208,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       mbar_init(&S->vfull[i], kConvThreads);
       mbar_init(&S->vempty[i], 1);
       mbar_init(&S->sfull[i], 1);
-      mbar_init(&S->sfree[i], kSoftThreads);
+      mbar_init(&S->pfull[i], 128);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&S->pair[i], 64);
-    mbar_init(&S->qfull, kSoftThreads);
-    mbar_init(&S->pfull, kSoftThreads);
-    mbar_init(&S->ofull, 1);
-    mbar_init(&S->drain, 1);
+    mbar_init(&S->qfull, QT * 128);
+    mbar_init(&S->done, 1);
     S->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 12) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&S->tmem)), "r"(512)
+  if (warp == MMA_WARP) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&S->tmem)),
+                 "r"(Shape::COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -138,99 +228,99 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 
   if (warp < 4) {
     // ---- codes to f16 ----
-    constexpr int KU = HD / 16;          // 16-code units of a key
-    constexpr int N = kTile * KU / 128;  // units a thread takes of a tile's keys (of its values as many)
+    const uint32_t bytes = (uint32_t)P * HD, page_blocks = (uint32_t)kv.layers * 2 * kv.kv_heads;
+    const uint32_t page_bytes = page_blocks * bytes;
+    const size_t head_block = (size_t)a.layer * 2 * kv.kv_heads + head;
+    const uint8_t *codes_k = kv.codes + head_block * bytes, *codes_v = codes_k + (size_t)kv.kv_heads * bytes;
+    const __half* open_k = kv.open + kv_block(kv, run.seq, a.layer, 0, head) * (size_t)bytes;
+    const __half* open_v = open_k + (size_t)kv.kv_heads * bytes;
     const int* table = kv.table + (size_t)run.seq * kv.pages_per_seq;
-    const __half* open_k = kv.open + kv_block(kv, run.seq, a.layer, 0, head) * bytes;
-    const __half* open_v = kv.open + kv_block(kv, run.seq, a.layer, 1, head) * bytes;
-    // Keys: unit i of a thread is row kr(i) and values 16 ku .. of it; eight
-    // lanes take eight rows, so that their stores spread over the banks.
-    // Values: pair vr(i) of positions and values 8 vu .. of both.
-    const int kr0 = (warp * 8 + (lane & 7)), ku0 = lane >> 3;
+    constexpr int KU = HD / 16;          // 16-code units of a key
+    constexpr int N = kTile * KU / 128;  // units a thread takes of a step's keys (of its values as many)
+    // Keys: unit i of a thread is row key_row(i) and values 16 key_unit(i) ..
+    // of it; eight lanes take eight rows, so that their stores spread over
+    // the banks. Values: pair val_pair(i) of positions and values 8
+    // val_unit(i) .. of both, four pairs and two units in eight lanes.
+    const int kr0 = warp * 8 + (lane & 7), ku0 = lane >> 3;
     const int vr0 = warp * 4 + (lane & 3), vu0 = lane >> 2;
-    constexpr int KSTEP = KU / 4;  // a warp covers 8 rows x 4 units: turns over the units
+    constexpr int KSTEP = KU / 4, VSTEP = HD / 64;
     auto key_row = [&](int i) { return kr0 + i / KSTEP * 32; };
     auto key_unit = [&](int i) { return ku0 + i % KSTEP * 4; };
-    constexpr int VU = HD / 8;  // 8-value units of a pair
-    constexpr int VSTEP = VU / 8;
     auto val_pair = [&](int i) { return vr0 + i / VSTEP * 16; };
     auto val_unit = [&](int i) { return vu0 + i % VSTEP * 8; };
+    // Lanes 0-7: the page of each group of 16 positions of a step, or -1
+    // (not in a full page, or past the end).
+    auto pages_of = [&](int step) {
+      const int pos = step * kTile + 16 * (lane & 7);
+      return pos < kend && pos < full ? table[pos >> kv.page_shift] : -1;
+    };
     uint4 kc[N], vc[N];
-    auto load_keys = [&](int tile) {
+    const uint4 none = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+    auto load_keys = [&](int step, int pg) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int pos = tile * kTile + key_row(i);
-        kc[i] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-        if (pos < kend && pos < full) {
-          const size_t b = kv_block(kv, table[pos >> kv.page_shift], a.layer, 0, head) * bytes;
-          kc[i] = __ldg((const uint4*)(kv.codes + b + (size_t)(pos & (P - 1)) * HD + 16 * key_unit(i)));
-        }
+        const int r = key_row(i), page = __shfl_sync(0xffffffffu, pg, r >> 4);
+        const uint32_t at = (uint32_t)((step * kTile + r) & (P - 1)) * HD + 16 * key_unit(i);
+        kc[i] = page < 0 ? none : __ldg((const uint4*)(codes_k + (size_t)(uint32_t)page * page_bytes + at));
       }
     };
-    auto load_values = [&](int tile) {
+    auto load_values = [&](int step, int pg) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int pos = tile * kTile + 2 * val_pair(i);
-        vc[i] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-        if (pos < kend && pos < full) {
-          const size_t b = kv_block(kv, table[pos >> kv.page_shift], a.layer, 1, head) * bytes;
-          vc[i] = __ldg((const uint4*)(kv.codes + b + (size_t)((pos & (P - 1)) >> 1) * (2 * HD) + 16 * val_unit(i)));
-        }
+        const int r = 2 * val_pair(i), page = __shfl_sync(0xffffffffu, pg, r >> 4);
+        const uint32_t at = (uint32_t)((step * kTile + r) & (P - 1)) * HD + 16 * val_unit(i);
+        vc[i] = page < 0 ? none : __ldg((const uint4*)(codes_v + (size_t)(uint32_t)page * page_bytes + at));
       }
     };
-    if (nt > 0) load_keys(t0);
+    int pg = nt > 0 ? pages_of(t0) : -1;
+    if (nt > 0) load_keys(t0, pg);
     for (int j = 0; j < nt; ++j) {
-      const int s = j & 1, tile = t0 + j;
-      load_values(tile);
-      // Scales of the tile's groups (thread i: group i).
+      const int step = t0 + j;
+      const int pg_next = j + 1 < nt ? pages_of(step + 1) : -1;
+      load_values(step, pg);
+      // Scales of the step's groups.
       float ks = 0.0f, vl = 0.0f, vi = 0.0f;
       if (threadIdx.x < 8) {
-        const int pos = tile * kTile + 16 * threadIdx.x;
-        if (pos < kend) {
-          ks = 1.0f;
-          vi = 1.0f;
-          if (pos < full) {
-            const size_t b = kv_block(kv, table[pos >> kv.page_shift], a.layer, 0, head);
-            ks = kv.scales[b];
-            const float vs = kv.scales[b + kv.kv_heads];
-            vl = vs > 0.0f ? __log2f(vs) : kZeroScaleLog2;
-            vi = vs > 0.0f ? __fdividef(1.0f, vs) : 2147483648.0f;
-          }
+        if (pg >= 0) {
+          const float* sc = kv.scales + (size_t)(uint32_t)pg * page_blocks + head_block;
+          const float vs = sc[kv.kv_heads];
+          ks = sc[0];
+          vl = vs > 0.0f ? __log2f(vs) : kZeroScaleLog2;
+          vi = vs > 0.0f ? __fdividef(1.0f, vs) : 2147483648.0f;
+        } else if (step * kTile + 16 * (int)threadIdx.x < kend) {
+          ks = vi = 1.0f;
         }
       }
-      if (!mbar_wait(&S->kempty[s], ((j >> 1) & 1) ^ 1, abort)) break;
-      if (threadIdx.x < 8) {
-        float* to = S->scales[j & 3][threadIdx.x];
-        to[0] = ks;
-        to[1] = vl;
-        to[2] = vi;
-      }
-      uint8_t* kt = k_s + s * TILE;
+      // Positions of the step in the open page: [full, kend).
+      const bool tail = (step + 1) * kTile > full && full < kend;
+      if (!mbar_wait(&S->kempty[j % KS], (j / KS & 1) ^ 1, abort)) break;
+      if (threadIdx.x < 8) *(float4*)S->scales[j & 3][threadIdx.x] = make_float4(ks, vl, vi, 0.0f);
+      uint8_t* kt = k_s + j % KS * TILE;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int r = key_row(i), u = key_unit(i), pos = tile * kTile + r;
-        uint4 x, y;
-        if (pos >= full && pos < kend) {
+        const int r = key_row(i), u = key_unit(i), pos = step * kTile + r;
+        uint4 x = make_uint4(codes_lo(kc[i].x), codes_hi(kc[i].x), codes_lo(kc[i].y), codes_hi(kc[i].y));
+        uint4 y = make_uint4(codes_lo(kc[i].z), codes_hi(kc[i].z), codes_lo(kc[i].w), codes_hi(kc[i].w));
+        if (tail && pos >= full && pos < kend) {
           const uint4* src = (const uint4*)(open_k + (size_t)(pos - full) * HD + 16 * u);
           x = src[0];
           y = src[1];
-        } else {
-          x = make_uint4(codes_lo(kc[i].x), codes_hi(kc[i].x), codes_lo(kc[i].y), codes_hi(kc[i].y));
-          y = make_uint4(codes_lo(kc[i].z), codes_hi(kc[i].z), codes_lo(kc[i].w), codes_hi(kc[i].w));
         }
         *(uint4*)(kt + tile_at(r, 2 * u)) = x;
         *(uint4*)(kt + tile_at(r, 2 * u + 1)) = y;
       }
       fence_async_smem();
-      mbar_arrive(&S->kfull[s]);
-      if (j + 1 < nt) load_keys(tile + 1);
-      if (!mbar_wait(&S->vempty[s], ((j >> 1) & 1) ^ 1, abort)) break;
-      uint8_t* vt = v_s + s * TILE;
+      mbar_arrive(&S->kfull[j % KS]);
+      pg = pg_next;
+      if (j + 1 < nt) load_keys(step + 1, pg);
+      if (!mbar_wait(&S->vempty[j % VS], (j / VS & 1) ^ 1, abort)) break;
+      uint8_t* vt = v_s + j % VS * TILE;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int r = 2 * val_pair(i), u = val_unit(i), pos = tile * kTile + r;
-        uint4 x, y;
-        if (pos >= full && pos < kend) {
+        const int r = 2 * val_pair(i), u = val_unit(i), pos = step * kTile + r;
+        uint4 x = make_uint4(codes_even(vc[i].x), codes_even(vc[i].y), codes_even(vc[i].z), codes_even(vc[i].w));
+        uint4 y = make_uint4(codes_odd(vc[i].x), codes_odd(vc[i].y), codes_odd(vc[i].z), codes_odd(vc[i].w));
+        if (tail && pos >= full && pos < kend) {
           // Pairs of the open page: words (position 0, position 1) of a value.
           const uint4* src = (const uint4*)(open_v + (size_t)(pos - full) * HD + 16 * u);
           const uint4 p = src[0], q = src[1];
@@ -238,223 +328,170 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                          __byte_perm(q.z, q.w, 0x5410));
           y = make_uint4(__byte_perm(p.x, p.y, 0x7632), __byte_perm(p.z, p.w, 0x7632), __byte_perm(q.x, q.y, 0x7632),
                          __byte_perm(q.z, q.w, 0x7632));
-        } else {
-          x = make_uint4(codes_even(vc[i].x), codes_even(vc[i].y), codes_even(vc[i].z), codes_even(vc[i].w));
-          y = make_uint4(codes_odd(vc[i].x), codes_odd(vc[i].y), codes_odd(vc[i].z), codes_odd(vc[i].w));
         }
         *(uint4*)(vt + tile_at(r, u)) = x;
         *(uint4*)(vt + tile_at(r + 1, u)) = y;
       }
       fence_async_smem();
-      mbar_arrive(&S->vfull[s]);
+      mbar_arrive(&S->vfull[j % VS]);
     }
-  } else if (warp == 12) {
+  } else if (warp == MMA_WARP) {
     if (lane == 0 && nt > 0) {
       const uint32_t qa = smem_u32(q_s), ka = smem_u32(k_s), va = smem_u32(v_s);
-      auto pv = [&](int j) -> bool {
-        if (!mbar_wait(&S->pfull, j & 1, abort) || !mbar_wait(&S->vfull[j & 1], (j >> 1) & 1, abort)) return false;
-        fence_after();
-        const uint32_t v = va + (j & 1) * TILE;
-#pragma unroll
-        for (int i = 0; i < kTile / 16; ++i) {
-          const uint64_t b = smem_desc_sw128_mn(v + i * 2048, kTile * 128);
-          mma_f16_ts(tmem + kColO, tmem + kColP + i * 8, b, idesc_f16n(HD, true), (j > 0 || i > 0) ? 1u : 0u);
-          if (LOW) mma_f16_ts(tmem + kColO, tmem + kColPLow + i * 8, b, idesc_f16n(HD, true), 1u);
-        }
-        mma_commit(&S->ofull);
-        mma_commit(&S->vempty[j & 1]);
-        return true;
-      };
-      bool ok = mbar_wait(&S->qfull, 0, abort);
-      for (int j = 0; j < nt && ok; ++j) {
-        const int s = j & 1;
-        if (!mbar_wait(&S->kfull[s], (j >> 1) & 1, abort) || !mbar_wait(&S->sfree[s], ((j >> 1) & 1) ^ 1, abort)) {
-          ok = false;
-          break;
-        }
-        fence_after();
-        const uint32_t k = ka + s * TILE;
+      auto scores = [&](int j, int t) {
+        const uint32_t k = ka + j % KS * TILE, q = qa + t * QB;
 #pragma unroll
         for (int i = 0; i < HD / 16; ++i) {
           const uint32_t at = (i >> 2) * (kTile * 128) + (i & 3) * 32;
           const uint64_t b = smem_desc_sw128(k + at);
-          mma_f16(tmem + s * kTile, smem_desc_sw128(qa + at), b, idesc_f16n(kTile), i > 0 ? 1u : 0u);
-          if (LOW) mma_f16(tmem + s * kTile, smem_desc_sw128(qa + TILE + at), b, idesc_f16n(kTile), 1u);
+          mma_f16(tmem + t * kTile, smem_desc_sw128(q + at), b, idesc_f16n(kTile), i > 0 ? 1u : 0u);
+          if (LOW) mma_f16(tmem + t * kTile, smem_desc_sw128(q + TILE + at), b, idesc_f16n(kTile), 1u);
         }
-        mma_commit(&S->sfull[s]);
-        mma_commit(&S->kempty[s]);
-        if (j > 0) ok = pv(j - 1);
+        mma_commit(&S->sfull[t]);
+      };
+      auto values = [&](int j, int t) {
+        const uint32_t v = va + j % VS * TILE, o = tmem + Shape::COL_O + t * kTile;
+#pragma unroll
+        for (int i = 0; i < kTile / 16; ++i) {
+          const uint64_t b = smem_desc_sw128_mn(v + i * 2048, kTile * 128);
+          const uint32_t p = tmem + t * kTile + (LOW ? 32 * (i >> 1) + 8 * (i & 1) : 8 * i);
+          mma_f16_ts(o, p, b, idesc_f16n(HD, true), (j > 0 || i > 0) ? 1u : 0u);
+          if (LOW) mma_f16_ts(o, p + 16, b, idesc_f16n(HD, true), 1u);
+        }
+      };
+      bool ok = mbar_wait(&S->qfull, 0, abort) && mbar_wait(&S->kfull[0], 0, abort);
+      if (ok) {
+        fence_after();
+        for (int t = 0; t < groups; ++t) scores(0, t);
+        mma_commit(&S->kempty[0]);
       }
-      if (ok) pv(nt - 1);
-      mma_commit(&S->drain);
+      for (int j = 0; j < nt && ok; ++j) {
+        if (!mbar_wait(&S->vfull[j % VS], j / VS & 1, abort)) break;
+        for (int t = 0; t < groups && ok; ++t) {
+          // A tile's P is ready; its product, then the next step's scores in
+          // the same place.
+          if (!mbar_wait(&S->pfull[t], j & 1, abort)) {
+            ok = false;
+            break;
+          }
+          fence_after();
+          values(j, t);
+          if (t == groups - 1) mma_commit(&S->vempty[j % VS]);
+          if (j + 1 < nt) {
+            if (t == 0 && !mbar_wait(&S->kfull[(j + 1) % KS], (j + 1) / KS & 1, abort)) {
+              ok = false;
+              break;
+            }
+            fence_after();
+            scores(j + 1, t);
+            if (t == groups - 1) mma_commit(&S->kempty[(j + 1) % KS]);
+          }
+        }
+      }
+      mma_commit(&S->done);
       const long long start = now_ns();
-      while (!mbar_test(&S->drain, 0) && now_ns() - start < TC_WAIT_NS) {
+      while (!mbar_test(&S->done, 0) && now_ns() - start < TC_WAIT_NS) {
       }
     }
   } else {
     // ---- softmax ----
-    const int quarter = warp & 3, half = (warp - 4) >> 2, q = quarter * 32 + lane;
-    const int c = c0 + q;
+    const int t = (warp - 4) >> 2, q = (warp & 3) * 32 + lane, c = c0 + t * kTile + q;
     const bool live = c < cols;
-    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t s_col = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * kTile;
+    const uint32_t o_col = s_col - t * kTile + Shape::COL_O + t * kTile;
     const int limit = !live ? 0 : a.causal ? min(run.len, run.first + c / g + 1) : run.len;
     int low_limit = live ? limit : 0x7fffffff;  // of the warp's rows: below it no mask is needed
 #pragma unroll
     for (int o = 16; o; o >>= 1) low_limit = min(low_limit, __shfl_xor_sync(0xffffffffu, low_limit, o));
-    int pairs = 0;
-    // The two threads of a column tell each other a number.
-    auto both_max = [&](float x, bool& ok) {
-      S->top[pairs & 1][half][q] = x;
-      mbar_arrive(&S->pair[quarter]);
-      ok = __all_sync(0xffffffffu, mbar_wait(&S->pair[quarter], pairs & 1, abort));
-      const float y = S->top[pairs & 1][half ^ 1][q];
-      ++pairs;
-      return fmaxf(x, y);
-    };
-    bool ok = true;
+    // The row, scaled into [1, 2) (its sign taken from the scale, so that the
+    // largest product is the largest score), as f16 value and remainder.
     float factor;
     {
-      // This thread's half of the row: values UH * half ..
-      const size_t at = live ? (size_t)(run.row0 + c / g) * a.q_stride + (size_t)(head * g + c % g) * HD + UH * half : 0;
-      float v[UH / 8][8];
-      float top = 0.0f;
+      const size_t at = live ? (size_t)(run.row0 + c / g) * a.q_stride + (size_t)(head * g + c % g) * HD : 0;
+      float top = 0.0f, v[8];
+#pragma unroll 4
+      for (int i = 0; i < HD / 8 && live; ++i) {
+        kv_load8(a.q, at + 8 * i, a.type, vec, v);
 #pragma unroll
-      for (int i = 0; i < UH / 8; ++i) {
-        if (live) {
-          kv_load8(a.q, at + 8 * i, a.type, vec, v[i]);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) v[i][k] = 0.0f;
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[i][k]));
+        for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[k]));
       }
-      top = both_max(top, ok);
       int e = 0;
       if (top > 0.0f && top <= 3.4e38f) e = max(-126, min(126, (int)((__float_as_uint(top) >> 23) & 255) - 127));
-      const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-      factor = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + e) << 23);
+      float down = __uint_as_float((uint32_t)(127 - e) << 23);
+      if (a.scale < 0.0f) down = -down;
+      factor = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll 4
+      for (int i = 0; i < HD / 8; ++i) {
+        if (live) {
+          kv_load8(a.q, at + 8 * i, a.type, vec, v);
+        } else {
 #pragma unroll
-      for (int i = 0; i < UH / 8; ++i) {
+          for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+        }
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float x = v[i][2 * k] * down, y = v[i][2 * k + 1] * down;
+          const float x = v[2 * k] * down, y = v[2 * k + 1] * down;
           const __half2 h = __floats2half2_rn(x, y);
           hi[k] = *(const uint32_t*)&h;
           lo[k] = pack_f16(x - __low2float(h), y - __high2float(h));
         }
-        const int to = tile_at(q, UH / 8 * half + i);
-        *(uint4*)(q_s + to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if (LOW) *(uint4*)(q_s + TILE + to) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        *(uint4*)(q_s + t * QB + tile_at(q, i)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (LOW) *(uint4*)(q_s + t * QB + TILE + tile_at(q, i)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
     }
     fence_async_smem();
     mbar_arrive(&S->qfull);
-    float m = kMInit, l = 0.0f;
-    for (int j = 0; j < nt && ok; ++j) {
-      const int s = j & 1, key0 = (t0 + j) * kTile + 64 * half;
+    float m = kMInit;
+    float2 l2 = make_float2(0.0f, 0.0f);
+    bool ok = true;
+    for (int j = 0; j < nt && t < groups; ++j) {
+      const int key0 = (t0 + j) * kTile;
       // Warp-uniform waits: the TMEM loads and stores below are warp-wide.
-      if (!__all_sync(0xffffffffu, mbar_wait(&S->sfull[s], (j >> 1) & 1, abort))) {
+      // The scores are ready, and the tile's products before them are done.
+      if (!__all_sync(0xffffffffu, mbar_wait(&S->sfull[t], j & 1, abort))) {
         ok = false;
         break;
       }
       fence_after();
-      float v[64];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        uint32_t r[32];
-        tmem_ld<32>(lanes + s * kTile + 64 * half + 32 * b, r);
-        tmem_wait_ld();
-#pragma unroll
-        for (int k = 0; k < 32; ++k) v[32 * b + k] = __uint_as_float(r[k]);
-      }
-      float f[4], vl[4], vi[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 x = *(const float4*)S->scales[j & 3][4 * half + i];
-        f[i] = factor * x.x;
-        vl[i] = x.y;
-        vi[i] = x.z;
-      }
-      fence_before();
-      mbar_arrive(&S->sfree[s]);
-      float top = kMInit;
-#pragma unroll
-      for (int k = 0; k < 64; ++k) v[k] = fmaf(v[k], f[k >> 4], vl[k >> 4]);
-      if (key0 + 64 > low_limit) {
-#pragma unroll
-        for (int k = 0; k < 64; ++k)
-          if (key0 + k >= limit) v[k] = -INFINITY;
-      }
-#pragma unroll
-      for (int k = 0; k < 64; ++k) top = fmaxf(top, v[k]);
-      top = both_max(top, ok);
-      if (!ok) break;
+      const bool mask = key0 + kTile > low_limit;
+      const float(*scales)[4] = S->scales[j & 3];
+      const float top = mask ? tile_top<true>(s_col, scales, factor, key0, limit)
+                             : tile_top<false>(s_col, scales, factor, key0, limit);
       float alpha = 1.0f;
       if (top > m + kRaise) {
         alpha = exp2_fast(m - (top - kBelow));
         m = top - kBelow;
-        l *= alpha;
+        l2.x *= alpha;
+        l2.y *= alpha;
       }
-      // P and O are free when the product before is done.
-      if (j > 0) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&S->ofull, (j - 1) & 1, abort))) {
-          ok = false;
-          break;
-        }
-        fence_after();
-        if (__any_sync(0xffffffffu, alpha != 1.0f)) {
+      if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
 #pragma unroll
-          for (int b = 0; b < UH / 32; ++b) {
-            uint32_t r[32];
-            tmem_ld<32>(lanes + kColO + UH * half + 32 * b, r);
-            tmem_wait_ld();
+        for (int b = 0; b < HD / 32; ++b) {
+          uint32_t r[32];
+          tmem_ld<32>(o_col + 32 * b, r);
+          tmem_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * alpha);
-            tmem_st32(lanes + kColO + UH * half + 32 * b, r);
-          }
+          for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * alpha);
+          tmem_st32(o_col + 32 * b, r);
         }
       }
-      uint32_t hi[32];
-#pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        const float x = exp2_fast(v[2 * k] - m), y = exp2_fast(v[2 * k + 1] - m);
-        l = fmaf(x + y, vi[k >> 3], l);
-        const __half2 h = __floats2half2_rn(x, y);
-        hi[k] = *(const uint32_t*)&h;
-        if (LOW) {
-          v[2 * k] = x - __low2float(h);
-          v[2 * k + 1] = y - __high2float(h);
-        }
-      }
-      tmem_st32(lanes + kColP + 32 * half, hi);
-      if (LOW) {
-#pragma unroll
-        for (int k = 0; k < 32; ++k) hi[k] = pack_f16(v[2 * k], v[2 * k + 1]);
-        tmem_st32(lanes + kColPLow + 32 * half, hi);
-      }
+      if (mask) tile_weights<true, LOW>(s_col, scales, factor, m, key0, limit, l2);
+      else tile_weights<false, LOW>(s_col, scales, factor, m, key0, limit, l2);
       tmem_wait_st();
       fence_before();
-      mbar_arrive(&S->pfull);
+      mbar_arrive(&S->pfull[t]);
     }
-    // The column's sums, joined over its two threads.
-    if (ok) {
-      S->top[pairs & 1][half][q] = l;
-      mbar_arrive(&S->pair[quarter]);
-      ok = __all_sync(0xffffffffu, mbar_wait(&S->pair[quarter], pairs & 1, abort));
-      l += S->top[pairs & 1][half ^ 1][q];
-    }
-    if (ok && nt > 0) ok = __all_sync(0xffffffffu, mbar_wait(&S->ofull, (nt - 1) & 1, abort));
-    if (ok) {
+    if (t < groups && ok && nt > 0) ok = __all_sync(0xffffffffu, mbar_wait(&S->done, 0, abort));
+    if (t < groups && ok) {
       fence_after();
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      float* part = (float*)workspace + kKvCounters + (((size_t)head * gridDim.x + block) * kTile + q) * (HD + 2);
+      const float l = l2.x + l2.y, inv = l == 0.0f ? 0.0f : 1.0f / l;
+      float* part = (float*)workspace + kKvCounters + (((size_t)head * gridDim.x + block) * COLS + t * kTile + q) * (HD + 2);
 #pragma unroll
-      for (int b = 0; b < UH / 32; ++b) {
+      for (int b = 0; b < HD / 32; ++b) {
         uint32_t r[32];
         if (nt > 0) {
-          tmem_ld<32>(lanes + kColO + UH * half + 32 * b, r);
+          tmem_ld<32>(o_col + 32 * b, r);
           tmem_wait_ld();
         } else {
 #pragma unroll
@@ -462,7 +499,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
         if (!live) continue;
         if (run.splits == 1) {
-          const size_t to = (size_t)(run.row0 + c / g) * a.out_stride + (size_t)(head * g + c % g) * HD + UH * half + 32 * b;
+          const size_t to = (size_t)(run.row0 + c / g) * a.out_stride + (size_t)(head * g + c % g) * HD + 32 * b;
 #pragma unroll
           for (int k = 0; k < 32; k += 8) {
             float x[8];
@@ -472,21 +509,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           }
         } else {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) part[UH * half + 32 * b + k] = __uint_as_float(r[k]);
+          for (int k = 0; k < 32; k += 2)
+            *(float2*)(part + 32 * b + k) = make_float2(__uint_as_float(r[k]), __uint_as_float(r[k + 1]));
         }
       }
-      if (run.splits > 1 && live && half == 0) {
-        part[HD] = m;
-        part[HD + 1] = l;
-      }
+      if (run.splits > 1 && live) *(float2*)(part + HD) = make_float2(m, l);
     }
   }
   if (run.splits > 1) __threadfence();
   fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == MMA_WARP) {
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Shape::COLS) : "memory");
   }
   if (threadIdx.x == 0 && S->abort) *(volatile int*)status = 1;
   if (run.splits == 1) return;
@@ -498,13 +533,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   __syncthreads();
   if (!S->last) return;
   __threadfence();
-  const float* first = (const float*)workspace + kKvCounters + ((size_t)head * gridDim.x + block - split) * kTile * (HD + 2);
-  for (int x = threadIdx.x; x < kTile * HD; x += kPromptThreads) {
+  const float* first = (const float*)workspace + kKvCounters + ((size_t)head * gridDim.x + block - split) * COLS * (HD + 2);
+  for (int x = threadIdx.x; x < COLS * HD; x += Shape::THREADS) {
     const int lc = x / HD, d = x % HD, c = c0 + lc;
     if (c >= cols) break;
     float top = kMInit, sum = 0.0f, val = 0.0f;
+#pragma unroll 4
     for (int i = 0; i < run.splits; ++i) {
-      const float* p = first + ((size_t)i * kTile + lc) * (HD + 2);
+      const float* p = first + ((size_t)i * COLS + lc) * (HD + 2);
       const float pm = __ldcg(p + HD), pl = __ldcg(p + HD + 1), pv = __ldcg(p + d);
       const float to = fmaxf(top, pm), fa = exp2_fast(top - to), fb = exp2_fast(pm - to);
       sum = fmaf(sum, fa, pl * fb);
@@ -516,42 +552,55 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   }
 }
 
-template <int HD, bool LOW>
+template <int HD, bool LOW, int QT>
 cudaError_t prompt(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& p, int vec,
                    int vec_out, void* ws, int* status, cudaStream_t s) {
-  constexpr int smem = prompt_smem<HD, LOW>();
+  constexpr int smem = prompt_smem<HD, LOW, QT>();
   static_assert(smem <= 227 * 1024, "the tiles fit in shared memory");
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   static DeviceOnce once;
   e = once.run(dev, [] {
-    return cudaFuncSetAttribute(k_kv_prompt<HD, LOW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    return cudaFuncSetAttribute(k_kv_prompt<HD, LOW, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   });
   if (e != cudaSuccess) return e;
-  k_kv_prompt<HD, LOW><<<dim3(p.blocks, kv.kv_heads), kPromptThreads, smem, s>>>(kv, runs, a, vec, vec_out, ws, status);
+  k_kv_prompt<HD, LOW, QT><<<dim3(p.blocks, kv.kv_heads), PromptShape<HD, LOW, QT>::THREADS, smem, s>>>(
+      kv, runs, a, vec, vec_out, ws, status);
   return cudaGetLastError();
+}
+template <int HD, bool LOW>
+cudaError_t prompt(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& p, int vec,
+                   int vec_out, void* ws, int* status, cudaStream_t s) {
+  return p.cols == 2 * kTile ? prompt<HD, LOW, 2>(kv, runs, a, p, vec, vec_out, ws, status, s)
+                             : prompt<HD, LOW, 1>(kv, runs, a, p, vec, vec_out, ws, status, s);
 }
 
 }  // namespace
 
-// A tile's positions are cut into shares only while the tiles leave SMs idle;
-// a share costs about a step and a half to start and to join (measured).
+// Two tiles a block while that leaves no SM idle (the two share the widened
+// codes, and one's products hide the other's softmax); positions are cut into
+// shares only while blocks leave SMs idle. A share costs about a step and a
+// half to start and to join.
 KvAttendPlan plan_kv_prompt(const KvView& kv, KvRuns& runs, const KvAttendArgs& a) {
   KvAttendPlan p;
-  p.cols = kTile;
   const int g = a.heads / kv.kv_heads, slots = current_sm_count();
   double tiles = 0, work = 0;
   int longest = 1;
-  for (int i = 0; i < runs.n; ++i) {
-    const double t = (double)(((size_t)runs.run[i].count * g + kTile - 1) / kTile);
-    const int steps = (runs.run[i].len + kTile - 1) / kTile;
-    tiles += t;
-    work += t * steps;
-    longest = std::max(longest, steps);
+  for (int pass = 0; pass < 2; ++pass) {
+    p.cols = pass == 0 ? 2 * kTile : kTile;
+    tiles = work = 0;
+    for (int i = 0; i < runs.n; ++i) {
+      const double t = (double)(((size_t)runs.run[i].count * g + p.cols - 1) / p.cols);
+      const int steps = (runs.run[i].len + kTile - 1) / kTile;
+      tiles += t;
+      work += t * steps;
+      longest = std::max(longest, steps);
+    }
+    tiles *= kv.kv_heads;
+    work *= kv.kv_heads;
+    if (tiles >= slots) break;
   }
-  tiles *= kv.kv_heads;
-  work *= kv.kv_heads;
   int share = longest;
   if (tiles < 2.0 * slots) {
     double best = (double)((int)((tiles + slots - 1) / slots)) * (longest + 1.5);
@@ -565,7 +614,7 @@ KvAttendPlan plan_kv_prompt(const KvView& kv, KvRuns& runs, const KvAttendArgs& 
       }
     }
   }
-  const size_t bytes = (size_t)kv.kv_heads * kTile * (kv.hd + 2) * 4;
+  const size_t bytes = (size_t)kv.kv_heads * p.cols * (kv.hd + 2) * 4;
   for (;; share = std::min(longest, 2 * share)) {
     p.blocks = 0;
     p.joins = false;
@@ -574,7 +623,7 @@ KvAttendPlan plan_kv_prompt(const KvView& kv, KvRuns& runs, const KvAttendArgs& 
       r.block0 = p.blocks;
       r.splits = std::max(1, ((r.len + kTile - 1) / kTile + share - 1) / share);
       p.joins |= r.splits > 1;
-      p.blocks += (int)(((size_t)r.count * g + kTile - 1) / kTile) * r.splits;
+      p.blocks += (int)(((size_t)r.count * g + p.cols - 1) / p.cols) * r.splits;
     }
     p.workspace = kKvCounters * 4 + p.blocks * bytes;
     if (!p.joins || ((size_t)p.blocks * kv.kv_heads <= kKvCounters && p.workspace <= kKvWorkspace)) break;
