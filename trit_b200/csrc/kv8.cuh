@@ -56,6 +56,29 @@ __device__ __forceinline__ void kv_load8(const void* p, size_t i, int type, bool
     }
   }
 }
+__device__ __forceinline__ void kv_load4(const void* p, size_t i, int type, bool vec, float (&v)[4]) {
+  if (!vec) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = kv_load(p, i + j, type);
+  } else if (type == kKvF32) {
+    const float4 a = *(const float4*)((const float*)p + i);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  } else {
+    const uint2 a = *(const uint2*)((const __half*)p + i);
+    const uint32_t w[2] = {a.x, a.y};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (type == kKvF16) {
+        const float2 f = __half22float2(*(const __half2*)&w[j]);
+        v[2 * j] = f.x;
+        v[2 * j + 1] = f.y;
+      } else {
+        v[2 * j] = __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+      }
+    }
+  }
+}
 __device__ __forceinline__ void kv_store8(void* p, size_t i, int type, bool vec, const float (&v)[8]) {
   if (!vec) {
 #pragma unroll

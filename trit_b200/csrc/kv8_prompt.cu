@@ -128,6 +128,7 @@ template <bool MASK, bool LOW>
 __device__ __forceinline__ void tile_weights(uint32_t s_col, const float (*scales)[4], float factor, float m, int key0,
                                              int limit, float2& sum) {
   uint32_t r[2][32];
+  float2 part[2] = {sum, make_float2(0.0f, 0.0f)};
   tmem_ld<32>(s_col, r[0]);
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
@@ -150,7 +151,7 @@ __device__ __forceinline__ void tile_weights(uint32_t s_col, const float (*scale
         }
         e.x = exp2_fast(e.x);
         e.y = exp2_fast(e.y);
-        sum = fma2(e, i2, sum);
+        part[k & 1] = fma2(e, i2, part[k & 1]);
         const __half2 p = __floats2half2_rn(e.x, e.y);
         out[8 * h + k] = *(const uint32_t*)&p;
         if (LOW) {
@@ -159,9 +160,12 @@ __device__ __forceinline__ void tile_weights(uint32_t s_col, const float (*scale
         }
       }
     }
+    // The sums are due here: put off, they would keep every weight alive.
+    asm volatile("" : "+f"(part[0].x), "+f"(part[0].y), "+f"(part[1].x), "+f"(part[1].y));
     if (LOW) tmem_st32(s_col + 32 * b, out);
     else tmem_st16(s_col + 16 * b, out);
   }
+  sum = make_float2(part[0].x + part[1].x, part[0].y + part[1].y);
 }
 
 template <int HD, bool LOW, int QT>
@@ -272,29 +276,30 @@ __global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape
         vc[i] = page < 0 ? none : __ldg((const uint4*)(codes_v + (size_t)(uint32_t)page * page_bytes + at));
       }
     };
-    int pg = nt > 0 ? pages_of(t0) : -1;
-    if (nt > 0) load_keys(t0, pg);
-    for (int j = 0; j < nt; ++j) {
-      const int step = t0 + j;
-      const int pg_next = j + 1 < nt ? pages_of(step + 1) : -1;
-      load_values(step, pg);
-      // Scales of the step's groups.
-      float ks = 0.0f, vl = 0.0f, vi = 0.0f;
+    // Lanes 0-7 of warp 0: the scales of a step's groups.
+    auto scales_of = [&](int step, int pg) {
+      float4 sc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (threadIdx.x < 8) {
         if (pg >= 0) {
-          const float* sc = kv.scales + (size_t)(uint32_t)pg * page_blocks + head_block;
-          const float vs = sc[kv.kv_heads];
-          ks = sc[0];
-          vl = vs > 0.0f ? __log2f(vs) : kZeroScaleLog2;
-          vi = vs > 0.0f ? __fdividef(1.0f, vs) : 2147483648.0f;
+          const float* x = kv.scales + (size_t)(uint32_t)pg * page_blocks + head_block;
+          sc.x = x[0];
+          sc.z = x[kv.kv_heads];
         } else if (step * kTile + 16 * (int)threadIdx.x < kend) {
-          ks = vi = 1.0f;
+          sc = make_float4(1.0f, 0.0f, 1.0f, 0.0f);  // f16
         }
       }
-      // Positions of the step in the open page: [full, kend).
-      const bool tail = (step + 1) * kTile > full && full < kend;
-      if (!mbar_wait(&S->kempty[j % KS], (j / KS & 1) ^ 1, abort)) break;
-      if (threadIdx.x < 8) *(float4*)S->scales[j & 3][threadIdx.x] = make_float4(ks, vl, vi, 0.0f);
+      return sc;
+    };
+    auto put_keys = [&](int j, float4 sc) -> bool {
+      const int step = t0 + j;
+      const bool tail = (step + 1) * kTile > full && full < kend;  // some of it in the open page
+      if (!mbar_wait(&S->kempty[j % KS], (j / KS & 1) ^ 1, abort)) return false;
+      if (threadIdx.x < 8) {
+        const float vs = sc.z;
+        sc.y = vs > 0.0f ? __log2f(vs) : kZeroScaleLog2;
+        sc.z = vs > 0.0f ? __fdividef(1.0f, vs) : 2147483648.0f;
+        *(float4*)S->scales[j & 3][threadIdx.x] = sc;
+      }
       uint8_t* kt = k_s + j % KS * TILE;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -311,9 +316,12 @@ __global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape
       }
       fence_async_smem();
       mbar_arrive(&S->kfull[j % KS]);
-      pg = pg_next;
-      if (j + 1 < nt) load_keys(step + 1, pg);
-      if (!mbar_wait(&S->vempty[j % VS], (j / VS & 1) ^ 1, abort)) break;
+      return true;
+    };
+    auto put_values = [&](int j) -> bool {
+      const int step = t0 + j;
+      const bool tail = (step + 1) * kTile > full && full < kend;
+      if (!mbar_wait(&S->vempty[j % VS], (j / VS & 1) ^ 1, abort)) return false;
       uint8_t* vt = v_s + j % VS * TILE;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -334,6 +342,26 @@ __global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape
       }
       fence_async_smem();
       mbar_arrive(&S->vfull[j % VS]);
+      return true;
+    };
+    // Keys run a step ahead of values where they have two buffers: the next
+    // step's scores come before this step's values are given back.
+    constexpr int LEAD = KS - 1;
+    int pgk = nt > 0 ? pages_of(t0) : -1, pgv = pgk;
+    float4 sc = scales_of(t0, pgk);
+    if (nt > 0) load_keys(t0, pgk);
+    for (int i = 0; i < nt + LEAD; ++i) {
+      const int jv = i - LEAD;  // values of step jv after keys of step i
+      const int pgk_next = i + 1 < nt ? pages_of(t0 + i + 1) : -1;
+      if (jv >= 0) load_values(t0 + jv, pgv);
+      if (i < nt && !put_keys(i, sc)) break;
+      pgv = LEAD ? pgk : pgk_next;
+      pgk = pgk_next;
+      if (i + 1 < nt) {
+        load_keys(t0 + i + 1, pgk);
+        sc = scales_of(t0 + i + 1, pgk);
+      }
+      if (jv >= 0 && !put_values(jv)) break;
     }
   } else if (warp == MMA_WARP) {
     if (lane == 0 && nt > 0) {
@@ -403,41 +431,48 @@ __global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape
     int low_limit = live ? limit : 0x7fffffff;  // of the warp's rows: below it no mask is needed
 #pragma unroll
     for (int o = 16; o; o >>= 1) low_limit = min(low_limit, __shfl_xor_sync(0xffffffffu, low_limit, o));
-    // The row, scaled into [1, 2) (its sign taken from the scale, so that the
-    // largest product is the largest score), as f16 value and remainder.
-    float factor;
+    // The warp's 32 rows, each scaled into [1, 2) (its sign taken from the
+    // scale, so that the largest product is the largest score), as f16 value
+    // and remainder. Lanes share rows, so that loads are whole lines.
+    float factor = 0.0f;
     {
-      const size_t at = live ? (size_t)(run.row0 + c / g) * a.q_stride + (size_t)(head * g + c % g) * HD : 0;
-      float top = 0.0f, v[8];
-#pragma unroll 4
-      for (int i = 0; i < HD / 8 && live; ++i) {
-        kv_load8(a.q, at + 8 * i, a.type, vec, v);
+      constexpr int RL = HD / 4, RW = 32 / RL;  // lanes a row, rows a turn
+      const int lr = lane / RL, d = lane % RL * 4;
+#pragma unroll 1
+      for (int i0 = 0; i0 < 32; i0 += 8 * RW) {
+        float v[8][4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[k]));
-      }
-      int e = 0;
-      if (top > 0.0f && top <= 3.4e38f) e = max(-126, min(126, (int)((__float_as_uint(top) >> 23) & 255) - 127));
-      float down = __uint_as_float((uint32_t)(127 - e) << 23);
-      if (a.scale < 0.0f) down = -down;
-      factor = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + e) << 23);
-#pragma unroll 4
-      for (int i = 0; i < HD / 8; ++i) {
-        if (live) {
-          kv_load8(a.q, at + 8 * i, a.type, vec, v);
-        } else {
+        for (int i = 0; i < 8; ++i) {
+          const int cc = c - lane + i0 + i * RW + lr;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+          for (int k = 0; k < 4; ++k) v[i][k] = 0.0f;
+          if (cc < cols)
+            kv_load4(a.q, (size_t)(run.row0 + cc / g) * a.q_stride + (size_t)(head * g + cc % g) * HD + d, a.type, vec, v[i]);
         }
-        uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float x = v[2 * k] * down, y = v[2 * k + 1] * down;
-          const __half2 h = __floats2half2_rn(x, y);
-          hi[k] = *(const uint32_t*)&h;
-          lo[k] = pack_f16(x - __low2float(h), y - __high2float(h));
+        for (int i = 0; i < 8; ++i) {
+          float top = fmaxf(fmaxf(fabsf(v[i][0]), fabsf(v[i][1])), fmaxf(fabsf(v[i][2]), fabsf(v[i][3])));
+#pragma unroll
+          for (int o = RL / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          int e = 0;
+          if (top > 0.0f && top <= 3.4e38f) e = max(-126, min(126, (int)((__float_as_uint(top) >> 23) & 255) - 127));
+          float down = __uint_as_float((uint32_t)(127 - e) << 23);
+          if (a.scale < 0.0f) down = -down;
+          const float f = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+          for (int z = 0; z < RW; ++z) {
+            const float fz = __shfl_sync(0xffffffffu, f, z * RL);
+            if (lane == i0 + i * RW + z) factor = fz;
+          }
+          const int r = (warp & 3) * 32 + i0 + i * RW + lr;
+          const __half2 h0 = __floats2half2_rn(v[i][0] * down, v[i][1] * down);
+          const __half2 h1 = __floats2half2_rn(v[i][2] * down, v[i][3] * down);
+          uint8_t* to = q_s + t * QB + tile_at(r, d >> 3) + (d & 4) * 2;
+          *(uint2*)to = make_uint2(*(const uint32_t*)&h0, *(const uint32_t*)&h1);
+          if (LOW)
+            *(uint2*)(to + TILE) = make_uint2(pack_f16(v[i][0] * down - __low2float(h0), v[i][1] * down - __high2float(h0)),
+                                              pack_f16(v[i][2] * down - __low2float(h1), v[i][3] * down - __high2float(h1)));
         }
-        *(uint4*)(q_s + t * QB + tile_at(q, i)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if (LOW) *(uint4*)(q_s + t * QB + TILE + tile_at(q, i)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
     }
     fence_async_smem();
