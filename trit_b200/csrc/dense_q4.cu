@@ -6,11 +6,11 @@
 //
 // The group sums run on mma m16n8k16 (M 16 matrix rows, N 8 columns): a code
 // becomes an exact f16 with one bitwise operation and one subtraction (or
-// fused multiply-add) for two codes, and a row of x is two f16 columns, the
-// value scaled by a power of two (the row's largest in [1, 2)) and its
-// remainder, 22 bits in all; rows rounded to 8 bits first (codes times an f16
-// scale, 18 bits) are exact in that form. Group sums and the sum over groups
-// are f32.
+// fused multiply-add) for two codes, and a row of x is two f16 columns: each
+// group of 32 values scaled by a power of two (its largest in [1, 2)) and the
+// remainders, 22 bits in all. A row rounded to 8 bits first is its codes,
+// exact in one column. The group's factor (the power of two, or the codes'
+// scale) joins d where the group sums, exact or in f32, are added in f32.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -60,21 +60,19 @@ __device__ __forceinline__ uint4 q4_load(const uint4* p) {
 }
 
 // One pass: up to 4 * NT rows of x. A block stages the rows' operand in
-// shared memory ([group][n-tile][lane] 16 bytes: both steps of 16), then
-// takes tiles of 16 matrix rows, whose chunks of 128 values its warps share;
-// their sums meet in shared memory.
+// shared memory ([group][n-tile][lane] 16 bytes: both steps of 16) while its
+// first weights are on the way, then takes tiles of 16 matrix rows, whose
+// chunks of 128 values its warps share; their sums meet in shared memory.
 template <int NT>
 __global__ void __launch_bounds__(kQ4Threads) k_q4(const __grid_constant__ DQ4 W, const float* x, int m, int quantize,
-                                                   int k0, int k1, float* y, int add) {
+                                                   int k0, int k1, int vec, float* y, int add) {
   extern __shared__ __align__(16) uint8_t q4_smem[];
-  uint4* xf = (uint4*)q4_smem;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, j = lane & 3;
   const int row0 = blockIdx.y * 4 * NT, rows = min(4 * NT, m - row0);
   const int c0 = k0 / kQ4Chunk, c1 = (k1 + kQ4Chunk - 1) / kQ4Chunk, nc = c1 - c0;  // this segment's chunks
-  const int groups = nc * 4;
+  uint4* xf = (uint4*)q4_smem;
+  float* factors = (float*)(xf + (size_t)nc * 4 * NT * 32);  // [group][4 * NT]
   __shared__ float s_sum[2][kQ4Warps][NT][64];
-  __shared__ float s_top[4 * NT][kQ4Warps];
-  __shared__ float s_up[4 * NT];
 
   // This warp's chunks: chunk (i % per) * warps + warp of tile i / per.
   const int tiles = (W.n + 15) / 16, mine = tiles > (int)blockIdx.x ? (tiles - 1 - blockIdx.x) / gridDim.x + 1 : 0;
@@ -100,52 +98,77 @@ __global__ void __launch_bounds__(kQ4Threads) k_q4(const __grid_constant__ DQ4 W
   for (int i = 0; i < kQ4Ahead; ++i)
     if (i < total) fetch(i);
 
-  // The rows' largest value gives their power of two.
-  for (int q = 0; q < rows; ++q) {
-    const float* src = x + (size_t)(row0 + q) * W.k;
-    float top = 0.0f;
-    for (int i = k0 + threadIdx.x; i < k1; i += kQ4Threads) top = fmaxf(top, fabsf(src[i]));
-    top = warp_max(top);
-    if (lane == 0) s_top[q][warp] = top;
-  }
-  __syncthreads();
-  if (threadIdx.x < 4 * NT) {
-    float top = 0.0f;
-    if ((int)threadIdx.x < rows)
-      for (int i = 0; i < kQ4Warps; ++i) top = fmaxf(top, s_top[threadIdx.x][i]);
-    int e = 0;
-    if (top > 0.0f && top <= 3.4e38f) e = max(-126, min(126, (int)((__float_as_uint(top) >> 23) & 255) - 127));
-    s_up[threadIdx.x] = __uint_as_float((uint32_t)(127 + e) << 23);
-  }
-  __syncthreads();
-  // A warp makes one row's operand of one group a turn: lane i takes value
-  // i of the group.
-  for (int u = warp; u < groups * 4 * NT; u += kQ4Warps) {
-    const int b = u / (4 * NT), q = u % (4 * NT), at = c0 * kQ4Chunk + b * 32 + lane;
-    float v = q < rows && at < k1 ? x[(size_t)(row0 + q) * W.k + at] : 0.0f;
-    if (quantize) {
-      const float scale = group_scale(warp_max(fabsf(v)));
-      v = (float)quantize_value(v, __fdiv_rn(1.0f, scale)) * round_f16(scale);
+  // The rows' operand: a thread takes 8 values of a group, four threads the
+  // group. Value i = 16 step + 4 jj + z of a group is half z / 2 of word
+  // (step, z % 2) of lanes (columns 2 (q % 4) and 2 (q % 4) + 1, jj).
+  const int units = nc * 16;  // of 8 values, a row
+  for (int u0 = 0; u0 < 4 * NT * units; u0 += kQ4Threads) {
+    const int u = u0 + threadIdx.x;  // row-major; units is a multiple of 16, so a group's threads stay together
+    const int q = u / units, at = u % units, b = at >> 2, first = k0 + at * 8;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    if (q < rows && first < k1) {  // k1 is k or whole chunks: whole groups of 32
+      const float* src = x + (size_t)(row0 + q) * W.k + first;
+      if (vec) {
+        const float4 a = *(const float4*)src, c = *(const float4*)(src + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = c.x; v[5] = c.y; v[6] = c.z; v[7] = c.w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = src[i];
+      }
     }
-    v = __fdiv_rn(v, s_up[q]);  // by a power of two
-    const __half hi = __float2half_rn(v), lo = __float2half_rn(v - __half2float(hi));
-    // Value i = 16 step + 4 j + z is half z / 2 of word (step, z % 2) of lane
-    // (column, j); columns 2 (q % 4) and 2 (q % 4) + 1.
-    const int step = lane >> 4, jj = (lane >> 2) & 3, z = lane & 3;
-    __half* to = (__half*)(xf + ((size_t)b * NT + q / 4) * 32 + (2 * (q & 3)) * 4 + jj) + (2 * step + (z & 1)) * 2 + (z >> 1);
-    to[0] = hi;
-    to[4 * 8] = lo;
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    if (q >= 4 * NT) continue;
+    float factor;
+    __half hi[8], lo[8];
+    if (quantize) {
+      const float scale = group_scale(top), inv = __fdiv_rn(1.0f, scale);
+      factor = round_f16(scale);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        // A value that is no number stays none.
+        const float c = v[i] * inv;
+        hi[i] = __float2half_rn(c == c ? (float)quantize_value(v[i], inv) : c);
+        lo[i] = __ushort_as_half(0);
+      }
+    } else {
+      int e = 0;
+      if (top > 0.0f && top <= 3.4e38f) e = max(-126, min(126, (int)((__float_as_uint(top) >> 23) & 255) - 127));
+      factor = __uint_as_float((uint32_t)(127 + e) << 23);
+      const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float a = v[i] * down;
+        hi[i] = __float2half_rn(a);
+        lo[i] = __float2half_rn(a - __half2float(hi[i]));
+      }
+    }
+    if ((at & 3) == 0) factors[b * 4 * NT + q] = factor;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      // Values 4 jj .. 4 jj + 3 of step `step`.
+      const int t = (at & 3) * 2 + h, step = t >> 2, jj = t & 3;
+      uint32_t* to = (uint32_t*)(xf + ((size_t)b * NT + (q >> 2)) * 32 + (2 * (q & 3)) * 4 + jj) + 2 * step;
+      const __half2 a0 = __halves2half2(hi[4 * h], hi[4 * h + 2]), a1 = __halves2half2(hi[4 * h + 1], hi[4 * h + 3]);
+      const __half2 b0 = __halves2half2(lo[4 * h], lo[4 * h + 2]), b1 = __halves2half2(lo[4 * h + 1], lo[4 * h + 3]);
+      *(uint2*)to = make_uint2(*(const uint32_t*)&a0, *(const uint32_t*)&a1);
+      *(uint2*)(to + 4 * 4) = make_uint2(*(const uint32_t*)&b0, *(const uint32_t*)&b1);
+    }
   }
   __syncthreads();
 
   int i = 0;
   for (int t = 0; t < mine; ++t) {
     const int tile = blockIdx.x + t * gridDim.x;
-    float acc[NT][4];
+    float acc[NT][2];
 #pragma unroll
-    for (int a = 0; a < NT; ++a)
-#pragma unroll
-      for (int z = 0; z < 4; ++z) acc[a][z] = 0.0f;
+    for (int a = 0; a < NT; ++a) acc[a][0] = acc[a][1] = 0.0f;
     for (int c = 0; c < per; ++c, ++i) {
       const uint4 wa = w[0][0], wb = w[0][1];
       const uint2 sa = sc[0][0], sb = sc[0][1];
@@ -161,7 +184,8 @@ __global__ void __launch_bounds__(kQ4Threads) k_q4(const __grid_constant__ DQ4 W
       const float2 s0 = __half22float2(*(const __half2*)&sa.x), s1 = __half22float2(*(const __half2*)&sa.y);
       const float2 s2 = __half22float2(*(const __half2*)&sb.x), s3 = __half22float2(*(const __half2*)&sb.y);
       const float fa[4] = {s0.x, s0.y, s1.x, s1.y}, fb[4] = {s2.x, s2.y, s3.x, s3.y};
-      const uint4* xg = xf + (size_t)(warp + c * kQ4Warps) * 4 * NT * 32 + lane;
+      const int group = (warp + c * kQ4Warps) * 4;
+      const uint4* xg = xf + (size_t)group * NT * 32 + lane;
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const uint32_t ha = ra[b] >> 8, hb = rb[b] >> 8;
@@ -170,22 +194,21 @@ __global__ void __launch_bounds__(kQ4Threads) k_q4(const __grid_constant__ DQ4 W
 #pragma unroll
         for (int a = 0; a < NT; ++a) {
           const uint4 f = xg[(b * NT + a) * 32];
+          const float factor = factors[(group + b) * 4 * NT + 4 * a + j];
           float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
           q4_mma(d, a00, a01, a02, a03, f.x, f.y);
           q4_mma(d, a10, a11, a12, a13, f.z, f.w);
-          acc[a][0] = fmaf(fa[b], d[0], acc[a][0]);
-          acc[a][1] = fmaf(fa[b], d[1], acc[a][1]);
-          acc[a][2] = fmaf(fb[b], d[2], acc[a][2]);
-          acc[a][3] = fmaf(fb[b], d[3], acc[a][3]);
+          // Columns 2 j and 2 j + 1 are one row's values and remainders.
+          acc[a][0] = fmaf(fa[b] * factor, d[0] + d[1], acc[a][0]);
+          acc[a][1] = fmaf(fb[b] * factor, d[2] + d[3], acc[a][1]);
         }
       }
     }
-    // Columns 2 j and 2 j + 1 are one row's value and remainder.
     float (*sum)[NT][64] = s_sum[t & 1];
 #pragma unroll
     for (int a = 0; a < NT; ++a) {
-      sum[warp][a][r * 4 + j] = acc[a][0] + acc[a][1];
-      sum[warp][a][(r + 8) * 4 + j] = acc[a][2] + acc[a][3];
+      sum[warp][a][r * 4 + j] = acc[a][0];
+      sum[warp][a][(r + 8) * 4 + j] = acc[a][1];
     }
     __syncthreads();
     for (int o = threadIdx.x; o < NT * 64; o += kQ4Threads) {
@@ -195,7 +218,6 @@ __global__ void __launch_bounds__(kQ4Threads) k_q4(const __grid_constant__ DQ4 W
       for (int z = 0; z < kQ4Warps; ++z) v += sum[z][a][o % 64];
       if (q < rows && at < W.n) {
         float* out = y + (size_t)(row0 + q) * W.n + at;
-        v *= s_up[q];
         *out = add ? *out + v : v;
       }
     }
@@ -261,22 +283,27 @@ cudaError_t pass(const DQ4& W, const float* x, int m, bool quantize, float* y, c
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   static DeviceOnce once;
+  static int by_registers = 1;  // blocks an SM (every device is the same GPU)
   e = once.run(dev, [] {
-    return cudaFuncSetAttribute(k_q4<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+    cudaFuncAttributes attr{};
+    cudaError_t r = cudaFuncGetAttributes(&attr, k_q4<NT>);
+    if (r != cudaSuccess) return r;
+    by_registers = std::max(1, 65536 / (attr.numRegs * kQ4Threads));
+    return cudaFuncSetAttribute(k_q4<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 190 * 1024);
   });
   if (e != cudaSuccess) return e;
   const int segment = kQ4Segment / NT, tiles = (W.n + 15) / 16, passes = (m + 4 * NT - 1) / (4 * NT);
+  const int vec = ((uintptr_t)x & 15) == 0;  // rows are multiples of 32 values
   for (int p0 = 0; p0 < passes; p0 += 65535) {
     const int np = std::min(passes - p0, 65535);
     for (int k0 = 0; k0 < W.k; k0 += segment) {
       const int k1 = std::min(W.k, k0 + segment);
-      const size_t smem = (size_t)((k1 - k0 + kQ4Chunk - 1) / kQ4Chunk) * 4 * NT * 512;
-      int per_sm = 0;
-      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k_q4<NT>, kQ4Threads, smem);
-      if (e != cudaSuccess) return e;
-      const int grid = std::min(tiles, std::max(1, per_sm) * current_sm_count());
+      const size_t smem = (size_t)((k1 - k0 + kQ4Chunk - 1) / kQ4Chunk) * 4 * NT * (512 + 16);
+      const size_t fixed = sizeof(float) * 2 * kQ4Warps * NT * 64 + 1024;
+      const int per_sm = std::max<int>(1, (int)std::min<size_t>(by_registers, 227 * 1024 / (smem + fixed)));
+      const int grid = std::min(tiles, per_sm * current_sm_count());
       k_q4<NT><<<dim3(grid, np), kQ4Threads, smem, s>>>(W, x + (size_t)p0 * 4 * NT * W.k, m - p0 * 4 * NT, quantize ? 1 : 0,
-                                                       k0, k1, y + (size_t)p0 * 4 * NT * W.n, k0 > 0 ? 1 : 0);
+                                                       k0, k1, vec, y + (size_t)p0 * 4 * NT * W.n, k0 > 0 ? 1 : 0);
       e = cudaGetLastError();
       if (e != cudaSuccess) return e;
     }
