@@ -10,7 +10,10 @@
 // group of 32 values scaled by a power of two (its largest in [1, 2)) and the
 // remainders, 22 bits in all. A row rounded to 8 bits first is its codes,
 // exact in one column. The group's factor (the power of two, or the codes'
-// scale) joins d where the group sums, exact or in f32, are added in f32.
+// scale) joins d where the group sums are added in f32. (Codes as subnormals
+// as they lie in the word, the 8 taken off the sum, save the subtractions but
+// lose seven bits: the tensor cores align products by the operands'
+// exponents.) Limited by instructions, about 140 a warp for 2048 weights.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -24,13 +27,23 @@ namespace {
 
 constexpr int kQ4Warps = 8;
 constexpr int kQ4Threads = kQ4Warps * 32;
-constexpr int kQ4Ahead = 3;  // chunks a warp has in flight
 constexpr int kQ4Chunk = 128;
+// A warp's ring of chunks (16 rows x 128 values: 1 KB of codes, 128 bytes of
+// scales), all but one of them on the way.
+constexpr int kQ4Stages = 8, kQ4Stage = 1024 + 128;
+constexpr int kQ4Ring = kQ4Warps * kQ4Stages * kQ4Stage;
 
+// D = A B and D += A B.
+__device__ __forceinline__ void q4_mma0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ void q4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -51,52 +64,54 @@ __device__ __forceinline__ uint32_t q4_high(uint32_t w) {
   const __half2 h = __hfma2(*(const __half2*)&x, a, b);
   return *(const uint32_t*)&h;
 }
-__device__ __forceinline__ uint4 q4_load(const uint4* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
 
 // One pass: up to 4 * NT rows of x. A block stages the rows' operand in
 // shared memory ([group][n-tile][lane] 16 bytes: both steps of 16) while its
-// first weights are on the way, then takes tiles of 16 matrix rows, whose
-// chunks of 128 values its warps share; their sums meet in shared memory.
+// first weights are on the way. `split` warps share a tile of 16 matrix rows,
+// each taking every split-th chunk of 128 values; their sums meet in shared
+// memory. Weights come by asynchronous copies into each warp's own ring.
 template <int NT>
-__global__ void __launch_bounds__(kQ4Threads) k_q4(const __grid_constant__ DQ4 W, const float* x, int m, int quantize,
-                                                   int k0, int k1, int vec, float* y, int add) {
+__global__ void __launch_bounds__(kQ4Threads, 2) k_q4(const __grid_constant__ DQ4 W, const float* x, int m, int quantize,
+                                                      int k0, int k1, int vec, int split, float* y, int add) {
   extern __shared__ __align__(16) uint8_t q4_smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, j = lane & 3;
   const int row0 = blockIdx.y * 4 * NT, rows = min(4 * NT, m - row0);
   const int c0 = k0 / kQ4Chunk, c1 = (k1 + kQ4Chunk - 1) / kQ4Chunk, nc = c1 - c0;  // this segment's chunks
-  uint4* xf = (uint4*)q4_smem;
+  uint4* xf = (uint4*)(q4_smem + kQ4Ring);
   float* factors = (float*)(xf + (size_t)nc * 4 * NT * 32);  // [group][4 * NT]
   __shared__ float s_sum[2][kQ4Warps][NT][64];
 
-  // This warp's chunks: chunk (i % per) * warps + warp of tile i / per.
-  const int tiles = (W.n + 15) / 16, mine = tiles > (int)blockIdx.x ? (tiles - 1 - blockIdx.x) / gridDim.x + 1 : 0;
-  const int per = warp < nc ? (nc - 1 - warp) / kQ4Warps + 1 : 0, total = per * mine;
-  const uint4* codes = (const uint4*)W.codes;
-  const uint2* scales = (const uint2*)W.scales;
-  uint4 w[kQ4Ahead][2];
-  uint2 sc[kQ4Ahead][2];
-  int ft = blockIdx.x, fc = warp;  // the next chunk to fetch
-  auto fetch = [&](int slot) {
-    const size_t at = (size_t)ft * W.chunks + c0 + fc;
-    w[slot][0] = q4_load(codes + at * 64 + lane);
-    w[slot][1] = q4_load(codes + at * 64 + 32 + lane);
-    sc[slot][0] = __ldg(scales + at * 16 + r);
-    sc[slot][1] = __ldg(scales + at * 16 + r + 8);
-    fc += kQ4Warps;
-    if (fc >= nc) {
-      fc = warp;
-      ft += gridDim.x;
+  const int part = warp % split, team = warp / split;
+  const int teams = gridDim.x * (kQ4Warps / split), first = blockIdx.x * (kQ4Warps / split) + team;
+  const int tiles = (W.n + 15) / 16, mine = tiles > first ? (tiles - 1 - first) / teams + 1 : 0;
+  const int per = part < nc ? (nc - 1 - part) / split + 1 : 0, total = per * mine;
+  uint8_t* ring = q4_smem + warp * (kQ4Stages * kQ4Stage);
+  const uint32_t ring32 = (uint32_t)__cvta_generic_to_shared(ring);
+  // The next chunk to fetch: its bytes, its place in the ring.
+  const uint8_t* codes = (const uint8_t*)W.codes + ((size_t)first * W.chunks + c0 + part) * 1024 + lane * 16;
+  const uint8_t* scales = (const uint8_t*)W.scales + ((size_t)first * W.chunks + c0 + part) * 128 + lane * 4;
+  const size_t turn = (size_t)teams * W.chunks - (size_t)per * split;  // chunks to the next tile's first
+  int left = total, fc = per, slot_in = 0;
+  auto fetch = [&]() {
+    if (left > 0) {
+      const uint32_t to = ring32 + slot_in;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + lane * 16), "l"(codes) : "memory");
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 512 + lane * 16), "l"(codes + 512) : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 1024 + lane * 4), "l"(scales) : "memory");
+      codes += (size_t)split * 1024;
+      scales += (size_t)split * 128;
+      if (--fc == 0) {
+        fc = per;
+        codes += turn * 1024;
+        scales += turn * 128;
+      }
+      --left;
+      slot_in = slot_in == (kQ4Stages - 1) * kQ4Stage ? 0 : slot_in + kQ4Stage;
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
-  for (int i = 0; i < kQ4Ahead; ++i)
-    if (i < total) fetch(i);
+  for (int i = 0; i < kQ4Stages - 1; ++i) fetch();
 
   // The rows' operand: a thread takes 8 values of a group, four threads the
   // group. Value i = 16 step + 4 jj + z of a group is half z / 2 of word
@@ -104,12 +119,12 @@ __global__ void __launch_bounds__(kQ4Threads) k_q4(const __grid_constant__ DQ4 W
   const int units = nc * 16;  // of 8 values, a row
   for (int u0 = 0; u0 < 4 * NT * units; u0 += kQ4Threads) {
     const int u = u0 + threadIdx.x;  // row-major; units is a multiple of 16, so a group's threads stay together
-    const int q = u / units, at = u % units, b = at >> 2, first = k0 + at * 8;
+    const int q = u / units, at = u % units, b = at >> 2, from = k0 + at * 8;
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-    if (q < rows && first < k1) {  // k1 is k or whole chunks: whole groups of 32
-      const float* src = x + (size_t)(row0 + q) * W.k + first;
+    if (q < rows && from < k1) {  // k1 is k or whole chunks: whole groups of 32
+      const float* src = x + (size_t)(row0 + q) * W.k + from;
       if (vec) {
         const float4 a = *(const float4*)src, c = *(const float4*)(src + 4);
         v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
@@ -124,7 +139,6 @@ __global__ void __launch_bounds__(kQ4Threads) k_q4(const __grid_constant__ DQ4 W
     for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    if (q >= 4 * NT) continue;
     float factor;
     __half hi[8], lo[8];
     if (quantize) {
@@ -149,6 +163,7 @@ __global__ void __launch_bounds__(kQ4Threads) k_q4(const __grid_constant__ DQ4 W
         lo[i] = __float2half_rn(a - __half2float(hi[i]));
       }
     }
+    if (q >= 4 * NT) continue;
     if ((at & 3) == 0) factors[b * 4 * NT + q] = factor;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -163,65 +178,82 @@ __global__ void __launch_bounds__(kQ4Threads) k_q4(const __grid_constant__ DQ4 W
   }
   __syncthreads();
 
-  int i = 0;
+  int slot = 0;
   for (int t = 0; t < mine; ++t) {
-    const int tile = blockIdx.x + t * gridDim.x;
-    float acc[NT][2];
+    const int tile = first + t * teams;
+    // Rows r and r + 8 of the tile, columns 2 j and 2 j + 1 (a row's values
+    // and remainders).
+    float acc[NT][4];
 #pragma unroll
-    for (int a = 0; a < NT; ++a) acc[a][0] = acc[a][1] = 0.0f;
-    for (int c = 0; c < per; ++c, ++i) {
-      const uint4 wa = w[0][0], wb = w[0][1];
-      const uint2 sa = sc[0][0], sb = sc[0][1];
-#pragma unroll
-      for (int z = 0; z + 1 < kQ4Ahead; ++z) {
-        w[z][0] = w[z + 1][0];
-        w[z][1] = w[z + 1][1];
-        sc[z][0] = sc[z + 1][0];
-        sc[z][1] = sc[z + 1][1];
-      }
-      if (i + kQ4Ahead < total) fetch(kQ4Ahead - 1);
+    for (int a = 0; a < NT; ++a) acc[a][0] = acc[a][1] = acc[a][2] = acc[a][3] = 0.0f;
+    const uint4* xg = xf + (size_t)part * 4 * NT * 32 + lane;
+    const float* fg = factors + part * 16 * NT + j;
+    for (int c = 0; c < per; ++c) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kQ4Stages - 2) : "memory");
+      __syncwarp();  // the scales are other lanes' copies; the slot before is free
+      fetch();
+      const uint8_t* in = ring + slot;
+      slot = slot == (kQ4Stages - 1) * kQ4Stage ? 0 : slot + kQ4Stage;
+      const uint4 wa = *(const uint4*)(in + lane * 16), wb = *(const uint4*)(in + 512 + lane * 16);
+      const uint2 sa = *(const uint2*)(in + 1024 + r * 8), sb = *(const uint2*)(in + 1024 + r * 8 + 64);
       const uint32_t ra[4] = {wa.x, wa.y, wa.z, wa.w}, rb[4] = {wb.x, wb.y, wb.z, wb.w};
       const float2 s0 = __half22float2(*(const __half2*)&sa.x), s1 = __half22float2(*(const __half2*)&sa.y);
       const float2 s2 = __half22float2(*(const __half2*)&sb.x), s3 = __half22float2(*(const __half2*)&sb.y);
       const float fa[4] = {s0.x, s0.y, s1.x, s1.y}, fb[4] = {s2.x, s2.y, s3.x, s3.y};
-      const int group = (warp + c * kQ4Warps) * 4;
-      const uint4* xg = xf + (size_t)group * NT * 32 + lane;
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const uint32_t ha = ra[b] >> 8, hb = rb[b] >> 8;
-        const uint32_t a00 = q4_low(ra[b]), a01 = q4_low(rb[b]), a02 = q4_low(ha), a03 = q4_low(hb);
-        const uint32_t a10 = q4_high(ra[b]), a11 = q4_high(rb[b]), a12 = q4_high(ha), a13 = q4_high(hb);
+        const uint32_t a0[4] = {q4_low(ra[b]), q4_low(rb[b]), q4_low(ha), q4_low(hb)};
+        const uint32_t a1[4] = {q4_high(ra[b]), q4_high(rb[b]), q4_high(ha), q4_high(hb)};
 #pragma unroll
         for (int a = 0; a < NT; ++a) {
           const uint4 f = xg[(b * NT + a) * 32];
-          const float factor = factors[(group + b) * 4 * NT + 4 * a + j];
-          float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          q4_mma(d, a00, a01, a02, a03, f.x, f.y);
-          q4_mma(d, a10, a11, a12, a13, f.z, f.w);
-          // Columns 2 j and 2 j + 1 are one row's values and remainders.
-          acc[a][0] = fmaf(fa[b] * factor, d[0] + d[1], acc[a][0]);
-          acc[a][1] = fmaf(fb[b] * factor, d[2] + d[3], acc[a][1]);
+          const float factor = fg[b * 4 * NT + 4 * a];
+          float d[4];
+          q4_mma0(d, a0[0], a0[1], a0[2], a0[3], f.x, f.y);
+          q4_mma(d, a1[0], a1[1], a1[2], a1[3], f.z, f.w);
+          const float da = fa[b] * factor, db = fb[b] * factor;
+          const float2 lo = fma2(make_float2(da, da), make_float2(d[0], d[1]), make_float2(acc[a][0], acc[a][1]));
+          const float2 hi = fma2(make_float2(db, db), make_float2(d[2], d[3]), make_float2(acc[a][2], acc[a][3]));
+          acc[a][0] = lo.x;
+          acc[a][1] = lo.y;
+          acc[a][2] = hi.x;
+          acc[a][3] = hi.y;
         }
       }
+      xg += (size_t)split * 4 * NT * 32;
+      fg += split * 16 * NT;
     }
-    float (*sum)[NT][64] = s_sum[t & 1];
-#pragma unroll
-    for (int a = 0; a < NT; ++a) {
-      sum[warp][a][r * 4 + j] = acc[a][0];
-      sum[warp][a][(r + 8) * 4 + j] = acc[a][1];
-    }
-    __syncthreads();
-    for (int o = threadIdx.x; o < NT * 64; o += kQ4Threads) {
-      const int a = o / 64, row = o % 64 / 4, q = a * 4 + o % 4, at = tile * 16 + row;
-      float v = 0.0f;
-#pragma unroll
-      for (int z = 0; z < kQ4Warps; ++z) v += sum[z][a][o % 64];
+    auto put = [&](int q, int at, float v) {
       if (q < rows && at < W.n) {
         float* out = y + (size_t)(row0 + q) * W.n + at;
         *out = add ? *out + v : v;
       }
+    };
+    if (split == 1) {
+#pragma unroll
+      for (int a = 0; a < NT; ++a) {
+        put(4 * a + j, tile * 16 + r, acc[a][0] + acc[a][1]);
+        put(4 * a + j, tile * 16 + r + 8, acc[a][2] + acc[a][3]);
+      }
+      continue;
+    }
+    float (*sum)[NT][64] = s_sum[t & 1];
+#pragma unroll
+    for (int a = 0; a < NT; ++a) {
+      sum[warp][a][r * 4 + j] = acc[a][0] + acc[a][1];
+      sum[warp][a][(r + 8) * 4 + j] = acc[a][2] + acc[a][3];
+    }
+    // The team's barrier (every warp of it has the same tiles).
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(split * 32) : "memory");
+    for (int o = part * 32 + lane; o < NT * 64; o += split * 32) {
+      const int a = o / 64;
+      float v = 0.0f;
+      for (int z = 0; z < split; ++z) v += sum[team * split + z][a][o % 64];
+      put(a * 4 + o % 4, tile * 16 + o % 64 / 4, v);
     }
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // Q4_0 blocks in file order to the tiles that k_q4 reads: codes
@@ -275,7 +307,9 @@ __global__ void __launch_bounds__(256) k_q4_expand(DQ4 W, int8_t* codes, __half*
   }
 }
 
-constexpr int kQ4Segment = 8192;  // values of k a pass stages (128 KB at 4 rows)
+// Values of k that a launch stages in what its ring and joins leave of shared
+// memory; longer rows take several, which add up in y.
+constexpr int kQ4Segment[5] = {0, 8192, 4096, 0, 2048};  // by NT
 
 template <int NT>
 cudaError_t pass(const DQ4& W, const float* x, int m, bool quantize, float* y, cudaStream_t s) {
@@ -283,27 +317,37 @@ cudaError_t pass(const DQ4& W, const float* x, int m, bool quantize, float* y, c
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   static DeviceOnce once;
-  static int by_registers = 1;  // blocks an SM (every device is the same GPU)
   e = once.run(dev, [] {
-    cudaFuncAttributes attr{};
-    cudaError_t r = cudaFuncGetAttributes(&attr, k_q4<NT>);
-    if (r != cudaSuccess) return r;
-    by_registers = std::max(1, 65536 / (attr.numRegs * kQ4Threads));
-    return cudaFuncSetAttribute(k_q4<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 190 * 1024);
+    return cudaFuncSetAttribute(k_q4<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                227 * 1024 - (int)sizeof(float) * 2 * kQ4Warps * NT * 64);
   });
   if (e != cudaSuccess) return e;
-  const int segment = kQ4Segment / NT, tiles = (W.n + 15) / 16, passes = (m + 4 * NT - 1) / (4 * NT);
+  constexpr int segment = kQ4Segment[NT];
+  const int tiles = (W.n + 15) / 16, passes = (m + 4 * NT - 1) / (4 * NT);
   const int vec = ((uintptr_t)x & 15) == 0;  // rows are multiples of 32 values
   for (int p0 = 0; p0 < passes; p0 += 65535) {
     const int np = std::min(passes - p0, 65535);
     for (int k0 = 0; k0 < W.k; k0 += segment) {
       const int k1 = std::min(W.k, k0 + segment);
-      const size_t smem = (size_t)((k1 - k0 + kQ4Chunk - 1) / kQ4Chunk) * 4 * NT * (512 + 16);
+      const int nc = (k1 - k0 + kQ4Chunk - 1) / kQ4Chunk;
+      const size_t smem = kQ4Ring + (size_t)nc * 4 * NT * (512 + 16);
       const size_t fixed = sizeof(float) * 2 * kQ4Warps * NT * 64 + 1024;
-      const int per_sm = std::max<int>(1, (int)std::min<size_t>(by_registers, 227 * 1024 / (smem + fixed)));
-      const int grid = std::min(tiles, per_sm * current_sm_count());
+      const int blocks = current_sm_count() * (2 * (smem + fixed) <= 227 * 1024 ? 2 : 1);
+      // Warps a tile: the fewest chunks for the busiest warp; of equals the
+      // fewest warps, which saves joins.
+      int split = 1;
+      long best = -1;
+      for (int z = 1; z <= kQ4Warps; z *= 2) {
+        const long teams = (long)blocks * (kQ4Warps / z);
+        const long longest = ((tiles + teams - 1) / teams) * ((nc + z - 1) / z);
+        if (best < 0 || longest < best) {
+          best = longest;
+          split = z;
+        }
+      }
+      const int per_block = kQ4Warps / split, grid = std::min((tiles + per_block - 1) / per_block, blocks);
       k_q4<NT><<<dim3(grid, np), kQ4Threads, smem, s>>>(W, x + (size_t)p0 * 4 * NT * W.k, m - p0 * 4 * NT, quantize ? 1 : 0,
-                                                       k0, k1, vec, y + (size_t)p0 * 4 * NT * W.n, k0 > 0 ? 1 : 0);
+                                                       k0, k1, vec, split, y + (size_t)p0 * 4 * NT * W.n, k0 > 0 ? 1 : 0);
       e = cudaGetLastError();
       if (e != cudaSuccess) return e;
     }
