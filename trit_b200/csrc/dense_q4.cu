@@ -48,17 +48,25 @@ __device__ __forceinline__ void q4_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// (w & mask) | one, one instruction while `one` is in a register (the compiler
+// would make two of two immediates).
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t q4_pick(uint32_t w, uint32_t one) {
+  uint32_t x;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(x) : "r"(w), "n"(MASK), "r"(one));
+  return x;
+}
 // Codes of the low halves of bytes 0 and 2 (shift w right by 8 for bytes 1
-// and 3) as f16 c - 8: 0x6400 | c is 1024 + c.
-__device__ __forceinline__ uint32_t q4_low(uint32_t w) {
-  const uint32_t x = (w & 0x000F000Fu) | 0x64006400u;
+// and 3) as f16 c - 8: 0x6400 | c is 1024 + c. `one`: 0x64006400.
+__device__ __forceinline__ uint32_t q4_low(uint32_t w, uint32_t one) {
+  const uint32_t x = q4_pick<0x000F000Fu>(w, one);
   const __half2 b = __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));
   const __half2 h = __hsub2(*(const __half2*)&x, b);
   return *(const uint32_t*)&h;
 }
 // The high halves: 0x6400 | 16 c is 1024 + 16 c; / 16 - 72 is c - 8, exactly.
-__device__ __forceinline__ uint32_t q4_high(uint32_t w) {
-  const uint32_t x = (w & 0x00F000F0u) | 0x64006400u;
+__device__ __forceinline__ uint32_t q4_high(uint32_t w, uint32_t one) {
+  const uint32_t x = q4_pick<0x00F000F0u>(w, one);
   const __half2 a = __halves2half2(__ushort_as_half(0x2C00), __ushort_as_half(0x2C00));
   const __half2 b = __halves2half2(__ushort_as_half(0xD480), __ushort_as_half(0xD480));
   const __half2 h = __hfma2(*(const __half2*)&x, a, b);
@@ -178,6 +186,8 @@ __global__ void __launch_bounds__(kQ4Threads, 2) k_q4(const __grid_constant__ DQ
   }
   __syncthreads();
 
+  uint32_t one;
+  asm volatile("mov.b32 %0, 0x64006400;" : "=r"(one));
   int slot = 0;
   for (int t = 0; t < mine; ++t) {
     const int tile = first + t * teams;
@@ -203,8 +213,8 @@ __global__ void __launch_bounds__(kQ4Threads, 2) k_q4(const __grid_constant__ DQ
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const uint32_t ha = ra[b] >> 8, hb = rb[b] >> 8;
-        const uint32_t a0[4] = {q4_low(ra[b]), q4_low(rb[b]), q4_low(ha), q4_low(hb)};
-        const uint32_t a1[4] = {q4_high(ra[b]), q4_high(rb[b]), q4_high(ha), q4_high(hb)};
+        const uint32_t a0[4] = {q4_low(ra[b], one), q4_low(rb[b], one), q4_low(ha, one), q4_low(hb, one)};
+        const uint32_t a1[4] = {q4_high(ra[b], one), q4_high(rb[b], one), q4_high(ha, one), q4_high(hb, one)};
 #pragma unroll
         for (int a = 0; a < NT; ++a) {
           const uint4 f = xg[(b * NT + a) * 32];
@@ -213,12 +223,10 @@ __global__ void __launch_bounds__(kQ4Threads, 2) k_q4(const __grid_constant__ DQ
           q4_mma0(d, a0[0], a0[1], a0[2], a0[3], f.x, f.y);
           q4_mma(d, a1[0], a1[1], a1[2], a1[3], f.z, f.w);
           const float da = fa[b] * factor, db = fb[b] * factor;
-          const float2 lo = fma2(make_float2(da, da), make_float2(d[0], d[1]), make_float2(acc[a][0], acc[a][1]));
-          const float2 hi = fma2(make_float2(db, db), make_float2(d[2], d[3]), make_float2(acc[a][2], acc[a][3]));
-          acc[a][0] = lo.x;
-          acc[a][1] = lo.y;
-          acc[a][2] = hi.x;
-          acc[a][3] = hi.y;
+          acc[a][0] = fmaf(da, d[0], acc[a][0]);
+          acc[a][1] = fmaf(da, d[1], acc[a][1]);
+          acc[a][2] = fmaf(db, d[2], acc[a][2]);
+          acc[a][3] = fmaf(db, d[3], acc[a][3]);
         }
       }
       xg += (size_t)split * 4 * NT * 32;
@@ -333,13 +341,13 @@ cudaError_t pass(const DQ4& W, const float* x, int m, bool quantize, float* y, c
       const size_t smem = kQ4Ring + (size_t)nc * 4 * NT * (512 + 16);
       const size_t fixed = sizeof(float) * 2 * kQ4Warps * NT * 64 + 1024;
       const int blocks = current_sm_count() * (2 * (smem + fixed) <= 227 * 1024 ? 2 : 1);
-      // Warps a tile: the fewest chunks for the busiest warp; of equals the
-      // fewest warps, which saves joins.
+      // Warps a tile: the least for the busiest warp, a join counted as two
+      // chunks (151936 x 2048: eight warps a tile 56 us, one 41).
       int split = 1;
       long best = -1;
       for (int z = 1; z <= kQ4Warps; z *= 2) {
         const long teams = (long)blocks * (kQ4Warps / z);
-        const long longest = ((tiles + teams - 1) / teams) * ((nc + z - 1) / z);
+        const long longest = ((tiles + teams - 1) / teams) * ((nc + z - 1) / z + (z > 1 ? 2 : 0));
         if (best < 0 || longest < best) {
           best = longest;
           split = z;
