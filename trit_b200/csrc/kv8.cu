@@ -756,6 +756,22 @@ __global__ void __launch_bounds__(256) k_kv_fork(const __grid_constant__ KvView 
       kv.table[(size_t)child * kv.pages_per_seq + i] = kv.table[(size_t)parent * kv.pages_per_seq + i];
   const int head = blockIdx.x % kv.kv_heads, which = blockIdx.x / kv.kv_heads % 2, layer = blockIdx.x / kv.kv_heads / 2;
   __half* to = kv.open + kv_block(kv, child, layer, which, head) * (size_t)(P * kv.hd);
+  if ((full + 1) * P > run.len) {
+    // The cut lies in the parent's open page: its f16 as they are (of values
+    // whole pairs of positions).
+    const uint4* from = (const uint4*)(kv.open + kv_block(kv, parent, layer, which, head) * (size_t)(P * kv.hd));
+    const int n = (which ? (rest + 1) / 2 * 2 : rest) * kv.hd / 8;
+    for (int i0 = 0; i0 < n; i0 += 1024) {
+      uint4 x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i0 + j * 256 + threadIdx.x < n) x[j] = from[i0 + j * 256 + threadIdx.x];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i0 + j * 256 + threadIdx.x < n) ((uint4*)to)[i0 + j * 256 + threadIdx.x] = x[j];
+    }
+    return;
+  }
   for (int i = threadIdx.x; i < rest * kv.hd; i += 256) {
     const int t = i / kv.hd, d = i % kv.hd;
     to[which ? ((t >> 1) * kv.hd + d) * 2 + (t & 1) : t * kv.hd + d] =
