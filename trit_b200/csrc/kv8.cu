@@ -243,7 +243,7 @@ struct AttendShape {
 template <int HD, bool SPLIT, int NT>
 __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS)
     k_kv_attend(const __grid_constant__ KvView kv, const __grid_constant__ KvRuns runs,
-                const __grid_constant__ KvAttendArgs a, int chunks, int splits, int vec, void* workspace) {
+                const __grid_constant__ KvAttendArgs a, int chunks, int splits, int vec, int vec_out, void* workspace) {
   using Shape = AttendShape<HD, NT>;
   constexpr int CL = NT * (SPLIT ? 4 : 8);   // columns a block
   constexpr int LT = SPLIT ? 1 : 2;          // columns a thread holds in an n-tile
@@ -611,30 +611,36 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS
     }
   __syncthreads();
   const int nsplit = run.splits;
-  // Partial results: [kv head][block][column][HD + 2] behind the counters.
+  // Partial results of a (kv head, block) behind the counters: [column][HD],
+  // then (m, l) of each column.
   float* part = (float*)workspace + kKvCounters + ((size_t)head * gridDim.x + blockIdx.x) * CL * (HD + 2);
-  for (int x = threadIdx.x; x < CL * HD; x += kAttendWarps * 32) {
+  auto put = [&](int c, int d, float sum, float4 v) {
+    const size_t at = (size_t)(run.row0 + c / g) * a.out_stride + (size_t)(head * g + c % g) * HD + d;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float x[4] = {sum == 0.0f ? 0.0f : v.x * inv, sum == 0.0f ? 0.0f : v.y * inv, sum == 0.0f ? 0.0f : v.z * inv,
+                        sum == 0.0f ? 0.0f : v.w * inv};
+    kv_store4(a.out, at, a.type, vec_out, x);
+  };
+  for (int x = 4 * threadIdx.x; x < CL * HD; x += 4 * kAttendWarps * 32) {
     const int lc = x / HD, d = x % HD, c = c0 + lc;
     if (c >= cols) break;
     float top = kMInit;
 #pragma unroll
     for (int w = 0; w < kAttendWarps; ++w) top = fmaxf(top, s_m[w][lc]);
-    float sum = 0.0f, val = 0.0f;
+    float sum = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int w = 0; w < kAttendWarps; ++w) {
-      const float f = exp2f(s_m[w][lc] - top);
+      const float f = exp2_fast(s_m[w][lc] - top);
+      const float4 q = *(const float4*)(s_o + ((size_t)w * CL + lc) * HD + d);
       sum = fmaf(f, s_l[w][lc], sum);
-      val = fmaf(f, s_o[((size_t)w * CL + lc) * HD + d], val);
+      v = make_float4(fmaf(f, q.x, v.x), fmaf(f, q.y, v.y), fmaf(f, q.z, v.z), fmaf(f, q.w, v.w));
     }
     if (nsplit == 1) {
-      const size_t at = (size_t)(run.row0 + c / g) * a.out_stride + (size_t)(head * g + c % g) * HD + d;
-      kv_store(a.out, at, a.type, sum == 0.0f ? 0.0f : val / sum);
+      put(c, d, sum, v);
     } else {
-      part[lc * (HD + 2) + d] = val;
-      if (d == 0) {
-        part[lc * (HD + 2) + HD] = top;
-        part[lc * (HD + 2) + HD + 1] = sum;
-      }
+      *(float4*)(part + x) = v;
+      if (d == 0) *(float2*)(part + CL * HD + 2 * lc) = make_float2(top, sum);
     }
   }
   if (nsplit == 1) return;
@@ -651,21 +657,13 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS
   if (!s_last) return;
   __threadfence();
   const float* first = part - (size_t)split * CL * (HD + 2);
-  for (int x = threadIdx.x; x < CL * HD; x += kAttendWarps * 32) {
+  for (int x = 4 * threadIdx.x; x < CL * HD; x += 4 * kAttendWarps * 32) {
     const int lc = x / HD, d = x % HD, c = c0 + lc;
     if (c >= cols) break;
-    float top = kMInit, sum = 0.0f, val = 0.0f;
-#pragma unroll 4
-    for (int i = 0; i < nsplit; ++i) {
-      const float* q = first + ((size_t)i * CL + lc) * (HD + 2);
-      const float qm = __ldcg(q + HD), ql = __ldcg(q + HD + 1), qv = __ldcg(q + d);
-      const float to = fmaxf(top, qm), fa = exp2f(top - to), fb = exp2f(qm - to);
-      sum = fmaf(sum, fa, ql * fb);
-      val = fmaf(val, fa, qv * fb);
-      top = to;
-    }
-    kv_store(a.out, (size_t)(run.row0 + c / g) * a.out_stride + (size_t)(head * g + c % g) * HD + d, a.type,
-             sum == 0.0f ? 0.0f : val / sum);
+    float sum = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    join_shares(first, (size_t)CL * (HD + 2), x, CL * HD + 2 * lc, nsplit, sum, v);
+    put(c, d, sum, v);
   }
 }
 
@@ -784,8 +782,10 @@ __global__ void k_kv_table(int* table, const __grid_constant__ KvEntries e) {
 }
 
 // ---------------------------------------------------------- page moves ----
-__global__ void __launch_bounds__(256) k_kv_move(const __grid_constant__ KvView kv, const int* moves) {
+__global__ void __launch_bounds__(256) k_kv_move(const __grid_constant__ KvView kv, const int* moves,
+                                                 unsigned long long* remap, unsigned epoch) {
   const int src = moves[2 * blockIdx.y], dst = moves[2 * blockIdx.y + 1];
+  if (remap && blockIdx.x == 0 && threadIdx.x == 0) remap[src] = (unsigned long long)epoch << 32 | (unsigned)dst;
   const size_t blocks = (size_t)kv.layers * 2 * kv.kv_heads, n = blocks * kv.page * kv.hd / 16;
   const uint4* a = (const uint4*)(kv.codes + (size_t)src * n * 16);
   uint4* b = (uint4*)(kv.codes + (size_t)dst * n * 16);
@@ -803,22 +803,18 @@ __global__ void __launch_bounds__(256) k_kv_move(const __grid_constant__ KvView 
     for (size_t i = threadIdx.x; i < blocks; i += 256) kv.scales[dst * blocks + i] = kv.scales[src * blocks + i];
 }
 
-__global__ void k_kv_remap_init(int* remap, int pages) {
-  const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i < pages) remap[i] = i;
-}
-__global__ void k_kv_remap_set(int* remap, const int* moves, int n) {
-  const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i < n) remap[moves[2 * i]] = moves[2 * i + 1];
-}
-__global__ void k_kv_remap(int* table, const int* remap, size_t entries) {
+// Table entries follow the moves: remap[page] holds (epoch, target) for the
+// pages that this compaction moved, and an older epoch for all others.
+__global__ void k_kv_remap(int* table, const unsigned long long* remap, unsigned epoch, size_t entries) {
   const size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x;
-  if (i < entries) table[i] = remap[table[i]];
+  if (i >= entries) return;
+  const unsigned long long to = remap[table[i]];
+  if ((unsigned)(to >> 32) == epoch) table[i] = (int)(unsigned)to;
 }
 
 template <int HD, bool SPLIT, int NT>
-cudaError_t attend(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& p, int vec, void* ws,
-                   cudaStream_t s) {
+cudaError_t attend(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& p, int vec,
+                   int vec_out, void* ws, cudaStream_t s) {
   constexpr int smem = AttendShape<HD, NT>::SMEM;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -829,7 +825,7 @@ cudaError_t attend(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, 
   });
   if (e != cudaSuccess) return e;
   k_kv_attend<HD, SPLIT, NT>
-      <<<dim3(p.blocks, kv.kv_heads), kAttendWarps * 32, smem, s>>>(kv, runs, a, p.chunks, p.splits, vec, ws);
+      <<<dim3(p.blocks, kv.kv_heads), kAttendWarps * 32, smem, s>>>(kv, runs, a, p.chunks, p.splits, vec, vec_out, ws);
   return cudaGetLastError();
 }
 
@@ -857,10 +853,11 @@ cudaError_t launch_kv_append(const KvView& kv, const KvRuns& runs, int layer, co
 // block reads its positions once for all of its columns).
 //
 // Positions are cut into shares of `c` steps a block, for one to four rounds
-// of blocks over the GPU: fewer rounds waste less on starting up, more even
-// out lengths that differ. The cost of a round is its longest share and about
-// four steps of start (measured: a block's first codes arrive after 2 us, a
-// step takes 0.5).
+// of blocks over the GPU: fewer rounds waste less on starting and joining,
+// more even out lengths that differ. A round costs its longest share and what
+// 48 steps do (measured, 32 heads on 8 and 128 wide: 64 streams of 601 to
+// 1279 positions take 54 us in shares of 64 steps, 57 whole, 65 in shares of
+// 20; 6 streams of 40001 to 65535 take 159 us in shares of 400, 186 of 96).
 KvAttendPlan plan_kv_attend(const KvView& kv, KvRuns& runs, const KvAttendArgs& a) {
   KvAttendPlan p;
   const int g = a.heads / kv.kv_heads, unit = a.type == kKvF32 ? 4 : 8;
@@ -888,16 +885,26 @@ KvAttendPlan plan_kv_attend(const KvView& kv, KvRuns& runs, const KvAttendArgs& 
   }
   tiles *= kv.kv_heads;
   work *= kv.kv_heads;
+  auto blocks = [&](int c) {
+    long n = 0;
+    if (runs.row_seq) return (long)tiles * ((longest + c - 1) / c);
+    for (int i = 0; i < runs.n; ++i)
+      n += (long)(((size_t)runs.run[i].count * g + p.cols - 1) / p.cols) * (((runs.run[i].len + 15) / 16 + c - 1) / c);
+    return n * kv.kv_heads;
+  };
+  constexpr double kStart = 48.0;
   int share = longest;
   if (tiles < 4.0 * slots && tiles <= kKvCounters) {
-    double best = (double)((int)((tiles + slots - 1) / slots)) * (longest + 4);
+    double best = (double)((int)((tiles + slots - 1) / slots)) * (longest + kStart);
     for (int rounds = 1; rounds <= 4; ++rounds) {
-      // sum ceil(steps / c) over the tiles is about work / c + tiles / 2.
+      // sum ceil(steps / c) over the tiles is about work / c + tiles / 2; the
+      // count must not pass the rounds, or a last round of a few blocks comes.
       const double room = (double)rounds * slots - 0.5 * tiles;
       if (room <= 0) continue;
-      const int c = std::max(16, (int)(work / room) + 1);
-      if (c < longest && rounds * (c + 4.0) < best) {
-        best = rounds * (c + 4.0);
+      int c = std::max(16, (int)(work / room) + 1);
+      while (c < longest && blocks(c) > (long)rounds * slots) c += std::max(1, c / 32);
+      if (c < longest && rounds * (c + kStart) < best) {
+        best = rounds * (c + kStart);
         share = c;
       }
     }
@@ -931,13 +938,14 @@ cudaError_t launch_kv_attend(const KvView& kv, const KvRuns& runs, const KvAtten
   if (p.joins && !ws) return cudaErrorInvalidValue;
   const size_t size = a.type == kKvF32 ? 4 : 2;
   const int vec = ((uintptr_t)a.q | a.q_stride * size) % 16 == 0;
+  const int vec_out = ((uintptr_t)a.out | a.out_stride * size) % 16 == 0;
   const bool two = p.cols == (a.type == kKvF32 ? 8 : 16);
   if (kv.hd == 128) {
-    if (a.type == kKvF32) return two ? attend<128, true, 2>(kv, runs, a, p, vec, ws, s) : attend<128, true, 1>(kv, runs, a, p, vec, ws, s);
-    return two ? attend<128, false, 2>(kv, runs, a, p, vec, ws, s) : attend<128, false, 1>(kv, runs, a, p, vec, ws, s);
+    if (a.type == kKvF32) return two ? attend<128, true, 2>(kv, runs, a, p, vec, vec_out, ws, s) : attend<128, true, 1>(kv, runs, a, p, vec, vec_out, ws, s);
+    return two ? attend<128, false, 2>(kv, runs, a, p, vec, vec_out, ws, s) : attend<128, false, 1>(kv, runs, a, p, vec, vec_out, ws, s);
   }
-  if (a.type == kKvF32) return two ? attend<64, true, 2>(kv, runs, a, p, vec, ws, s) : attend<64, true, 1>(kv, runs, a, p, vec, ws, s);
-  return two ? attend<64, false, 2>(kv, runs, a, p, vec, ws, s) : attend<64, false, 1>(kv, runs, a, p, vec, ws, s);
+  if (a.type == kKvF32) return two ? attend<64, true, 2>(kv, runs, a, p, vec, vec_out, ws, s) : attend<64, true, 1>(kv, runs, a, p, vec, vec_out, ws, s);
+  return two ? attend<64, false, 2>(kv, runs, a, p, vec, vec_out, ws, s) : attend<64, false, 1>(kv, runs, a, p, vec, vec_out, ws, s);
 }
 
 cudaError_t launch_kv_read(const KvView& kv, const KvRuns& runs, int layer, void* k, void* v, int type, int max_count,
@@ -963,19 +971,19 @@ cudaError_t launch_kv_table(const KvView& kv, const KvEntries& e, cudaStream_t s
   return cudaGetLastError();
 }
 
-cudaError_t launch_kv_move(const KvView& kv, const int* moves, int n, cudaStream_t s) {
+cudaError_t launch_kv_move(const KvView& kv, const int* moves, int n, unsigned long long* remap, unsigned epoch,
+                           cudaStream_t s) {
   const size_t vec = (size_t)kv.layers * 2 * kv.kv_heads * kv.page * kv.hd / 16;
   const int x = (int)std::max<size_t>(1, std::min<size_t>((vec + 2047) / 2048, 64));
-  for (int i = 0; i < n; i += 65535) k_kv_move<<<dim3(x, std::min(n - i, 65535)), 256, 0, s>>>(kv, moves + 2 * i);
+  for (int i = 0; i < n; i += 65535)
+    k_kv_move<<<dim3(x, std::min(n - i, 65535)), 256, 0, s>>>(kv, moves + 2 * i, remap, epoch);
   return cudaGetLastError();
 }
 
-cudaError_t launch_kv_remap(const KvView& kv, const int* moves, int n, int* remap, int pages, int sequences,
+cudaError_t launch_kv_remap(const KvView& kv, const unsigned long long* remap, unsigned epoch, int sequences,
                             cudaStream_t s) {
   const size_t entries = (size_t)sequences * kv.pages_per_seq;
-  k_kv_remap_init<<<(pages + 255) / 256, 256, 0, s>>>(remap, pages);
-  k_kv_remap_set<<<(n + 255) / 256, 256, 0, s>>>(remap, moves, n);
-  k_kv_remap<<<(unsigned)((entries + 255) / 256), 256, 0, s>>>(kv.table, remap, entries);
+  k_kv_remap<<<(unsigned)((entries + 255) / 256), 256, 0, s>>>(kv.table, remap, epoch, entries);
   return cudaGetLastError();
 }
 

@@ -79,6 +79,27 @@ __device__ __forceinline__ void kv_load4(const void* p, size_t i, int type, bool
     }
   }
 }
+__device__ __forceinline__ void kv_store4(void* p, size_t i, int type, bool vec, const float (&v)[4]) {
+  if (!vec) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) kv_store(p, i + j, type, v[j]);
+  } else if (type == kKvF32) {
+    *(float4*)((float*)p + i) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    uint32_t w[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (type == kKvF16) {
+        const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+        w[j] = *(const uint32_t*)&h;
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+        w[j] = *(const uint32_t*)&h;
+      }
+    }
+    *(uint2*)((__half*)p + i) = make_uint2(w[0], w[1]);
+  }
+}
 __device__ __forceinline__ void kv_store8(void* p, size_t i, int type, bool vec, const float (&v)[8]) {
   if (!vec) {
 #pragma unroll
@@ -160,6 +181,32 @@ __device__ __forceinline__ void find_run(const KvRuns& runs, int block, int chun
   const int at = block - run.block0;
   chunk = at / run.splits;
   split = at % run.splits;
+}
+
+// Four values of a column, joined over its shares in their order: share i's
+// values at first + i * step + at, its (m, l) at first + i * step + ml.
+__device__ __forceinline__ void join_shares(const float* first, size_t step, int at, int ml, int shares, float& sum,
+                                            float4& v) {
+  float top = kMInit;
+  for (int i0 = 0; i0 < shares; i0 += 4) {
+    float4 x[4];
+    float2 s[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i0 + j < shares) {
+        x[j] = __ldcg((const float4*)(first + (size_t)(i0 + j) * step + at));
+        s[j] = __ldcg((const float2*)(first + (size_t)(i0 + j) * step + ml));
+      }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i0 + j < shares) {
+        const float to = fmaxf(top, s[j].x), fa = exp2_fast(top - to), fb = exp2_fast(s[j].x - to);
+        sum = fmaf(sum, fa, s[j].y * fb);
+        v = make_float4(fmaf(v.x, fa, x[j].x * fb), fmaf(v.y, fa, x[j].y * fb), fmaf(v.z, fa, x[j].z * fb),
+                        fmaf(v.w, fa, x[j].w * fb));
+        top = to;
+      }
+  }
 }
 
 }  // namespace

@@ -106,10 +106,11 @@ struct KvEntries {
 };
 cudaError_t launch_kv_table(const KvView& kv, const KvEntries& e, cudaStream_t s);
 // Page moves[2i] -> moves[2i + 1] (device pairs; no page is both read and
-// written).
-cudaError_t launch_kv_move(const KvView& kv, const int* moves, int n, cudaStream_t s);
-// Entries of the first pages_used[...] of every table row follow the moves.
-cudaError_t launch_kv_remap(const KvView& kv, const int* moves, int n, int* remap, int pages, int sequences,
+// written); with `remap`, the moved pages' targets are noted there under
+// `epoch`, and launch_kv_remap makes the table's entries follow.
+cudaError_t launch_kv_move(const KvView& kv, const int* moves, int n, unsigned long long* remap, unsigned epoch,
+                           cudaStream_t s);
+cudaError_t launch_kv_remap(const KvView& kv, const unsigned long long* remap, unsigned epoch, int sequences,
                             cudaStream_t s);
 
 struct KvOptions {
@@ -190,7 +191,9 @@ class KvCache {
   MinHeap free_seqs_, free_pages_;
   std::vector<int> refs_;  // sequences that hold each page
   void* workspace_ = nullptr;
-  int *moves_ = nullptr, *remap_ = nullptr, *status_ = nullptr;
+  int *moves_ = nullptr, *status_ = nullptr;
+  unsigned long long* remap_ = nullptr;  // [pages] (epoch, target) of the last compaction that moved it
+  unsigned epoch_ = 0;
   cudaEvent_t order_ = nullptr;
   unsigned long long last_stream_ = 0;
   bool used_ = false, capturing_ = false;

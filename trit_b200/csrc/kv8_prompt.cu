@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape
     if (t < groups && ok) {
       fence_after();
       const float l = l2.x + l2.y, inv = l == 0.0f ? 0.0f : 1.0f / l;
-      float* part = (float*)workspace + kKvCounters + (((size_t)head * gridDim.x + block) * COLS + t * kTile + q) * (HD + 2);
+      float* part = (float*)workspace + kKvCounters + ((size_t)head * gridDim.x + block) * COLS * (HD + 2);
 #pragma unroll
       for (int b = 0; b < HD / 32; ++b) {
         uint32_t r[32];
@@ -544,11 +544,11 @@ __global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape
           }
         } else {
 #pragma unroll
-          for (int k = 0; k < 32; k += 2)
-            *(float2*)(part + 32 * b + k) = make_float2(__uint_as_float(r[k]), __uint_as_float(r[k + 1]));
+          for (int k = 0; k < 32; k += 4)
+            *(uint4*)(part + (t * kTile + q) * HD + 32 * b + k) = make_uint4(r[k], r[k + 1], r[k + 2], r[k + 3]);
         }
       }
-      if (run.splits > 1 && live) *(float2*)(part + HD) = make_float2(m, l);
+      if (run.splits > 1 && live) *(float2*)(part + COLS * HD + 2 * (t * kTile + q)) = make_float2(m, l);
     }
   }
   if (run.splits > 1) __threadfence();
@@ -569,21 +569,16 @@ __global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape
   if (!S->last) return;
   __threadfence();
   const float* first = (const float*)workspace + kKvCounters + ((size_t)head * gridDim.x + block - split) * COLS * (HD + 2);
-  for (int x = threadIdx.x; x < COLS * HD; x += Shape::THREADS) {
+  for (int x = 4 * threadIdx.x; x < COLS * HD; x += 4 * Shape::THREADS) {
     const int lc = x / HD, d = x % HD, c = c0 + lc;
     if (c >= cols) break;
-    float top = kMInit, sum = 0.0f, val = 0.0f;
-#pragma unroll 4
-    for (int i = 0; i < run.splits; ++i) {
-      const float* p = first + ((size_t)i * COLS + lc) * (HD + 2);
-      const float pm = __ldcg(p + HD), pl = __ldcg(p + HD + 1), pv = __ldcg(p + d);
-      const float to = fmaxf(top, pm), fa = exp2_fast(top - to), fb = exp2_fast(pm - to);
-      sum = fmaf(sum, fa, pl * fb);
-      val = fmaf(val, fa, pv * fb);
-      top = to;
-    }
-    kv_store(a.out, (size_t)(run.row0 + c / g) * a.out_stride + (size_t)(head * g + c % g) * HD + d, a.type,
-             sum == 0.0f ? 0.0f : val / sum);
+    float sum = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    join_shares(first, (size_t)COLS * (HD + 2), x, COLS * HD + 2 * lc, run.splits, sum, v);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float y[4] = {sum == 0.0f ? 0.0f : v.x * inv, sum == 0.0f ? 0.0f : v.y * inv, sum == 0.0f ? 0.0f : v.z * inv,
+                        sum == 0.0f ? 0.0f : v.w * inv};
+    kv_store4(a.out, (size_t)(run.row0 + c / g) * a.out_stride + (size_t)(head * g + c % g) * HD + d, a.type, vec_out, y);
   }
 }
 
@@ -615,11 +610,13 @@ cudaError_t prompt(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, 
 
 // Two tiles a block while that leaves no SM idle (the two share the widened
 // codes, and one's products hide the other's softmax); positions are cut into
-// shares only while blocks leave SMs idle. A share costs about a step and a
-// half to start and to join.
+// shares while blocks leave SMs idle. A share costs what 12 steps do to start
+// and to join (measured: 7 streams of 300 to 2111 positions, 33 to 300 rows
+// each, 53 us whole, 70 in shares of 10 steps).
 KvAttendPlan plan_kv_prompt(const KvView& kv, KvRuns& runs, const KvAttendArgs& a) {
   KvAttendPlan p;
-  const int g = a.heads / kv.kv_heads, slots = current_sm_count();
+  const int g = a.heads / kv.kv_heads;
+  int slots = current_sm_count();
   double tiles = 0, work = 0;
   int longest = 1;
   for (int pass = 0; pass < 2; ++pass) {
@@ -636,15 +633,16 @@ KvAttendPlan plan_kv_prompt(const KvView& kv, KvRuns& runs, const KvAttendArgs& 
     work *= kv.kv_heads;
     if (tiles >= slots) break;
   }
+  if (p.cols == kTile && !(a.type == kKvF32 && kv.hd == 128)) slots *= 2;  // two blocks an SM
   int share = longest;
   if (tiles < 2.0 * slots) {
-    double best = (double)((int)((tiles + slots - 1) / slots)) * (longest + 1.5);
+    double best = (double)((int)((tiles + slots - 1) / slots)) * (longest + 12.0);
     for (int rounds = 1; rounds <= 2; ++rounds) {
       const double room = (double)rounds * slots - 0.5 * tiles;
       if (room <= 0) continue;
       const int c = std::max(2, (int)(work / room) + 1);
-      if (c < longest && rounds * (c + 1.5) < best) {
-        best = rounds * (c + 1.5);
+      if (c < longest && rounds * (c + 12.0) < best) {
+        best = rounds * (c + 12.0);
         share = c;
       }
     }

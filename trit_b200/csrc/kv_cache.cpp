@@ -57,7 +57,8 @@ KvCache::KvCache(const KvOptions& o) : opt_(o) {
     TRIT_CUDA(cudaMalloc(&view_.open, open));
     TRIT_CUDA(cudaMalloc(&view_.table, table));
     TRIT_CUDA(cudaMalloc(&moves_, (size_t)o.pages * 8));
-    TRIT_CUDA(cudaMalloc(&remap_, (size_t)o.pages * 4));
+    TRIT_CUDA(cudaMalloc(&remap_, (size_t)o.pages * 8));
+    TRIT_CUDA(cudaMemset(remap_, 0, (size_t)o.pages * 8));
     TRIT_CUDA(cudaMalloc(&workspace_, kKvWorkspace));
     TRIT_CUDA(cudaHostAlloc(&status_, 4, cudaHostAllocDefault));
     *status_ = 0;
@@ -245,7 +246,7 @@ void KvCache::copy(const int* ids, size_t n, int* out, cudaStream_t s) {
   // memory), and no page is both read and written.
   if (pages) {
     TRIT_CUDA(cudaMemcpyAsync(moves_, moves.data(), moves.size() * 4, cudaMemcpyHostToDevice, s));
-    TRIT_CUDA(launch_kv_move(view_, moves_, (int)pages, s));
+    TRIT_CUDA(launch_kv_move(view_, moves_, (int)pages, nullptr, 0, s));
     set_entries(entries, s);
   }
   leave(s);
@@ -486,8 +487,9 @@ int64_t KvCache::compact(cudaStream_t s) {
   enter(s, "compact");
   const int n = (int)(moves.size() / 2);
   TRIT_CUDA(cudaMemcpyAsync(moves_, moves.data(), moves.size() * 4, cudaMemcpyHostToDevice, s));
-  TRIT_CUDA(launch_kv_move(view_, moves_, n, s));
-  TRIT_CUDA(launch_kv_remap(view_, moves_, n, remap_, opt_.pages, opt_.sequences, s));
+  ++epoch_;
+  TRIT_CUDA(launch_kv_move(view_, moves_, n, remap_, epoch_, s));
+  TRIT_CUDA(launch_kv_remap(view_, remap_, epoch_, opt_.sequences, s));
   for (int i = 0; i < n; ++i) {
     refs_[moves[2 * i + 1]] = refs_[moves[2 * i]];
     refs_[moves[2 * i]] = 0;
