@@ -291,16 +291,25 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS
     vinv = vs > 0.0f ? __fdividef(1.0f, vs) : 2147483648.0f;
   };
   if (ncode && fbase + lane <= last_page) pid = table[fbase + lane];
-  uint8_t* mine = smem + (size_t)warp * STAGES * Shape::UNIT + lane * 16;
-  const uint8_t* codes_k = kv.codes + head_scale * bytes + r * HD + 16 * j;
-  const uint8_t* codes_v = kv.codes + (head_scale + kv.kv_heads) * bytes + j * (2 * HD) + 16 * r;
-  // Every lane copies the bytes that it will itself take as operands, so
-  // only its own wait stands between.
+  // A unit of codes is two runs of 16 HD bytes, each copied as it lies, 512
+  // bytes an instruction (whole lines: copies by operand, half lines at a
+  // time, reached 4.3 of 6.5 TB/s). In shared memory 16-byte chunks swap
+  // places within a row so that operands are read without conflicts: chunk c
+  // of key r at c ^ 4 (r % 2) (128 wide), of value pair p at c ^ 2 (p % 4).
+  uint8_t* stages = smem + (size_t)warp * STAGES * Shape::UNIT;
+  const uint8_t* codes_k = kv.codes + head_scale * bytes + lane * 16;
+  const uint8_t* codes_v = codes_k + (size_t)kv.kv_heads * bytes;
+  const int put_k = HD == 128 ? (lane >> 3) * 128 + ((lane & 7) ^ ((lane >> 3 & 1) << 2)) * 16 : lane * 16;
+  const int put_v = HD * 16 + (HD == 128 ? (lane >> 4) * 256 + ((lane & 15) ^ ((lane >> 4) << 1)) * 16
+                                         : (lane >> 3) * 128 + ((lane & 7) ^ ((lane >> 3) << 1)) * 16);
+  const int get_k = HD == 128 ? r * 128 + (j ^ ((r & 1) << 2)) * 16 : r * 64 + j * 16;
+  const int get_v = HD * 16 + j * (2 * HD) + (r ^ (j << 1)) * 16;
+  // Of the open page every lane copies the bytes that it will itself take.
   int slot_in = 0, slot_out = 0, ahead = 0;  // ahead: units fetched
   auto fetch = [&]() {
     const int unit = ahead++;
     if (unit < units) {
-      uint8_t* to = mine + slot_in * Shape::UNIT;
+      uint8_t* to = stages + slot_in * Shape::UNIT;
       slot_in = slot_in == STAGES - 1 ? 0 : slot_in + 1;
       if (unit < ncode) {
         const int step = s0 + unit;
@@ -314,17 +323,16 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS
         const size_t at = (size_t)page * page_bytes + (uint32_t)(step & ((1 << page_steps) - 1)) * (16 * HD);
         const uint8_t *kp = codes_k + at, *vp = codes_v + at;
 #pragma unroll
-        for (int b = 0; b < KB; ++b) {
-          copy16(to + (2 * b) * 512, kp + 64 * b);
-          copy16(to + (2 * b + 1) * 512, kp + 64 * b + 8 * HD);
-          copy16(to + (2 * KB + 2 * b) * 512, vp + 128 * b);
-          copy16(to + (2 * KB + 2 * b + 1) * 512, vp + 128 * b + 4 * 2 * HD);
-        }
+        for (int i = 0; i < HD / 32; ++i) copy16(to + put_k + i * 512, kp + i * 512);
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i)
+          copy16(to + (HD == 128 ? (put_v ^ ((i & 1) << 6)) : put_v) + i * 512, vp + i * 512);
       } else {
         const int tok = (f1 - full + (unit - ncode) / 2) * 16, which = (unit - ncode) & 1;
         const __half* x = kv.open + kv_block(kv, run.seq, a.layer, which, head) * bytes;
         x += which ? (size_t)(tok / 2 + j) * (2 * HD) + 16 * r : (size_t)(tok + r) * HD + 16 * j;
         const int half = which ? 4 * 2 * HD : 8 * HD, wide = which ? 128 : 64;
+        to += lane * 16;
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
           copy16(to + (4 * b) * 512, x + wide * b);
@@ -337,7 +345,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   auto next = [&]() {  // the unit that is consumed next
-    const uint4* in = (const uint4*)(mine + slot_out * Shape::UNIT);
+    const uint8_t* in = stages + slot_out * Shape::UNIT;
     slot_out = slot_out == STAGES - 1 ? 0 : slot_out + 1;
     return in;
   };
@@ -496,12 +504,14 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS
   int unit = 0;
   for (; unit < ncode; unit += 2) {
     const bool two = unit + 1 < ncode;
+    __syncwarp();  // the units before are read
     fetch();
     fetch();
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    __syncwarp();
     float ks[2], lv[2], iv[2];
     int key0[2];
-    const uint4* in[2];
+    const uint8_t* in[2];
 #pragma unroll
     for (int z = 0; z < 2; ++z) {
       const int step = s0 + unit + z;
@@ -528,7 +538,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS
     for (int b = 0; b < KB; ++b)
 #pragma unroll
       for (int z = 0; z < 2; ++z) {
-        const uint4 k0 = in[z][(2 * b) * 32], k1 = in[z][(2 * b + 1) * 32];
+        const uint8_t* at = in[z] + (get_k ^ (b << 6));
+        const uint4 k0 = *(const uint4*)at, k1 = *(const uint4*)(at + 8 * HD);
         const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -542,7 +553,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS
     for (int z = 0; z < 2; ++z)
 #pragma unroll
       for (int b = 0; b < KB; ++b) {
-        const uint4 v0 = in[z][(2 * KB + 2 * b) * 32], v1 = in[z][(2 * KB + 2 * b + 1) * 32];
+        const uint8_t* at = in[z] + get_v + b * 128;
+        const uint4 v0 = *(const uint4*)at, v1 = *(const uint4*)(at + 8 * HD);
         const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -556,11 +568,12 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS
   for (unit = ncode; unit < units; ++unit) {
     const bool keys = ((unit - ncode) & 1) == 0;
     if (keys) {
+      __syncwarp();
       while (ahead < min(units, unit + STAGES)) fetch();
       asm volatile("cp.async.wait_all;" ::: "memory");
       clear();
     }
-    const uint4* in = next();
+    const uint4* in = (const uint4*)(next() + lane * 16);
 #pragma unroll
     for (int b = 0; b < KB; ++b)
 #pragma unroll
