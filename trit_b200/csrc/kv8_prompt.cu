@@ -10,9 +10,8 @@
 //               open page's f16 is copied. Codes are loaded half a step ahead
 //               in registers, page numbers a step ahead.
 //   warps 4-    softmax, four warps a tile: a thread owns one query column
-//               (one TMEM lane). Two passes over its scores in TMEM: the
-//               largest, then P, which takes the place of the scores there
-//               and is the second product's first operand.
+//               (one TMEM lane). One pass over its scores in TMEM; P takes
+//               their place and is the second product's first operand.
 //   last warp   owns TMEM and issues the products, for two tiles in turn: while
 //               one tile's run, the other's softmax does.
 //
@@ -93,71 +92,86 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 
-// The largest score of a row of S (128 TMEM columns from s_col), each group
-// of 16 with its scales; positions from `limit` on do not count.
-template <bool MASK>
-__device__ __forceinline__ float tile_top(uint32_t s_col, const float (*scales)[4], float factor, int key0, int limit) {
-  float top = kMInit;
-#pragma unroll
-  for (int b = 0; b < 2; ++b) {
-    uint32_t r[2][32];
-    tmem_ld<32>(s_col + 64 * b, r[0]);
-    tmem_ld<32>(s_col + 64 * b + 32, r[1]);
-    tmem_wait_ld();
-#pragma unroll
-    for (int h = 0; h < 4; ++h) {
-      const uint32_t* x = r[h >> 1] + 16 * (h & 1);
-      const float2 sc = *(const float2*)scales[4 * b + h];
-      float y[4];
-#pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        float v = __uint_as_float(x[k]);
-        if (MASK && key0 + 64 * b + 16 * h + k >= limit) v = -INFINITY;
-        y[k & 3] = k < 4 ? v : fmaxf(y[k & 3], v);
-      }
-      const float v = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
-      top = fmaxf(top, MASK && v == -INFINITY ? v : fmaf(v, factor * sc.x, sc.y));
-    }
-  }
-  return top;
-}
-
-// S to P in its place: 2^(t - m) as f16 (and its remainder: 16 columns of
-// each in turn), and their sums over the value scales.
-template <bool MASK, bool LOW>
-__device__ __forceinline__ void tile_weights(uint32_t s_col, const float (*scales)[4], float factor, float m, int key0,
-                                             int limit, float2& sum) {
-  uint32_t r[2][32];
+// A row's scores (128 TMEM columns from s_col) to P in their place, 32 at a
+// time: t = log2 of a weight over the value scale, P = 2^(t - m) as f16 (and
+// its remainder: 16 columns of each in turn), `sum` of P over the value
+// scales. When a t passes m by kRaise (a vote of the warp: its rows share the
+// branch) m becomes a whole number near the largest, so that what is scaled by
+// the difference, the sum, O and this row's earlier P, keeps its bits.
+// Positions from `limit` on get no weight.
+template <int HD, bool MASK, bool LOW>
+__device__ __forceinline__ void tile_weights(uint32_t s_col, uint32_t o_col, bool scale_o, const float (*scales)[4],
+                                             float factor, int key0, int limit, float& m, float2& sum) {
   float2 part[2] = {sum, make_float2(0.0f, 0.0f)};
-  tmem_ld<32>(s_col, r[0]);
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
+    uint32_t r[32];
+    tmem_ld<32>(s_col + 32 * b, r);
     tmem_wait_ld();
-    if (b < 3) tmem_ld<32>(s_col + 32 * b + 32, r[(b + 1) & 1]);
-    const uint32_t* x = r[b & 1];
-    uint32_t out[32];
+    float2 x[16];
+    float top[4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float4 sc = *(const float4*)scales[2 * b + h];
-      const float f = factor * sc.x, d = sc.y - m;
-      const float2 f2 = make_float2(f, f), d2 = make_float2(d, d), i2 = make_float2(sc.z, sc.z);
+      const float2 sc = *(const float2*)scales[2 * b + h];
+      const float f = factor * sc.x;
+      const float2 f2 = make_float2(f, f), d2 = make_float2(sc.y, sc.y);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        float2 e = fma2(make_float2(__uint_as_float(x[16 * h + 2 * k]), __uint_as_float(x[16 * h + 2 * k + 1])), f2, d2);
+        float2 t = fma2(make_float2(__uint_as_float(r[16 * h + 2 * k]), __uint_as_float(r[16 * h + 2 * k + 1])), f2, d2);
         if (MASK) {
           const int key = key0 + 32 * b + 16 * h + 2 * k;
-          if (key >= limit) e.x = -INFINITY;
-          if (key + 1 >= limit) e.y = -INFINITY;
+          if (key >= limit) t.x = -INFINITY;
+          if (key + 1 >= limit) t.y = -INFINITY;
         }
-        e.x = exp2_fast(e.x);
-        e.y = exp2_fast(e.y);
-        part[k & 1] = fma2(e, i2, part[k & 1]);
-        const __half2 p = __floats2half2_rn(e.x, e.y);
-        out[8 * h + k] = *(const uint32_t*)&p;
-        if (LOW) {
-          const float2 low = sub2(e, __half22float2(p));
-          out[16 + 8 * h + k] = pack_f16(low.x, low.y);
+        x[8 * h + k] = t;
+        const float y = fmaxf(t.x, t.y);
+        top[k & 3] = h == 0 && k < 4 ? y : fmaxf(top[k & 3], y);
+      }
+    }
+    const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    if (__any_sync(0xffffffffu, most > m + kRaise)) {
+      float alpha = 1.0f;
+      if (most > m + kRaise) {
+        const float to = floorf(most) - kBelow;
+        alpha = exp2_fast(m - to);
+        m = to;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) part[i] = make_float2(part[i].x * alpha, part[i].y * alpha);
+      const __half2 alpha2 = __float2half2_rn(alpha);
+#pragma unroll 1
+      for (int c = 0; c < (LOW ? 32 : 16) * b; c += 16) {
+        uint32_t p[16];
+        tmem_ld<16>(s_col + c, p);
+        tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const __half2 h = __hmul2(*(const __half2*)&p[k], alpha2);
+          p[k] = *(const uint32_t*)&h;
         }
+        tmem_st16(s_col + c, p);
+      }
+#pragma unroll 1
+      for (int c = 0; c < (scale_o ? HD : 0); c += 16) {
+        uint32_t p[16];
+        tmem_ld<16>(o_col + c, p);
+        tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) p[k] = __float_as_uint(__uint_as_float(p[k]) * alpha);
+        tmem_st16(o_col + c, p);
+      }
+    }
+    uint32_t out[32];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const float iv = scales[2 * b + (k >> 3)][2];
+      float2 e = make_float2(exp2_fast(x[k].x - m), exp2_fast(x[k].y - m));
+      part[k & 1] = fma2(e, make_float2(iv, iv), part[k & 1]);
+      const __half2 p = __floats2half2_rn(e.x, e.y);
+      out[k] = *(const uint32_t*)&p;
+      if (LOW) {
+        const float2 low = sub2(e, __half22float2(p));
+        out[16 + k] = pack_f16(low.x, low.y);
       }
     }
     // The sums are due here: put off, they would keep every weight alive.
@@ -491,28 +505,8 @@ __global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape
       fence_after();
       const bool mask = key0 + kTile > low_limit;
       const float(*scales)[4] = S->scales[j & 3];
-      const float top = mask ? tile_top<true>(s_col, scales, factor, key0, limit)
-                             : tile_top<false>(s_col, scales, factor, key0, limit);
-      float alpha = 1.0f;
-      if (top > m + kRaise) {
-        alpha = exp2_fast(m - (top - kBelow));
-        m = top - kBelow;
-        l2.x *= alpha;
-        l2.y *= alpha;
-      }
-      if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-#pragma unroll
-        for (int b = 0; b < HD / 32; ++b) {
-          uint32_t r[32];
-          tmem_ld<32>(o_col + 32 * b, r);
-          tmem_wait_ld();
-#pragma unroll
-          for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * alpha);
-          tmem_st32(o_col + 32 * b, r);
-        }
-      }
-      if (mask) tile_weights<true, LOW>(s_col, scales, factor, m, key0, limit, l2);
-      else tile_weights<false, LOW>(s_col, scales, factor, m, key0, limit, l2);
+      if (mask) tile_weights<HD, true, LOW>(s_col, o_col, j > 0, scales, factor, key0, limit, m, l2);
+      else tile_weights<HD, false, LOW>(s_col, o_col, j > 0, scales, factor, key0, limit, m, l2);
       tmem_wait_st();
       fence_before();
       mbar_arrive(&S->pfull[t]);
