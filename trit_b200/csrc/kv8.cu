@@ -232,19 +232,21 @@ __device__ __forceinline__ void copy16(void* smem, const void* global) {
                : "memory");
 }
 
-template <int HD, int NT>
+template <int HD, bool SPLIT, int NT>
 struct AttendShape {
   static constexpr int UNIT = HD * 32;  // bytes of 16 positions' codes, or of their f16 keys (or values)
   static constexpr int STAGES = HD == 128 && NT == 1 ? 4 : 6;
   static constexpr int BLOCKS = HD == 128 && NT == 2 ? 2 : 3;  // an SM (registers)
-  static constexpr int SMEM = kAttendWarps * STAGES * UNIT;
+  static constexpr int STAGE_BYTES = kAttendWarps * STAGES * UNIT;
+  // Sums that f32 rows put aside (see kKvChain): HD / 8 values a lane and tile.
+  static constexpr int SMEM = STAGE_BYTES + (SPLIT ? kAttendWarps * NT * HD / 8 * 32 * 4 : 0);
 };
 
 template <int HD, bool SPLIT, int NT>
-__global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS)
+__global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, SPLIT, NT>::BLOCKS)
     k_kv_attend(const __grid_constant__ KvView kv, const __grid_constant__ KvRuns runs,
                 const __grid_constant__ KvAttendArgs a, int chunks, int splits, int vec, int vec_out, void* workspace) {
-  using Shape = AttendShape<HD, NT>;
+  using Shape = AttendShape<HD, SPLIT, NT>;
   constexpr int CL = NT * (SPLIT ? 4 : 8);   // columns a block
   constexpr int LT = SPLIT ? 1 : 2;          // columns a thread holds in an n-tile
   constexpr int KB = HD / 64;                // 64-wide blocks of a key
@@ -421,6 +423,25 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS
     }
   }
 
+  // f32 rows: the tensor cores cut what they add to a sum short, so a sum
+  // loses up to 2^-24 of itself with every product; after kKvChain positions
+  // it is put aside in shared memory and begun anew.
+  float* aside = (float*)(smem + Shape::STAGE_BYTES) + warp * (NT * HD / 8 * 32) + lane;
+  auto put_aside = [&](bool add) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int k = 0; k < MT; ++k)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          float* to = aside + ((t * MT + k) * 2 + y) * 32;
+          const float v = o[t][k][2 * y] + o[t][k][2 * y + 1];
+          *to = add ? *to + v : v;
+          o[t][k][2 * y] = o[t][k][2 * y + 1] = 0.0f;
+        }
+  };
+  if (SPLIT) put_aside(false);
+
   // Scores of two steps of 16 positions to P^T and the running sums. s[z][t]:
   // positions key0[z] + r and key0[z] + r + 8 of the thread's columns.
   auto softmax = [&](float (&s)[2][NT][4], const int (&key0)[2], const float (&ks)[2], const float (&lv)[2],
@@ -449,7 +470,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS
 #pragma unroll
           for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
           if (top > m[t][i] + kRaise) {
-            const float to = top - kBelow, alpha = exp2_fast(m[t][i] - to);
+            const float to = floorf(top) - kBelow, alpha = exp2_fast(m[t][i] - to);
             m[t][i] = to;
             l[t][i] *= alpha;
 #pragma unroll
@@ -457,6 +478,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS
               if (SPLIT) {
 #pragma unroll
                 for (int y = 0; y < 4; ++y) o[t][k][y] *= alpha;
+#pragma unroll
+                for (int y = 0; y < 2; ++y) aside[((t * MT + k) * 2 + y) * 32] *= alpha;
               } else {
                 o[t][k][i] *= alpha;
                 o[t][k][2 + i] *= alpha;
@@ -504,6 +527,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS
   int unit = 0;
   for (; unit < ncode; unit += 2) {
     const bool two = unit + 1 < ncode;
+    if (SPLIT && unit > 0 && unit % (kKvChain / 16) == 0) put_aside(true);
     __syncwarp();  // the units before are read
     fetch();
     fetch();
@@ -534,6 +558,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS
       }
     }
     clear();
+    float s2[2][NT][4] = {};  // the second half of 128-wide keys (f32 rows: shorter chains)
 #pragma unroll
     for (int b = 0; b < KB; ++b)
 #pragma unroll
@@ -545,9 +570,18 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS
         for (int q = 0; q < 4; ++q) {
           const uint32_t a0 = codes_lo(w0[q]), a1 = codes_lo(w1[q]), a2 = codes_hi(w0[q]), a3 = codes_hi(w1[q]);
 #pragma unroll
-          for (int t = 0; t < NT; ++t) mma16816(s[z][t], a0, a1, a2, a3, qf[t][b][q][0], qf[t][b][q][1]);
+          for (int t = 0; t < NT; ++t)
+            mma16816(SPLIT && b ? s2[z][t] : s[z][t], a0, a1, a2, a3, qf[t][b][q][0], qf[t][b][q][1]);
         }
       }
+    if (SPLIT && KB == 2) {
+#pragma unroll
+      for (int z = 0; z < 2; ++z)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[z][t][x] += s2[z][t][x];
+    }
     softmax(s, key0, ks, lv, iv, p);
 #pragma unroll
     for (int z = 0; z < 2; ++z)
@@ -601,7 +635,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
   float* s_o = (float*)smem;  // [warps][CL][HD]
-  static_assert(Shape::SMEM >= kAttendWarps * CL * HD * 4, "the sums fit where the loads were");
+  static_assert(Shape::STAGE_BYTES >= kAttendWarps * CL * HD * 4, "the sums fit where the loads were");
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -618,15 +652,18 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, NT>::BLOCKS
 #pragma unroll
       for (int k = 0; k < MT; ++k) {
         const int d = KB == 1 ? 8 * r + 2 * k : 64 * (k >> 2) + 8 * r + 2 * (k & 3);
-        *(float2*)(to + d) = SPLIT ? make_float2(o[t][k][0] + o[t][k][1], o[t][k][2] + o[t][k][3])
-                                   : make_float2(o[t][k][i], o[t][k][2 + i]);
+        float2 v = make_float2(o[t][k][i], o[t][k][2 + i]);
+        if (SPLIT)
+          v = make_float2(o[t][k][0] + o[t][k][1] + aside[(t * MT + k) * 64],
+                          o[t][k][2] + o[t][k][3] + aside[(t * MT + k) * 64 + 32]);
+        *(float2*)(to + d) = v;
       }
     }
   __syncthreads();
   const int nsplit = run.splits;
   // Partial results of a (kv head, block) behind the counters: [column][HD],
   // then (m, l) of each column.
-  float* part = (float*)workspace + kKvCounters + ((size_t)head * gridDim.x + blockIdx.x) * CL * (HD + 2);
+  float* part = (float*)workspace + kKvHead + ((size_t)head * gridDim.x + blockIdx.x) * CL * (HD + 2);
   auto put = [&](int c, int d, float sum, float4 v) {
     const size_t at = (size_t)(run.row0 + c / g) * a.out_stride + (size_t)(head * g + c % g) * HD + d;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -828,7 +865,7 @@ __global__ void k_kv_remap(int* table, const unsigned long long* remap, unsigned
 template <int HD, bool SPLIT, int NT>
 cudaError_t attend(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& p, int vec,
                    int vec_out, void* ws, cudaStream_t s) {
-  constexpr int smem = AttendShape<HD, NT>::SMEM;
+  constexpr int smem = AttendShape<HD, SPLIT, NT>::SMEM;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -939,7 +976,7 @@ KvAttendPlan plan_kv_attend(const KvView& kv, KvRuns& runs, const KvAttendArgs& 
         p.blocks += (int)(((size_t)r.count * g + p.cols - 1) / p.cols) * r.splits;
       }
     }
-    p.workspace = kKvCounters * 4 + p.blocks * bytes;
+    p.workspace = p.joins ? kKvHead * 4 + p.blocks * bytes : 0;
     if (!p.joins || ((size_t)p.blocks * kv.kv_heads <= kKvCounters && p.workspace <= kKvWorkspace)) break;
   }
   return p;

@@ -73,11 +73,16 @@ cudaError_t launch_kv_append(const KvView& kv, const KvRuns& runs, int layer, co
 struct KvAttendPlan {
   int blocks = 0, cols = 0, chunks = 1, splits = 1;
   bool joins = false;
-  size_t workspace = 0;  // bytes, with joins
+  // Bytes of workspace, and where in it (in floats) sums are put aside, in how
+  // many places.
+  size_t workspace = 0, aside = 0;
+  int places = 0;
 };
-// The workspace: f32 partial results behind one counter a tile, which is
-// zero between calls. No plan needs more.
-constexpr size_t kKvCounters = 8192, kKvWorkspace = 32u << 20;
+// The workspace begins with words that are zero between calls: a counter a
+// tile whose shares meet, and a flag a place where a block of many rows puts
+// sums aside. No plan needs more.
+constexpr size_t kKvCounters = 8192, kKvPlaces = 1024, kKvHead = kKvCounters + kKvPlaces;
+constexpr size_t kKvWorkspace = 64u << 20;
 KvAttendPlan plan_kv_attend(const KvView& kv, KvRuns& runs, const KvAttendArgs& a);
 cudaError_t launch_kv_attend(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& plan,
                              void* workspace, cudaStream_t s);

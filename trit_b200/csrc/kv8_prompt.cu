@@ -52,7 +52,7 @@ struct PromptSmem {
   // of the step two later are in use, which the softmax of this one precedes.
   float scales[4][8][4];
   uint32_t tmem;
-  int abort, last;
+  int abort, last, place;
 };
 
 // D = A B (+ D when `accumulate`), A in TMEM.
@@ -101,7 +101,7 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
 // Positions from `limit` on get no weight.
 template <int HD, bool MASK, bool LOW>
 __device__ __forceinline__ void tile_weights(uint32_t s_col, uint32_t o_col, bool scale_o, const float (*scales)[4],
-                                             float factor, int key0, int limit, float& m, float2& sum) {
+                                             float factor, int key0, int limit, float& m, float2& sum, float& carry) {
   float2 part[2] = {sum, make_float2(0.0f, 0.0f)};
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
@@ -138,6 +138,7 @@ __device__ __forceinline__ void tile_weights(uint32_t s_col, uint32_t o_col, boo
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) part[i] = make_float2(part[i].x * alpha, part[i].y * alpha);
+      carry *= alpha;
       const __half2 alpha2 = __float2half2_rn(alpha);
 #pragma unroll 1
       for (int c = 0; c < (LOW ? 32 : 16) * b; c += 16) {
@@ -191,10 +192,15 @@ constexpr int prompt_smem() {
 template <int HD, bool LOW, int QT>
 __global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape<HD, LOW, QT>::BLOCKS)
     k_kv_prompt(const __grid_constant__ KvView kv, const __grid_constant__ KvRuns runs,
-                const __grid_constant__ KvAttendArgs a, int vec, int vec_out, void* workspace, int* status) {
+                const __grid_constant__ KvAttendArgs a, int vec, int vec_out, void* workspace, size_t aside_at,
+                int places, int* status) {
   using Shape = PromptShape<HD, LOW, QT>;
   constexpr int TILE = Shape::TILE, KS = Shape::KS, VS = Shape::VS, QB = (LOW ? 2 : 1) * TILE;
   constexpr int COLS = QT * kTile;
+  // Steps whose values are summed in one go: f32 rows add O up in the
+  // workspace (in a place that the block takes for its time; 32 columns of a
+  // warp side by side) and begin anew.
+  constexpr int CHAIN = LOW ? kKvChain / kTile : 1 << 30;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* q_s = base;                  // [QT][value, remainder]
@@ -231,6 +237,18 @@ __global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape
     mbar_init(&S->qfull, QT * 128);
     mbar_init(&S->done, 1);
     S->abort = 0;
+    S->place = -1;
+    if (LOW && nt > CHAIN) {
+      // As many places as blocks run at once: one is free.
+      unsigned* flags = (unsigned*)workspace + kKvCounters;
+      int at = (int)(blockIdx.x + blockIdx.y * gridDim.x) % places;
+      for (int i = 0; i < 1 << 20 && S->place < 0; ++i) {
+        if (atomicExch(flags + at, 1u) == 0) S->place = at;
+        at = at + 1 == places ? 0 : at + 1;
+      }
+      if (S->place < 0) S->abort = 1;
+      __threadfence();
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == MMA_WARP) {
@@ -397,7 +415,7 @@ __global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape
         for (int i = 0; i < kTile / 16; ++i) {
           const uint64_t b = smem_desc_sw128_mn(v + i * 2048, kTile * 128);
           const uint32_t p = tmem + t * kTile + (LOW ? 32 * (i >> 1) + 8 * (i & 1) : 8 * i);
-          mma_f16_ts(o, p, b, idesc_f16n(HD, true), (j > 0 || i > 0) ? 1u : 0u);
+          mma_f16_ts(o, p, b, idesc_f16n(HD, true), (j % CHAIN > 0 || i > 0) ? 1u : 0u);
           if (LOW) mma_f16_ts(o, p + 16, b, idesc_f16n(HD, true), 1u);
         }
       };
@@ -491,9 +509,25 @@ __global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape
     }
     fence_async_smem();
     mbar_arrive(&S->qfull);
-    float m = kMInit;
+    float m = kMInit, carry = 1.0f;  // carry: what O put aside is to be scaled by
     float2 l2 = make_float2(0.0f, 0.0f);
-    bool ok = true;
+    bool ok = true, aside = false;
+    float* part = (float*)workspace + kKvHead + ((size_t)head * gridDim.x + block) * COLS * (HD + 2);
+    float* total = (float*)workspace + aside_at + ((size_t)max(S->place, 0) * COLS + t * kTile + (warp & 3) * 32) * HD + lane;
+    // 32 values of O, with what was put aside of them.
+    auto whole = [&](int b, uint32_t (&r)[32]) {
+      tmem_ld<32>(o_col + 32 * b, r);
+      if (LOW && aside) {
+        float x[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) x[k] = __ldcg(total + (32 * b + k) * 32);
+        tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(fmaf(x[k], carry, __uint_as_float(r[k])));
+      } else {
+        tmem_wait_ld();
+      }
+    };
     for (int j = 0; j < nt && t < groups; ++j) {
       const int key0 = (t0 + j) * kTile;
       // Warp-uniform waits: the TMEM loads and stores below are warp-wide.
@@ -503,10 +537,33 @@ __global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape
         break;
       }
       fence_after();
+      if (LOW && j > 0 && j % CHAIN == 0) {
+        const bool add = aside && __all_sync(0xffffffffu, carry == 1.0f);
+#pragma unroll 1
+        for (int b = 0; b < HD / 32; ++b) {
+          uint32_t r[32];
+          if (add) {
+            tmem_ld<32>(o_col + 32 * b, r);
+            tmem_wait_ld();
+            // Nothing waits for these; the same thread reads them back.
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(total + (32 * b + k) * 32),
+                           "f"(__uint_as_float(r[k]))
+                           : "memory");
+          } else {
+            whole(b, r);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) __stcg(total + (32 * b + k) * 32, __uint_as_float(r[k]));
+          }
+        }
+        aside = true;
+        carry = 1.0f;
+      }
       const bool mask = key0 + kTile > low_limit;
       const float(*scales)[4] = S->scales[j & 3];
-      if (mask) tile_weights<HD, true, LOW>(s_col, o_col, j > 0, scales, factor, key0, limit, m, l2);
-      else tile_weights<HD, false, LOW>(s_col, o_col, j > 0, scales, factor, key0, limit, m, l2);
+      if (mask) tile_weights<HD, true, LOW>(s_col, o_col, j % CHAIN > 0, scales, factor, key0, limit, m, l2, carry);
+      else tile_weights<HD, false, LOW>(s_col, o_col, j % CHAIN > 0, scales, factor, key0, limit, m, l2, carry);
       tmem_wait_st();
       fence_before();
       mbar_arrive(&S->pfull[t]);
@@ -515,26 +572,24 @@ __global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape
     if (t < groups && ok) {
       fence_after();
       const float l = l2.x + l2.y, inv = l == 0.0f ? 0.0f : 1.0f / l;
-      float* part = (float*)workspace + kKvCounters + ((size_t)head * gridDim.x + block) * COLS * (HD + 2);
-#pragma unroll
+#pragma unroll 1
       for (int b = 0; b < HD / 32; ++b) {
         uint32_t r[32];
         if (nt > 0) {
-          tmem_ld<32>(o_col + 32 * b, r);
-          tmem_wait_ld();
+          whole(b, r);
         } else {
 #pragma unroll
           for (int k = 0; k < 32; ++k) r[k] = 0;
         }
         if (!live) continue;
         if (run.splits == 1) {
-          const size_t to = (size_t)(run.row0 + c / g) * a.out_stride + (size_t)(head * g + c % g) * HD + 32 * b;
+          const size_t out_at = (size_t)(run.row0 + c / g) * a.out_stride + (size_t)(head * g + c % g) * HD;
 #pragma unroll
           for (int k = 0; k < 32; k += 8) {
             float x[8];
 #pragma unroll
             for (int z = 0; z < 8; ++z) x[z] = l == 0.0f ? 0.0f : __uint_as_float(r[k + z]) * inv;
-            kv_store8(a.out, to + k, a.type, vec_out, x);
+            kv_store8(a.out, out_at + 32 * b + k, a.type, vec_out, x);
           }
         } else {
 #pragma unroll
@@ -545,7 +600,7 @@ __global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape
       if (run.splits > 1 && live) *(float2*)(part + COLS * HD + 2 * (t * kTile + q)) = make_float2(m, l);
     }
   }
-  if (run.splits > 1) __threadfence();
+  if (run.splits > 1 || S->place >= 0) __threadfence();
   fence_before();
   __syncthreads();
   if (warp == MMA_WARP) {
@@ -553,6 +608,7 @@ __global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Shape::COLS) : "memory");
   }
   if (threadIdx.x == 0 && S->abort) *(volatile int*)status = 1;
+  if (threadIdx.x == 0 && S->place >= 0) atomicExch((unsigned*)workspace + kKvCounters + S->place, 0u);
   if (run.splits == 1) return;
   // The block that comes last of a tile's shares joins them, in their order.
   if (threadIdx.x == 0) {
@@ -562,7 +618,7 @@ __global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape
   __syncthreads();
   if (!S->last) return;
   __threadfence();
-  const float* first = (const float*)workspace + kKvCounters + ((size_t)head * gridDim.x + block - split) * COLS * (HD + 2);
+  const float* first = (const float*)workspace + kKvHead + ((size_t)head * gridDim.x + block - split) * COLS * (HD + 2);
   for (int x = 4 * threadIdx.x; x < COLS * HD; x += 4 * Shape::THREADS) {
     const int lc = x / HD, d = x % HD, c = c0 + lc;
     if (c >= cols) break;
@@ -590,7 +646,7 @@ cudaError_t prompt(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, 
   });
   if (e != cudaSuccess) return e;
   k_kv_prompt<HD, LOW, QT><<<dim3(p.blocks, kv.kv_heads), PromptShape<HD, LOW, QT>::THREADS, smem, s>>>(
-      kv, runs, a, vec, vec_out, ws, status);
+      kv, runs, a, vec, vec_out, ws, p.aside, p.places, status);
   return cudaGetLastError();
 }
 template <int HD, bool LOW>
@@ -652,7 +708,12 @@ KvAttendPlan plan_kv_prompt(const KvView& kv, KvRuns& runs, const KvAttendArgs& 
       p.joins |= r.splits > 1;
       p.blocks += (int)(((size_t)r.count * g + p.cols - 1) / p.cols) * r.splits;
     }
-    p.workspace = kKvCounters * 4 + p.blocks * bytes;
+    // The partial results of shares, then the sums that f32 rows put aside.
+    const size_t partial = p.joins ? p.blocks * bytes : 0;
+    p.aside = a.type == kKvF32 ? kKvHead + partial / 4 : 0;
+    p.workspace = p.aside || p.joins ? kKvHead * 4 + partial : 0;
+    p.places = std::min<int>(kKvPlaces, 2 * current_sm_count());  // at most two blocks run on an SM
+    if (p.aside) p.workspace += (size_t)p.places * p.cols * kv.hd * 4;
     if (!p.joins || ((size_t)p.blocks * kv.kv_heads <= kKvCounters && p.workspace <= kKvWorkspace)) break;
   }
   return p;
@@ -661,7 +722,7 @@ KvAttendPlan plan_kv_prompt(const KvView& kv, KvRuns& runs, const KvAttendArgs& 
 cudaError_t launch_kv_prompt(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& p, void* ws,
                              int* status, cudaStream_t s) {
   if (p.blocks <= 0) return cudaSuccess;
-  if (runs.row_seq || (p.joins && !ws)) return cudaErrorInvalidValue;
+  if (runs.row_seq || (p.workspace && !ws)) return cudaErrorInvalidValue;
   const size_t size = a.type == kKvF32 ? 4 : 2;
   const int vec = ((uintptr_t)a.q | a.q_stride * size) % 16 == 0, vec_out = ((uintptr_t)a.out | a.out_stride * size) % 16 == 0;
   const bool low = a.type == kKvF32;

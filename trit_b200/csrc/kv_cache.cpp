@@ -65,7 +65,7 @@ KvCache::KvCache(const KvOptions& o) : opt_(o) {
     // The attention reads whole steps of 16 positions of an open page, also
     // those behind its end: they must hold numbers from the start.
     TRIT_CUDA(cudaMemset(view_.open, 0, open));
-    TRIT_CUDA(cudaMemset(workspace_, 0, kKvCounters * 4));
+    TRIT_CUDA(cudaMemset(workspace_, 0, kKvHead * 4));
     TRIT_CUDA(cudaMemset(view_.table, 0, table));
     TRIT_CUDA(cudaDeviceSynchronize());
     TRIT_CUDA(cudaEventCreateWithFlags(&order_, cudaEventDisableTiming));
@@ -417,15 +417,15 @@ void KvCache::attend_runs(KvRuns& runs, KvAttendArgs& a, bool prompt, cudaStream
   for (int i = 0; i < runs.n; ++i) a.max_len = std::max(a.max_len, runs.run[i].len);
   const KvAttendPlan plan = prompt ? plan_kv_prompt(view_, runs, a) : plan_kv_attend(view_, runs, a);
   void* ws = workspace_;
-  if (capturing_ && plan.joins) {
+  if (capturing_ && plan.workspace) {
     // A captured call's workspace belongs to its graph: two graphs of one
     // cache, or a graph and a call, may then run at once.
     TRIT_CUDA(cudaMallocAsync(&ws, plan.workspace, s));
-    TRIT_CUDA(cudaMemsetAsync(ws, 0, kKvCounters * 4, s));
+    TRIT_CUDA(cudaMemsetAsync(ws, 0, kKvHead * 4, s));
   }
   if (prompt) TRIT_CUDA(launch_kv_prompt(view_, runs, a, plan, ws, status_, s));
   else TRIT_CUDA(launch_kv_attend(view_, runs, a, plan, ws, s));
-  if (capturing_ && plan.joins) TRIT_CUDA(cudaFreeAsync(ws, s));
+  if (capturing_ && plan.workspace) TRIT_CUDA(cudaFreeAsync(ws, s));
   runs.n = 0;
 }
 
