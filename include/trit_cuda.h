@@ -308,8 +308,9 @@ TritDense *trit_dense_q8_0(const void *blocks, size_t n, size_t k, int table, in
  * in another order than a Q8_0 layer's. A call of more than 32 rows with
  * table = 0 (n a multiple of 32, k of 128) runs on the int8 tensor cores from
  * an int8 copy of the weights that the first such call makes (n x k bytes
- * more). The other calls use no scratch memory: they may overlap, and may be
- * captured. NULL on failure. (The reference expands Q4_0 tensors when it
+ * more; not in a capture), and like a Q8_0 layer's calls they share scratch
+ * memory: order them on one stream. The other calls use none: they may
+ * overlap, and may be captured after the first. NULL on failure. (The reference expands Q4_0 tensors when it
  * loads them, src/cpu/ggml_quants.rs:1-6.) */
 TritDense *trit_dense_q4_0(const void *blocks, size_t n, size_t k, int table, int device);
 
@@ -371,9 +372,10 @@ int trit_dense_q8_0_forward_static(const void *codes, const void *scales, size_t
  * In a stream capture only trit_cuda_kv_attend and trit_cuda_kv_read are
  * taken; a replay reads the positions that the sequences had when it was
  * captured, and the caller orders it after the calls it depends on. The
- * graph owns the memory it works in. The sequences must stay as they were:
- * a replay after a trit_cuda_kv_release, trit_cuda_kv_compact or
- * trit_cuda_kv_extend of them reads what now lies there.
+ * graph owns the memory it works in. The cache must outlive the graph, and
+ * the sequences must stay as they were: a replay after a
+ * trit_cuda_kv_release, trit_cuda_kv_compact or trit_cuda_kv_append of them
+ * reads what now lies there.
  *
  * A call that fails on its arguments changes nothing. */
 

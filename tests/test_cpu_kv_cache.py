@@ -18,6 +18,8 @@ from trit_b200 import Dense, KvCache, TritError, lm
     (dict(kv_heads=2, pages=4, sequences=0), "sequences"),
     (dict(kv_heads=2, pages=4, max_tokens=0), "max_tokens"),
     (dict(kv_heads=2, pages=4, colour=1), "unknown key colour"),
+    (dict(kv_heads=2, pages=4, sequences=1024, max_tokens=1 << 26, page_tokens=16), "2\\^31 or more"),
+    (dict(kv_heads=1024, pages=4, layers=4096, page_tokens=128), "4 GB or more"),
 ])
 def test_bad_cache_options(options, words):
     with pytest.raises(TritError, match=words):

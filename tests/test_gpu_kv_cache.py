@@ -319,6 +319,102 @@ def test_pages_far_into_the_pool():
         assert np.array_equal(contents(kv, 0, c[0], kv_heads, hd)[0], held(k64, page))
 
 
+# Enough rows and heads for the kernel of many rows (8192 columns in a call, 64 in a run).
+@pytest.mark.parametrize("hd, page, heads, kv_heads", [(128, 64, 16, 4), (64, 16, 20, 4), (128, 128, 15, 5), (64, 32, 16, 16)])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompts(hd, page, heads, kv_heads, dtype, causal):
+    lens, counts = [300, 700, 129, 257, 31], [300, 200, 128, 1, 31]
+    if not causal:
+        lens, counts = lens + [0, 1], counts + [70, 70]
+    with KvCache(kv_heads=kv_heads, pages=128, head_dim=hd, page_tokens=page, sequences=8, max_tokens=1024) as kv:
+        seqs = kv.open(len(lens))
+        data = [(rows(i, n, kv_heads, hd, dtype=dtype), rows(50 + i, n, kv_heads, hd, dtype=dtype)) for i, n in enumerate(lens)]
+        fill(kv, 0, seqs, [(k[0], v[0]) for k, v in data], dtype)
+        q, q64 = rows(99, sum(counts), heads, hd, dtype=dtype)
+        scale = 0.1 if causal else -0.1
+        out = run_attend(kv, 0, seqs, q, counts, heads, scale, dtype, causal)
+        check_attend(out, q64, [held(k[1], page) for k, _ in data], [held(v[1], page) for _, v in data], counts, scale, dtype, causal)
+
+
+@pytest.mark.parametrize("size", [1.0, 40.0, 1e-6])
+def test_prompts_of_any_scores(size):
+    """Sharp and flat softmaxes whose largest score comes late, over pages of values of very different size."""
+    hd, page, t, heads = 128, 16, 400, 32
+    (q, q64), (k, k64), (v, v64) = rows(1, t, heads, hd), rows(2, t, 1, hd), rows(3, t, 1, hd)
+    ramp = torch.linspace(0.01, 1.0, t, device="cuda")[:, None, None] * size
+    q, k = q * size, k * ramp
+    v[160:176] = 0
+    v[176:192] *= 1000
+    q64, k64, v64 = (x.double().cpu().numpy() for x in (q, k, v))
+    with KvCache(kv_heads=1, pages=32, head_dim=hd, page_tokens=page, sequences=1, max_tokens=512) as kv:
+        s = kv.open(1)
+        fill(kv, 0, s, [(k, v)])
+        out = run_attend(kv, 0, s, q, [t], heads, 0.09, "f32")
+        check_attend(out, q64, [held(k64, page)], [held(v64, page)], [t], 0.09, "f32")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_many_rows_behind_a_long_context(dtype, hd):
+    """Few tiles of many rows, so that their positions are shared out and the shares joined; the output may be the query."""
+    page, t, m, heads = 32, 6000, 300, 32
+    (k, k64), (v, v64), (q, q64) = rows(1, t, 1, hd, dtype=dtype), rows(2, t, 1, hd, dtype=dtype), rows(3, m, heads, hd, dtype=dtype)
+    with KvCache(kv_heads=1, pages=200, head_dim=hd, page_tokens=page, sequences=2, max_tokens=8192) as kv:
+        s = kv.open(1)
+        fill(kv, 0, s, [(k, v)], dtype)
+        for causal in (True, False):
+            out = q.clone()
+            torch.cuda.synchronize()
+            kv.attend(0, s, [m], out.data_ptr(), out.data_ptr(), heads=heads, scale=0.11, dtype=dtype, causal=causal)
+            torch.cuda.synchronize()
+            check_attend(out, q64, [held(k64, page)], [held(v64, page)], [m], 0.11, dtype, causal=causal)
+
+
+def test_many_rows_of_long_sequences_unshared():
+    """So many tiles that none is shared out: every warp walks all of its positions in one go."""
+    hd, page, t, n = 128, 64, 1500, 600
+    (k, k64), (v, v64), (q, q64) = rows(1, t, 4, hd), rows(2, t, 4, hd), rows(3, n, 4, hd)
+    with KvCache(kv_heads=4, pages=32, head_dim=hd, page_tokens=page, sequences=1, max_tokens=2048) as kv:
+        s = kv.open(1)
+        fill(kv, 0, s, [(k, v)])
+        out = run_attend(kv, 0, s * n, q, [1] * n, 4, 0.09, "f32", causal=False)
+        want, tol = attend(q64, held(k64, page), held(v64, page), 0.09, False)
+        assert (np.abs(out.double().cpu().numpy() - want) <= tol).all()
+
+
+def test_calls_from_two_threads():
+    """Two host threads on two streams, each with its sequences: calls take turns, results are each one's own."""
+    import threading
+
+    hd, page, t = 64, 16, 50
+    errors = []
+    with KvCache(kv_heads=2, pages=64, head_dim=hd, page_tokens=page, sequences=8, max_tokens=64) as kv:
+        def work(seed):
+            try:
+                stream = torch.cuda.Stream()
+                for i in range(20):
+                    s = kv.open(1)
+                    (k, k64), (v, v64), (q, q64) = (rows(seed + 3 * i + j, t, 2, hd) for j in range(3))
+                    out = torch.empty_like(q)
+                    torch.cuda.synchronize()
+                    kv.extend(s, [t], stream=stream.cuda_stream)
+                    kv.append(0, s, [t], k.data_ptr(), v.data_ptr(), stream=stream.cuda_stream)
+                    kv.attend(0, s, [t], q.data_ptr(), out.data_ptr(), heads=2, scale=0.125, stream=stream.cuda_stream)
+                    stream.synchronize()
+                    check_attend(out, q64, [held(k64, page)], [held(v64, page)], [t], 0.125, "f32")
+                    kv.release(s)
+            except BaseException as e:  # noqa: BLE001
+                errors.append(e)
+
+        threads = [threading.Thread(target=work, args=(1000 * i,)) for i in range(2)]
+        for x in threads:
+            x.start()
+        for x in threads:
+            x.join()
+    assert not errors, errors
+
+
 def test_steps_as_a_decoder_makes_them():
     """Everything together: prompts, steps that append and attend, a branch, a gap that closes; on two streams in turn
     without a wait between the calls."""
@@ -398,6 +494,33 @@ def test_captured_attention():
         assert kv.length(s[0]) == t + 1
         kv.append(0, s, [1], x.data_ptr(), x.data_ptr())
         torch.cuda.synchronize()
+
+
+def test_captured_prompt():
+    """The kernel of many rows, with what it puts aside and shares out, in two graphs replayed at once."""
+    hd, page, t, m, heads = 128, 64, 3000, 300, 32
+    (k, _), (v, _) = rows(1, t, 1, hd), rows(2, t, 1, hd)
+    with KvCache(kv_heads=1, pages=64, head_dim=hd, page_tokens=page, sequences=1, max_tokens=4096) as kv:
+        s = kv.open(1)
+        fill(kv, 0, s, [(k, v)])
+        qs = [rows(i, m, heads, hd)[0] for i in (3, 4)]
+        want = [run_attend(kv, 0, s, q, [m], heads, 0.1, "f32") for q in qs]
+        outs, graphs, streams = [torch.zeros_like(q) for q in qs], [], [torch.cuda.Stream() for _ in qs]
+        for q, out, stream in zip(qs, outs, streams):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=stream):
+                kv.attend(0, s, [m], q.data_ptr(), out.data_ptr(), heads=heads, scale=0.1, stream=stream.cuda_stream)
+            graphs.append(g)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for out in outs:
+                out.zero_()
+            torch.cuda.synchronize()
+            for g, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(o, w) for o, w in zip(outs, want))
 
 
 def test_refusals():

@@ -1026,7 +1026,7 @@ void Lm::attention_q8(int layer, int m, int max_tk, const std::vector<std::pair<
   };
   if (!causal_) {
     r.run[r.n++] = KvRun{0, 0, 0, m, m};
-    go(m, kv_prompt_run(m, group));
+    go(m, kv_prompt_run(m, group, kKvF32, (int64_t)m * cfg_.heads));
   } else if (!runs) {
     r.n = m;
     r.row_seq = row_stream_;
@@ -1037,7 +1037,7 @@ void Lm::attention_q8(int layer, int m, int max_tk, const std::vector<std::pair<
     bool prompt = false;
     for (const auto& run : *runs) {
       const int row = run.first, count = run.second;
-      const bool many = kv_prompt_run(count, group);
+      const bool many = kv_prompt_run(count, group, kKvF32, (int64_t)m * cfg_.heads);
       if (r.n && (many != prompt || r.n == kKvRuns)) {
         go(most, prompt);
         most = 0;
@@ -1965,6 +1965,7 @@ std::unique_ptr<DenseOp> dense_q4_0(const void* blocks, size_t n, size_t k, int 
 // same codes and scales: its weights are expanded once and kept.
 void DenseOp::forward_q4(const float* x, size_t m, float* y, cudaStream_t s) {
   constexpr size_t kWideRows = 33;
+  if (m > (size_t)INT32_MAX) throw Error("a call has at most 2^31 - 1 rows");
   if (m < kWideRows || !tc_ok) {
     TRIT_CUDA(launch_q4(w4, x, (int)m, !table, y, s));
     return;

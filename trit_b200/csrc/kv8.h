@@ -91,10 +91,17 @@ cudaError_t launch_kv_attend(const KvView& kv, const KvRuns& runs, const KvAtten
 KvAttendPlan plan_kv_prompt(const KvView& kv, KvRuns& runs, const KvAttendArgs& a);
 cudaError_t launch_kv_prompt(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& plan,
                              void* workspace, int* status, cudaStream_t s);
-// Whether a run's rows are worth the kernel of many rows: it takes a
-// tile of 128 query columns at the cost of one, the other kernel reads the
-// positions again for every 4 to 16 columns.
-inline bool kv_prompt_run(int count, int group) { return (size_t)count * group > 32; }
+// Whether a run's rows are worth the kernel of many rows. It takes 128 or 256
+// query columns (a row of a head of the group) at the cost of one, the other
+// reads the positions again for every 4 to 16; but it starts late, so the call
+// has to bring enough columns over all kv heads as well. Measured, 32 heads on
+// 8, 128 wide, us for few / many: f32, 32 runs of 1000 positions, 32 columns
+// 87 / 104, 48 121 / 105; one run of 2000, 256 columns 38 / 43, 512 68 / 46;
+// bf16, 32 runs, 48 columns 72 / 80, 64 92 / 84; one run, 512 columns 38 / 56,
+// 1024 67 / 56.
+inline bool kv_prompt_run(int64_t count, int group, int type, int64_t columns) {
+  return type == kKvF32 ? count * group >= 40 && columns >= 4096 : count * group >= 64 && columns >= 8192;
+}
 // Positions first .. first + count of each run as values, rows of
 // [kv_heads][hd] from row0 on.
 cudaError_t launch_kv_read(const KvView& kv, const KvRuns& runs, int layer, void* k, void* v, int type, int max_count,

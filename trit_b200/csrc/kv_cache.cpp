@@ -38,6 +38,8 @@ KvOptions KvOptions::parse(const char* text) {
     throw Error("options: page_tokens is 16, 32, 64 or 128");
   if ((size_t)o.layers * 2 * o.kv_heads * o.page * o.hd >> 32)
     throw Error("options: a page of all layers and heads holds 4 GB or more");
+  if ((size_t)o.sequences * std::max(1, o.max_tokens / o.page) > (size_t)INT32_MAX)
+    throw Error("options: sequences * max_tokens / page_tokens is 2^31 or more");
   return o;
 }
 
@@ -401,7 +403,7 @@ void KvCache::attend(int layer, const int* ids, const int64_t* counts, size_t n,
   for (size_t i = 0; i < n; ++i) {
     const Seq& p = seqs_[ids[i]];
     if (!counts[i]) continue;
-    KvRuns& to = kv_prompt_run((int)counts[i], group) ? many : few;
+    KvRuns& to = kv_prompt_run(counts[i], group, type, total * heads) ? many : few;
     to.run[to.n++] = KvRun{ids[i], (int)(p.len - counts[i]), row, (int)counts[i], (int)p.len};
     row += (int)counts[i];
     if (to.n == kKvRuns) attend_runs(to, a, &to == &many, s);
