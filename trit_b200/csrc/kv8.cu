@@ -9,6 +9,7 @@
 // values alone, not on how many calls brought them.
 #include <algorithm>
 
+#include "device.cuh"
 #include "kernels.h"
 #include "kv8.cuh"
 
@@ -30,20 +31,24 @@ __device__ __forceinline__ int nearest_code(float x, float scale, float inv) {
   return x < 0.0f ? -c : c;
 }
 
-// Codes + 128 of 8 values, packed in order. x * inv is within 4e-5 of
-// x / scale (two roundings of a number below 128), so rounding it is exact
-// unless it lands within 1e-4 of a border; those go through nearest_code.
-// Adding 1.5 * 2^23 rounds, and leaves the code in the low bits.
+// Codes + 128 of 8 values, packed in order. Adding 1.5 * 2^23 rounds x * inv
+// to the nearest whole number t and leaves the code in the low bits. x * inv
+// is within 127 * 2^-24 (8e-6) of x / scale, so t is the nearest code unless
+// x * inv lies within 1e-5 of a border; units with a value within 2e-5 of one
+// go through nearest_code.
 __device__ __forceinline__ uint2 codes8(const float (&v)[8], float scale, float inv) {
+  constexpr float kRound = 12582912.0f + 128.0f;
+  const float2 by = make_float2(inv, inv), up = make_float2(kRound, kRound), back = make_float2(kRound, kRound);
   uint32_t c[8];
   float far = 0.0f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float y = __fmul_rn(v[j], inv), r = __fadd_rn(y, 12582912.0f + 128.0f);
-    c[j] = __float_as_uint(r);
-    far = fmaxf(far, fabsf(__fsub_rn(y, __fsub_rn(r, 12582912.0f + 128.0f))));
+  for (int j = 0; j < 8; j += 2) {
+    const float2 x = make_float2(v[j], v[j + 1]), r = fma2(x, by, up), t = sub2(back, r), d = fma2(x, by, t);
+    c[j] = __float_as_uint(r.x);
+    c[j + 1] = __float_as_uint(r.y);
+    far = fmaxf(fmaxf(far, fabsf(d.x)), fabsf(d.y));
   }
-  if (far > 0.4999f) {
+  if (far > 0.49998f) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) c[j] = (uint32_t)(nearest_code(v[j], scale, inv) + 128);
   }
@@ -51,6 +56,15 @@ __device__ __forceinline__ uint2 codes8(const float (&v)[8], float scale, float 
   w.x = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
   w.y = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
   return w;
+}
+
+// The largest magnitudes of 8 f16, even and odd places; NaN if one is.
+__device__ __forceinline__ __half2 largest8(uint4 h) {
+  const uint32_t w[4] = {h.x, h.y, h.z, h.w};
+  __half2 m = __habs2(*(const __half2*)&w[0]);
+#pragma unroll
+  for (int j = 1; j < 4; ++j) m = __hmax2_nan(m, __habs2(*(const __half2*)&w[j]));
+  return m;
 }
 
 // ------------------------------------------------------------- append ----
@@ -112,16 +126,17 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const __grid_const
       } else {
         float f[8];
         kv_load8(src, (size_t)(run.row0 + page * P + t - run.first) * stride + (size_t)head * HD + 8 * u, type, vec, f);
-        __half x[8];
+        h = make_uint4(pack_f16(f[0], f[1]), pack_f16(f[2], f[3]), pack_f16(f[4], f[5]), pack_f16(f[6], f[7]));
+        const __half2 far = largest8(h);
+        if (!(__low2float(far) <= kF16Max && __high2float(far) <= kF16Max)) {  // an infinity or NaN among them
+          __half x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = to_cache_f16(f[j]);
-        h = *(const uint4*)x;
+          for (int j = 0; j < 8; ++j) x[j] = to_cache_f16(f[j]);
+          h = *(const uint4*)x;
+        }
       }
       held[i] = h;
-      const uint32_t w[4] = {h.x, h.y, h.z, h.w};
-      __half2 m = __habs2(*(const __half2*)&w[0]);
-#pragma unroll
-      for (int j = 1; j < 4; ++j) m = __hmax2(m, __habs2(*(const __half2*)&w[j]));
+      const __half2 m = largest8(h);
       top = fmaxf(top, fmaxf(__low2float(m), __high2float(m)));
     }
     if (full) {
@@ -779,11 +794,21 @@ __global__ void __launch_bounds__(256) k_kv_read(const __grid_constant__ KvView 
         w[1][0] = q1.x;
         w[1][1] = q1.y;
       }
+      // 0x4B000000 | c is 2^23 + c; both steps are exact up to the product's
+      // rounding.
+      const float2 base = make_float2(-8388736.0f, -8388736.0f), by = make_float2(scale, scale);
 #pragma unroll
       for (int z = 0; z < 2; ++z)
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          x[z][j] = __fmul_rn((float)((int)(w[z][j >> 2] >> (8 * (j & 3)) & 255u) - 128), scale);
+        for (int j = 0; j < 8; j += 2) {
+          const uint32_t q = w[z][j >> 2];
+          const float2 y = mul2(add2(make_float2(__uint_as_float(__byte_perm(q, 0x4B000000u, 0x7540 + (j & 3))),
+                                                 __uint_as_float(__byte_perm(q, 0x4B000000u, 0x7541 + (j & 3)))),
+                                     base),
+                                by);
+          x[z][j] = y.x;
+          x[z][j + 1] = y.y;
+        }
     }
 #pragma unroll
     for (int z = 0; z < 2; ++z) {
