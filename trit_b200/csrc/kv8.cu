@@ -74,7 +74,12 @@ __device__ __forceinline__ __half2 largest8(uint4 h) {
 // so that the second does not overwrite what the first still reads. The
 // page's share passes through shared memory as f16, eight values a thread
 // and turn, while its largest value is found.
-// Bound by bytes: rows in (2 or 4 bytes a value), codes out.
+// Its bytes are the rows in (2 or 4 a value) and the codes out; a block waits
+// for its rows, then rounds them, so few rows cost latency (64 streams, one
+// row each, 9 us) and many cost instructions as well: 5 streams of 1301 bf16
+// rows on 8 heads 128 wide 19 us a layer, 2.1 TB/s (256 threads a block: four
+// layers and their reads 132 us, with 128 threads 137; when rounding took
+// twice the instructions 147, with 512 threads 179).
 constexpr int kAppendThreads = 256;
 
 template <int HD>
@@ -203,10 +208,11 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const __grid_const
 // the positions; a warp walks its positions 16 at a time:
 //   S^T = K Q^T   mma m16n8k16, M 16 positions, N 8 columns, K the head
 //   O^T += V^T P^T               M 16 of the head's values, K 16 positions
-// with codes loaded straight into the registers that hold an operand (16
-// bytes a lane, whole 32-byte sectors), one byte permute and one subtraction
-// turning two codes into two exact f16 (0x6400 | u is 1024 + u). The order of
-// a product's inner index is free, so it is taken as the loads bring it.
+// two steps an iteration. Codes come by asynchronous copies of whole lines
+// into the warp's own ring in shared memory, 4 or 6 steps deep, and from
+// there 16 bytes a lane; one byte permute and one subtraction turn two codes
+// into two exact f16 (0x6400 | u is 1024 + u). The order of a product's inner
+// index is free, so it is taken as the bytes lie.
 //
 // The products are exact in f16 but for Q and P. A query is scaled by a
 // power of two into [1, 2) and, for f32 rows, split into two f16 columns
@@ -217,9 +223,13 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const __grid_const
 // the page's value scale rides in the exponent and the value product takes
 // the bare codes; the denominator adds p / value scale. M is raised only when
 // a t passes it by 14 (p stays below 2^14 in f16), which a vote of the warp
-// finds; then M becomes the top less 7.
+// finds; then M becomes the top's whole part less 7 (whole, so that a raise
+// scales the sums exactly).
 //
-// Bound by the codes' bytes: 2 hd bytes a position and kv head.
+// Bound by the codes' bytes, 2 hd a position and kv head, where contexts are
+// long: 32 heads on 8, 128 wide, 6 streams of 40001 to 65535 positions take
+// 127 us, 5.1 TB/s. 64 streams of 601 to 1279 take 39 us (3.3 TB/s): starting
+// and joining blocks and uneven lengths. One of 217 takes 7.5 us, latency.
 constexpr int kAttendWarps = 4;
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -745,6 +755,8 @@ __device__ __forceinline__ float kv_value(const KvView& kv, int seq, int len, in
 }
 
 // A unit is 8 values of a pair of positions: the 16 codes that lie together.
+// Bound by codes in and values out; 6505 positions on 8 heads 128 wide as
+// bf16 take 10 us (4 TB/s of both), 64 short reads 8.5 us, latency.
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv_read(const __grid_constant__ KvView kv, const __grid_constant__ KvRuns runs,
                                                  int layer, void* k, void* v, int type, int vec) {
@@ -819,7 +831,8 @@ __global__ void __launch_bounds__(256) k_kv_read(const __grid_constant__ KvView 
   }
 }
 
-// Block (x, run): one (layer, keys or values, head) of the open page.
+// Block (x, run): one (layer, keys or values, head) of the open page. A fork
+// moves at most one page, so it is latency: 5 to 6 us.
 __global__ void __launch_bounds__(256) k_kv_fork(const __grid_constant__ KvView kv, const __grid_constant__ KvRuns runs,
                                                  int copy_table) {
   const KvRun& run = runs.run[blockIdx.y];
@@ -857,6 +870,8 @@ __global__ void k_kv_table(int* table, const __grid_constant__ KvEntries e) {
 }
 
 // ---------------------------------------------------------- page moves ----
+// Bound by bytes, each read and written once: 163 us for 0.5 GB of pages (6.6
+// TB/s of DRAM traffic both ways, what a plain copy reaches).
 __global__ void __launch_bounds__(256) k_kv_move(const __grid_constant__ KvView kv, const int* moves,
                                                  unsigned long long* remap, unsigned epoch) {
   const int src = moves[2 * blockIdx.y], dst = moves[2 * blockIdx.y + 1];
@@ -930,9 +945,10 @@ cudaError_t launch_kv_append(const KvView& kv, const KvRuns& runs, int layer, co
 // Positions are cut into shares of `c` steps a block, for one to four rounds
 // of blocks over the GPU: fewer rounds waste less on starting and joining,
 // more even out lengths that differ. A round costs its longest share and what
-// 48 steps do (measured, 32 heads on 8 and 128 wide: 64 streams of 601 to
-// 1279 positions take 54 us in shares of 64 steps, 57 whole, 65 in shares of
-// 20; 6 streams of 40001 to 65535 take 159 us in shares of 400, 186 of 96).
+// 48 steps do (measured while a copy still took half lines, which made all of
+// it slower than now; 32 heads on 8 and 128 wide: 64 streams of 601 to 1279
+// positions took 54 us in shares of 64 steps, 57 whole, 65 in shares of 20; 6
+// streams of 40001 to 65535 took 159 us in shares of 400, 186 of 96).
 KvAttendPlan plan_kv_attend(const KvView& kv, KvRuns& runs, const KvAttendArgs& a) {
   KvAttendPlan p;
   const int g = a.heads / kv.kv_heads, unit = a.type == kKvF32 ? 4 : 8;
