@@ -111,6 +111,29 @@ def test_odd_values():
         assert np.array_equal(gk, held(x, page)) and np.array_equal(gv, held(-x, page))
 
 
+def test_codes_beside_every_border():
+    """Pages whose values are the f16 numbers next to (n + 1/2) scale, at scales of many sizes: the code is the nearest,
+    exactly, wherever the page's scale puts the border."""
+    page, hd, pages = 16, 64, 200
+    rng = np.random.default_rng(3)
+    tops = np.concatenate([[65504.0, 127.0, 63.5, 1.0, 6e-8, 1.2e-7], np.exp(rng.uniform(np.log(1e-6), np.log(6e4), pages - 6))])
+    tops = tops.astype(np.float16).astype(np.float64)
+    scale = (tops / 127).astype(np.float32).astype(np.float64)
+    n = rng.integers(-127, 127, (pages, page * hd))
+    x = ((n + 0.5) * scale[:, None]).astype(np.float16)
+    step = rng.integers(-1, 2, x.shape)
+    x = np.where(step < 0, np.nextafter(x, np.float16(-np.inf)), np.where(step > 0, np.nextafter(x, np.float16(np.inf)), x))
+    x = np.clip(x.astype(np.float64), -tops[:, None], tops[:, None])
+    x[:, 0] = tops
+    x = x.astype(np.float32).reshape(pages * page, 1, hd)
+    with KvCache(kv_heads=1, pages=pages, head_dim=hd, page_tokens=page, sequences=1, max_tokens=pages * page) as kv:
+        s = kv.open(1)
+        d = torch.from_numpy(x).cuda()
+        fill(kv, 0, s, [(d, -d)])
+        gk, gv = contents(kv, 0, s[0], 1, hd)
+        assert np.array_equal(gk, held(x, page)) and np.array_equal(gv, held(-x, page))
+
+
 @pytest.mark.parametrize("kv_heads, group", [(1, 1), (2, 2), (1, 3), (2, 4), (1, 5), (1, 8), (1, 20)])
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_next_token(kv_heads, group, dtype):
