@@ -84,6 +84,10 @@ def peaks():
         return FALLBACK_HBM_GBS, "fallback"
 
 
+# Bytes of a cached value (the 8-bit cache's scales, 4 bytes a page and head, left out).
+KV_BYTES = {"f16": 2, "f32": 4, "q8": 1}
+
+
 def algorithmic_bytes(info: dict, streams: int, positions: list[int], kv_bytes: int) -> dict:
     """Bytes one greedy step must move: every weight once (products, norms,
     the output table), each stream's KV cache up to its position, and one
@@ -315,6 +319,8 @@ def measure(w: dict, args, r: dp.Rank, steps: int, warmup: int, decode: str, exa
     prompt_len = w["prompt"] + w.get("rows", 0)
     tc_attention = bool(getattr(args, "tc_attention", False))
     exact = exact and not tc_attention
+    if args.kv == "q8":
+        decode = "layered"  # the 8-bit cache decodes layered
     opts = {"device": r.local, "kv": args.kv, "max_context": prompt_len + w["new"] + 8, "exact": exact}
     tp = max(1, getattr(args, "tp", 1) or 1)
     group = r.rank // tp  # ranks of one tensor-parallel group serve the same streams
@@ -376,12 +382,12 @@ def measure(w: dict, args, r: dp.Rank, steps: int, warmup: int, decode: str, exa
     value = steps_all / (decode_max / 1e3)
     e2e = made_all / wall_max
     positions = [prompt_len + i for i in range(w["new"] - 1)]
-    alg = algorithmic_bytes(info, S, positions, 2 if args.kv == "f16" else 4)
+    alg = algorithmic_bytes(info, S, positions, KV_BYTES[args.kv])
     hbm, peak_kind = peaks()
     greedy_steps = decode_steps / S  # forwards of the whole batch
     per_step_s = decode_ms / 1e3 / max(1.0, greedy_steps)
     achieved = alg["total"] / per_step_s / 1e9 / tp  # per GPU: a group's ranks share the step's bytes
-    path = "tree-order sums" if not exact else "exact reference order"
+    path = "tree-order sums" if not exact else "exact reference order" if args.kv != "q8" else "8-bit cache"
     kernel = {"generate": f"decode step (persistent kernel, {path})" if decode == "persistent" else "layered step",
               "answer": f"decode step (persistent kernel, {path})" if decode == "persistent" else "layered step",
               "batch": "batched decode step (layered kernels, one CUDA graph)"}[w["kind"]]
@@ -392,7 +398,7 @@ def measure(w: dict, args, r: dp.Rank, steps: int, warmup: int, decode: str, exa
         "config": {"workload": w["workload"], "model": w["model"], "global_batch": S * r.world // tp,
                    "seq_len": prompt_len + w["new"], "parallelism": (f"dp{r.world} (independent streams, no collective)" if tp == 1 else
                                    f"tp{tp} x dp{r.world // tp} (NCCL all-reduce of o/down partials, argmax keys)"),
-                   "decode": decode if w["kind"] != "batch" else "batched", "exact": exact,
+                   "decode": decode if w["kind"] != "batch" else "batched", "exact": exact and args.kv != "q8",
                    "prompt_attention": "tensor cores (f16)" if tc_attention else "exact", "kv_cache": args.kv,
                    "l2": f"weights {alg['weights'] / 1e6:.0f} MB > 126 MB L2; no flush"},
         "e2e": {"value": e2e, "unit": "tok/s", "h2d_bytes_per_step": h2d, "d2h_bytes_per_step": S * w["new"] * 4},
@@ -593,7 +599,7 @@ def main() -> None:
     ap.add_argument("--tc-attention", action="store_true",
                     help="prompt attention on the tensor cores (f16 flash attention; not bit-exact)")
     ap.add_argument("--prefill-rows", type=int, help="rows a prompt pass (engine option)")
-    ap.add_argument("--kv", default="f16")
+    ap.add_argument("--kv", default="f16", choices=sorted(KV_BYTES))
     ap.add_argument("--tp", type=int, default=1,
                     help="tensor-parallel group size (ranks of a group split each layer; --gpus a multiple of it)")
     ap.add_argument("--reps", type=int, default=1000, help="repetitions per case of the op sweep")

@@ -93,7 +93,8 @@ void trit_cuda_free_text(char *text);
  *                   "q8" holds 8-bit codes with a scale a page and kv head
  *                   (see trit_cuda_kv_new), about half the memory and bytes
  *                   of "f16": logits drift (a value by about 1 %), decoding
- *                   runs layered, pages of 16, 32, 64 or 128 positions, at
+ *                   runs layered (slower than "f16" for one stream, faster
+ *                   for a batch), pages of 16, 32, 64 or 128 positions, at
  *                   most 16 prefixes at once
  *   "max_context":  positions per stream (4096)
  *   "max_streams":  stream slots for trit_lm_generate_batch (1)
