@@ -134,6 +134,9 @@ __device__ __forceinline__ void tile_weights(uint32_t s_col, uint32_t o_col, boo
     }
     const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
     if (__any_sync(0xffffffffu, most > m + kRaise)) {
+      // Stores to TMEM are asynchronous: the P of the blocks before, and O
+      // where one of them raised m too, are read back below.
+      tmem_wait_st();
       float alpha = 1.0f;
       if (most > m + kRaise) {
         const float to = floorf(most) - kBelow;
