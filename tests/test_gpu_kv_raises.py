@@ -77,3 +77,20 @@ def test_the_maximum_rises_in_every_block(dtype, causal, rise):
     rng = np.random.default_rng(3)
     sizes = rng.choice([1.0, 1.0, 1.0, 0.75, 0.5, -1.0, 0.0], m)
     check(rise * (np.arange(t) // 32), sizes, rng.standard_normal((t, HD)), dtype, 128, causal)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("top", [24.5, 25.0, 26.0, 28.0])
+def test_a_late_maximum_far_above(dtype, top):
+    """One step: low scores, many just below what raises the maximum, then one 18 to 21 powers of two above those. The
+    output is the many's share alone, 2e-4 and less, which one f16 factor between the two maxima cannot hold."""
+    t, m = 127, 256
+    key = np.zeros(t)
+    key[32:96] = 6.9
+    key[96] = top
+    v = np.zeros((t, HD))
+    v[:96] = 1.0
+    v[:, HD // 2:] *= np.linspace(0.5, 1.5, t)[:, None]
+    sizes = np.ones(m)
+    sizes[1::3] = 0.97
+    check(key, sizes, v, dtype, 128)

@@ -101,7 +101,8 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
 // its remainder: 16 columns of each in turn), `sum` of P over the value
 // scales. When a t passes m by kRaise (a vote of the warp: its rows share the
 // branch) m becomes a whole number near the largest, so that what is scaled by
-// the difference, the sum, O and this row's earlier P, keeps its bits.
+// the difference, the sum, O and this row's earlier P, keeps its bits (of P
+// those from 2^-32 of the new largest on, f16's last place).
 // Positions from `limit` on get no weight.
 template <int HD, bool MASK, bool LOW>
 __device__ __forceinline__ void tile_weights(uint32_t s_col, uint32_t o_col, bool scale_o, const float (*scales)[4],
@@ -146,7 +147,8 @@ __device__ __forceinline__ void tile_weights(uint32_t s_col, uint32_t o_col, boo
 #pragma unroll
       for (int i = 0; i < 2; ++i) part[i] = make_float2(part[i].x * alpha, part[i].y * alpha);
       carry *= alpha;
-      const __half2 alpha2 = __float2half2_rn(alpha);
+      // P is scaled in f32: alpha falls below f16 (2^-25 and less) where P
+      // times alpha need not.
 #pragma unroll 1
       for (int c = 0; c < (LOW ? 32 : 16) * b; c += 16) {
         uint32_t p[16];
@@ -154,8 +156,8 @@ __device__ __forceinline__ void tile_weights(uint32_t s_col, uint32_t o_col, boo
         tmem_wait_ld();
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          const __half2 h = __hmul2(*(const __half2*)&p[k], alpha2);
-          p[k] = *(const uint32_t*)&h;
+          const float2 f = __half22float2(*(const __half2*)&p[k]);
+          p[k] = pack_f16(f.x * alpha, f.y * alpha);
         }
         tmem_st16(s_col + c, p);
       }
