@@ -157,9 +157,9 @@ __global__ void __launch_bounds__(kQ4Threads, 2) k_q4(const __grid_constant__ DQ
       factor = round_f16(scale);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        // A value that is no number stays none.
-        const float c = v[i] * inv;
-        hi[i] = __float2half_rn(c == c ? (float)quantize_value(v[i], inv) : c);
+        // NaN stays NaN; a zero is code 0 although `inv` may be infinite (a
+        // largest value below 3.8e-37).
+        hi[i] = __float2half_rn(v[i] == v[i] ? (float)quantize_value(v[i], inv) : v[i]);
         lo[i] = __ushort_as_half(0);
       }
     } else {
