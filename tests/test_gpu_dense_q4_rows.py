@@ -45,3 +45,19 @@ def test_groups_of_tiny_values_and_zeros(rows, tiny):
     x[-1, 64:] = 0
     x[-1, 96:128:2] = tiny
     check(Dense.q4_0(blocks, n, k).forward(x), x, w)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_rows_that_are_not_numbers(rows):
+    """A row with NaN or an infinity gives no numbers, and changes no other."""
+    n, k = 64, 256
+    blocks, w = layer(n, k, 4)
+    x = np.random.default_rng(rows).standard_normal((rows, k)).astype(np.float32)
+    bad = {r: v for r, v in zip((0, rows // 2, rows - 1), (np.nan, np.inf, -np.nan))}
+    for i, (r, v) in enumerate(bad.items()):
+        x[r, 37 * i + 3] = v
+    got = Dense.q4_0(blocks, n, k).forward(x)
+    assert not np.isfinite(got[list(bad)]).any()
+    good = [r for r in range(rows) if r not in bad]
+    if good:
+        check(got[good], x[good], w)

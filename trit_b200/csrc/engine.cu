@@ -1992,7 +1992,8 @@ void DenseOp::forward_q4(const float* x, size_t m, float* y, cudaStream_t s) {
     rows_cap = m;
     TRIT_CUDA(make_tc_frame_map(&tc_x, xq, (m + 63) / 64 * 64, (size_t)mat.k));
   }
-  TRIT_CUDA(launch_norm_quant(x, (int)m, mat.k, nullptr, 0.0f, mat.agroup, mat.half, xq, xs, s));
+  // NaN stays NaN, as in the 4-bit kernel.
+  TRIT_CUDA(launch_norm_quant(x, (int)m, mat.k, nullptr, 0.0f, mat.agroup, mat.half, xq, xs, s, nullptr, true));
   TRIT_CUDA(launch_gemm_tc(tc_w, tc_x, mat, xs, (int)m, kEpOut, y, mat.n, 1.0f, tc_status, s));
 }
 

@@ -31,9 +31,10 @@ enum Epilogue : int { kEpOut = 0, kEpResid = 1, kEpSilu = 2 };
 cudaError_t launch_embed(const DTable& T, const int* ids, int m, float* x, float mult, cudaStream_t s);
 cudaError_t launch_scale(float* x, size_t n, float mult, cudaStream_t s);
 // RmsNorm (weights w; null: none) of m rows, times `scale` (null: none),
-// then the activation quantizer in groups of `group`.
+// then the activation quantizer in groups of `group`. keep_nan (rows as they
+// are only): NaN makes its group's scale NaN instead of a code 0.
 cudaError_t launch_norm_quant(const float* x, int m, int d, const float* w, float eps, int group, int half,
-                              int8_t* xq, float* xs, cudaStream_t s, const float* scale = nullptr);
+                              int8_t* xq, float* xs, cudaStream_t s, const float* scale = nullptr, bool keep_nan = false);
 cudaError_t launch_gemv(const DMat& W, const int8_t* xq, const float* xs, int m, int mode, float* y, int ldy,
                         float resid_mult, cudaStream_t s);
 cudaError_t launch_qk_rope_append(float* qkv, int m, const DConfig& cfg, const float* q_norm, const float* k_norm,

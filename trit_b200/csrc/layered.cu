@@ -1476,8 +1476,10 @@ cudaError_t launch_scale(float* x, size_t n, float mult, cudaStream_t s) {
 // Quantized::grouped of rows with no norm and no scale (the attention
 // output, h): the groups of a row are independent, so a row's groups spread
 // over `gridDim.y` blocks (a warp a group, as k_norm_quant quantizes them).
+// keep_nan: a group with a NaN gets scale NaN, so that its products are none
+// either (without, a NaN is code 0, the reference's rule).
 template <int G>
-__global__ void __launch_bounds__(256) k_quant_rows(const float* x, int d, int half, int8_t* xq, float* xs) {
+__global__ void __launch_bounds__(256) k_quant_rows(const float* x, int d, int half, int keep_nan, int8_t* xq, float* xs) {
   const int r = blockIdx.x, groups = d / G;
   const int per = (groups + gridDim.y - 1) / gridDim.y;
   const int g0 = blockIdx.y * per, g1 = min(groups, g0 + per);
@@ -1487,7 +1489,13 @@ __global__ void __launch_bounds__(256) k_quant_rows(const float* x, int d, int h
     float v[G / 32];
 #pragma unroll
     for (int i = 0; i < G / 32; ++i) v[i] = row[g * G + lane * (G / 32) + i];
-    const float scale = warp_quantize_group<G>(v, xq + (size_t)r * d + g * G, half);
+    float scale = warp_quantize_group<G>(v, xq + (size_t)r * d + g * G, half);
+    if (keep_nan) {
+      bool none = false;
+#pragma unroll
+      for (int i = 0; i < G / 32; ++i) none |= v[i] != v[i];
+      if (__any_sync(0xffffffffu, none)) scale = __int_as_float(0x7fffffff);
+    }
     if (lane == 0) xs[(size_t)r * groups + g] = scale;
   }
 }
@@ -1537,14 +1545,15 @@ cudaError_t launch_silu_quant(const float* g, int m, int units, int group, int h
 }
 
 cudaError_t launch_norm_quant(const float* x, int m, int d, const float* w, float eps, int group, int half,
-                              int8_t* xq, float* xs, cudaStream_t s, const float* scale) {
+                              int8_t* xq, float* xs, cudaStream_t s, const float* scale, bool keep_nan) {
   if (!w && !scale) {
     const int splits = free_quant_splits(m, d / group);
-    if (group == 32) k_quant_rows<32><<<dim3(m, splits), 256, 0, s>>>(x, d, half, xq, xs);
-    else k_quant_rows<128><<<dim3(m, splits), 256, 0, s>>>(x, d, half, xq, xs);
+    if (group == 32) k_quant_rows<32><<<dim3(m, splits), 256, 0, s>>>(x, d, half, keep_nan, xq, xs);
+    else k_quant_rows<128><<<dim3(m, splits), 256, 0, s>>>(x, d, half, keep_nan, xq, xs);
     LAUNCH_CHECK();
     return cudaSuccess;
   }
+  if (keep_nan) return cudaErrorInvalidValue;
   const int groups = d / group, splits = quant_splits(m, groups), per = (groups + splits - 1) / splits;
   const size_t row = (size_t)d * 4, wslice = w ? (size_t)per * group * 4 : 0;
   if (row > kNormSmem) return cudaErrorInvalidValue;           // d <= 12224
