@@ -24,7 +24,10 @@ namespace trit {
 constexpr int kQ8Prefixes = 16;
 
 void CudaCheck::ok(cudaError_t e, const char* what) {
-  if (e != cudaSuccess) throw Error(std::string("CUDA: ") + cudaGetErrorString(e) + " (" + what + ")");
+  if (e == cudaSuccess) return;
+  // Taken off the thread, or the next launch's check would find it there.
+  cudaGetLastError();
+  throw Error(std::string("CUDA: ") + cudaGetErrorString(e) + " (" + what + ")");
 }
 
 Options Options::parse(const char* text, bool lenient) {
