@@ -1963,6 +1963,36 @@ std::unique_ptr<DenseOp> dense_q4_0(const void* blocks, size_t n, size_t k, int 
   return op;
 }
 
+// The int8 copy of a 4-bit layer's weights, all of it or none.
+void DenseOp::make_wide() {
+  struct Buffers {
+    void *codes = nullptr, *scales = nullptr, *status = nullptr;
+    ~Buffers() {
+      for (void* b : {codes, scales, status})
+        if (b) cudaFree(b);
+    }
+  } b;
+  const size_t n = w4.n, k = w4.k;
+  TRIT_CUDA(cudaMalloc(&b.codes, n * k));
+  TRIT_CUDA(cudaMalloc(&b.scales, n * (k / 32) * 2));
+  TRIT_CUDA(cudaMalloc(&b.status, 4));
+  TRIT_CUDA(cudaMemsetAsync(b.status, 0, 4, stream));
+  TRIT_CUDA(launch_q4_expand(w4, (int8_t*)b.codes, b.scales, stream));
+  TRIT_CUDA(cudaStreamSynchronize(stream));
+  DMat wide = mat;
+  wide.kind = kQ8_0; wide.agroup = 32; wide.half = 1;
+  wide.codes = b.codes;
+  wide.scales = b.scales;
+  TcMap map{};
+  TRIT_CUDA(make_tc_weight_map(&map, wide, wide.codes));
+  mat = wide;
+  tc_w = map;
+  wide_codes = (int8_t*)b.codes;
+  wide_scales = b.scales;
+  tc_status = (int*)b.status;
+  b = Buffers{};
+}
+
 // Up to 16 rows the 4-bit kernel, which reads the weights once a pass. From
 // kWideRows rows of 8-bit activations on, the int8 tensor-core product of the
 // same codes and scales: its weights are expanded once and kept.
@@ -1973,19 +2003,7 @@ void DenseOp::forward_q4(const float* x, size_t m, float* y, cudaStream_t s) {
     TRIT_CUDA(launch_q4(w4, x, (int)m, !table, y, s));
     return;
   }
-  if (!wide_codes) {
-    const size_t n = w4.n, k = w4.k;
-    TRIT_CUDA(cudaMalloc(&wide_scales, n * (k / 32) * 2));
-    TRIT_CUDA(cudaMalloc(&tc_status, 4));
-    TRIT_CUDA(cudaMemset(tc_status, 0, 4));
-    TRIT_CUDA(cudaMalloc(&wide_codes, n * k));
-    TRIT_CUDA(launch_q4_expand(w4, wide_codes, wide_scales, stream));
-    TRIT_CUDA(cudaStreamSynchronize(stream));
-    mat.kind = kQ8_0; mat.agroup = 32; mat.half = 1;
-    mat.codes = wide_codes;
-    mat.scales = wide_scales;
-    TRIT_CUDA(make_tc_weight_map(&tc_w, mat, mat.codes));
-  }
+  if (!wide_codes) make_wide();
   if (m > rows_cap) {
     if (xq) TRIT_CUDA(cudaFree(xq));
     if (xs) TRIT_CUDA(cudaFree(xs));

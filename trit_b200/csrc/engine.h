@@ -316,6 +316,7 @@ struct DenseOp {
   int8_t* wide_codes = nullptr;
   void* wide_scales = nullptr;
   ~DenseOp();
+  void make_wide();
   void forward_q4(const float* x, size_t m, float* y, cudaStream_t s);
   void forward_device(const float* x, size_t m, float* y, cudaStream_t s);
 };
