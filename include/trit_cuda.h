@@ -306,14 +306,15 @@ TritDense *trit_dense_q8_0(const void *blocks, size_t n, size_t k, int table, in
  * d (c - 8)), kept in 4 bits on the GPU. k is a multiple of 32. table = 0:
  * rows of x are rounded to int8 codes in groups of 32 with f16-rounded
  * scales, as in a Q8_0 layer; table = 1: f32 rows as they are. A row with a
- * NaN gives NaN (a Q8_0 layer takes it for 0). Sums are f32,
- * in another order than a Q8_0 layer's. A call of more than 32 rows with
- * table = 0 (n a multiple of 32, k of 128) runs on the int8 tensor cores from
- * an int8 copy of the weights that the first such call makes (n x k bytes
- * more; not in a capture), and like a Q8_0 layer's calls they share scratch
- * memory: order them on one stream. The other calls use none: they may
- * overlap, and may be captured after the first. NULL on failure. (The reference expands Q4_0 tensors when it
- * loads them, src/cpu/ggml_quants.rs:1-6.) */
+ * NaN gives NaN (a Q8_0 layer takes it for 0). Sums are f32, in another order
+ * than a Q8_0 layer's. A call of more than 32 rows with table = 0 (n a
+ * multiple of 32, k of 128) runs on the int8 tensor cores from an int8 copy of
+ * the weights that the first such call makes (n x k bytes more; refused in a
+ * capture). Outside of a capture such calls share scratch memory, as a Q8_0
+ * layer's do: order them on one stream; a captured one's belongs to its graph.
+ * The other calls use none: they may overlap, and may be captured after the
+ * first. NULL on failure. (The reference expands Q4_0 tensors when it loads
+ * them, src/cpu/ggml_quants.rs:1-6.) */
 TritDense *trit_dense_q4_0(const void *blocks, size_t n, size_t k, int table, int device);
 
 /* out (rows x n) = x (rows x k) times the layer, both in host memory.

@@ -2003,19 +2003,41 @@ void DenseOp::forward_q4(const float* x, size_t m, float* y, cudaStream_t s) {
     TRIT_CUDA(launch_q4(w4, x, (int)m, !table, y, s));
     return;
   }
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  TRIT_CUDA(cudaStreamIsCapturing(s, &capture));
+  const bool capturing = capture != cudaStreamCaptureStatusNone;
+  if (!wide_codes && capturing)
+    throw Error("the stream is being captured, and the first call of more than 32 rows makes the layer's int8 copy");
   if (!wide_codes) make_wide();
-  if (m > rows_cap) {
+  const size_t frames = (m + 63) / 64 * 64, codes = frames * (size_t)mat.k, scales = m * (size_t)(mat.k / 32) * 4;
+  int8_t* q = xq;
+  float* qs = xs;
+  TcMap frame_map = tc_x;
+  if (capturing) {
+    // A captured call's scratch belongs to its graph: it outlives the layer's
+    // own, which a larger call replaces, and graphs may run at once.
+    TRIT_CUDA(cudaMallocAsync(&q, codes, s));
+    TRIT_CUDA(cudaMallocAsync(&qs, scales, s));
+    TRIT_CUDA(make_tc_frame_map(&frame_map, q, frames, (size_t)mat.k));
+  } else if (m > rows_cap) {
     if (xq) TRIT_CUDA(cudaFree(xq));
     if (xs) TRIT_CUDA(cudaFree(xs));
     xq = nullptr; xs = nullptr; rows_cap = 0;
-    TRIT_CUDA(cudaMalloc(&xq, (m + 63) / 64 * 64 * (size_t)mat.k));
-    TRIT_CUDA(cudaMalloc(&xs, m * (size_t)(mat.k / 32) * 4));
+    TRIT_CUDA(cudaMalloc(&xq, codes));
+    TRIT_CUDA(cudaMalloc(&xs, scales));
+    TRIT_CUDA(make_tc_frame_map(&tc_x, xq, frames, (size_t)mat.k));
     rows_cap = m;
-    TRIT_CUDA(make_tc_frame_map(&tc_x, xq, (m + 63) / 64 * 64, (size_t)mat.k));
+    q = xq;
+    qs = xs;
+    frame_map = tc_x;
   }
   // NaN stays NaN, as in the 4-bit kernel.
-  TRIT_CUDA(launch_norm_quant(x, (int)m, mat.k, nullptr, 0.0f, mat.agroup, mat.half, xq, xs, s, nullptr, true));
-  TRIT_CUDA(launch_gemm_tc(tc_w, tc_x, mat, xs, (int)m, kEpOut, y, mat.n, 1.0f, tc_status, s));
+  TRIT_CUDA(launch_norm_quant(x, (int)m, mat.k, nullptr, 0.0f, mat.agroup, mat.half, q, qs, s, nullptr, true));
+  TRIT_CUDA(launch_gemm_tc(tc_w, frame_map, mat, qs, (int)m, kEpOut, y, mat.n, 1.0f, tc_status, s));
+  if (capturing) {
+    TRIT_CUDA(cudaFreeAsync(q, s));
+    TRIT_CUDA(cudaFreeAsync(qs, s));
+  }
 }
 
 void DenseOp::forward_device(const float* x, size_t m, float* y, cudaStream_t s) {
