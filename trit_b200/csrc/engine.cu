@@ -1053,6 +1053,19 @@ void Lm::attention_q8(int layer, int m, int max_tk, const std::vector<std::pair<
   }
 }
 
+// The shares that a decode step of m rows cuts its positions into when the
+// longest row has max_tk of them.
+int Lm::q8_shares(int m, int max_tk) const {
+  KvAttendArgs a;
+  a.heads = cfg_.heads;
+  a.max_len = max_tk;
+  KvRuns r;
+  r.n = m;
+  r.row_seq = row_stream_;
+  r.row_pos = row_pos_;
+  return plan_kv_attend(kv8_->view(), r, a).splits;
+}
+
 // CausalLm::set_ffn_scales (causal_lm.rs:305-307): the normed MLP input of
 // layer l times scales[l] (hidden, :458-463); null clears them.
 void Lm::set_ffn_scales(const float* scales) {
@@ -1829,7 +1842,11 @@ void Lm::generate_batch(size_t S, const int* const* prompts, const size_t* lens,
     if (steps > 1 && clock_.on) {
       for (int i = 1; i < steps; ++i) step();  // per-kernel clocks: no graph
     } else if (steps > 1) {
-      if (!batch_graph_ || batch_graph_streams_ != (int)S || batch_graph_tmax_ < tmax) {
+      // Over the 8-bit cache the graph also holds how the attention shares out
+      // its positions, which decides the order of its sums: the call's own, not
+      // an earlier, longer call's.
+      const int shares = kv8_ ? q8_shares((int)S, tmax) : 0;
+      if (!batch_graph_ || batch_graph_streams_ != (int)S || batch_graph_tmax_ < tmax || batch_graph_shares_ != shares) {
         if (batch_graph_) cudaGraphExecDestroy(batch_graph_);
         batch_graph_ = nullptr;
         int counted = timing_.gpu_launches;
@@ -1849,6 +1866,7 @@ void Lm::generate_batch(size_t S, const int* const* prompts, const size_t* lens,
         timing_.gpu_launches = counted;  // captured, not run
         batch_graph_streams_ = (int)S;
         batch_graph_tmax_ = tmax;
+        batch_graph_shares_ = shares;
       }
       for (int i = 1; i < steps; ++i) TRIT_CUDA(cudaGraphLaunch(batch_graph_, stream_));
       timing_.gpu_launches += per_step * (steps - 1);

@@ -177,6 +177,7 @@ class Lm {
               const int* host_stream = nullptr, const int* host_pos = nullptr);
   void attention_q8(int layer, int m, int max_tk, const std::vector<std::pair<int, int>>* runs, const int* host_stream,
                     const int* host_pos);
+  int q8_shares(int m, int max_tk) const;
   void setup_tensor_cores();
   // The final norm, the output table and the best token of nb rows at x
   // (row stride ldx) into tokens; with tensor parallelism the ranks' best
@@ -266,7 +267,7 @@ class Lm {
   int* batch_tok_ = nullptr;    // device [max_new][streams]
   size_t batch_tok_cap_ = 0;
   cudaGraphExec_t batch_graph_ = nullptr;  // one captured greedy step
-  int batch_graph_streams_ = 0, batch_graph_tmax_ = 0;
+  int batch_graph_streams_ = 0, batch_graph_tmax_ = 0, batch_graph_shares_ = 0;
   // tensor-core products
   bool tc_ready_ = false;
   std::vector<TcMap> tc_w_;     // [layer][qkv, out, gate_up, down]
