@@ -303,11 +303,11 @@ TritDense *trit_dense_q8_0(const void *blocks, size_t n, size_t k, int table, in
 /* A layer from ggml Q4_0 blocks of an `n x k` row-major matrix (18 bytes a
  * block of 32 weights: an f16 scale d and 32 codes c of 4 bits, code i in the
  * low half of byte i and code 16 + i in its high half; the weight is
- * d (c - 8)), kept in 4 bits on the GPU. k is a multiple of 32. table = 0:
- * rows of x are rounded to int8 codes in groups of 32 with f16-rounded
- * scales, as in a Q8_0 layer; table = 1: f32 rows as they are. A row with a
- * NaN gives NaN (a Q8_0 layer takes it for 0). Sums are f32, in another order
- * than a Q8_0 layer's. A call of more than 32 rows with table = 0 (n a
+ * d (c - 8)), kept in 4 bits on the GPU. k is a multiple of 32; n and k are at
+ * most 2^31 - 16384. table = 0: rows of x are rounded to int8 codes in groups
+ * of 32 with f16-rounded scales, as in a Q8_0 layer; table = 1: f32 rows as
+ * they are. A row with a NaN gives NaN (a Q8_0 layer takes it for 0). Sums are
+ * f32, in another order than a Q8_0 layer's. A call of more than 32 rows with table = 0 (n a
  * multiple of 32, k of 128) runs on the int8 tensor cores from an int8 copy of
  * the weights that the first such call makes (n x k bytes more; refused in a
  * capture). Outside of a capture such calls share scratch memory, as a Q8_0

@@ -1953,7 +1953,10 @@ std::unique_ptr<DenseOp> dense_q8_0(const void* blocks, size_t n, size_t k, int 
 
 std::unique_ptr<DenseOp> dense_q4_0(const void* blocks, size_t n, size_t k, int device, bool table) {
   if (n == 0 || k == 0 || k % 32) throw Error("Q4_0 rows are whole blocks of 32");
-  if (n > INT32_MAX || k > INT32_MAX) throw Error("a layer has at most 2^31 - 1 rows and columns");
+  // Rows are counted in tiles of 16 and columns in segments of up to 8192, in
+  // 32 bits.
+  constexpr size_t kMost = (1u << 31) - 16384;
+  if (n > kMost || k > kMost) throw Error("a Q4_0 layer has at most 2^31 - 16384 rows and columns");
   auto op = std::make_unique<DenseOp>();
   op->device = device;
   op->table = table;
