@@ -10,7 +10,9 @@ namespace trit {
 namespace {
 
 constexpr float kF16Max = 65504.0f;
-constexpr float kMInit = -1e30f;  // "no key yet": finite, so that differences stay numbers
+// "No key yet": finite, so that differences are no NaN, and below every score
+// (the lowest f32).
+constexpr float kMInit = -3.4028234663852886e38f;
 
 __host__ __device__ __forceinline__ size_t kv_block(const KvView& kv, int page_or_seq, int layer, int which, int head) {
   return (((size_t)page_or_seq * kv.layers + layer) * 2 + which) * kv.kv_heads + head;
