@@ -380,7 +380,9 @@ void KvCache::attend(int layer, const int* ids, const int64_t* counts, size_t n,
       throw Error(std::to_string(counts[i]) + " causal rows for a sequence of " + std::to_string(p.len) + " positions");
     if (p.filled[layer] != p.len)
       throw Error("sequence " + std::to_string(ids[i]) + " has positions that were not appended yet");
-    total += counts[i];
+    // Rows without causal order are not bounded by the sequence: checked
+    // before they add up past 64 bits.
+    if (counts[i] > INT32_MAX || (total += counts[i]) > INT32_MAX) throw Error("more than 2^31 rows in a call");
   }
   if (total * (heads / opt_.kv_heads) > INT32_MAX) throw Error("more than 2^31 rows of heads in a call");
   if (!total) return;
