@@ -94,13 +94,19 @@ cudaError_t launch_kv_prompt(const KvView& kv, const KvRuns& runs, const KvAtten
 // Whether a run's rows are worth the kernel of many rows. It takes 128 or 256
 // query columns (a row of a head of the group) at the cost of one, the other
 // reads the positions again for every 4 to 16; but it starts late, so the call
-// has to bring enough columns over all kv heads as well. Measured, 32 heads on
-// 8, 128 wide, us for few / many: f32, 32 runs of 1000 positions, 32 columns
-// 87 / 104, 48 121 / 105; one run of 2000, 256 columns 38 / 43, 512 68 / 46;
-// bf16, 32 runs, 48 columns 72 / 80, 64 92 / 84; one run, 512 columns 38 / 56,
-// 1024 67 / 56.
+// has to bring enough columns over all kv heads as well. Measured on 32 heads
+// on 8, 40 on 8 and 8 on 8, 128 wide, and 16 on 4, 32 on 4 and 16 on 16, 64
+// wide, over 500 to 4000 positions; us for few / many:
+// - columns a run, 24 runs of 1500 positions: f32, 32 on 8, 48 columns 112 /
+//   132, 64 154 / 133; 16 on 4, 48 39 / 39, 64 43 / 39; 16 on 16, 64 142 / 147,
+//   80 174 / 147. bf16, 32 on 8, 64 87 / 96, 96 118 / 99; 16 on 4, 64 26 / 32,
+//   96 41 / 34; 16 on 16, 64 84 / 109, 96 119 / 112. The lengths move the
+//   border by a quarter either way.
+// - columns a call, one run: f32, 32 on 8, over 2000 positions 2048 37 / 43,
+//   4096 65 / 46; over 500 4096 30 / 35, 8192 48 / 35. bf16 over 2000 4096 37 /
+//   56, 8192 66 / 57; over 500 8192 31 / 39, 16384 49 / 46; over 6000 4096 85 / 74.
 inline bool kv_prompt_run(int64_t count, int group, int type, int64_t columns) {
-  return type == kKvF32 ? count * group >= 40 && columns >= 4096 : count * group >= 64 && columns >= 8192;
+  return type == kKvF32 ? count * group >= 64 && columns >= 4096 : count * group >= 96 && columns >= 8192;
 }
 // Positions first .. first + count of each run as values, rows of
 // [kv_heads][hd] from row0 on.
