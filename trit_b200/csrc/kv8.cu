@@ -216,8 +216,12 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const __grid_const
 //
 // The products are exact in f16 but for Q and P. A query is scaled by a
 // power of two into [1, 2) and, for f32 rows, split into two f16 columns
-// (value and remainder: 22 bits); P likewise. For f16 and bf16 rows P is one
-// f16 (2^-11, below the rounding of the output). Sums are f32.
+// (value and remainder: 22 bits); P likewise. f16 rows are f16 in one column,
+// and their P has its remainder in a second operand of the same columns (one
+// f16, 2^-11 of a weight, is as much as the output's own rounding: 24 streams
+// of up to 1500 positions were 2.9e-4 off instead of 2.0e-4, at 20.5 us instead
+// of 22.6). For bf16 rows P is one f16, an eighth of the output's rounding:
+// 1.7e-3 off with either. Sums are f32.
 //
 // Softmax: p = 2^(t - M) with t = log2(e) scale q.k + log2(value scale), so
 // the page's value scale rides in the exponent and the value product takes
@@ -257,8 +261,10 @@ __device__ __forceinline__ void copy16(void* smem, const void* global) {
                : "memory");
 }
 
-template <int HD, bool SPLIT, int NT>
+// TYPE (KvType): f32 rows split Q and P, f16 rows P.
+template <int HD, int TYPE, int NT>
 struct AttendShape {
+  static constexpr bool SPLIT = TYPE == kKvF32;
   static constexpr int UNIT = HD * 32;  // bytes of 16 positions' codes, or of their f16 keys (or values)
   static constexpr int STAGES = HD == 128 && NT == 1 ? 4 : 6;
   static constexpr int BLOCKS = HD == 128 && NT == 2 ? 2 : 3;  // an SM (registers)
@@ -267,11 +273,13 @@ struct AttendShape {
   static constexpr int SMEM = STAGE_BYTES + (SPLIT ? kAttendWarps * NT * HD / 8 * 32 * 4 : 0);
 };
 
-template <int HD, bool SPLIT, int NT>
-__global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, SPLIT, NT>::BLOCKS)
+template <int HD, int TYPE, int NT>
+__global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, TYPE, NT>::BLOCKS)
     k_kv_attend(const __grid_constant__ KvView kv, const __grid_constant__ KvRuns runs,
                 const __grid_constant__ KvAttendArgs a, int chunks, int splits, int vec, int vec_out, void* workspace) {
-  using Shape = AttendShape<HD, SPLIT, NT>;
+  using Shape = AttendShape<HD, TYPE, NT>;
+  constexpr bool SPLIT = Shape::SPLIT;
+  constexpr int PB = TYPE == kKvF16 ? 2 : 1;  // operands of P: with its remainder
   constexpr int CL = NT * (SPLIT ? 4 : 8);   // columns a block
   constexpr int LT = SPLIT ? 1 : 2;          // columns a thread holds in an n-tile
   constexpr int KB = HD / 64;                // 64-wide blocks of a key
@@ -470,7 +478,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, SPLIT, NT>:
   // Scores of two steps of 16 positions to P^T and the running sums. s[z][t]:
   // positions key0[z] + r and key0[z] + r + 8 of the thread's columns.
   auto softmax = [&](float (&s)[2][NT][4], const int (&key0)[2], const float (&ks)[2], const float (&lv)[2],
-                     const float (&iv)[2], uint32_t (&p)[2][NT][2]) {
+                     const float (&iv)[2], uint32_t (&p)[2][NT][PB][2]) {
     float x[2][NT][LT][2];
     bool raise = false;
 #pragma unroll
@@ -533,12 +541,16 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, SPLIT, NT>:
           } else {
             w = pack_f16(e[0][h], e[LT - 1][h]);
           }
-          p[z][t][h] = transpose8(w);
+          p[z][t][0][h] = transpose8(w);
+          if (PB == 2) {
+            const float2 hi = __half22float2(*(const __half2*)&w);
+            p[z][t][PB - 1][h] = transpose8(pack_f16(e[0][h] - hi.x, e[LT - 1][h] - hi.y));
+          }
         }
       }
   };
 
-  uint32_t p[2][NT][2];
+  uint32_t p[2][NT][PB][2];
   float s[2][NT][4];
   auto clear = [&]() {
 #pragma unroll
@@ -619,7 +631,9 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, SPLIT, NT>:
         for (int q = 0; q < 4; ++q) {
           const uint32_t a0 = codes_lo(w0[q]), a1 = codes_hi(w0[q]), a2 = codes_lo(w1[q]), a3 = codes_hi(w1[q]);
 #pragma unroll
-          for (int t = 0; t < NT; ++t) mma16816(o[t][4 * b + q], a0, a1, a2, a3, p[z][t][0], p[z][t][1]);
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int x = 0; x < PB; ++x) mma16816(o[t][4 * b + q], a0, a1, a2, a3, p[z][t][x][0], p[z][t][x][1]);
         }
       }
   }
@@ -644,8 +658,13 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, SPLIT, NT>:
           const int q = 2 * z + y;
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            if (keys) mma16816(s[0][t], w0[2 * y], w1[2 * y], w0[2 * y + 1], w1[2 * y + 1], qf[t][b][q][0], qf[t][b][q][1]);
-            else mma16816(o[t][4 * b + q], w0[2 * y], w0[2 * y + 1], w1[2 * y], w1[2 * y + 1], p[0][t][0], p[0][t][1]);
+            if (keys) {
+              mma16816(s[0][t], w0[2 * y], w1[2 * y], w0[2 * y + 1], w1[2 * y + 1], qf[t][b][q][0], qf[t][b][q][1]);
+            } else {
+#pragma unroll
+              for (int x = 0; x < PB; ++x)
+                mma16816(o[t][4 * b + q], w0[2 * y], w0[2 * y + 1], w1[2 * y], w1[2 * y + 1], p[0][t][x][0], p[0][t][x][1]);
+            }
           }
         }
       }
@@ -902,21 +921,31 @@ __global__ void k_kv_remap(int* table, const unsigned long long* remap, unsigned
   if ((unsigned)(to >> 32) == epoch) table[i] = (int)(unsigned)to;
 }
 
-template <int HD, bool SPLIT, int NT>
+template <int HD, int TYPE, int NT>
 cudaError_t attend(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& p, int vec,
                    int vec_out, void* ws, cudaStream_t s) {
-  constexpr int smem = AttendShape<HD, SPLIT, NT>::SMEM;
+  constexpr int smem = AttendShape<HD, TYPE, NT>::SMEM;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   static DeviceOnce once;
   e = once.run(dev, [] {
-    return cudaFuncSetAttribute(k_kv_attend<HD, SPLIT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    return cudaFuncSetAttribute(k_kv_attend<HD, TYPE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   });
   if (e != cudaSuccess) return e;
-  k_kv_attend<HD, SPLIT, NT>
+  k_kv_attend<HD, TYPE, NT>
       <<<dim3(p.blocks, kv.kv_heads), kAttendWarps * 32, smem, s>>>(kv, runs, a, p.chunks, p.splits, vec, vec_out, ws);
   return cudaGetLastError();
+}
+template <int TYPE>
+cudaError_t attend(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& p, int vec,
+                   int vec_out, void* ws, cudaStream_t s) {
+  const bool two = p.cols == (TYPE == kKvF32 ? 8 : 16);
+  if (kv.hd == 128)
+    return two ? attend<128, TYPE, 2>(kv, runs, a, p, vec, vec_out, ws, s)
+               : attend<128, TYPE, 1>(kv, runs, a, p, vec, vec_out, ws, s);
+  return two ? attend<64, TYPE, 2>(kv, runs, a, p, vec, vec_out, ws, s)
+             : attend<64, TYPE, 1>(kv, runs, a, p, vec, vec_out, ws, s);
 }
 
 }  // namespace
@@ -1030,13 +1059,9 @@ cudaError_t launch_kv_attend(const KvView& kv, const KvRuns& runs, const KvAtten
   const size_t size = a.type == kKvF32 ? 4 : 2;
   const int vec = ((uintptr_t)a.q | a.q_stride * size) % 16 == 0;
   const int vec_out = ((uintptr_t)a.out | a.out_stride * size) % 16 == 0;
-  const bool two = p.cols == (a.type == kKvF32 ? 8 : 16);
-  if (kv.hd == 128) {
-    if (a.type == kKvF32) return two ? attend<128, true, 2>(kv, runs, a, p, vec, vec_out, ws, s) : attend<128, true, 1>(kv, runs, a, p, vec, vec_out, ws, s);
-    return two ? attend<128, false, 2>(kv, runs, a, p, vec, vec_out, ws, s) : attend<128, false, 1>(kv, runs, a, p, vec, vec_out, ws, s);
-  }
-  if (a.type == kKvF32) return two ? attend<64, true, 2>(kv, runs, a, p, vec, vec_out, ws, s) : attend<64, true, 1>(kv, runs, a, p, vec, vec_out, ws, s);
-  return two ? attend<64, false, 2>(kv, runs, a, p, vec, vec_out, ws, s) : attend<64, false, 1>(kv, runs, a, p, vec, vec_out, ws, s);
+  if (a.type == kKvF32) return attend<kKvF32>(kv, runs, a, p, vec, vec_out, ws, s);
+  if (a.type == kKvF16) return attend<kKvF16>(kv, runs, a, p, vec, vec_out, ws, s);
+  return attend<kKvBF16>(kv, runs, a, p, vec, vec_out, ws, s);
 }
 
 cudaError_t launch_kv_read(const KvView& kv, const KvRuns& runs, int layer, void* k, void* v, int type, int max_count,

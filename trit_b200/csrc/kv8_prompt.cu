@@ -16,15 +16,17 @@
 //               one tile's run, the other's softmax does.
 //
 // f32 rows take two products each (Q and P as f16 value and remainder, 22
-// bits, summed in one accumulator), f16 and bf16 rows one (a row scaled by a
-// power of two; P rounded to 2^-11, below the output's rounding). Scales are
-// applied as in k_kv_attend: the key scale to S, the value scale in the
+// bits, summed in one accumulator), f16 rows two for P V only (they are f16
+// already), bf16 rows one (P rounded to 2^-11, an eighth of the output's
+// rounding); 16-bit rows are scaled by a power of two. Scales are applied as
+// in k_kv_attend: the key scale to S, the value scale in the
 // exponent of P. The floor is the tensor cores' 4 * 128 * 128 * hd operations
 // a tile and step, twice that for f32 rows. What bounds it is the softmax: one
 // thread a column takes about 5400 cycles a step's tile, the products of two
 // tiles 4100, and a step of two tiles about 8400. 4000 causal f32 rows, 32
-// heads on 8, 128 wide: 470 us, 279 TFLOP/s (558 as multiplied), the tensor
-// pipe busy 31 %; putting sums aside is 50 us of it.
+// heads on 8, 128 wide: 475 us, 276 TFLOP/s (552 as multiplied), the tensor
+// pipe busy 31 %; putting sums aside is 50 us of it. As f16 rows 342 us (275
+// without P's remainder), as bf16 rows 276 us, 475 TFLOP/s.
 #include <algorithm>
 
 #include "device.cuh"
@@ -38,9 +40,11 @@ namespace {
 constexpr int kTile = 128;  // query columns of a tile, and positions a step
 constexpr int kConvThreads = 128;
 
-// QT: query tiles a block. V is in one buffer where two do not fit.
-template <int HD, bool LOW, int QT>
+// QT: query tiles a block. V is in one buffer where two do not fit. TYPE
+// (KvType): f32 rows have remainders of Q and P, f16 rows of P.
+template <int HD, int TYPE, int QT>
 struct PromptShape {
+  static constexpr bool LOW = TYPE == kKvF32;
   static constexpr int TILE = kTile * HD * 2;  // bytes of an f16 tile
   static constexpr int BLOCKS = QT == 1 && !(LOW && HD == 128) ? 2 : 1;  // an SM
   static constexpr int KS = QT == 1 && HD == 128 ? 1 : 2, VS = (QT == 1 || LOW) && HD == 128 ? 1 : 2;
@@ -98,7 +102,7 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
 
 // A row's scores (128 TMEM columns from s_col) to P in their place, 32 at a
 // time: t = log2 of a weight over the value scale, P = 2^(t - m) as f16 (and
-// its remainder: 16 columns of each in turn), `sum` of P over the value
+// its remainder where LOW: 16 columns of each in turn), `sum` of P over the value
 // scales. When a t passes m by kRaise (a vote of the warp: its rows share the
 // branch) m becomes a whole number near the largest, so that what is scaled by
 // the difference, the sum, O and this row's earlier P, keeps its bits (of P
@@ -192,18 +196,19 @@ __device__ __forceinline__ void tile_weights(uint32_t s_col, uint32_t o_col, boo
   sum = make_float2(part[0].x + part[1].x, part[0].y + part[1].y);
 }
 
-template <int HD, bool LOW, int QT>
+template <int HD, int TYPE, int QT>
 constexpr int prompt_smem() {
-  using Shape = PromptShape<HD, LOW, QT>;
-  return 1024 + (QT * (LOW ? 2 : 1) + Shape::KS + Shape::VS) * Shape::TILE + (int)sizeof(PromptSmem);
+  using Shape = PromptShape<HD, TYPE, QT>;
+  return 1024 + (QT * (Shape::LOW ? 2 : 1) + Shape::KS + Shape::VS) * Shape::TILE + (int)sizeof(PromptSmem);
 }
 
-template <int HD, bool LOW, int QT>
-__global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape<HD, LOW, QT>::BLOCKS)
+template <int HD, int TYPE, int QT>
+__global__ void __launch_bounds__(PromptShape<HD, TYPE, QT>::THREADS, PromptShape<HD, TYPE, QT>::BLOCKS)
     k_kv_prompt(const __grid_constant__ KvView kv, const __grid_constant__ KvRuns runs,
                 const __grid_constant__ KvAttendArgs a, int vec, int vec_out, void* workspace, size_t aside_at,
                 int places, int* status) {
-  using Shape = PromptShape<HD, LOW, QT>;
+  using Shape = PromptShape<HD, TYPE, QT>;
+  constexpr bool LOW = Shape::LOW, LOWP = TYPE != kKvBF16;
   constexpr int TILE = Shape::TILE, KS = Shape::KS, VS = Shape::VS, QB = (LOW ? 2 : 1) * TILE;
   constexpr int COLS = QT * kTile;
   // Steps whose values are summed in one go: f32 rows add O up in the
@@ -423,9 +428,9 @@ __global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape
 #pragma unroll
         for (int i = 0; i < kTile / 16; ++i) {
           const uint64_t b = smem_desc_sw128_mn(v + i * 2048, kTile * 128);
-          const uint32_t p = tmem + t * kTile + (LOW ? 32 * (i >> 1) + 8 * (i & 1) : 8 * i);
+          const uint32_t p = tmem + t * kTile + (LOWP ? 32 * (i >> 1) + 8 * (i & 1) : 8 * i);
           mma_f16_ts(o, p, b, idesc_f16n(HD, true), (j % CHAIN > 0 || i > 0) ? 1u : 0u);
-          if (LOW) mma_f16_ts(o, p + 16, b, idesc_f16n(HD, true), 1u);
+          if (LOWP) mma_f16_ts(o, p + 16, b, idesc_f16n(HD, true), 1u);
         }
       };
       bool ok = mbar_wait(&S->qfull, 0, abort) && mbar_wait(&S->kfull[0], 0, abort);
@@ -571,8 +576,8 @@ __global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape
       }
       const bool mask = key0 + kTile > low_limit;
       const float(*scales)[4] = S->scales[j & 3];
-      if (mask) tile_weights<HD, true, LOW>(s_col, o_col, j % CHAIN > 0, scales, factor, key0, limit, m, l2, carry);
-      else tile_weights<HD, false, LOW>(s_col, o_col, j % CHAIN > 0, scales, factor, key0, limit, m, l2, carry);
+      if (mask) tile_weights<HD, true, LOWP>(s_col, o_col, j % CHAIN > 0, scales, factor, key0, limit, m, l2, carry);
+      else tile_weights<HD, false, LOWP>(s_col, o_col, j % CHAIN > 0, scales, factor, key0, limit, m, l2, carry);
       tmem_wait_st();
       fence_before();
       mbar_arrive(&S->pfull[t]);
@@ -641,28 +646,32 @@ __global__ void __launch_bounds__(PromptShape<HD, LOW, QT>::THREADS, PromptShape
   }
 }
 
-template <int HD, bool LOW, int QT>
+template <int HD, int TYPE, int QT>
 cudaError_t prompt(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& p, int vec,
                    int vec_out, void* ws, int* status, cudaStream_t s) {
-  constexpr int smem = prompt_smem<HD, LOW, QT>();
+  constexpr int smem = prompt_smem<HD, TYPE, QT>();
   static_assert(smem <= 227 * 1024, "the tiles fit in shared memory");
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   static DeviceOnce once;
   e = once.run(dev, [] {
-    return cudaFuncSetAttribute(k_kv_prompt<HD, LOW, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    return cudaFuncSetAttribute(k_kv_prompt<HD, TYPE, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   });
   if (e != cudaSuccess) return e;
-  k_kv_prompt<HD, LOW, QT><<<dim3(p.blocks, kv.kv_heads), PromptShape<HD, LOW, QT>::THREADS, smem, s>>>(
+  k_kv_prompt<HD, TYPE, QT><<<dim3(p.blocks, kv.kv_heads), PromptShape<HD, TYPE, QT>::THREADS, smem, s>>>(
       kv, runs, a, vec, vec_out, ws, p.aside, p.places, status);
   return cudaGetLastError();
 }
-template <int HD, bool LOW>
+template <int TYPE>
 cudaError_t prompt(const KvView& kv, const KvRuns& runs, const KvAttendArgs& a, const KvAttendPlan& p, int vec,
                    int vec_out, void* ws, int* status, cudaStream_t s) {
-  return p.cols == 2 * kTile ? prompt<HD, LOW, 2>(kv, runs, a, p, vec, vec_out, ws, status, s)
-                             : prompt<HD, LOW, 1>(kv, runs, a, p, vec, vec_out, ws, status, s);
+  const bool two = p.cols == 2 * kTile;
+  if (kv.hd == 128)
+    return two ? prompt<128, TYPE, 2>(kv, runs, a, p, vec, vec_out, ws, status, s)
+               : prompt<128, TYPE, 1>(kv, runs, a, p, vec, vec_out, ws, status, s);
+  return two ? prompt<64, TYPE, 2>(kv, runs, a, p, vec, vec_out, ws, status, s)
+             : prompt<64, TYPE, 1>(kv, runs, a, p, vec, vec_out, ws, status, s);
 }
 
 }  // namespace
@@ -734,12 +743,9 @@ cudaError_t launch_kv_prompt(const KvView& kv, const KvRuns& runs, const KvAtten
   if (runs.row_seq || (p.workspace && !ws)) return cudaErrorInvalidValue;
   const size_t size = a.type == kKvF32 ? 4 : 2;
   const int vec = ((uintptr_t)a.q | a.q_stride * size) % 16 == 0, vec_out = ((uintptr_t)a.out | a.out_stride * size) % 16 == 0;
-  const bool low = a.type == kKvF32;
-  if (kv.hd == 128)
-    return low ? prompt<128, true>(kv, runs, a, p, vec, vec_out, ws, status, s)
-               : prompt<128, false>(kv, runs, a, p, vec, vec_out, ws, status, s);
-  return low ? prompt<64, true>(kv, runs, a, p, vec, vec_out, ws, status, s)
-             : prompt<64, false>(kv, runs, a, p, vec, vec_out, ws, status, s);
+  if (a.type == kKvF32) return prompt<kKvF32>(kv, runs, a, p, vec, vec_out, ws, status, s);
+  if (a.type == kKvF16) return prompt<kKvF16>(kv, runs, a, p, vec, vec_out, ws, status, s);
+  return prompt<kKvBF16>(kv, runs, a, p, vec, vec_out, ws, status, s);
 }
 
 }  // namespace trit
