@@ -457,8 +457,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendShape<HD, TYPE, NT>::
   }
 
   // f32 rows: the tensor cores cut what they add to a sum short, so a sum
-  // loses up to 2^-24 of itself with every product; after kKvChain positions
-  // it is put aside in shared memory and begun anew.
+  // loses up to 2^-24 of itself with every product, 2^-25 on average; after
+  // kKvChain positions it is put aside in shared memory and begun anew.
   float* aside = (float*)(smem + Shape::STAGE_BYTES) + warp * (NT * HD / 8 * 32) + lane;
   auto put_aside = [&](bool add) {
 #pragma unroll
@@ -973,11 +973,12 @@ cudaError_t launch_kv_append(const KvView& kv, const KvRuns& runs, int layer, co
 //
 // Positions are cut into shares of `c` steps a block, for one to four rounds
 // of blocks over the GPU: fewer rounds waste less on starting and joining,
-// more even out lengths that differ. A round costs its longest share and what
-// 48 steps do (measured while a copy still took half lines, which made all of
-// it slower than now; 32 heads on 8 and 128 wide: 64 streams of 601 to 1279
-// positions took 54 us in shares of 64 steps, 57 whole, 65 in shares of 20; 6
-// streams of 40001 to 65535 took 159 us in shares of 400, 186 of 96).
+// more even out lengths that differ. A round costs its longest share and
+// kStart steps. Measured with kStart at 12 / 24 / 48 / 96, us: 64 streams of
+// 601 to 1279 positions, 32 heads on 8 and 128 wide, 45.5 / 40.4 / 40.5 / 40.6;
+// 6 of 40001 to 65535, bf16, 130 / 122 / 122 / 122; 24 of up to 1500, four rows
+// each, 16 on 16 and 64 wide, 20.8 / 18.2 / 18.2 / 18.2; 128 of 100 to 600, 16 on
+// 2 and 64 wide, 25.5 / 26.2 / 25.6 / 26.7.
 KvAttendPlan plan_kv_attend(const KvView& kv, KvRuns& runs, const KvAttendArgs& a) {
   KvAttendPlan p;
   const int g = a.heads / kv.kv_heads, unit = a.type == kKvF32 ? 4 : 8;

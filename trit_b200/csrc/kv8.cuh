@@ -136,8 +136,8 @@ __device__ __forceinline__ void halves8(uint4 h, float (&v)[8]) {
 
 constexpr float kRaise = 14.0f, kBelow = 7.0f;
 // Positions whose values f32 rows sum up on the tensor cores in one go: their
-// sums are cut short, not rounded, and lose about 2^-25 of themselves with
-// every product (60000 positions in one chain of k_kv_attend: 1.4e-5).
+// sums are cut short, not rounded, and lose up to 2^-24 of themselves with
+// every product, 2^-25 on average (60000 positions in one chain of k_kv_attend: 1.4e-5).
 constexpr int kKvChain = 256;
 constexpr float kZeroScaleLog2 = -31.0f;  // below every f16 page's scale (6e-8 / 127)
 
