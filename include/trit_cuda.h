@@ -423,7 +423,8 @@ int trit_cuda_kv_append(TritKv *kv, int32_t layer, const int32_t *seqs, const in
  * h / (heads / kv_heads). causal = 1: the rows stand at the sequence's last
  * counts[i] positions, each seeing the positions up to its own; causal = 0:
  * every row sees all positions (an encoder's states). Zeros where there is
- * none. `out` may be `q`, with the same stride. Returns 0, or -1. */
+ * none. Sums are f32; a weight of the softmax holds 22 bits, of bf16 rows 11. A
+ * query with a NaN gives NaN. `out` may be `q`, with the same stride. Returns 0, or -1. */
 int trit_cuda_kv_attend(TritKv *kv, int32_t layer, const int32_t *seqs, const int64_t *counts, size_t n, const void *q,
                         size_t q_stride, int32_t heads, int type, float scale, int causal, void *out,
                         size_t out_stride, void *stream);

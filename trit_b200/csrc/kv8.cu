@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const __grid_const
 //
 // Bound by the codes' bytes, 2 hd a position and kv head, where contexts are
 // long: 32 heads on 8, 128 wide, 6 streams of 40001 to 65535 positions take
-// 127 us, 5.1 TB/s. 64 streams of 601 to 1279 take 39 us (3.3 TB/s): starting
+// 129 us, 5.0 TB/s. 64 streams of 601 to 1279 take 39 us (3.3 TB/s): starting
 // and joining blocks and uneven lengths. One of 217 takes 7.5 us, latency.
 constexpr int kAttendWarps = 4;
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
