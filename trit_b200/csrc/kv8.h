@@ -198,6 +198,7 @@ class KvCache {
   void check_layer(int layer) const;
   // Orders stream s behind everything this cache queued on other streams.
   void enter(cudaStream_t s, const char* what, bool may_capture = false);
+  void refuse_capture(cudaStream_t s, const char* what);
   void leave(cudaStream_t s);
   void attend_runs(KvRuns& runs, KvAttendArgs& a, bool prompt, cudaStream_t s);
   void set_entries(const std::vector<std::pair<int, int>>& entries, cudaStream_t s);

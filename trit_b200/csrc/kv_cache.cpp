@@ -133,14 +133,26 @@ void KvCache::check_layer(int layer) const {
     throw Error("layer " + std::to_string(layer) + " of a cache of " + std::to_string(opt_.layers) + " layers");
 }
 
+namespace {
+bool is_capturing(cudaStream_t s) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  TRIT_CUDA(cudaStreamIsCapturing(s, &st));
+  return st != cudaStreamCaptureStatusNone;
+}
+}  // namespace
+
+void KvCache::refuse_capture(cudaStream_t s, const char* what) {
+  TRIT_CUDA(cudaSetDevice(opt_.device));
+  capturing_ = false;
+  if (is_capturing(s))
+    throw Error(std::string(what) + ": the stream is being captured, and a replay would write the same positions again");
+}
+
 void KvCache::enter(cudaStream_t s, const char* what, bool may_capture) {
   TRIT_CUDA(cudaSetDevice(opt_.device));
   if (take_failure()) throw Error("an attention call before this one gave up waiting for its pipeline");
-  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-  TRIT_CUDA(cudaStreamIsCapturing(s, &st));
-  capturing_ = st != cudaStreamCaptureStatusNone;
-  if (capturing_ && !may_capture)
-    throw Error(std::string(what) + ": the stream is being captured, and a replay would write the same positions again");
+  if (may_capture) capturing_ = is_capturing(s);
+  else refuse_capture(s, what);
   if (capturing_ || !used_) return;
   unsigned long long id = 0;
   TRIT_CUDA(cudaStreamGetId(s, &id));
@@ -271,6 +283,7 @@ void KvCache::release(const int* ids, size_t n) {
 void KvCache::extend(const int* ids, const int64_t* counts, size_t n, cudaStream_t s) {
   std::vector<char> seen(opt_.sequences, 0);
   size_t pages = 0;
+  bool grows = false;
   for (size_t i = 0; i < n; ++i) {
     const Seq& q = seq(ids[i]);
     if (seen[ids[i]]++) throw Error("sequence " + std::to_string(ids[i]) + " is named twice");
@@ -279,11 +292,13 @@ void KvCache::extend(const int* ids, const int64_t* counts, size_t n, cudaStream
       throw Error("sequence " + std::to_string(ids[i]) + ": " + std::to_string(q.len) + " + " + std::to_string(counts[i]) +
                   " positions exceed max_tokens " + std::to_string(opt_.max_tokens));
     pages += (q.len + counts[i]) / opt_.page - q.pages.size();
+    grows |= counts[i] > 0;
   }
   if (pages > free_pages_.size())
     throw Error(std::to_string(pages) + " pages asked, " + std::to_string(free_pages_.size()) + " of " +
                 std::to_string(opt_.pages) + " are free");
   if (pages) enter(s, "extend");
+  else if (grows) refuse_capture(s, "extend");
   std::vector<std::pair<int, int>> entries;
   for (size_t i = 0; i < n; ++i) {
     Seq& q = seqs_[ids[i]];
