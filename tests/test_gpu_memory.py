@@ -1,10 +1,8 @@
 """Calls after one that found no memory: nothing is lost, and the next call is
 not blamed for it."""
-import numpy as np
 import pytest
 
-from tests.test_gpu_dense_q4 import layer
-from trit_b200 import Dense, KvCache, TritError
+from trit_b200 import KvCache, TritError
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
