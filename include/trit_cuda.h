@@ -53,6 +53,7 @@ typedef struct TritLm TritLm;
 typedef struct TritLmPrefix TritLmPrefix;
 typedef struct TritDense TritDense;
 typedef struct TritKv TritKv;
+typedef struct TritRotary TritRotary;
 
 /* A tensor-parallel group's id (NCCL's unique id as 256 hex characters
  * and a NUL, into out of cap >= 257 bytes), made once on one rank and
@@ -317,6 +318,31 @@ TritDense *trit_dense_q8_0(const void *blocks, size_t n, size_t k, int table, in
  * them, src/cpu/ggml_quants.rs:1-6.) */
 TritDense *trit_dense_q4_0(const void *blocks, size_t n, size_t k, int table, int device);
 
+/* A layer of 8-bit floating point from an `n x k` row-major matrix of e4m3
+ * numbers (`codes`, a byte each: 1 sign, 4 exponent and 3 fraction bits, largest
+ * 448, no infinities) with an f32 scale for each block of 128 x 128 (`scales`,
+ * ceil(n / 128) x ceil(k / 128), row-major), both in host memory. A weight is
+ * code * scale. k is a multiple of 16 up to 2^24, n at most 2^31 - 256. Rows of
+ * x are 8-bit rows: e4m3 numbers with an f32 scale for each 128 of a row, which
+ * trit_cuda_rms_norm writes; rows of values are rounded to such first. Each
+ * block's products are summed on the tensor cores, the blocks in f32. Calls use
+ * no memory of the layer's but its weights, so they may overlap and be captured.
+ * NULL on failure. (No counterpart in the reference.) */
+TritDense *trit_dense_fp8(const void *codes, const float *scales, size_t n, size_t k, int device);
+
+/* out (rows x n) from 8-bit rows (`codes` rows x k bytes, 16-byte aligned, and
+ * `scales` rows x ceil(k / 128)), in device memory, for a layer of
+ * trit_dense_fp8. `type` is that of out: 0 for f32, 1 for f16, 2 for bf16;
+ * out_stride is in elements between rows (0: packed). Queued on `cuda_stream`
+ * (NULL: the default stream); does not wait. Returns 0, or -1. */
+int trit_dense_forward_codes(TritDense *layer, const void *codes, const float *scales, size_t rows, void *out,
+                             size_t out_stride, int type, void *cuda_stream);
+
+/* trit_dense_forward_codes of rows of values (of `type`, as out), which are
+ * rounded to 8-bit rows first, as trit_cuda_rms_norm rounds them. */
+int trit_dense_forward_rows(TritDense *layer, const void *x, size_t x_stride, size_t rows, void *out, size_t out_stride,
+                            int type, void *cuda_stream);
+
 /* out (rows x n) = x (rows x k) times the layer, both in host memory.
  * Returns 0, or -1. (Dense::forward, gemm.rs:500-542.) */
 int trit_dense_forward(TritDense *layer, const float *x, size_t rows, float *out);
@@ -444,6 +470,71 @@ int64_t trit_cuda_kv_length(const TritKv *kv, int32_t seq);
 
 /* Full pages in use and in all. Returns 0, or -1. */
 int trit_cuda_kv_pages(const TritKv *kv, int64_t *used, int64_t *total);
+
+/* ---- rows between the products and the cache ----
+ *
+ * For callers that run their own decoder beside trit_cuda_kv_* and layers of
+ * trit_dense_fp8. Device pointers throughout, all on one GPU, which is found
+ * from them; `type` is 0 for f32, 1 for f16, 2 for bf16; strides are elements
+ * between rows (0: packed); `cuda_stream` is a cudaStream_t of that GPU (NULL:
+ * the default stream). Calls queue their work there, do not wait, allocate
+ * nothing and keep nothing, so any of them may overlap and be captured. A
+ * call that fails on its arguments changes nothing. Two tensors of a call are
+ * the same (pointer and stride) or share no element. No counterpart in the
+ * reference, whose decoder does these steps inside CausalLm. */
+
+/* RMSNorm of rows of `width` values (up to 2^24), behind the residual's
+ * addition and in front of 8-bit rows:
+ *   h = x + residual, rounded to `type` and written to `sum` (NULL: to
+ *       `residual`); without a residual (NULL) h = x, and sum is NULL
+ *   s = f32(1 / sqrt(mean(h^2) + eps)), its sum in 64 bits
+ *   y = h * f32(s * weight), in f32 (a power of two goes from s to h first
+ *       where s is beyond 2^100 or 2^-100, so that s keeps its bits)
+ *   out (NULL: none) = y rounded to `type`; out may be x
+ *   codes, scales (NULL: none) = y as 8-bit rows: rows x width e4m3 numbers and
+ *       an f32 scale for each 128 of a row (rows x ceil(width / 128)),
+ *       scale = max(f32(max|y| / 448), 2^-126), 1 where all are zero,
+ *       code = e4m3(f32(y * f32(1 / scale))), ties to even
+ * A group of 128 with a NaN or an infinity has the scale NaN. `weight` is f32
+ * (weight_type 0) or of `type`. x and residual may be one tensor. Returns 0, or -1. (RmsNorm,
+ * src/layers.rs:128-153.) */
+int trit_cuda_rms_norm(const void *x, size_t x_stride, const void *residual, size_t residual_stride, void *sum,
+                       size_t sum_stride, const void *weight, int weight_type, size_t rows, size_t width, int type,
+                       double eps, void *out, size_t out_stride, void *codes, float *scales, void *cuda_stream);
+
+/* Rotary positions. `options_json` is an object: "head_dim" (needed; even, up
+ * to 512), "rotary_dim" (head_dim: how many of a head's first values turn;
+ * even), "layout" ("halves": pairs i, i + rotary_dim / 2; or "interleaved":
+ * pairs 2 i, 2 i + 1), "theta" (1e6), "scaling", and its settings. The
+ * frequency of pair i is f = theta^(-2 i / rotary_dim) radians a position, or
+ *   "linear":  f / factor
+ *   "ntk":     that of theta * factor^(d / (d - 2)), d = rotary_dim
+ *   "yarn":    between the pairs that turn `fast` (32) and `slow` (1) times
+ *              over `trained` positions, rounded outwards, a straight line from
+ *              f to f / factor; rotated values times 0.1 ln(factor) + 1
+ *   "bands":   f for wavelengths below trained / high (4), f / factor for those
+ *              above trained / low (1), a straight line over f between
+ * "frequencies" gives them instead (rotary_dim / 2 numbers), and
+ * "attention_factor" the factor of the rotated values. The handle holds no
+ * device memory and serves every GPU, also several threads at once. NULL on
+ * failure. (Rotary::halves, src/layers.rs:276-335.) */
+TritRotary *trit_cuda_rotary_new(const char *options_json);
+
+/* Frees a handle. NULL is a no-op. */
+void trit_cuda_rotary_free(TritRotary *rotary);
+
+/* The frequencies, at most `cap` of them into `out`, and the factor of the
+ * rotated values (NULL: not wanted). Returns their count, or -1. */
+int64_t trit_cuda_rotary_frequencies(const TritRotary *rotary, double *out, size_t cap, double *factor);
+
+/* Turns the pairs of q (rows x q_heads x head_dim) and k (rows x k_heads x
+ * head_dim; 0 heads and NULL: no such tensor) by position * frequency, which is
+ * formed in 64 bits (positions up to 2^53 either way; a negative one turns
+ * back). `positions` has one number a row. q_out and k_out: NULL for in place.
+ * Values of a head behind rotary_dim stay as they are. Returns 0, or -1. */
+int trit_cuda_rotary_apply(const TritRotary *rotary, const int64_t *positions, size_t rows, const void *q, size_t q_stride,
+                           int32_t q_heads, void *q_out, size_t q_out_stride, const void *k, size_t k_stride,
+                           int32_t k_heads, void *k_out, size_t k_out_stride, int type, void *cuda_stream);
 
 #ifdef __cplusplus
 }

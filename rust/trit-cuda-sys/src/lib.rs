@@ -41,6 +41,10 @@ pub mod ffi {
     pub struct TritKv {
         _p: [u8; 0],
     }
+    #[repr(C)]
+    pub struct TritRotary {
+        _p: [u8; 0],
+    }
 
     #[link(name = "trit_cuda")]
     extern "C" {
@@ -114,6 +118,16 @@ pub mod ffi {
             -> *mut TritDense;
         pub fn trit_dense_q4_0(blocks: *const c_void, n: usize, k: usize, table: c_int, device: c_int)
             -> *mut TritDense;
+        pub fn trit_dense_fp8(codes: *const c_void, scales: *const f32, n: usize, k: usize, device: c_int)
+            -> *mut TritDense;
+        pub fn trit_dense_forward_codes(
+            layer: *mut TritDense, codes: *const c_void, scales: *const f32, rows: usize, out: *mut c_void,
+            out_stride: usize, kind: c_int, cuda_stream: *mut c_void,
+        ) -> c_int;
+        pub fn trit_dense_forward_rows(
+            layer: *mut TritDense, x: *const c_void, x_stride: usize, rows: usize, out: *mut c_void,
+            out_stride: usize, kind: c_int, cuda_stream: *mut c_void,
+        ) -> c_int;
         pub fn trit_dense_forward(layer: *mut TritDense, x: *const f32, rows: usize, out: *mut f32) -> c_int;
         pub fn trit_dense_forward_device(
             layer: *mut TritDense, x: *const f32, rows: usize, out: *mut f32, cuda_stream: *mut c_void,
@@ -147,6 +161,22 @@ pub mod ffi {
         pub fn trit_cuda_kv_compact(kv: *mut TritKv, stream: *mut c_void) -> i64;
         pub fn trit_cuda_kv_length(kv: *const TritKv, seq: i32) -> i64;
         pub fn trit_cuda_kv_pages(kv: *const TritKv, used: *mut i64, total: *mut i64) -> c_int;
+        pub fn trit_cuda_rms_norm(
+            x: *const c_void, x_stride: usize, residual: *const c_void, residual_stride: usize, sum: *mut c_void,
+            sum_stride: usize, weight: *const c_void, weight_kind: c_int, rows: usize, width: usize, kind: c_int,
+            eps: f64, out: *mut c_void, out_stride: usize, codes: *mut c_void, scales: *mut f32,
+            cuda_stream: *mut c_void,
+        ) -> c_int;
+        pub fn trit_cuda_rotary_new(options_json: *const c_char) -> *mut TritRotary;
+        pub fn trit_cuda_rotary_free(rotary: *mut TritRotary);
+        pub fn trit_cuda_rotary_frequencies(
+            rotary: *const TritRotary, out: *mut f64, cap: usize, factor: *mut f64,
+        ) -> i64;
+        pub fn trit_cuda_rotary_apply(
+            rotary: *const TritRotary, positions: *const i64, rows: usize, q: *const c_void, q_stride: usize,
+            q_heads: i32, q_out: *mut c_void, q_out_stride: usize, k: *const c_void, k_stride: usize, k_heads: i32,
+            k_out: *mut c_void, k_out_stride: usize, kind: c_int, cuda_stream: *mut c_void,
+        ) -> c_int;
         pub fn trit_dense_free(layer: *mut TritDense);
         pub fn trit_dense_q8_0_forward_static(
             codes: *const c_void, scales: *const c_void, n: usize, k: usize, x: *const f32, rows: usize,

@@ -12,6 +12,7 @@
 #include "engine.h"
 #include "kv8.h"
 #include "nccl_link.h"
+#include "rows.h"
 
 struct TritLm {
   std::unique_ptr<trit::Lm> lm;
@@ -21,11 +22,15 @@ struct TritLmPrefix {
   const TritLm* owner = nullptr;
 };
 struct TritDense {
-  std::unique_ptr<trit::DenseOp> op;
+  std::unique_ptr<trit::DenseOp> op;     // Q8_0 and Q4_0 layers
+  std::unique_ptr<trit::DenseFp8> fp8;   // or this
   std::mutex mu;
 };
 struct TritKv {
   std::unique_ptr<trit::KvCache> kv;
+};
+struct TritRotary {
+  std::unique_ptr<trit::Rotary> rotary;
 };
 
 namespace {
@@ -60,6 +65,18 @@ int64_t copy_out(const std::vector<int>& toks, int32_t* out, size_t cap) {
   size_t n = std::min(cap, toks.size());
   for (size_t i = 0; i < n; ++i) out[i] = toks[i];
   return (int64_t)toks.size();
+}
+
+// A call that only layers of 8-bit floating point take.
+template <class F>
+int on_fp8(TritDense* layer, F body) {
+  return guard<int>(-1, [&]() {
+    need(layer, "layer");
+    if (!layer->fp8) throw trit::Error("the layer's weights are not 8-bit floating point (trit_dense_fp8)");
+    std::lock_guard<std::mutex> lock(layer->mu);
+    body(*layer->fp8);
+    return 0;
+  });
 }
 
 // A call on a cache: under its mutex, failures as everywhere.
@@ -362,12 +379,109 @@ TritDense* trit_dense_q4_0(const void* blocks, size_t n, size_t k, int table, in
   });
 }
 
+TritDense* trit_dense_fp8(const void* codes, const float* scales, size_t n, size_t k, int device) {
+  return guard<TritDense*>(nullptr, [&]() {
+    need(codes, "codes");
+    need(scales, "scales");
+    auto h = std::make_unique<TritDense>();
+    h->fp8 = std::make_unique<trit::DenseFp8>(codes, scales, n, k, device);
+    return h.release();
+  });
+}
+
+int trit_dense_forward_rows(TritDense* layer, const void* x, size_t x_stride, size_t rows, void* out, size_t out_stride,
+                            int type, void* cuda_stream) {
+  return on_fp8(layer, [&](trit::DenseFp8& d) {
+    d.forward_rows(x, x_stride, rows, out, out_stride, type, (cudaStream_t)cuda_stream);
+  });
+}
+
+int trit_dense_forward_codes(TritDense* layer, const void* codes, const float* scales, size_t rows, void* out,
+                             size_t out_stride, int type, void* cuda_stream) {
+  return on_fp8(layer, [&](trit::DenseFp8& d) {
+    d.forward_codes(codes, scales, rows, out, out_stride, type, (cudaStream_t)cuda_stream);
+  });
+}
+
+int trit_cuda_rms_norm(const void* x, size_t x_stride, const void* residual, size_t residual_stride, void* sum,
+                       size_t sum_stride, const void* weight, int weight_type, size_t rows, size_t width, int type,
+                       double eps, void* out, size_t out_stride, void* codes, float* scales, void* cuda_stream) {
+  return guard<int>(-1, [&]() {
+    if (weight_type != type && weight_type != trit::kRowF32) throw trit::Error("the weight's type is f32 or that of the rows");
+    trit::NormArgs a;
+    a.x = x;
+    a.residual = residual;
+    a.sum = sum;
+    a.weight = weight;
+    a.out = out;
+    a.codes = (uint8_t*)codes;
+    a.scales = scales;
+    a.x_stride = x_stride;
+    a.residual_stride = residual_stride;
+    a.sum_stride = sum_stride;
+    a.out_stride = out_stride;
+    a.type = type;
+    a.weight_f32 = weight_type == trit::kRowF32;
+    a.eps = eps;
+    trit::rms_norm(a, rows, width, (cudaStream_t)cuda_stream);
+    return 0;
+  });
+}
+
+TritRotary* trit_cuda_rotary_new(const char* options_json) {
+  return guard<TritRotary*>(nullptr, [&]() {
+    auto h = std::make_unique<TritRotary>();
+    h->rotary = trit::Rotary::parse(options_json);
+    return h.release();
+  });
+}
+
+void trit_cuda_rotary_free(TritRotary* rotary) { delete rotary; }
+
+int64_t trit_cuda_rotary_frequencies(const TritRotary* rotary, double* out, size_t cap, double* factor) {
+  return guard<int64_t>(-1, [&]() {
+    need(rotary, "rotary");
+    const auto& f = rotary->rotary->frequencies;
+    if (cap) need(out, "out");
+    for (size_t i = 0; i < std::min(cap, f.size()); ++i) out[i] = f[i];
+    if (factor) *factor = rotary->rotary->table.factor;
+    return (int64_t)f.size();
+  });
+}
+
+int trit_cuda_rotary_apply(const TritRotary* rotary, const int64_t* positions, size_t rows, const void* q, size_t q_stride,
+                           int32_t q_heads, void* q_out, size_t q_out_stride, const void* k, size_t k_stride,
+                           int32_t k_heads, void* k_out, size_t k_out_stride, int type, void* cuda_stream) {
+  return guard<int>(-1, [&]() {
+    need(rotary, "rotary");
+    trit::RotaryArgs a;
+    a.positions = positions;
+    a.q = q;
+    a.k = k;
+    a.q_out = q_out;
+    a.k_out = k_out;
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.q_out_stride = q_out_stride;
+    a.k_out_stride = k_out_stride;
+    a.q_heads = q_heads;
+    a.k_heads = k_heads;
+    a.type = type;
+    rotary->rotary->apply(a, rows, (cudaStream_t)cuda_stream);
+    return 0;
+  });
+}
+
 int trit_dense_forward(TritDense* layer, const float* x, size_t rows, float* out) {
   return guard<int>(-1, [&]() {
     need(layer, "layer");
     need(x, "x");
     need(out, "out");
     std::lock_guard<std::mutex> lock(layer->mu);
+    if (layer->fp8) {
+      layer->fp8->forward_host(x, rows, out);
+      return 0;
+    }
     trit::DenseOp& op = *layer->op;
     TRIT_CUDA(cudaSetDevice(op.device));
     size_t k = op.table ? op.tab.k : op.mat.k, n = op.table ? op.tab.n : op.mat.n;
@@ -396,6 +510,11 @@ int trit_dense_forward_device(TritDense* layer, const float* x, size_t rows, flo
     need(x, "x");
     need(out, "out");
     std::lock_guard<std::mutex> lock(layer->mu);
+    if (layer->fp8) {
+      trit::DenseFp8& d = *layer->fp8;
+      d.forward_rows(x, 0, rows, out, 0, trit::kRowF32, cuda_stream ? (cudaStream_t)cuda_stream : d.stream());
+      return 0;
+    }
     trit::DenseOp& op = *layer->op;
     TRIT_CUDA(cudaSetDevice(op.device));
     op.forward_device(x, rows, out, cuda_stream ? (cudaStream_t)cuda_stream : op.stream);

@@ -40,6 +40,7 @@
 
 #include "device.cuh"
 #include "kernels.h"
+#include "rows.h"
 #include "tc.cuh"
 
 namespace trit {
@@ -72,14 +73,6 @@ struct TcShape {
   static constexpr int CW = N / 2;                   // columns an epilogue warp folds
   static constexpr int CTAS = N == 64 ? 1 : 2;       // CTAs an SM holds (TMEM, shared memory)
 };
-
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
-      "[%2];" ::"r"(smem_u32(dst)),
-      "l"((uint64_t)map), "r"(smem_u32(bar)), "r"(x), "r"(y)
-      : "memory");
-}
 
 // Instruction descriptor of kind::i8: D s32 (bits 4-5 = 2), A and B s8
 // (bits 7-9, 10-12 = 1), both K-major, N >> 3 at bit 17, M >> 4 at bit 24.
@@ -767,6 +760,19 @@ cudaError_t make_tc_map(TcMap* out, const void* base, size_t rows, size_t k, int
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+cudaError_t make_fp8_map(TcMap* out, const void* base, size_t rows, size_t k, int box_rows) {
+  EncodeTiled enc = encoder();
+  if (!enc) return cudaErrorNotSupported;
+  if (!rows || !k || k % 16 || ((uintptr_t)base & 15) || box_rows % 8 || box_rows > 256) return cudaErrorInvalidValue;
+  cuuint64_t dims[2] = {k, rows};
+  cuuint64_t strides[1] = {k};
+  cuuint32_t box[2] = {TC_KT, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc((CUtensorMap*)out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box,
+                   estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
 cudaError_t make_tc_weight_map(TcMap* out, const DMat& W, const void* codes8) {
   return make_tc_map(out, codes8, (size_t)W.n, (size_t)W.k, TC_M);
 }

@@ -58,6 +58,15 @@ __device__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort) {
   }
 }
 
+// A box of a 2-D tensor map (in constant or parameter memory) to shared memory.
+__device__ __forceinline__ void tma_load_2d(void* dst, const void* map, uint64_t* bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"((uint64_t)map), "r"(smem_u32(bar)), "r"(x), "r"(y)
+      : "memory");
+}
+
 // Shared-memory matrix descriptor, K-major with the 128-byte swizzle: rows
 // of 128 bytes, 8-row groups 1024 bytes apart (SBO); the leading offset is
 // unused for this layout (encoded 1). `addr` may step through the 128-byte

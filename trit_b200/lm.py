@@ -103,6 +103,20 @@ def library() -> ctypes.CDLL:
         "trit_cuda_kv_compact": (ctypes.c_int64, [ctypes.c_void_p, ctypes.c_void_p]),
         "trit_cuda_kv_length": (ctypes.c_int64, [ctypes.c_void_p, ctypes.c_int32]),
         "trit_cuda_kv_pages": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+        "trit_dense_fp8": (ctypes.c_void_p, [ctypes.c_void_p, ctypes.c_void_p, _size, _size, ctypes.c_int]),
+        "trit_dense_forward_codes": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, _size,
+                                                    ctypes.c_void_p, _size, ctypes.c_int, ctypes.c_void_p]),
+        "trit_dense_forward_rows": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, _size, _size, ctypes.c_void_p, _size,
+                                                   ctypes.c_int, ctypes.c_void_p]),
+        "trit_cuda_rms_norm": (ctypes.c_int, [ctypes.c_void_p, _size, ctypes.c_void_p, _size, ctypes.c_void_p, _size,
+                                              ctypes.c_void_p, ctypes.c_int, _size, _size, ctypes.c_int, ctypes.c_double,
+                                              ctypes.c_void_p, _size, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+        "trit_cuda_rotary_new": (ctypes.c_void_p, [ctypes.c_char_p]),
+        "trit_cuda_rotary_free": (None, [ctypes.c_void_p]),
+        "trit_cuda_rotary_frequencies": (ctypes.c_int64, [ctypes.c_void_p, _f64p, _size, _f64p]),
+        "trit_cuda_rotary_apply": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, _size, ctypes.c_void_p, _size, ctypes.c_int32,
+                                                  ctypes.c_void_p, _size, ctypes.c_void_p, _size, ctypes.c_int32,
+                                                  ctypes.c_void_p, _size, ctypes.c_int, ctypes.c_void_p]),
         "trit_dense_forward": (ctypes.c_int, [ctypes.c_void_p, _f32p, _size, _f32p]),
         "trit_dense_forward_device": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, _size, ctypes.c_void_p,
                                                      ctypes.c_void_p]),
@@ -366,7 +380,8 @@ class CausalLm:
 
 
 class Dense:
-    """One product layer from ggml Q8_0 blocks (Dense, src/cpu/gemm.rs:14-24), or from Q4_0 blocks."""
+    """One product layer from ggml Q8_0 blocks (Dense, src/cpu/gemm.rs:14-24), from Q4_0 blocks, or of 8-bit
+    floating point with block scales."""
 
     def __init__(self, handle: int, n: int, k: int, table: bool):
         self._handle, self.n, self.k, self.table = handle, n, k, table
@@ -393,6 +408,21 @@ class Dense:
             raise _error()
         return cls(h, n, k, table)
 
+    @classmethod
+    def fp8(cls, codes: np.ndarray, scales: np.ndarray, n: int, k: int, device: int = 0) -> "Dense":
+        """A layer of e4m3 weights (codes: n x k bytes) with an f32 scale for each block of 128 x 128
+        (ceil(n / 128) x ceil(k / 128)) (trit_dense_fp8). Rows of x are e4m3 with a scale for each 128 of a row."""
+        b = np.ascontiguousarray(codes, dtype=np.uint8)
+        s = np.ascontiguousarray(scales, dtype=np.float32)
+        if b.size != n * k:
+            raise TritError(f"{b.size} bytes are not the numbers of a {n}x{k} matrix")
+        if s.size != (n + 127) // 128 * ((k + 127) // 128):
+            raise TritError(f"{s.size} scales are not those of the 128 x 128 blocks of a {n}x{k} matrix")
+        h = library().trit_dense_fp8(b.ctypes.data, s.ctypes.data, n, k, device)
+        if not h:
+            raise _error()
+        return cls(h, n, k, False)
+
     def forward(self, x: np.ndarray) -> np.ndarray:
         """Dense::forward (gemm.rs:500-506): rows x k -> rows x n."""
         xs = np.ascontiguousarray(x, dtype=np.float32).reshape(-1, self.k)
@@ -405,6 +435,20 @@ class Dense:
         if library().trit_dense_forward_device(self._handle, x_ptr, rows, out_ptr, stream) != 0:
             raise _error()
 
+    def forward_codes(self, codes_ptr: int, scales_ptr: int, rows: int, out_ptr: int, dtype: str = "f32", out_stride: int = 0,
+                      stream: int | None = None) -> None:
+        """out (rows x n of `dtype`) from 8-bit rows, as rms_norm writes them (layers of Dense.fp8). Device pointers;
+        `stream` is a cudaStream_t handle (None: the default stream)."""
+        if library().trit_dense_forward_codes(self._handle, codes_ptr, scales_ptr, rows, out_ptr, out_stride, _type(dtype),
+                                              stream) != 0:
+            raise _error()
+
+    def forward_rows(self, x_ptr: int, rows: int, out_ptr: int, dtype: str = "f32", x_stride: int = 0, out_stride: int = 0,
+                     stream: int | None = None) -> None:
+        """forward_codes of rows of `dtype`, rounded to 8-bit rows first."""
+        if library().trit_dense_forward_rows(self._handle, x_ptr, x_stride, rows, out_ptr, out_stride, _type(dtype), stream) != 0:
+            raise _error()
+
     def close(self) -> None:
         if getattr(self, "_handle", None):
             library().trit_dense_free(self._handle)
@@ -414,7 +458,69 @@ class Dense:
         self.close()
 
 
-_KV_TYPES = {"f32": 0, "f16": 1, "bf16": 2}
+_TYPES = {"f32": 0, "f16": 1, "bf16": 2}
+
+
+def _type(dtype: str) -> int:
+    if dtype not in _TYPES:
+        raise TritError(f"dtype {dtype!r} is not one of {', '.join(_TYPES)}")
+    return _TYPES[dtype]
+
+
+def rms_norm(x_ptr: int, weight_ptr: int, rows: int, width: int, out_ptr: int | None = None, codes_ptr: int | None = None,
+             scales_ptr: int | None = None, residual_ptr: int | None = None, sum_ptr: int | None = None, dtype: str = "f32",
+             weight_dtype: str = "f32", eps: float = 1e-6, x_stride: int = 0, residual_stride: int = 0, sum_stride: int = 0,
+             out_stride: int = 0, stream: int | None = None) -> None:
+    """RMSNorm of rows x width values of `dtype` (trit_cuda_rms_norm): h = x + residual goes to sum_ptr (None: to the
+    residual), its norm to out_ptr as values and to codes_ptr (e4m3 bytes) and scales_ptr (f32, one for each 128 of a
+    row) as 8-bit rows. Device pointers; `stream` is a cudaStream_t handle (None: the default stream)."""
+    if library().trit_cuda_rms_norm(x_ptr, x_stride, residual_ptr, residual_stride, sum_ptr, sum_stride, weight_ptr,
+                                    _type(weight_dtype), rows, width, _type(dtype), eps, out_ptr, out_stride, codes_ptr,
+                                    scales_ptr, stream) != 0:
+        raise _error()
+
+
+class Rotary:
+    """Rotary positions of queries and keys (trit_cuda_rotary_*, include/trit_cuda.h)."""
+
+    def __init__(self, head_dim: int, **options):
+        """Options are the keys of trit_cuda_rotary_new (rotary_dim, layout, theta, scaling and its settings,
+        frequencies, attention_factor); None stands for a key that is not given."""
+        self._handle = None
+        text = json.dumps({k: v for k, v in dict(options, head_dim=head_dim).items() if v is not None}).encode()
+        lib = library()
+        self._handle = lib.trit_cuda_rotary_new(text)
+        if not self._handle:
+            raise _error()
+        self._free = lib.trit_cuda_rotary_free
+
+    def close(self) -> None:
+        if getattr(self, "_handle", None):
+            self._free(self._handle)
+            self._handle = None
+
+    def __del__(self):
+        self.close()
+
+    def frequencies(self) -> tuple[list[float], float]:
+        """Radians a position of every pair, and the factor of the rotated values."""
+        lib, factor = library(), ctypes.c_double()
+        n = lib.trit_cuda_rotary_frequencies(self._handle, None, 0, ctypes.byref(factor))
+        if n < 0:
+            raise _error()
+        out = np.zeros(n, dtype=np.float64)
+        if lib.trit_cuda_rotary_frequencies(self._handle, _ptr(out, _f64p), n, None) < 0:
+            raise _error()
+        return out.tolist(), factor.value
+
+    def apply(self, positions_ptr: int, rows: int, q_ptr: int | None, q_heads: int, k_ptr: int | None = None, k_heads: int = 0,
+              dtype: str = "f32", q_stride: int = 0, k_stride: int = 0, q_out_ptr: int | None = None,
+              k_out_ptr: int | None = None, q_out_stride: int = 0, k_out_stride: int = 0, stream: int | None = None) -> None:
+        """Turns q (rows x q_heads x head_dim) and k by the rows' positions (64-bit integers), in place where no
+        output is given. Device pointers; strides in elements between rows (0: packed)."""
+        if library().trit_cuda_rotary_apply(self._handle, positions_ptr, rows, q_ptr, q_stride, q_heads, q_out_ptr, q_out_stride,
+                                            k_ptr, k_stride, k_heads, k_out_ptr, k_out_stride, _type(dtype), stream) != 0:
+            raise _error()
 
 
 def _words(values: Iterable[int], kind: str = "i", n: int | None = None) -> tuple[array, int]:
@@ -462,12 +568,6 @@ class KvCache:
     def __exit__(self, *exc):
         self.close()
 
-    @staticmethod
-    def _type(dtype: str) -> int:
-        if dtype not in _KV_TYPES:
-            raise TritError(f"dtype {dtype!r} is not one of {', '.join(_KV_TYPES)}")
-        return _KV_TYPES[dtype]
-
     def open(self, n: int = 1) -> list[int]:
         """n new sequences without positions."""
         out, to = _words(bytes(4 * max(n, 0)))
@@ -514,7 +614,7 @@ class KvCache:
         ids, at = _words(seqs)
         n, n_at = _words(counts, "q", len(ids))
         if library().trit_cuda_kv_append(self._handle, layer, at, n_at, len(ids), k_ptr, k_stride, v_ptr, v_stride,
-                                         self._type(dtype), stream) != 0:
+                                         _type(dtype), stream) != 0:
             raise _error()
 
     def attend(self, layer: int, seqs: Sequence[int], counts: Sequence[int], q_ptr: int, out_ptr: int, heads: int,
@@ -525,7 +625,7 @@ class KvCache:
         ids, at = _words(seqs)
         n, n_at = _words(counts, "q", len(ids))
         if library().trit_cuda_kv_attend(self._handle, layer, at, n_at, len(ids), q_ptr, q_stride, heads,
-                                         self._type(dtype), scale, 1 if causal else 0, out_ptr, out_stride,
+                                         _type(dtype), scale, 1 if causal else 0, out_ptr, out_stride,
                                          stream) != 0:
             raise _error()
 
@@ -536,7 +636,7 @@ class KvCache:
         ids, at = _words(seqs)
         f, f_at = _words(firsts, "q", len(ids))
         n, n_at = _words(counts, "q", len(ids))
-        if library().trit_cuda_kv_read(self._handle, layer, at, f_at, n_at, len(ids), k_ptr, v_ptr, self._type(dtype),
+        if library().trit_cuda_kv_read(self._handle, layer, at, f_at, n_at, len(ids), k_ptr, v_ptr, _type(dtype),
                                        stream) != 0:
             raise _error()
 
