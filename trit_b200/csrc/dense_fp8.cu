@@ -11,11 +11,8 @@
 //   warp 0     TMA producer: a stage is 128 values of k of the tile's rows of
 //              x and w, with the 128-byte swizzle;
 //   warp 1     issues four MMAs (K = 32) a stage into one of the TMEM buffers;
-//   warps 2..  epilogue: load a block's sums from TMEM, add them up, and write
+//   warps 4..  epilogue: load a block's sums from TMEM, add them up, and write
 //              the tile through shared memory in whole lines.
-// With CTAS = 2 a pair of blocks shares a tile of 256 rows: each holds its own
-// 128 rows of x and half of the tile's rows of w, and the first one's MMAs
-// (cta_group::2) read both, which halves what a block loads of w.
 // Every wait is bounded in time and reports through a status word.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -33,24 +30,29 @@ namespace {
 
 constexpr int F8_K = 128;  // values (bytes) of k a stage: one swizzle line, one scale block
 
-// CTAS blocks a tile; AR rows of x are loaded a block (the MMA's other rows
-// read what lies behind them, and nobody reads their sums); BN rows of w a tile.
-template <int CTAS, int AR, int BN>
+// AR rows of x are loaded (the MMA's other rows read what lies behind them,
+// and nobody reads their sums); BN rows of w a tile.
+template <int AR, int BN>
 struct F8Shape {
-  static constexpr int BR = BN / CTAS;  // rows of w a block loads
-  static constexpr int STAGE = (AR + BR) * F8_K;
+  static constexpr int STAGE = (AR + BN) * F8_K;
   static constexpr int COLUMN_WARPS = BN >= 128 ? 2 : 1;      // epilogue warps that share a tile's columns
   static constexpr int CW = BN / COLUMN_WARPS;                // columns of each
   static constexpr int ROW_WARPS = (AR + 31) / 32;            // of the four TMEM quarters, those with rows
-  static constexpr int THREADS = 64 + 128 * COLUMN_WARPS;
+  static constexpr int THREADS = 128 + 128 * COLUMN_WARPS;
   static constexpr int BUFS = BN >= 256 ? 2 : 4;
-  static constexpr int COLS = BUFS * BN < 32 ? 32 : BUFS * BN;  // of TMEM
+  static constexpr int COLS = BUFS * BN;                      // of TMEM
   static constexpr int STAGING = ROW_WARPS * COLUMN_WARPS * 4096;
   static constexpr int TAIL = (128 - AR) * F8_K > STAGING ? (128 - AR) * F8_K : STAGING;  // behind the stages
-  static constexpr int BLOCKS = CTAS == 2 || BN >= 128 ? 1 : 2;  // an SM holds
+  static constexpr int BLOCKS = BN >= 128 ? 1 : 2;            // an SM holds
   static constexpr int ROOM = (BLOCKS == 1 ? 226 : 113) * 1024 - 1024 - TAIL;
   static constexpr int STAGES = ROOM / STAGE < 12 ? ROOM / STAGE : 12;
   static constexpr int SMEM = 1024 + STAGES * STAGE + TAIL;
+  // 128 sums and two loads of 32 a thread do not fit the block's even share of
+  // the registers: the epilogue takes what the other roles do not need. The
+  // shares add up to the launch's 384 threads x 168.
+  static constexpr bool SPLIT = CW == 128;
+  static constexpr int REGS = 168, REGS_FEW = 72, REGS_MANY = 216;
+  static_assert(!SPLIT || (THREADS == 384 && 128 * REGS_FEW + 256 * REGS_MANY == THREADS * REGS), "register shares");
 };
 struct F8Sync {
   uint64_t full[12], empty[12], tfull[4], tempty[4], drain;
@@ -58,57 +60,27 @@ struct F8Sync {
   int abort;
 };
 
-template <int CTAS>
+// One lane of the warp, in a form that the compiler knows to be one: the
+// instructions behind it take uniform registers (0.30 -> 0.17 us a stage of
+// small MMAs against `lane == 0`).
+__device__ __forceinline__ bool elected() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
 __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  const uint32_t z = 0;
-  if constexpr (CTAS == 1)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d_tmem),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(z));
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}" ::"r"(d_tmem),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(z));
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
 }
 // Instruction descriptor of kind::f8f6f4: D f32 (bits 4-5 = 1), A and B e4m3
 // (bits 7-9, 10-12 = 0), both K-major, N >> 3 at bit 17, M >> 4 at bit 24.
 __host__ __device__ constexpr uint32_t idesc_f8(int m, int n) {
   return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-// The MMAs issued so far arrive at *bar once they are done; of a pair, at both
-// blocks' (the same place in each).
-template <int CTAS>
-__device__ __forceinline__ void commit_f8(uint64_t* bar) {
-  if constexpr (CTAS == 1)
-    mma_commit(bar);
-  else
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-                     smem_u32(bar)),
-                 "h"((uint16_t)3)
-                 : "memory");
-}
-// The address of the pair's first block's copy of a shared variable.
-__device__ __forceinline__ uint32_t first_of_pair(const void* p) {
-  uint32_t r;
-  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
-  return r;
-}
-// A copy whose bytes count at the first block's barrier.
-__device__ __forceinline__ void tma_load_pair(void* dst, const void* map, uint32_t bar, int x, int y) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], "
-      "[%2];" ::"r"(smem_u32(dst)),
-      "l"((uint64_t)map), "r"(bar), "r"(x), "r"(y)
-      : "memory");
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 // Tiles in groups of 8 row tiles, so that the tiles in work at a time share
 // their rows of x and w in L2.
 __device__ __forceinline__ void tile_place(long long t, int row_tiles, int col_tiles, int* r, int* c) {
@@ -207,19 +179,17 @@ __device__ __forceinline__ void store_tile(const float2 (&acc)[CW / 2], uint8_t*
   }
 }
 
-template <int CTAS, int AR, int BN>
-__global__ void __launch_bounds__(F8Shape<CTAS, AR, BN>::THREADS, F8Shape<CTAS, AR, BN>::BLOCKS)
+template <int AR, int BN>
+__global__ void __launch_bounds__(F8Shape<AR, BN>::THREADS, F8Shape<AR, BN>::BLOCKS)
     k_fp8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ Fp8Args a) {
-  using S = F8Shape<CTAS, AR, BN>;
+  using S = F8Shape<AR, BN>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ F8Sync sync;
   F8Sync* y = &sync;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = CTAS == 2 ? blockIdx.x & 1 : 0;
-  const int row_tiles = (a.m + CTAS * 128 - 1) / (CTAS * 128), col_tiles = (a.n + BN - 1) / BN;
+  const int row_tiles = (a.m + 127) / 128, col_tiles = (a.n + BN - 1) / BN;
   const long long tiles = (long long)row_tiles * col_tiles;
-  const long long first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
   volatile int* abort = &y->abort;
 
   if (threadIdx.x == 0) {
@@ -229,37 +199,30 @@ __global__ void __launch_bounds__(F8Shape<CTAS, AR, BN>::THREADS, F8Shape<CTAS, 
     }
     for (int i = 0; i < S::BUFS; ++i) {
       mbar_init(&y->tfull[i], 1);
-      mbar_init(&y->tempty[i], CTAS * S::ROW_WARPS * S::COLUMN_WARPS);
+      mbar_init(&y->tempty[i], S::ROW_WARPS * S::COLUMN_WARPS);
     }
     mbar_init(&y->drain, 1);
     y->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    if constexpr (CTAS == 1) {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&y->tmem)), "r"(S::COLS)
-                   : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    } else {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&y->tmem)), "r"(S::COLS)
-                   : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    }
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&y->tmem)), "r"(S::COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   fence_before();
   __syncthreads();
-  if constexpr (CTAS == 2) cluster_sync();
   fence_after();
   const uint32_t tmem = y->tmem;
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < 4) {
+    if constexpr (S::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::REGS_FEW));
+    if (warp == 0 && elected()) {
       uint32_t it = 0;
       bool ok = true;
-      for (long long t = first; t < tiles && ok; t += step) {
+      for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
         int r, c;
         tile_place(t, row_tiles, col_tiles, &r, &c);
-        const int m0 = (r * CTAS + rank) * 128, n0 = c * BN + rank * S::BR;
         for (int b = 0; b < a.blocks; ++b, ++it) {
           const uint32_t i = it % S::STAGES;
           if (!mbar_wait(&y->empty[i], ((it / S::STAGES) & 1) ^ 1, abort)) {
@@ -267,32 +230,24 @@ __global__ void __launch_bounds__(F8Shape<CTAS, AR, BN>::THREADS, F8Shape<CTAS, 
             break;
           }
           uint8_t* to = base + i * S::STAGE;
-          if constexpr (CTAS == 1) {
-            mbar_expect_tx(&y->full[i], S::STAGE);
-            tma_load_2d(to, &xmap, &y->full[i], b * F8_K, m0);
-            tma_load_2d(to + AR * F8_K, &wmap, &y->full[i], b * F8_K, n0);
-          } else {
-            // The pair's four copies count at the first block's barrier.
-            if (rank == 0) mbar_expect_tx(&y->full[i], 2 * S::STAGE);
-            const uint32_t bar = first_of_pair(&y->full[i]);
-            tma_load_pair(to, &xmap, bar, b * F8_K, m0);
-            tma_load_pair(to + AR * F8_K, &wmap, bar, b * F8_K, n0);
-          }
+          mbar_expect_tx(&y->full[i], S::STAGE);
+          tma_load_2d(to, &xmap, &y->full[i], b * F8_K, r * 128);
+          tma_load_2d(to + AR * F8_K, &wmap, &y->full[i], b * F8_K, c * BN);
         }
       }
       if (!ok) {
-        // Copies in flight wait for nothing: let them land before the block's memory is released.
-        const long long t0 = now_ns();
-        while (now_ns() - t0 < 20000000ll) {
+        // Let the copies in flight land before the block's memory is released.
+        for (uint32_t z = it > S::STAGES ? it - S::STAGES : 0; z < it; ++z) {
+          const long long t0 = now_ns();
+          while (!mbar_test(&y->full[z % S::STAGES], (z / S::STAGES) & 1) && now_ns() - t0 < TC_WAIT_NS) {
+          }
         }
       }
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    } else if (warp == 1 && elected()) {
       const uint32_t s0 = smem_u32(base);
       uint32_t it = 0;
       bool ok = true;
-      for (long long t = first; t < tiles && ok; t += step) {
+      for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
         for (int b = 0; b < a.blocks; ++b, ++it) {
           const uint32_t i = it % S::STAGES, u = it % S::BUFS;
           if (!mbar_wait(&y->tempty[u], ((it / S::BUFS) & 1) ^ 1, abort) ||
@@ -303,126 +258,116 @@ __global__ void __launch_bounds__(F8Shape<CTAS, AR, BN>::THREADS, F8Shape<CTAS, 
           fence_after();
 #pragma unroll
           for (int j = 0; j < F8_K / 32; ++j)
-            mma_f8<CTAS>(tmem + u * BN, smem_desc_sw128(s0 + i * S::STAGE + j * 32),
-                         smem_desc_sw128(s0 + i * S::STAGE + AR * F8_K + j * 32), idesc_f8(CTAS * 128, BN), j ? 1u : 0u);
-          commit_f8<CTAS>(&y->tfull[u]);
-          commit_f8<CTAS>(&y->empty[i]);
+            mma_f8(tmem + u * BN, smem_desc_sw128(s0 + i * S::STAGE + j * 32),
+                   smem_desc_sw128(s0 + i * S::STAGE + AR * F8_K + j * 32), idesc_f8(128, BN), j ? 1u : 0u);
+          mma_commit(&y->tfull[u]);
+          mma_commit(&y->empty[i]);
         }
       }
       // Every MMA issued has finished once `drain` completes.
-      commit_f8<CTAS>(&y->drain);
+      mma_commit(&y->drain);
       const long long t0 = now_ns();
       while (!mbar_test(&y->drain, 0) && now_ns() - t0 < TC_WAIT_NS) {
       }
     }
-  } else if ((warp & 3) < S::ROW_WARPS) {
-    const int quarter = warp & 3, part = (warp - 2) >> 2;
-    uint8_t* staging = base + S::STAGES * S::STAGE + (part * S::ROW_WARPS + quarter) * 4096;
-    const uint32_t tl = tmem + ((uint32_t)(quarter * 32) << 16) + part * S::CW;
-    const bool vec = a.blocks % 4 == 0 && ((uintptr_t)a.x_scales & 15) == 0;
-    uint32_t it = 0;
-    bool ok = true;
-    for (long long t = first; t < tiles && ok; t += step) {
-      int r, c;
-      tile_place(t, row_tiles, col_tiles, &r, &c);
-      const long long row0 = ((long long)r * CTAS + rank) * 128 + quarter * 32;
-      const int col0 = c * BN + part * S::CW;
-      const bool live = row0 + lane < a.m;
-      const float* sx = a.x_scales + (size_t)(live ? row0 + lane : 0) * a.blocks;
-      // Every 32 blocks a lane loads the scale of w of one of them. A tile's
-      // columns lie in one block of w; past n they read the last block's.
-      const float* sw = a.w_scales + (size_t)min(col0 / 128, (a.n - 1) / 128) * a.blocks;
-      float2 acc[S::CW / 2];
+  } else {
+    if constexpr (S::SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::REGS_MANY));
+    const int quarter = warp & 3, part = (warp - 4) >> 2;
+    if (quarter < S::ROW_WARPS) {
+      constexpr int LD = S::CW >= 64 ? 32 : 16;  // columns a load; the next ones are on the way while these are added
+      uint8_t* staging = base + S::STAGES * S::STAGE + (part * S::ROW_WARPS + quarter) * 4096;
+      const uint32_t tl = tmem + ((uint32_t)(quarter * 32) << 16) + part * S::CW;
+      const bool vec = a.blocks % 4 == 0 && ((uintptr_t)a.x_scales & 15) == 0;
+      uint32_t it = 0;
+      bool ok = true;
+      for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        int r, c;
+        tile_place(t, row_tiles, col_tiles, &r, &c);
+        const long long row0 = (long long)r * 128 + quarter * 32;
+        const int col0 = c * BN + part * S::CW;
+        const bool live = row0 + lane < a.m;
+        const float* sx = a.x_scales + (size_t)(live ? row0 + lane : 0) * a.blocks;
+        // Every 32 blocks a lane loads the scale of w of one of them. A warp's
+        // columns lie in one block of w; past n they read the last block's.
+        const float* sw = a.w_scales + (size_t)min(col0 / 128, (a.n - 1) / 128) * a.blocks;
+        float2 acc[S::CW / 2];
 #pragma unroll
-      for (int i = 0; i < S::CW / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
-      float4 next = scales4(sx, 0, a.blocks, live, vec);
-      float sws = 0.0f;
-      for (int b0 = 0; b0 < a.blocks && ok; b0 += 4) {
-        if ((b0 & 31) == 0) sws = b0 + lane < a.blocks ? __ldg(sw + b0 + lane) : 0.0f;
-        const float4 now = next;
-        next = scales4(sx, b0 + 4, a.blocks, live, vec);
+        for (int i = 0; i < S::CW / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
+        float4 next = scales4(sx, 0, a.blocks, live, vec);
+        float sws = 0.0f;
+        for (int b0 = 0; b0 < a.blocks && ok; b0 += 4) {
+          if ((b0 & 31) == 0) sws = b0 + lane < a.blocks ? __ldg(sw + b0 + lane) : 0.0f;
+          const float4 now = next;
+          next = scales4(sx, b0 + 4, a.blocks, live, vec);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (b0 + j >= a.blocks) break;
-          const float xj = j == 0 ? now.x : j == 1 ? now.y : j == 2 ? now.z : now.w;
-          const float scale = xj * __shfl_sync(0xffffffffu, sws, (b0 + j) & 31);
-          const float2 s2 = make_float2(scale, scale);
-          const uint32_t u = it % S::BUFS;
-          if (!__all_sync(0xffffffffu, mbar_wait(&y->tfull[u], (it / S::BUFS) & 1, abort))) {
-            ok = false;
-            break;
-          }
-          ++it;
-          fence_after();
-          const uint32_t from = tl + u * BN;
-          // 16 columns a load; the next ones are on the way while these are added.
-          uint32_t v[2][16];
-          tmem_ld<16>(from, v[0]);
-#pragma unroll
-          for (int q = 0; q < S::CW / 16; ++q) {
-            tmem_wait_ld();
-            if (q + 1 < S::CW / 16) {
-              tmem_ld<16>(from + (q + 1) * 16, v[(q + 1) & 1]);
-            } else {
-              fence_before();
-              if (lane == 0) {
-                if constexpr (CTAS == 1)
-                  mbar_arrive(&y->tempty[u]);
-                else
-                  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(first_of_pair(&y->tempty[u]))
-                               : "memory");
-              }
+          for (int j = 0; j < 4; ++j) {
+            if (b0 + j >= a.blocks) break;
+            const float xj = j == 0 ? now.x : j == 1 ? now.y : j == 2 ? now.z : now.w;
+            const float scale = xj * __shfl_sync(0xffffffffu, sws, (b0 + j) & 31);
+            const float2 s2 = make_float2(scale, scale);
+            const uint32_t u = it % S::BUFS;
+            if (!__all_sync(0xffffffffu, mbar_wait(&y->tfull[u], (it / S::BUFS) & 1, abort))) {
+              ok = false;
+              break;
             }
+            ++it;
+            fence_after();
+            const uint32_t from = tl + u * BN;
+            uint32_t v[2][LD];
+            tmem_ld<LD>(from, v[0]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              acc[q * 8 + i] = fma2(make_float2(__uint_as_float(v[q & 1][2 * i]), __uint_as_float(v[q & 1][2 * i + 1])), s2,
-                                    acc[q * 8 + i]);
+            for (int q = 0; q < S::CW / LD; ++q) {
+              tmem_wait_ld();
+              if (q + 1 < S::CW / LD) {
+                tmem_ld<LD>(from + (q + 1) * LD, v[(q + 1) & 1]);
+              } else {
+                fence_before();
+                if (lane == 0) mbar_arrive(&y->tempty[u]);
+              }
+#pragma unroll
+              for (int i = 0; i < LD / 2; ++i)
+                acc[q * (LD / 2) + i] = fma2(make_float2(__uint_as_float(v[q & 1][2 * i]), __uint_as_float(v[q & 1][2 * i + 1])),
+                                             s2, acc[q * (LD / 2) + i]);
+            }
           }
         }
+        if (ok && row0 < a.m) store_tile<S::CW>(acc, staging, a, row0, col0, lane);
       }
-      if (ok && row0 < a.m) store_tile<S::CW>(acc, staging, a, row0, col0, lane);
     }
   }
   fence_before();
   __syncthreads();
-  // A pair ends together: the first block's MMAs read the second's memory, and both arrive at its barriers.
-  if constexpr (CTAS == 2) cluster_sync();
   if (warp == 1) {
     fence_after();
-    if constexpr (CTAS == 1)
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
-    else
-      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
   }
   if (threadIdx.x == 0 && y->abort) *(volatile int*)a.status = 1;
 }
 
-template <int CTAS, int AR, int BN>
+template <int AR, int BN>
 cudaError_t run(const TcMap* w, const TcMap& x, const Fp8Args& a, cudaStream_t s) {
-  using S = F8Shape<CTAS, AR, BN>;
+  using S = F8Shape<AR, BN>;
   static_assert(S::STAGES >= 3 && S::STAGES <= 12 && S::SMEM + (int)sizeof(F8Sync) <= 227 * 1024, "shared memory");
-  static_assert(S::COLS * S::BLOCKS <= 512, "TMEM");
-  static_assert(S::CW <= 128 && S::CW % 16 == 0, "columns of an epilogue warp");
+  static_assert(S::COLS * S::BLOCKS <= 512 && (S::COLS & (S::COLS - 1)) == 0, "TMEM");
+  static_assert(S::CW <= 128 && S::CW % 32 == 0, "columns of an epilogue warp");
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   static DeviceOnce once;
-  e = once.run(dev, [] { return cudaFuncSetAttribute(k_fp8<CTAS, AR, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); });
+  e = once.run(dev, [] {
+    cudaFuncAttributes f;
+    cudaError_t r = cudaFuncGetAttributes(&f, k_fp8<AR, BN>);
+    // A launch with fewer registers than the shares add up to would wait for them without end.
+    if (r == cudaSuccess && S::SPLIT && f.numRegs != S::REGS) r = cudaErrorInvalidKernelImage;
+    if (r != cudaSuccess) return r;
+    return cudaFuncSetAttribute(k_fp8<AR, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+  });
   if (e != cudaSuccess) return e;
-  const long long rows = (a.m + CTAS * 128 - 1LL) / (CTAS * 128), tiles = rows * ((a.n + BN - 1) / BN);
-  const int teams = current_sm_count() * S::BLOCKS / CTAS;
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3((unsigned)std::min<long long>(tiles, teams) * CTAS);
-  config.blockDim = dim3(S::THREADS);
-  config.dynamicSmemBytes = S::SMEM;
-  config.stream = s;
-  cudaLaunchAttribute cluster{};
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim = {CTAS, 1, 1};
-  config.attrs = &cluster;
-  config.numAttrs = 1;
-  constexpr int box = S::BR == 32 ? 0 : S::BR == 64 ? 1 : S::BR == 128 ? 2 : 3;
-  return cudaLaunchKernelEx(&config, k_fp8<CTAS, AR, BN>, *(const CUtensorMap*)&x, *(const CUtensorMap*)&w[box], a);
+  const long long tiles = (a.m + 127LL) / 128 * ((a.n + BN - 1) / BN);
+  const int grid = (int)std::min<long long>(tiles, current_sm_count() * S::BLOCKS);
+  constexpr int box = BN == 32 ? 0 : BN == 64 ? 1 : BN == 128 ? 2 : 3;
+  k_fp8<AR, BN><<<grid, S::THREADS, S::SMEM, s>>>(*(const CUtensorMap*)&x, *(const CUtensorMap*)&w[box], a);
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -433,12 +378,12 @@ int fp8_row_box(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128
 cudaError_t launch_fp8(const TcMap* w, const TcMap& x, const Fp8Args& a, cudaStream_t s) {
   if (a.m <= 0) return cudaSuccess;
   switch (fp8_row_box(a.m)) {
-    case 16: return run<1, 16, 32>(w, x, a, s);
-    case 32: return run<1, 32, 32>(w, x, a, s);
-    case 64: return run<1, 64, 64>(w, x, a, s);
+    case 16: return run<16, 32>(w, x, a, s);
+    case 32: return run<32, 32>(w, x, a, s);
+    case 64: return run<64, 64>(w, x, a, s);
   }
-  if (a.m <= 512) return run<1, 128, 128>(w, x, a, s);
-  return run<2, 128, 256>(w, x, a, s);
+  if (a.m <= 512) return run<128, 128>(w, x, a, s);
+  return run<128, 256>(w, x, a, s);
 }
 
 }  // namespace trit
