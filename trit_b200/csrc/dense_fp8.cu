@@ -8,8 +8,10 @@
 // Rows of x are the MMA's M (a TMEM lane each), so a thread's scale of x is one
 // register a block and that of w the same for all its columns: one packed
 // multiply-add for two sums. Warp roles:
-//   warp 0     TMA producer: a stage is 128 values of k of the tile's rows of
-//              x and w, with the 128-byte swizzle;
+//   warp 0     producer: a stage is 128 values of k of the tile's rows of x (a
+//              tensor copy) and w (bulk copies: w is kept in units of 64 rows x
+//              128 values as the MMA reads them, a unit's next ones behind it,
+//              so that a tile of w is one run of memory);
 //   warp 1     issues four MMAs (K = 32) a stage into one of the TMEM buffers;
 //   warps 4..  epilogue: load a block's sums from TMEM, add them up, and write
 //              the tile through shared memory in whole lines.
@@ -29,29 +31,31 @@ namespace trit {
 namespace {
 
 constexpr int F8_K = 128;  // values (bytes) of k a stage: one swizzle line, one scale block
+constexpr int F8_UNIT = 64, F8_UNIT_BYTES = F8_UNIT * F8_K;  // rows of a unit of w
 
 // AR rows of x are loaded (the MMA's other rows read what lies behind them,
 // and nobody reads their sums); BN rows of w a tile.
-template <int AR, int BN>
+template <int AR, int BN, int BLOCKS_>
 struct F8Shape {
   static constexpr int STAGE = (AR + BN) * F8_K;
   static constexpr int COLUMN_WARPS = BN >= 128 ? 2 : 1;      // epilogue warps that share a tile's columns
   static constexpr int CW = BN / COLUMN_WARPS;                // columns of each
   static constexpr int ROW_WARPS = (AR + 31) / 32;            // of the four TMEM quarters, those with rows
   static constexpr int THREADS = 128 + 128 * COLUMN_WARPS;
-  static constexpr int BUFS = BN >= 256 ? 2 : 4;
+  static constexpr int BUFS = BN * 4 * BLOCKS_ > 512 ? 2 : 4;
   static constexpr int COLS = BUFS * BN;                      // of TMEM
   static constexpr int STAGING = ROW_WARPS * COLUMN_WARPS * 4096;
   static constexpr int TAIL = (128 - AR) * F8_K > STAGING ? (128 - AR) * F8_K : STAGING;  // behind the stages
-  static constexpr int BLOCKS = BN >= 128 ? 1 : 2;            // an SM holds
-  static constexpr int ROOM = (BLOCKS == 1 ? 226 : 113) * 1024 - 1024 - TAIL;
+  static constexpr int BLOCKS = BLOCKS_;                      // an SM holds
+  static constexpr int ROOM = 226 * 1024 / BLOCKS - 2048 - 1024 - TAIL;  // (a block's own 1 KB, and its static memory)
   static constexpr int STAGES = ROOM / STAGE < 12 ? ROOM / STAGE : 12;
   static constexpr int SMEM = 1024 + STAGES * STAGE + TAIL;
   // 128 sums and two loads of 32 a thread do not fit the block's even share of
   // the registers: the epilogue takes what the other roles do not need. The
   // shares add up to the launch's 384 threads x 168.
+  static constexpr bool SPLITS = BN < 256;  // k may be split over a cluster
   static constexpr bool SPLIT = CW == 128;
-  static constexpr int REGS = 168, REGS_FEW = 72, REGS_MANY = 216;
+  static constexpr int REGS = 168, REGS_FEW = 56, REGS_MANY = 224;
   static_assert(!SPLIT || (THREADS == 384 && 128 * REGS_FEW + 256 * REGS_MANY == THREADS * REGS), "register shares");
 };
 struct F8Sync {
@@ -81,12 +85,17 @@ __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a, uint64_t b, 
 __host__ __device__ constexpr uint32_t idesc_f8(int m, int n) {
   return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
+// `bytes` consecutive bytes to shared memory.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
 // Tiles in groups of 8 row tiles, so that the tiles in work at a time share
 // their rows of x and w in L2.
-__device__ __forceinline__ void tile_place(long long t, int row_tiles, int col_tiles, int* r, int* c) {
-  const long long group = t / (8LL * col_tiles);
-  const int rows = min(8LL, row_tiles - group * 8);
-  const long long at = t - group * 8 * col_tiles;
+__device__ __forceinline__ void tile_place(uint32_t t, uint32_t row_tiles, uint32_t col_tiles, int* r, int* c) {
+  const uint32_t group = t / (8 * col_tiles), rows = min(8u, row_tiles - group * 8), at = t - group * 8 * col_tiles;
   *r = (int)(group * 8 + at % rows);
   *c = (int)(at / rows);
 }
@@ -115,9 +124,9 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, bool f16) {
 // A warp's 32 rows (a lane each) x CW columns to out, through 4 KB of shared
 // memory of its own: 16-byte unit u of row r lies at u ^ (r % 8).
 template <int CW>
-__device__ __forceinline__ void store_tile(const float2 (&acc)[CW / 2], uint8_t* staging, const Fp8Args& a, long long row0,
+__device__ __forceinline__ void store_tile(const float2 (&acc)[CW / 2], uint8_t* staging, const Fp8Args& a, int row0,
                                            int col0, int lane) {
-  const int rows = (int)min(32LL, a.m - row0);
+  const int rows = min(32, a.m - row0);
   const bool f32 = a.type == kRowF32, f16 = a.type == kRowF16;
   const int size = f32 ? 4 : 2;
   const bool vec = (((uintptr_t)a.out | a.out_stride * size) & 15) == 0;
@@ -127,6 +136,7 @@ __device__ __forceinline__ void store_tile(const float2 (&acc)[CW / 2], uint8_t*
     __syncwarp();
     if (vec) {
       const int u = lane % units, per = 32 / units, values = 16 / size;
+#pragma unroll 4
       for (int r = lane / units; r < rows; r += per) {
         const uint4 v = *(const uint4*)(staging + r * 128 + ((u ^ (r & 7)) << 4));
         const int at = col + u * values;
@@ -144,6 +154,7 @@ __device__ __forceinline__ void store_tile(const float2 (&acc)[CW / 2], uint8_t*
       }
     } else {
       const int values = units * 16 / size;
+#pragma unroll 8
       for (int r = 0; r < rows; ++r) {
         for (int i = lane; i < values && col + i < a.n; i += 32) {
           const uint8_t* from = staging + r * 128 + (((i * size >> 4) ^ (r & 7)) << 4) + (i * size & 15);
@@ -179,17 +190,89 @@ __device__ __forceinline__ void store_tile(const float2 (&acc)[CW / 2], uint8_t*
   }
 }
 
-template <int AR, int BN>
-__global__ void __launch_bounds__(F8Shape<AR, BN>::THREADS, F8Shape<AR, BN>::BLOCKS)
-    k_fp8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ Fp8Args a) {
-  using S = F8Shape<AR, BN>;
+__device__ __forceinline__ int cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return (int)r;
+}
+__device__ __forceinline__ int cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctaid.x;" : "=r"(r));
+  return (int)r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// A split's sums in shared memory, [row][BN] f32, over the stages, which are
+// all read by then: 16-byte unit u of row r lies at u ^ (r % 8).
+template <int CW, int BN>
+__device__ __forceinline__ void put_part(const float2 (&acc)[CW / 2], uint8_t* part, int row, int col0) {
+#pragma unroll
+  for (int u = 0; u < CW / 4; ++u)
+    *(float4*)(part + (size_t)row * BN * 4 + (((col0 / 4 + u) ^ (row & 7)) << 4)) =
+        make_float4(acc[2 * u].x, acc[2 * u].y, acc[2 * u + 1].x, acc[2 * u + 1].y);
+}
+// Each block of the cluster adds up its share of the tile, always from the
+// first split to the last, and writes it out.
+template <int BN>
+__device__ __forceinline__ void join_parts(const uint8_t* part, const Fp8Args& a, int row0, int rows, int col0, int split,
+                                           int splits) {
+  const int units = rows * (BN / 4), u0 = units * split / splits, u1 = units * (split + 1) / splits;
+  const bool f32 = a.type == kRowF32, f16 = a.type == kRowF16;
+  const int size = f32 ? 4 : 2;
+  const bool vec = (((uintptr_t)a.out | a.out_stride * size) & (4 * size - 1)) == 0;
+  for (int i = u0 + (int)threadIdx.x; i < u1; i += (int)blockDim.x) {
+    const int r = i / (BN / 4), u = i % (BN / 4), at = col0 + u * 4;
+    const uint32_t mine = smem_u32(part) + r * BN * 4 + ((u ^ (r & 7)) << 4);
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int z = 0; z < splits; ++z) {
+      uint32_t from;
+      float w[4];
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(mine), "r"(z));
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(w[0]), "=f"(w[1]), "=f"(w[2]), "=f"(w[3])
+                   : "r"(from)
+                   : "memory");
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += w[j];
+    }
+    uint8_t* p = (uint8_t*)a.out + ((size_t)(row0 + r) * a.out_stride + at) * size;
+    if (vec && at + 4 <= a.n) {
+      if (f32) *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
+      else *(uint2*)p = make_uint2(pack2(v[0], v[1], f16), pack2(v[2], v[3], f16));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (at + j >= a.n) break;
+        if (f32) ((float*)p)[j] = v[j];
+        else ((uint16_t*)p)[j] = (uint16_t)pack2(v[j], 0.0f, f16);
+      }
+    }
+  }
+}
+
+// A kernel that is launched while the one before it in its stream still runs:
+// nothing that one wrote may be read, and nothing written, before this.
+__device__ __forceinline__ void after_kernel_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets the next such kernel start as this one's blocks leave room.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <int AR, int BN, int BLOCKS>
+__global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
+    k_fp8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Fp8Args a) {
+  using S = F8Shape<AR, BN, BLOCKS>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ F8Sync sync;
   F8Sync* y = &sync;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row_tiles = (a.m + 127) / 128, col_tiles = (a.n + BN - 1) / BN;
-  const long long tiles = (long long)row_tiles * col_tiles;
+  const uint32_t row_tiles = ((uint32_t)a.m + 127) / 128, col_tiles = ((uint32_t)a.n + BN - 1) / BN, tiles = row_tiles * col_tiles;
+  // The blocks of a cluster share a tile, each with a part of k.
+  const int splits = S::SPLITS ? cluster_size() : 1, split = S::SPLITS ? cluster_rank() : 0;
+  const int lo = S::SPLITS ? (int)((long long)a.blocks * split / splits) : 0;
+  const int hi = S::SPLITS ? (int)((long long)a.blocks * (split + 1) / splits) : a.blocks;
+  const uint32_t first = blockIdx.x / splits, step = gridDim.x / splits;
   volatile int* abort = &y->abort;
 
   if (threadIdx.x == 0) {
@@ -214,41 +297,58 @@ __global__ void __launch_bounds__(F8Shape<AR, BN>::THREADS, F8Shape<AR, BN>::BLO
   __syncthreads();
   fence_after();
   const uint32_t tmem = y->tmem;
+  let_next_start();
 
   if (warp < 4) {
     if constexpr (S::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::REGS_FEW));
     if (warp == 0 && elected()) {
       uint32_t it = 0;
       bool ok = true;
-      for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      // What does not depend on the kernel before, the first stages' weights,
+      // is on its way before that kernel has ended.
+      uint32_t early = 0;
+      for (uint32_t t = first; t < tiles && ok; t += step) {
         int r, c;
         tile_place(t, row_tiles, col_tiles, &r, &c);
-        for (int b = 0; b < a.blocks; ++b, ++it) {
+        const int units = min(BN / F8_UNIT, (a.n + F8_UNIT - 1) / F8_UNIT - c * (BN / F8_UNIT));
+        const uint8_t* w = a.w + (size_t)c * (BN / F8_UNIT) * a.blocks * F8_UNIT_BYTES;
+        auto weights = [&](int b, uint32_t i) {
+          mbar_expect_tx(&y->full[i], AR * F8_K + units * F8_UNIT_BYTES);
+          for (int z = 0; z < units; ++z)
+            bulk_load(base + i * S::STAGE + AR * F8_K + z * F8_UNIT_BYTES, w + ((size_t)z * a.blocks + b) * F8_UNIT_BYTES,
+                      F8_UNIT_BYTES, &y->full[i]);
+        };
+        if (it == 0) {
+          for (; early < S::STAGES && lo + (int)early < hi; ++early) weights(lo + early, early);
+          after_kernel_before();
+        }
+        for (int b = lo; b < hi; ++b, ++it) {
           const uint32_t i = it % S::STAGES;
-          if (!mbar_wait(&y->empty[i], ((it / S::STAGES) & 1) ^ 1, abort)) {
-            ok = false;
-            break;
+          if (it >= early) {
+            if (!mbar_wait(&y->empty[i], ((it / S::STAGES) & 1) ^ 1, abort)) {
+              ok = false;
+              break;
+            }
+            weights(b, i);
           }
-          uint8_t* to = base + i * S::STAGE;
-          mbar_expect_tx(&y->full[i], S::STAGE);
-          tma_load_2d(to, &xmap, &y->full[i], b * F8_K, r * 128);
-          tma_load_2d(to + AR * F8_K, &wmap, &y->full[i], b * F8_K, c * BN);
+          tma_load_2d(base + i * S::STAGE, &xmap, &y->full[i], b * F8_K, r * 128);
         }
       }
       if (!ok) {
-        // Let the copies in flight land before the block's memory is released.
-        for (uint32_t z = it > S::STAGES ? it - S::STAGES : 0; z < it; ++z) {
-          const long long t0 = now_ns();
+        // Let the copies in flight land before the block's memory is released
+        // (a stage whose rows were not asked for any more does not fill).
+        const long long t0 = now_ns();
+        const uint32_t end = max(it, early);
+        for (uint32_t z = end > S::STAGES ? end - S::STAGES : 0; z < end; ++z)
           while (!mbar_test(&y->full[z % S::STAGES], (z / S::STAGES) & 1) && now_ns() - t0 < TC_WAIT_NS) {
           }
-        }
       }
     } else if (warp == 1 && elected()) {
       const uint32_t s0 = smem_u32(base);
       uint32_t it = 0;
       bool ok = true;
-      for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        for (int b = 0; b < a.blocks; ++b, ++it) {
+      for (uint32_t t = first; t < tiles && ok; t += step) {
+        for (int b = lo; b < hi; ++b, ++it) {
           const uint32_t i = it % S::STAGES, u = it % S::BUFS;
           if (!mbar_wait(&y->tempty[u], ((it / S::BUFS) & 1) ^ 1, abort) ||
               !mbar_wait(&y->full[i], (it / S::STAGES) & 1, abort)) {
@@ -273,17 +373,17 @@ __global__ void __launch_bounds__(F8Shape<AR, BN>::THREADS, F8Shape<AR, BN>::BLO
   } else {
     if constexpr (S::SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::REGS_MANY));
     const int quarter = warp & 3, part = (warp - 4) >> 2;
+    after_kernel_before();
     if (quarter < S::ROW_WARPS) {
-      constexpr int LD = S::CW >= 64 ? 32 : 16;  // columns a load; the next ones are on the way while these are added
       uint8_t* staging = base + S::STAGES * S::STAGE + (part * S::ROW_WARPS + quarter) * 4096;
       const uint32_t tl = tmem + ((uint32_t)(quarter * 32) << 16) + part * S::CW;
       const bool vec = a.blocks % 4 == 0 && ((uintptr_t)a.x_scales & 15) == 0;
       uint32_t it = 0;
       bool ok = true;
-      for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      for (uint32_t t = first; t < tiles && ok; t += step) {
         int r, c;
         tile_place(t, row_tiles, col_tiles, &r, &c);
-        const long long row0 = (long long)r * 128 + quarter * 32;
+        const int row0 = r * 128 + quarter * 32;  // m is at most 2^31 - 256
         const int col0 = c * BN + part * S::CW;
         const bool live = row0 + lane < a.m;
         const float* sx = a.x_scales + (size_t)(live ? row0 + lane : 0) * a.blocks;
@@ -293,50 +393,59 @@ __global__ void __launch_bounds__(F8Shape<AR, BN>::THREADS, F8Shape<AR, BN>::BLO
         float2 acc[S::CW / 2];
 #pragma unroll
         for (int i = 0; i < S::CW / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
-        float4 next = scales4(sx, 0, a.blocks, live, vec);
-        float sws = 0.0f;
-        for (int b0 = 0; b0 < a.blocks && ok; b0 += 4) {
-          if ((b0 & 31) == 0) sws = b0 + lane < a.blocks ? __ldg(sw + b0 + lane) : 0.0f;
-          const float4 now = next;
-          next = scales4(sx, b0 + 4, a.blocks, live, vec);
+        float4 now = make_float4(0.0f, 0.0f, 0.0f, 0.0f), next = scales4(sx, lo & ~3, hi, live, vec);
+        float sws = lo + lane < hi ? __ldg(sw + lo + lane) : 0.0f;
+        for (int b = lo; b < hi; ++b, ++it) {
+          if ((b & 3) == 0 || b == lo) {
+            now = next;
+            for (int i = 0; S::SPLITS && i < (b & 3); ++i) now = make_float4(now.y, now.z, now.w, 0.0f);
+            next = scales4(sx, (b & ~3) + 4, hi, live, vec);
+          }
+          if (b > lo && ((b - lo) & 31) == 0) sws = b + lane < hi ? __ldg(sw + b + lane) : 0.0f;
+          const float scale = now.x * __shfl_sync(0xffffffffu, sws, (b - lo) & 31);
+          now = make_float4(now.y, now.z, now.w, 0.0f);
+          const float2 s2 = make_float2(scale, scale);
+          const uint32_t u = it % S::BUFS;
+          if (!__all_sync(0xffffffffu, mbar_wait(&y->tfull[u], (it / S::BUFS) & 1, abort))) {
+            ok = false;
+            break;
+          }
+          fence_after();
+          // 64 columns on the way at a time; the next ones while these are added.
+          const uint32_t from = tl + u * BN;
+          uint32_t v[2][32];
+          tmem_ld<32>(from, v[0]);
+          tmem_ld<32>(from + 32, v[1]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (b0 + j >= a.blocks) break;
-            const float xj = j == 0 ? now.x : j == 1 ? now.y : j == 2 ? now.z : now.w;
-            const float scale = xj * __shfl_sync(0xffffffffu, sws, (b0 + j) & 31);
-            const float2 s2 = make_float2(scale, scale);
-            const uint32_t u = it % S::BUFS;
-            if (!__all_sync(0xffffffffu, mbar_wait(&y->tfull[u], (it / S::BUFS) & 1, abort))) {
-              ok = false;
-              break;
-            }
-            ++it;
-            fence_after();
-            const uint32_t from = tl + u * BN;
-            uint32_t v[2][LD];
-            tmem_ld<LD>(from, v[0]);
-#pragma unroll
-            for (int q = 0; q < S::CW / LD; ++q) {
+          for (int q = 0; q < S::CW / 32; ++q) {
+            if (q % 2 == 0) {
               tmem_wait_ld();
-              if (q + 1 < S::CW / LD) {
-                tmem_ld<LD>(from + (q + 1) * LD, v[(q + 1) & 1]);
-              } else {
+              if (q + 2 == S::CW / 32) {
                 fence_before();
                 if (lane == 0) mbar_arrive(&y->tempty[u]);
               }
-#pragma unroll
-              for (int i = 0; i < LD / 2; ++i)
-                acc[q * (LD / 2) + i] = fma2(make_float2(__uint_as_float(v[q & 1][2 * i]), __uint_as_float(v[q & 1][2 * i + 1])),
-                                             s2, acc[q * (LD / 2) + i]);
             }
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              acc[q * 16 + i] = fma2(make_float2(__uint_as_float(v[q & 1][2 * i]), __uint_as_float(v[q & 1][2 * i + 1])), s2,
+                                     acc[q * 16 + i]);
+            if (q + 2 < S::CW / 32) tmem_ld<32>(from + (q + 2) * 32, v[q & 1]);
           }
         }
-        if (ok && row0 < a.m) store_tile<S::CW>(acc, staging, a, row0, col0, lane);
+        if (S::SPLITS && splits > 1) put_part<S::CW, BN>(acc, base, quarter * 32 + lane, part * S::CW);
+        else if (ok && row0 < a.m) store_tile<S::CW>(acc, staging, a, row0, col0, lane);
       }
     }
   }
   fence_before();
   __syncthreads();
+  if (S::SPLITS && splits > 1) {
+    cluster_sync();
+    int r, c;
+    tile_place(first, row_tiles, col_tiles, &r, &c);
+    join_parts<BN>(base, a, r * 128, min(AR, a.m - r * 128), c * BN, split, splits);
+    cluster_sync();  // nobody leaves while others read its part
+  }
   if (warp == 1) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
@@ -344,46 +453,86 @@ __global__ void __launch_bounds__(F8Shape<AR, BN>::THREADS, F8Shape<AR, BN>::BLO
   if (threadIdx.x == 0 && y->abort) *(volatile int*)a.status = 1;
 }
 
-template <int AR, int BN>
-cudaError_t run(const TcMap* w, const TcMap& x, const Fp8Args& a, cudaStream_t s) {
-  using S = F8Shape<AR, BN>;
+template <int AR, int BN, int BLOCKS>
+cudaError_t run(const TcMap& x, const Fp8Args& a, int splits, cudaStream_t s) {
+  using S = F8Shape<AR, BN, BLOCKS>;
   static_assert(S::STAGES >= 3 && S::STAGES <= 12 && S::SMEM + (int)sizeof(F8Sync) <= 227 * 1024, "shared memory");
+  static_assert(AR * BN * 4 <= S::STAGES * S::STAGE, "a split's sums");
   static_assert(S::COLS * S::BLOCKS <= 512 && (S::COLS & (S::COLS - 1)) == 0, "TMEM");
-  static_assert(S::CW <= 128 && S::CW % 32 == 0, "columns of an epilogue warp");
+  static_assert(S::CW <= 128 && S::CW % 64 == 0 && BN % F8_UNIT == 0, "columns of an epilogue warp");
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   static DeviceOnce once;
   e = once.run(dev, [] {
     cudaFuncAttributes f;
-    cudaError_t r = cudaFuncGetAttributes(&f, k_fp8<AR, BN>);
+    cudaError_t r = cudaFuncGetAttributes(&f, k_fp8<AR, BN, BLOCKS>);
     // A launch with fewer registers than the shares add up to would wait for them without end.
     if (r == cudaSuccess && S::SPLIT && f.numRegs != S::REGS) r = cudaErrorInvalidKernelImage;
     if (r != cudaSuccess) return r;
-    return cudaFuncSetAttribute(k_fp8<AR, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    return cudaFuncSetAttribute(k_fp8<AR, BN, BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
   });
   if (e != cudaSuccess) return e;
   const long long tiles = (a.m + 127LL) / 128 * ((a.n + BN - 1) / BN);
-  const int grid = (int)std::min<long long>(tiles, current_sm_count() * S::BLOCKS);
-  constexpr int box = BN == 32 ? 0 : BN == 64 ? 1 : BN == 128 ? 2 : 3;
-  k_fp8<AR, BN><<<grid, S::THREADS, S::SMEM, s>>>(*(const CUtensorMap*)&x, *(const CUtensorMap*)&w[box], a);
-  return cudaGetLastError();
+  if (tiles >> 30) return cudaErrorInvalidValue;  // an output of 2^42 values or more
+  cudaLaunchConfig_t config{};
+  // Blocks take tile after tile; those of a cluster have one.
+  config.gridDim = dim3((unsigned)(splits > 1 ? tiles * splits : std::min<long long>(tiles, current_sm_count() * BLOCKS)));
+  config.blockDim = dim3(S::THREADS);
+  config.dynamicSmemBytes = S::SMEM;
+  config.stream = s;
+  cudaLaunchAttribute attrs[2] = {};
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim = {(unsigned)splits, 1, 1};
+  config.attrs = attrs;
+  config.numAttrs = splits > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&config, k_fp8<AR, BN, BLOCKS>, *(const CUtensorMap*)&x, a);
+}
+
+// Rows of bytes to the units that k_fp8 reads: [n / 64][k / 128][64 rows][128
+// bytes], 16-byte chunk c of row r at c ^ (r % 8), zero past either end. One
+// thread a chunk.
+__global__ void __launch_bounds__(256) k_fp8_pack(const uint8_t* codes, size_t n, size_t k, uint8_t* w) {
+  const size_t blocks = (k + F8_K - 1) / F8_K, chunks = (n + F8_UNIT - 1) / F8_UNIT * blocks * (F8_UNIT_BYTES / 16);
+  for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < chunks; i += (size_t)gridDim.x * 256) {
+    const size_t unit = i / (F8_UNIT_BYTES / 16);
+    const int at = (int)(i % (F8_UNIT_BYTES / 16)), r = at / 8, c = (at % 8) ^ (r & 7);
+    const size_t row = unit / blocks * F8_UNIT + r, col = unit % blocks * F8_K + c * 16;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (row < n && col < k) v = *(const uint4*)(codes + row * k + col);  // k is a multiple of 16
+    ((uint4*)w)[i] = v;
+  }
 }
 
 }  // namespace
 
-int fp8_weight_box(int index) { return 32 << index; }
-int fp8_row_box(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128; }
+int fp8_row_box(int m) { return m <= 16 ? 16 : m <= 64 ? 64 : 128; }
+size_t fp8_packed_bytes(size_t n, size_t k) {
+  return (n + F8_UNIT - 1) / F8_UNIT * ((k + F8_K - 1) / F8_K) * F8_UNIT_BYTES;
+}
+cudaError_t launch_fp8_pack(const uint8_t* codes, size_t n, size_t k, uint8_t* w, cudaStream_t s) {
+  k_fp8_pack<<<148 * 8, 256, 0, s>>>(codes, n, k, w);
+  return cudaGetLastError();
+}
 
-cudaError_t launch_fp8(const TcMap* w, const TcMap& x, const Fp8Args& a, cudaStream_t s) {
+cudaError_t launch_fp8(const TcMap& x, const Fp8Args& a, cudaStream_t s) {
   if (a.m <= 0) return cudaSuccess;
-  switch (fp8_row_box(a.m)) {
-    case 16: return run<16, 32>(w, x, a, s);
-    case 32: return run<32, 32>(w, x, a, s);
-    case 64: return run<64, 64>(w, x, a, s);
-  }
-  if (a.m <= 512) return run<128, 128>(w, x, a, s);
-  return run<128, 256>(w, x, a, s);
+  const long long sms = current_sm_count();
+  const auto tiles = [&](int bn) { return (a.m + 127LL) / 128 * ((a.n + bn - 1) / bn); };
+  // As many blocks of a cluster as there is room for beside each other.
+  const auto splits = [&](long long tiles, long long room) {
+    int z = 1;
+    while (z < 8 && tiles * z * 2 <= room && a.blocks / (z * 2) >= (z < 4 ? 2 : 4)) z *= 2;
+    return z;
+  };
+  const int box = fp8_row_box(a.m);
+  if (box == 16) return run<16, 64, 2>(x, a, splits(tiles(64), 2 * sms), s);
+  if (box == 64) return run<64, 64, 2>(x, a, splits(tiles(64), 2 * sms), s);
+  const auto waves = [&](int bn) { return (double)((tiles(bn) + sms - 1) / sms); };
+  if (waves(128) * 0.385 < waves(256) * 0.6) return run<128, 128, 1>(x, a, splits(tiles(128), sms), s);
+  return run<128, 256, 1>(x, a, 1, s);
 }
 
 }  // namespace trit

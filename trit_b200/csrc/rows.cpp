@@ -295,15 +295,21 @@ DenseFp8::DenseFp8(const void* codes, const float* scales, size_t n, size_t k, i
   OnDevice on(device);
   const size_t blocks = ((n + 127) / 128) * ((k + 127) / 128);
   try {
-    TRIT_CUDA(cudaMalloc(&codes_, n * k));
+    TRIT_CUDA(cudaMalloc(&codes_, fp8_packed_bytes(n, k)));
     TRIT_CUDA(cudaMalloc(&scales_, blocks * 4));
     TRIT_CUDA(cudaStreamCreateWithFlags(&stream_, cudaStreamNonBlocking));
     TRIT_CUDA(cudaHostAlloc(&status_, 4, cudaHostAllocDefault));
     *status_ = 0;
-    TRIT_CUDA(cudaMemcpy(codes_, codes, n * k, cudaMemcpyHostToDevice));
-    TRIT_CUDA(cudaMemcpy(scales_, scales, blocks * 4, cudaMemcpyHostToDevice));
-    TRIT_CUDA(cudaDeviceSynchronize());
-    for (int i = 0; i < 4; ++i) TRIT_CUDA(make_fp8_map(&maps_[i], codes_, n, k, fp8_weight_box(i)));
+    // On the layer's stream: a plain cudaMemcpy may return before its last
+    // bytes are there, and that stream does not wait for it.
+    uint8_t* raw = nullptr;
+    TRIT_CUDA(cudaMalloc(&raw, n * k));
+    cudaError_t e = cudaMemcpyAsync(scales_, scales, blocks * 4, cudaMemcpyHostToDevice, stream_);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(raw, codes, n * k, cudaMemcpyHostToDevice, stream_);
+    if (e == cudaSuccess) e = launch_fp8_pack(raw, n, k, codes_, stream_);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(stream_);
+    cudaFree(raw);
+    TRIT_CUDA(e);
   } catch (...) {
     release();
     throw;
@@ -342,6 +348,7 @@ void DenseFp8::product(const void* codes, const float* scales, size_t m, void* o
   TcMap map;
   TRIT_CUDA(make_fp8_map(&map, codes, m, k_, fp8_row_box((int)m)));
   Fp8Args a;
+  a.w = codes_;
   a.x_scales = scales;
   a.w_scales = scales_;
   a.out = out;
@@ -351,7 +358,7 @@ void DenseFp8::product(const void* codes, const float* scales, size_t m, void* o
   a.blocks = (int)((k_ + kFp8Group - 1) / kFp8Group);
   a.type = type;
   a.status = status_;
-  TRIT_CUDA(launch_fp8(maps_, map, a, s));
+  TRIT_CUDA(launch_fp8(map, a, s));
 }
 
 void DenseFp8::forward_codes(const void* codes, const float* scales, size_t m, void* out, size_t out_stride, int type,

@@ -108,14 +108,14 @@ class DenseFp8 {
 
   int device_;
   size_t n_, k_;
-  uint8_t* codes_ = nullptr;  // [n][k]
+  uint8_t* codes_ = nullptr;  // packed (launch_fp8_pack)
   float* scales_ = nullptr;   // [ceil(n / 128)][ceil(k / 128)]
   cudaStream_t stream_ = nullptr;
   int* status_ = nullptr;     // pinned: a wait inside a product ran out
-  TcMap maps_[4];             // boxes of 32, 64, 128 and 256 weight rows
 };
 
 struct Fp8Args {
+  const uint8_t* w = nullptr;  // packed (launch_fp8_pack)
   const float* x_scales = nullptr;
   const float* w_scales = nullptr;
   void* out = nullptr;
@@ -127,9 +127,10 @@ struct Fp8Args {
 // A TMA map of 8-bit numbers [rows][k], row stride k, boxes of 128 values x
 // box_rows rows with the 128-byte swizzle; past either end reads zero.
 cudaError_t make_fp8_map(TcMap* out, const void* base, size_t rows, size_t k, int box_rows);
-// Box rows of the weights' maps, and of the rows' map for m rows.
-int fp8_weight_box(int index);
-int fp8_row_box(int m);
-cudaError_t launch_fp8(const TcMap* weight_maps, const TcMap& rows, const Fp8Args& a, cudaStream_t s);
+int fp8_row_box(int m);  // its box rows for m rows
+// The weights [n][k] in the order that the product reads them.
+size_t fp8_packed_bytes(size_t n, size_t k);
+cudaError_t launch_fp8_pack(const uint8_t* codes, size_t n, size_t k, uint8_t* w, cudaStream_t s);
+cudaError_t launch_fp8(const TcMap& x, const Fp8Args& a, cudaStream_t s);
 
 }  // namespace trit
