@@ -24,6 +24,7 @@
 #include <algorithm>
 
 #include "device.cuh"
+#include "launch.cuh"
 #include "rows.h"
 #include "tc.cuh"
 
@@ -153,15 +154,28 @@ __device__ __forceinline__ void store_tile(const float2 (&acc)[CW / 2], uint8_t*
         }
       }
     } else {
-      const int values = units * 16 / size;
+      // Rows that start anywhere: a lane stores four bytes where they are
+      // aligned, so with an odd start of 16-bit rows a lane's two values begin
+      // one earlier, and lane 0 has the first and the last one alone.
+      const int live = min(units * 16 / size, a.n - col);
 #pragma unroll 8
-      for (int r = 0; r < rows; ++r) {
-        for (int i = lane; i < values && col + i < a.n; i += 32) {
-          const uint8_t* from = staging + r * 128 + (((i * size >> 4) ^ (r & 7)) << 4) + (i * size & 15);
-          uint8_t* p = out + ((size_t)r * a.out_stride + col + i) * size;
-          if (f32) *(uint32_t*)p = *(const uint32_t*)from;
-          else *(uint16_t*)p = *(const uint16_t*)from;
+      for (int r = 0; r < 32; ++r) {
+        if (r >= rows) break;
+        const uint8_t* from = staging + r * 128;
+        uint8_t* p = out + ((size_t)r * a.out_stride + col) * size;
+        if (f32) {
+          if (lane < live) ((uint32_t*)p)[lane] = *(const uint32_t*)(from + ((lane / 4 ^ (r & 7)) << 4) + (lane & 3) * 4);
+          continue;
         }
+        const auto get = [&](int e) { return *(const uint16_t*)(from + ((e / 8 ^ (r & 7)) << 4) + (e & 7) * 2); };
+        const int odd = (int)((uintptr_t)p >> 1 & 1), e = 2 * lane - odd;
+        if (e >= 0 && e + 1 < live) {
+          *(uint32_t*)(p + 2 * e) = (uint32_t)get(e) | (uint32_t)get(e + 1) << 16;
+        } else {
+          if (e < 0 && live > 0) ((uint16_t*)p)[0] = get(0);
+          if (e >= 0 && e < live) ((uint16_t*)p)[e] = get(e);
+        }
+        if (odd && lane == 0 && live == 64) ((uint16_t*)p)[63] = get(63);
       }
     }
     __syncwarp();
@@ -251,12 +265,6 @@ __device__ __forceinline__ void join_parts(const uint8_t* part, const Fp8Args& a
     }
   }
 }
-
-// A kernel that is launched while the one before it in its stream still runs:
-// nothing that one wrote may be read, and nothing written, before this.
-__device__ __forceinline__ void after_kernel_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-// Lets the next such kernel start as this one's blocks leave room.
-__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <int AR, int BN, int BLOCKS>
 __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
@@ -411,25 +419,23 @@ __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
             break;
           }
           fence_after();
-          // 64 columns on the way at a time; the next ones while these are added.
+          // 32 columns a load; the next ones are on the way while these are added.
           const uint32_t from = tl + u * BN;
           uint32_t v[2][32];
           tmem_ld<32>(from, v[0]);
-          tmem_ld<32>(from + 32, v[1]);
 #pragma unroll
           for (int q = 0; q < S::CW / 32; ++q) {
-            if (q % 2 == 0) {
-              tmem_wait_ld();
-              if (q + 2 == S::CW / 32) {
-                fence_before();
-                if (lane == 0) mbar_arrive(&y->tempty[u]);
-              }
+            tmem_wait_ld();
+            if (q + 1 < S::CW / 32) {
+              tmem_ld<32>(from + (q + 1) * 32, v[(q + 1) & 1]);
+            } else {
+              fence_before();
+              if (lane == 0) mbar_arrive(&y->tempty[u]);
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i)
               acc[q * 16 + i] = fma2(make_float2(__uint_as_float(v[q & 1][2 * i]), __uint_as_float(v[q & 1][2 * i + 1])), s2,
                                      acc[q * 16 + i]);
-            if (q + 2 < S::CW / 32) tmem_ld<32>(from + (q + 2) * 32, v[q & 1]);
           }
         }
         if (S::SPLITS && splits > 1) put_part<S::CW, BN>(acc, base, quarter * 32 + lane, part * S::CW);
@@ -475,20 +481,10 @@ cudaError_t run(const TcMap& x, const Fp8Args& a, int splits, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   const long long tiles = (a.m + 127LL) / 128 * ((a.n + BN - 1) / BN);
   if (tiles >> 30) return cudaErrorInvalidValue;  // an output of 2^42 values or more
-  cudaLaunchConfig_t config{};
   // Blocks take tile after tile; those of a cluster have one.
-  config.gridDim = dim3((unsigned)(splits > 1 ? tiles * splits : std::min<long long>(tiles, current_sm_count() * BLOCKS)));
-  config.blockDim = dim3(S::THREADS);
-  config.dynamicSmemBytes = S::SMEM;
-  config.stream = s;
-  cudaLaunchAttribute attrs[2] = {};
-  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attrs[0].val.programmaticStreamSerializationAllowed = 1;
-  attrs[1].id = cudaLaunchAttributeClusterDimension;
-  attrs[1].val.clusterDim = {(unsigned)splits, 1, 1};
-  config.attrs = attrs;
-  config.numAttrs = splits > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&config, k_fp8<AR, BN, BLOCKS>, *(const CUtensorMap*)&x, a);
+  const long long grid = splits > 1 ? tiles * splits : std::min<long long>(tiles, current_sm_count() * BLOCKS);
+  return launch_early(k_fp8<AR, BN, BLOCKS>, dim3((unsigned)grid), dim3(S::THREADS), S::SMEM, s, (unsigned)splits,
+                      *(const CUtensorMap*)&x, a);
 }
 
 // Rows of bytes to the units that k_fp8 reads: [n / 64][k / 128][64 rows][128

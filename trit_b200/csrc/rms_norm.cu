@@ -12,12 +12,16 @@
 // gets the scale NaN.
 //
 // Bound by bytes: a row is read once and stays in registers between the sum
-// and the output. A thread holds 8 neighbouring values at a time, so 16
-// threads hold a group and share its maximum with shuffles.
+// and the output. It takes few instructions to be so: a thread holds 16 values
+// of a group (two runs of 8, so that a warp's loads are whole lines), 8 threads
+// share the group's maximum with shuffles, and the two quotients, the row's
+// root and the products are written with what is exact and cheap.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include "device.cuh"
+#include "launch.cuh"
 #include "rows.h"
 
 namespace trit {
@@ -86,74 +90,27 @@ __device__ __forceinline__ void store8(T* p, int left, const float (&v)[8]) {
   }
 }
 
-__device__ __forceinline__ double warp_sum_f64(double v) {
+// The sum over TEAM threads (a power of two, up to a warp).
+template <int TEAM>
+__device__ __forceinline__ double lanes_sum(double v) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = TEAM / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-
-// Two e4m3 numbers, the first in the low byte.
-__device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
-  return r;
-}
-
-// The codes and the scale of 8 values whose group the 16 threads of this half
-// warp hold. Every thread of the warp takes part.
-template <bool VEC>
-__device__ __forceinline__ void put_codes(const float (&y)[8], uint8_t* codes, float* scale_at, int left) {
-  uint32_t most = 0;  // the bits of |y| are ordered as its values, infinity and NaN above all
-#pragma unroll
-  for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(y[i]) & 0x7fffffffu);
-#pragma unroll
-  for (int o = 8; o; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-  float scale = 1.0f;
-  if (most >= 0x7f800000u) scale = __uint_as_float(0x7fffffffu);
-  else if (most) scale = fmaxf(__fdiv_rn(__uint_as_float(most), 448.0f), 1.17549435e-38f);
-  if (left <= 0) return;
-  const float inv = __fdiv_rn(1.0f, scale);
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = e4m3x2(__fmul_rn(y[2 * i], inv), __fmul_rn(y[2 * i + 1], inv));
-  if constexpr (VEC) {
-    *(uint2*)codes = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < left) codes[i] = (uint8_t)(w[i / 2] >> (8 * (i & 1)));
-  }
-  if ((threadIdx.x & 15) == 0) *scale_at = scale;
-}
-
-template <class T, bool VEC>
-__device__ __forceinline__ void finish8(const NormArgs& a, size_t row, int at, int left, const float (&y)[8]) {
-  if (a.out) store8<T, VEC>((T*)a.out + row * a.out_stride + at, left, y);
-  if (a.codes)
-    put_codes<VEC>(y, a.codes + row * a.width + at,
-                   a.scales + row * ((a.width + kFp8Group - 1) / kFp8Group) + at / kFp8Group, left);
-}
-
-// h of 8 values: x, or its sum with the residual, which is stored.
-template <class T, bool VEC>
-__device__ __forceinline__ void sum8(const NormArgs& a, size_t row, int at, int left, float (&h)[8], const float (&r)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) h[i] = to_f32(from_f32<T>(__fadd_rn(h[i], r[i])));
-  store8<T, VEC>((T*)a.sum + row * a.sum_stride + at, left, h);
-}
-
-// The block's (TEAM threads') sum of a value a thread.
+// The sum of a value a thread over the team: a part of a warp, or the block.
 template <int TEAM>
 __device__ __forceinline__ double team_sum(double v) {
-  v = warp_sum_f64(v);
-  if constexpr (TEAM > 32) {
+  if constexpr (TEAM <= 32) {
+    return lanes_sum<TEAM>(v);
+  } else {
     __shared__ double part[TEAM / 32];
+    v = lanes_sum<32>(v);
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = warp_sum_f64((threadIdx.x & 31) < TEAM / 32 ? part[threadIdx.x & 31] : 0.0);
+    return lanes_sum<TEAM / 32>(part[threadIdx.x & (TEAM / 32 - 1)]);
   }
-  return v;
 }
+
 // s as f32(s 2^e) and 2^-e, e = 0 but where s or its product with h's bits
 // would leave f32's exponents: rows of f32 beyond 2^100 or, without eps, below
 // 2^-100.
@@ -161,119 +118,215 @@ struct Factor {
   float s = 1.0f, h = 1.0f;
 };
 __device__ __forceinline__ Factor norm_factor(double sum, const NormArgs& a) {
-  const double s = rsqrt(sum / a.width + a.eps);
+  const double d = sum * a.inv_width + a.eps;
+  if (d > 0x1p-90 && d < 0x1p90) {
+    // From the f32 approximation y (off by 2^-22): with e = 1 - d y^2,
+    // 1 / sqrt(d) = y (1 - e)^(-1/2) = y (1 + e / 2 + 3 e^2 / 8 + ...); the
+    // next term is below 2^-63.
+    const double y = (double)rsqrtf((float)d), e = fma(-d * y, y, 1.0);
+    return Factor{(float)fma(y * e, fma(e, 0.375, 0.5), y), 1.0f};
+  }
+  const double s = rsqrt(d);
   if (s < 0x1p-100 && s > 0.0) return Factor{(float)(s * 0x1p64), 0x1p-64f};
   if (s > 0x1p100) return Factor{(float)(s * 0x1p-64), 0x1p64f};
   return Factor{(float)s, 1.0f};
 }
 
-// y from h: the norm's factor times the weights, or the rows as they are.
-template <class T, bool VEC>
-__device__ __forceinline__ void norm8(const NormArgs& a, int at, int left, const Factor& f, float (&v)[8]) {
-  if (!a.weight) return;
-  float w[8];
-  if (a.weight_f32) load8<float, VEC>((const float*)a.weight + at, left, w);
-  else load8<T, VEC>((const T*)a.weight + at, left, w);
-  if (f.h != 1.0f) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= f.h;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], __fmul_rn(f.s, w[i]));
+// The largest |v|; NaN where there is one.
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Two e4m3 numbers, the first in the low byte.
+__device__ __forceinline__ uint32_t e4m3x2(float2 v) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(v.y), "f"(v.x));
+  return r;
 }
 
-// A row of up to TEAM * 8 * VPT values, held in registers. A team of one warp
-// shares its block with seven others.
-template <class T, int TEAM, int VPT, bool VEC>
-__global__ void __launch_bounds__(TEAM == 32 ? 256 : TEAM) k_norm(const __grid_constant__ NormArgs a) {
-  const int t = TEAM == 32 ? threadIdx.x & 31 : threadIdx.x;
-  const size_t row = TEAM == 32 ? blockIdx.x * (size_t)8 + (threadIdx.x >> 5) : blockIdx.x;
-  if (row >= (size_t)a.rows) return;  // a whole warp
-  float h[VPT][8];
-  const T* x = (const T*)a.x + row * a.x_stride;
+// A thread's 16 values: runs of 8 at `at` and at + 64 of the row; left: how
+// many of the row's values there are from each on.
+struct Place {
+  int at, left0, left1;
+  __device__ __forceinline__ Place(int unit, int width)
+      : at((unit >> 3) * kFp8Group + (unit & 7) * 8), left0(width - at), left1(width - at - 64) {}
+};
+template <class T, bool VEC>
+__device__ __forceinline__ void load16(const T* p, const Place& u, float (&v)[16]) {
+  load8<T, VEC>(p + u.at, u.left0, *(float (*)[8])v);
+  load8<T, VEC>(p + u.at + 64, u.left1, *(float (*)[8])(v + 8));
+}
+template <class T, bool VEC>
+__device__ __forceinline__ void store16(T* p, const Place& u, const float (&v)[16]) {
+  store8<T, VEC>(p + u.at, u.left0, *(const float (*)[8])v);
+  store8<T, VEC>(p + u.at + 64, u.left1, *(const float (*)[8])(v + 8));
+}
+template <bool VEC>
+__device__ __forceinline__ void store_codes8(uint8_t* p, int left, const uint32_t (&w)[4]) {
+  if constexpr (VEC) {
+    if (left > 0) *(uint2*)p = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+  } else {
 #pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    const int at = (t + j * TEAM) * 8;
-    load8<T, VEC>(x + at, a.width - at, h[j]);
+    for (int i = 0; i < 8; ++i)
+      if (i < left) p[i] = (uint8_t)(w[i / 2] >> (8 * (i & 1)));
   }
+}
+
+// The codes and the scale of a group that 8 neighbouring threads hold. Every
+// thread of the warp takes part.
+template <bool VEC>
+__device__ __forceinline__ void put_codes(const float (&y)[16], const Place& u, uint8_t* codes, float* scales) {
+  float most = max_abs(y[0], y[1], y[2]);
+#pragma unroll
+  for (int i = 3; i < 15; i += 2) most = max_abs(most, y[i], y[i + 1]);
+  most = max_abs(most, y[15], 0.0f);
+#pragma unroll
+  for (int o = 4; o; o >>= 1) most = max_abs(most, __shfl_xor_sync(0xffffffffu, most, o), 0.0f);
+  // max / 448 through 64 bits: with X the 24 bits of max, the quotient lies at
+  // least 1 / 14 of an f32 step from the border between two f32 (2 X 2^s is
+  // even, 7 (2 j + 1) odd), the 64-bit product within 2^-28 of a step.
+  float scale = fmaxf((float)((double)most * (1.0 / 448.0)), 1.17549435e-38f);
+  if (most == 0.0f) scale = 1.0f;
+  if (!(most < __uint_as_float(0x7f800000u))) scale = __uint_as_float(0x7fffffffu);
+  const float inv = __frcp_rn(scale);
+  const float2 i2 = make_float2(inv, inv);
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = e4m3x2(mul2(make_float2(y[2 * i], y[2 * i + 1]), i2));
+  store_codes8<VEC>(codes + u.at, u.left0, *(const uint32_t (*)[4])w);
+  store_codes8<VEC>(codes + u.at + 64, u.left1, *(const uint32_t (*)[4])(w + 4));
+  if ((threadIdx.x & 7) == 0 && u.left0 > 0) scales[u.at / kFp8Group] = scale;
+}
+
+template <class T, bool VEC>
+__device__ __forceinline__ void weights16(const NormArgs& a, const Place& u, float (&w)[16]) {
+  if (a.weight_f32) load16<float, VEC>((const float*)a.weight, u, w);
+  else load16<T, VEC>((const T*)a.weight, u, w);
+}
+// y: h times the norm's factor and the weights.
+__device__ __forceinline__ void norm16(const Factor& f, const float (&w)[16], float (&v)[16]) {
+  if (f.h != 1.0f) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] *= f.h;
+  }
+  const float2 s2 = make_float2(f.s, f.s);
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) {
+    const float2 y = mul2(make_float2(v[i], v[i + 1]), mul2(s2, make_float2(w[i], w[i + 1])));
+    v[i] = y.x;
+    v[i + 1] = y.y;
+  }
+}
+
+// h: x, or its sum with the residual, which is stored.
+template <class T, bool VEC>
+__device__ __forceinline__ void sum16(const NormArgs& a, size_t row, const Place& u, const float (&r)[16], float (&h)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) h[i] = to_f32(from_f32<T>(__fadd_rn(h[i], r[i])));
+  store16<T, VEC>((T*)a.sum + row * a.sum_stride, u, h);
+}
+template <class T, bool VEC>
+__device__ __forceinline__ void finish16(const NormArgs& a, size_t row, const Place& u, const float (&y)[16]) {
+  if (a.out) store16<T, VEC>((T*)a.out + row * a.out_stride, u, y);
+  if (a.codes)
+    put_codes<VEC>(y, u, a.codes + row * a.width, a.scales + row * ((a.width + kFp8Group - 1) / kFp8Group));
+}
+__device__ __forceinline__ double add_squares(const float (&h)[16], double sum) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) sum = fma((double)h[i], (double)h[i], sum);
+  return sum;
+}
+
+// A row of up to TEAM * 16 * U values, held in registers. Teams of a warp or
+// less share a block.
+template <class T, int TEAM, int U, bool VEC>
+__global__ void __launch_bounds__(TEAM <= 32 ? 256 : TEAM) k_norm(const __grid_constant__ NormArgs a) {
+  let_next_start();
+  after_kernel_before();
+  const int t = threadIdx.x % TEAM;
+  const size_t at = TEAM <= 32 ? blockIdx.x * (size_t)(256 / TEAM) + threadIdx.x / TEAM : blockIdx.x;
+  // A team behind the last row has no values, but takes part in the shuffles.
+  const int width = at < (size_t)a.rows ? a.width : 0;
+  const size_t row = at < (size_t)a.rows ? at : 0;
+  float h[U][16], w[U][16];
+#pragma unroll
+  for (int j = 0; j < U; ++j) load16<T, VEC>((const T*)a.x + row * a.x_stride, Place(t + j * TEAM, width), h[j]);
   if (a.residual) {
-    const T* res = (const T*)a.residual + row * a.residual_stride;
-    float r[VPT][8];
+    float r[U][16];
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      const int at = (t + j * TEAM) * 8;
-      load8<T, VEC>(res + at, a.width - at, r[j]);
-    }
+    for (int j = 0; j < U; ++j)
+      load16<T, VEC>((const T*)a.residual + row * a.residual_stride, Place(t + j * TEAM, width), r[j]);
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      const int at = (t + j * TEAM) * 8;
-      sum8<T, VEC>(a, row, at, a.width - at, h[j], r[j]);
-    }
+    for (int j = 0; j < U; ++j) sum16<T, VEC>(a, row, Place(t + j * TEAM, width), r[j], h[j]);
   }
-  Factor f;
   if (a.weight) {
     double sum = 0.0;
 #pragma unroll
-    for (int j = 0; j < VPT; ++j)
+    for (int j = 0; j < U; ++j) {
+      weights16<T, VEC>(a, Place(t + j * TEAM, width), w[j]);
+      sum = add_squares(h[j], sum);
+    }
+    const Factor f = norm_factor(team_sum<TEAM>(sum), a);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum = fma((double)h[j][i], (double)h[j][i], sum);
-    f = norm_factor(team_sum<TEAM>(sum), a);
+    for (int j = 0; j < U; ++j) norm16(f, w[j], h[j]);
   }
 #pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    const int at = (t + j * TEAM) * 8, left = a.width - at;
-    norm8<T, VEC>(a, at, left, f, h[j]);
-    finish8<T, VEC>(a, row, at, left, h[j]);
-  }
+  for (int j = 0; j < U; ++j) finish16<T, VEC>(a, row, Place(t + j * TEAM, width), h[j]);
 }
 
 // Rows of any width: the second pass reads h again (the sum where there is a
 // residual), each thread what it read or wrote itself.
 template <class T, bool VEC>
 __global__ void __launch_bounds__(1024) k_norm_long(const __grid_constant__ NormArgs a) {
+  let_next_start();
+  after_kernel_before();
   const size_t row = blockIdx.x;
   const T* x = (const T*)a.x + row * a.x_stride;
-  const int all = (a.width + 8 * 1024 - 1) / (8 * 1024) * (8 * 1024);  // every thread takes every turn
+  const int turns = (a.width + 16 * 1024 - 1) / (16 * 1024);  // every thread takes every turn
   double sum = 0.0;
-  for (int at = threadIdx.x * 8; at < all; at += 8 * 1024) {
-    float h[8];
-    load8<T, VEC>(x + at, a.width - at, h);
+  for (int j = 0; j < turns; ++j) {
+    const Place u(j * 1024 + threadIdx.x, a.width);
+    float h[16];
+    load16<T, VEC>(x, u, h);
     if (a.residual) {
-      float r[8];
-      load8<T, VEC>((const T*)a.residual + row * a.residual_stride + at, a.width - at, r);
-      sum8<T, VEC>(a, row, at, a.width - at, h, r);
+      float r[16];
+      load16<T, VEC>((const T*)a.residual + row * a.residual_stride, u, r);
+      sum16<T, VEC>(a, row, u, r, h);
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fma((double)h[i], (double)h[i], sum);
+    sum = add_squares(h, sum);
   }
   const Factor f = a.weight ? norm_factor(team_sum<1024>(sum), a) : Factor();
   const T* from = a.residual ? (const T*)a.sum + row * a.sum_stride : x;
-  for (int at = threadIdx.x * 8; at < all; at += 8 * 1024) {
-    const int left = a.width - at;
-    float h[8];
-    load8<T, VEC>(from + at, left, h);
-    norm8<T, VEC>(a, at, left, f, h);
-    finish8<T, VEC>(a, row, at, left, h);
+  for (int j = 0; j < turns; ++j) {
+    const Place u(j * 1024 + threadIdx.x, a.width);
+    float h[16];
+    load16<T, VEC>(from, u, h);
+    if (a.weight) {
+      float w[16];
+      weights16<T, VEC>(a, u, w);
+      norm16(f, w, h);
+    }
+    finish16<T, VEC>(a, row, u, h);
   }
 }
 
-template <class T, int TEAM, int VPT, bool VEC>
+template <class T, int TEAM, int U, bool VEC>
 cudaError_t run(const NormArgs& a, cudaStream_t s) {
-  const int per = TEAM == 32 ? 8 : 1;
-  k_norm<T, TEAM, VPT, VEC><<<(a.rows + per - 1) / per, TEAM == 32 ? 256 : TEAM, 0, s>>>(a);
-  return cudaGetLastError();
+  const int per = TEAM <= 32 ? 256 / TEAM : 1;
+  return launch_early(k_norm<T, TEAM, U, VEC>, dim3((a.rows + per - 1) / per), dim3(TEAM <= 32 ? 256 : TEAM), 0, s, 1, a);
 }
 
 template <class T, bool VEC>
 cudaError_t dispatch(const NormArgs& a, cudaStream_t s) {
   const int w = a.width;
-  if (w <= 256) return run<T, 32, 1, VEC>(a, s);
-  if (w <= 1024) return run<T, 32, 4, VEC>(a, s);
-  if (w <= 2048) return run<T, 256, 1, VEC>(a, s);
-  if (w <= 4096) return run<T, 256, 2, VEC>(a, s);
-  if (w <= 8192) return run<T, 512, 2, VEC>(a, s);
-  k_norm_long<T, VEC><<<a.rows, 1024, 0, s>>>(a);
-  return cudaGetLastError();
+  if (w <= 128) return run<T, 8, 1, VEC>(a, s);
+  if (w <= 512) return run<T, 32, 1, VEC>(a, s);
+  if (w <= 1024) return run<T, 64, 1, VEC>(a, s);
+  if (w <= 2048) return run<T, 128, 1, VEC>(a, s);
+  if (w <= 4096) return run<T, 256, 1, VEC>(a, s);
+  if (w <= 8192) return run<T, 512, 1, VEC>(a, s);
+  return launch_early(k_norm_long<T, VEC>, dim3(a.rows), dim3(1024), 0, s, 1, a);
 }
 
 template <class T>
@@ -286,8 +339,10 @@ cudaError_t by_alignment(const NormArgs& a, cudaStream_t s) {
 
 }  // namespace
 
-cudaError_t launch_rms_norm(const NormArgs& a, cudaStream_t s) {
-  if (a.rows <= 0) return cudaSuccess;
+cudaError_t launch_rms_norm(const NormArgs& args, cudaStream_t s) {
+  if (args.rows <= 0) return cudaSuccess;
+  NormArgs a = args;
+  a.inv_width = 1.0 / a.width;
   if (a.type == kRowF32) return by_alignment<float>(a, s);
   if (a.type == kRowF16) return by_alignment<__half>(a, s);
   return by_alignment<__nv_bfloat16>(a, s);

@@ -7,20 +7,22 @@
 // p t_i is formed in 64 bits and brought to an eighth of a turn around a
 // quarter turn before anything is rounded to f32, so positions of any size
 // lose nothing. A block computes the angles of its rows once for all heads
-// while its first values load. Bound by bytes, each read and written once.
+// while its first values load; a thread then keeps those of its pairs in
+// registers. Bound by bytes, each read and written once.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
 
+#include "launch.cuh"
 #include "rows.h"
 
 namespace trit {
 namespace {
 
 constexpr int kRotaryThreads = 256;
-constexpr int kRotaryAhead = 2;  // units a thread loads before it works on the first
+constexpr int kRotaryAhead = 4;  // heads a thread loads before it works on the first
 
 template <class T>
 __device__ __forceinline__ float wide(T v) {
@@ -58,27 +60,16 @@ __device__ __forceinline__ void store(T* p, const Pack<T, V>& r) {
   }
 }
 
-// n / d for n < 2^31 by a multiplication.
-struct Divide {
-  uint32_t by = 1, mul = 0, shift = 0;
-  explicit Divide(uint32_t d) : by(d) {
-    // ceil(2^(32 + shift) / d) with 2^shift >= d: the error stays below 1 / d.
-    while ((1ull << shift) < d) ++shift;
-    mul = (uint32_t)(((1ull << (32 + shift)) + d - 1) / d - (1ull << 32));
-  }
-  __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
-    return (uint32_t)(((unsigned long long)__umulhi(n, mul) + n) >> shift);
-  }
-};
-
-// The work on a row: `units` of V values (halves: V pairs, both their halves),
-// head after head, queries before keys, and behind the rotated units of a
-// head the copied ones.
+// How a block of threads shares out its rows and heads. A unit is V values, or
+// V pairs of halves; `at` counts a head's units, those that turn first. A
+// thread keeps one unit's place and row, so that it reads its angles once, and
+// goes through every `head_lanes`-th head.
 struct RotaryWork {
   RotaryArgs a;
-  int hd, rd, turning, per_head;  // units of a head that turn, and all of them
-  int rows_per_block, heads_per_block;
-  Divide by_row, by_head, by_pairs;
+  int turning, per_head;  // units of a head that turn, and all of them
+  int lanes;              // units of a head side by side: per_head, at most the block
+  int rows, head_lanes;   // rows of a block; threads a unit and row
+  int heads;              // of a block
 };
 
 // cos and sin of t turns, times f.
@@ -97,99 +88,83 @@ __device__ __forceinline__ float2 turn(double t, float f) {
 template <class T, int V, bool INTER, bool ALIGNED>
 __global__ void __launch_bounds__(kRotaryThreads) k_rotary(const __grid_constant__ RotaryTable table,
                                                            const __grid_constant__ RotaryWork w) {
-  extern __shared__ float2 angles[];  // [rows of the block][pairs]
+  constexpr int PV = INTER ? V / 2 : V;  // pairs of a unit
+  extern __shared__ float2 angles[];     // [row][pair of its unit][unit]: a warp's units lie side by side
   const RotaryArgs& a = w.a;
-  const int row0 = blockIdx.x * w.rows_per_block, rows = min(w.rows_per_block, a.rows - row0);
-  const int head0 = blockIdx.y * w.heads_per_block, heads = min(w.heads_per_block, a.q_heads + a.k_heads - head0);
-  const int pairs = w.rd / 2, row_units = heads * w.per_head, units = rows * row_units;
-  // by_row is for a full set of heads; the last blocks of a row divide.
-  const bool full = heads == w.heads_per_block;
+  const int pairs = table.rotary_dim / 2, slots = w.turning * PV;
+  const int row0 = blockIdx.x * w.rows, rows = min(w.rows, a.rows - row0);
+  const int head_end = min((int)(blockIdx.y + 1) * w.heads, a.q_heads + a.k_heads);
+  const int lane = threadIdx.x % w.lanes, team = threadIdx.x / w.lanes, r = team % w.rows, head_lane = team / w.rows;
+  const int first = r < rows && head_lane < w.head_lanes ? (int)blockIdx.y * w.heads + head_lane : head_end;
+  const T* const q = (const T*)a.q + (size_t)(row0 + r) * a.q_stride;
+  const T* const k = (const T*)a.k + (size_t)(row0 + r) * a.k_stride;
+  T* const qo = (T*)a.q_out + (size_t)(row0 + r) * a.q_out_stride;
+  T* const ko = (T*)a.k_out + (size_t)(row0 + r) * a.k_out_stride;
+  const int hd = table.head_dim, rd = table.rotary_dim;
 
-  struct Unit {
-    const T* from;
-    T* to;
-    int row, at;  // the unit's place in its head; -1: none
-  };
-  auto find = [&](int u) {
-    Unit r;
-    r.at = -1;
-    if (u >= units) return r;
-    r.row = full ? w.by_row(u) : u / row_units;
-    const int rem = u - r.row * row_units, h = w.by_head(rem);
-    r.at = rem - h * w.per_head;
-    const int head = head0 + h;
-    const size_t row = row0 + r.row;
-    if (head < a.q_heads) {
-      r.from = (const T*)a.q + row * a.q_stride + (size_t)head * w.hd;
-      r.to = (T*)a.q_out + row * a.q_out_stride + (size_t)head * w.hd;
-    } else {
-      r.from = (const T*)a.k + row * a.k_stride + (size_t)(head - a.q_heads) * w.hd;
-      r.to = (T*)a.k_out + row * a.k_out_stride + (size_t)(head - a.q_heads) * w.hd;
-    }
-    return r;
-  };
   using P = Pack<T, V>;
-  auto fetch = [&](const Unit& r, P& lo, P& hi) {
-    if (r.at < 0) return;
-    if (INTER) {
-      lo = load<T, V, ALIGNED>(r.from + r.at * V);
-    } else if (r.at < w.turning) {
-      lo = load<T, V, ALIGNED>(r.from + r.at * V);
-      hi = load<T, V, ALIGNED>(r.from + r.at * V + pairs);
-    } else {
-      lo = load<T, V, ALIGNED>(r.from + w.rd + (r.at - w.turning) * V);
+  P lo[kRotaryAhead], hi[kRotaryAhead];
+  // The unit's values of the next heads from h on.
+  auto fetch = [&](int at, int h) {
+#pragma unroll
+    for (int i = 0; i < kRotaryAhead; ++i) {
+      const int head = h + i * w.head_lanes;
+      if (head >= head_end) break;
+      const T* from = head < a.q_heads ? q + head * hd : k + (head - a.q_heads) * hd;
+      if (INTER || at < w.turning) from += at * V;
+      else from += rd + (at - w.turning) * V;
+      lo[i] = load<T, V, ALIGNED>(from);
+      if (!INTER && at < w.turning) hi[i] = load<T, V, ALIGNED>(from + pairs);
     }
   };
-  Unit unit[kRotaryAhead];
-  P lo[kRotaryAhead], hi[kRotaryAhead];
-#pragma unroll
-  for (int i = 0; i < kRotaryAhead; ++i) {
-    unit[i] = find(threadIdx.x + i * kRotaryThreads);
-    fetch(unit[i], lo[i], hi[i]);
-  }
+  let_next_start();
+  after_kernel_before();
+  if (first < head_end && lane < w.per_head) fetch(lane, first);
   for (int i = threadIdx.x; i < rows * pairs; i += kRotaryThreads) {
-    const int r = w.by_pairs(i);
-    angles[i] = turn((double)a.positions[row0 + r] * table.turns[i - r * pairs], table.factor);
+    const int row = i / pairs, p = i - row * pairs;
+    angles[row * slots + p % PV * w.turning + p / PV] =
+        turn((double)__ldg(a.positions + row0 + row) * table.turns[p], table.factor);
   }
   __syncthreads();
-  for (int u0 = 0; u0 < units; u0 += kRotaryAhead * kRotaryThreads) {
+  for (int at = lane; at < w.per_head; at += w.lanes) {
+    float2 cs[PV];
+    // An interleaved unit may reach behind the last pair: those values stay.
+    const int turns = at < w.turning ? min(PV, pairs - at * PV) : 0;
 #pragma unroll
-    for (int i = 0; i < kRotaryAhead; ++i) {
-      const Unit& r = unit[i];
-      if (r.at < 0) continue;
-      const float2* cs = angles + r.row * pairs;
-      if (INTER) {
-        P o = lo[i];
-        const int first = r.at * V;
+    for (int j = 0; j < PV; ++j)
+      cs[j] = j < turns ? angles[r * slots + j * w.turning + at] : make_float2(1.0f, 0.0f);
+    for (int h = first; h < head_end; h += kRotaryAhead * w.head_lanes) {
+      if (at != lane || h != first) fetch(at, h);
 #pragma unroll
-        for (int j = 0; j < V; j += 2) {
-          if (first + j >= w.rd) break;  // rd is even: a pair turns as a whole
-          const float2 t = cs[(first + j) / 2];
-          const float x = wide(lo[i].v[j]), y = wide(lo[i].v[j + 1]);
-          o.v[j] = narrow<T>(x * t.x - y * t.y);
-          o.v[j + 1] = narrow<T>(y * t.x + x * t.y);
+      for (int i = 0; i < kRotaryAhead; ++i) {
+        const int head = h + i * w.head_lanes;
+        if (head >= head_end) break;
+        T* to = head < a.q_heads ? qo + head * hd : ko + (head - a.q_heads) * hd;
+        if (INTER) {
+          P o = lo[i];
+#pragma unroll
+          for (int j = 0; j < PV; ++j) {
+            const float x = wide(lo[i].v[2 * j]), y = wide(lo[i].v[2 * j + 1]);
+            if (j < turns) {
+              o.v[2 * j] = narrow<T>(x * cs[j].x - y * cs[j].y);
+              o.v[2 * j + 1] = narrow<T>(y * cs[j].x + x * cs[j].y);
+            }
+          }
+          store<T, V, ALIGNED>(to + at * V, o);
+        } else if (at < w.turning) {
+          P x, y;
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float u = wide(lo[i].v[j]), v = wide(hi[i].v[j]);
+            x.v[j] = narrow<T>(u * cs[j].x - v * cs[j].y);
+            y.v[j] = narrow<T>(v * cs[j].x + u * cs[j].y);
+          }
+          store<T, V, ALIGNED>(to + at * V, x);
+          store<T, V, ALIGNED>(to + at * V + pairs, y);
+        } else {
+          store<T, V, ALIGNED>(to + rd + (at - w.turning) * V, lo[i]);
         }
-        store<T, V, ALIGNED>(r.to + first, o);
-      } else if (r.at < w.turning) {
-        P p, q;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float2 t = cs[r.at * V + j];
-          const float x = wide(lo[i].v[j]), y = wide(hi[i].v[j]);
-          p.v[j] = narrow<T>(x * t.x - y * t.y);
-          q.v[j] = narrow<T>(y * t.x + x * t.y);
-        }
-        store<T, V, ALIGNED>(r.to + r.at * V, p);
-        store<T, V, ALIGNED>(r.to + r.at * V + pairs, q);
-      } else {
-        store<T, V, ALIGNED>(r.to + w.rd + (r.at - w.turning) * V, lo[i]);
       }
-    }
-    if (u0 + kRotaryAhead * kRotaryThreads >= units) break;
-#pragma unroll
-    for (int i = 0; i < kRotaryAhead; ++i) {
-      unit[i] = find(u0 + (kRotaryAhead + i) * kRotaryThreads + threadIdx.x);
-      fetch(unit[i], lo[i], hi[i]);
     }
   }
 }
@@ -199,22 +174,27 @@ cudaError_t run(const RotaryTable& t, const RotaryArgs& a, cudaStream_t s) {
   const int pairs = t.rotary_dim / 2, heads = a.q_heads + a.k_heads;
   // In place, the values behind the pairs stay as they are.
   const bool still = a.q == a.q_out && a.k == a.k_out;
-  const int turning = INTER ? ((still ? t.rotary_dim : t.head_dim) + V - 1) / V : pairs / V;
-  const int per_head = INTER || still ? turning : turning + (t.head_dim - t.rotary_dim) / V;
-  // Blocks of several rows, so that a thread has a few units; where the rows
-  // alone do not fill the SMs, a block takes a part of the heads.
-  const int row_units = heads * per_head;
-  const int rows = std::max(1, std::min(std::min(4, 4 * kRotaryThreads / std::max(1, row_units)), a.rows));
-  const int row_blocks = (a.rows + rows - 1) / rows;
-  const int wanted = 2 * current_sm_count();
-  int parts = std::max(1, std::min(heads, wanted / row_blocks));
-  while (parts > 1 && (heads + parts - 1) / parts * per_head * rows < kRotaryThreads / 2) --parts;
-  const int heads_per_block = (heads + parts - 1) / parts;
-  const RotaryWork w{a, t.head_dim, t.rotary_dim, turning, per_head, rows, heads_per_block,
-                     Divide(heads_per_block * per_head), Divide(per_head), Divide(pairs)};
-  k_rotary<T, V, INTER, ALIGNED><<<dim3(row_blocks, (heads + heads_per_block - 1) / heads_per_block), kRotaryThreads,
-                                   (size_t)rows * pairs * sizeof(float2), s>>>(t, w);
-  return cudaGetLastError();
+  RotaryWork w{a};
+  w.turning = INTER ? (t.rotary_dim + V - 1) / V : pairs / V;
+  w.per_head = still ? w.turning : INTER ? t.head_dim / V : w.turning + (t.head_dim - t.rotary_dim) / V;
+  w.lanes = std::min(w.per_head, kRotaryThreads);
+  const int teams = kRotaryThreads / w.lanes;
+  // Many rows: a thread goes through about eight heads. Few: a block has one
+  // row, and its heads are cut so that the blocks fill the SMs.
+  const long long threads = (long long)a.rows * heads * w.lanes / 8;
+  if (threads >= (long long)current_sm_count() * 512) {
+    w.head_lanes = std::min(teams, (heads + 7) / 8);
+    w.rows = std::min(std::min(teams / w.head_lanes, 8), a.rows);
+    w.heads = heads;
+  } else {
+    w.rows = 1;
+    const int parts = std::max(1, std::min((heads + teams - 1) / teams * kRotaryAhead, 2 * current_sm_count() / a.rows));
+    w.heads = (heads + parts - 1) / parts;
+    w.head_lanes = std::min(teams, w.heads);
+  }
+  return launch_early(k_rotary<T, V, INTER, ALIGNED>,
+                      dim3((a.rows + w.rows - 1) / w.rows, (heads + w.heads - 1) / w.heads), dim3(kRotaryThreads),
+                      (size_t)w.rows * w.turning * (INTER ? V / 2 : V) * sizeof(float2), s, 1, t, w);
 }
 
 // The widest units that the sizes, strides and addresses allow.

@@ -52,7 +52,7 @@ struct NormArgs {
   size_t x_stride = 0, residual_stride = 0, sum_stride = 0, out_stride = 0;
   int rows = 0, width = 0;
   int type = 0, weight_f32 = 0;
-  double eps = 0.0;
+  double eps = 0.0, inv_width = 0.0;  // (the latter set by the launch)
 };
 cudaError_t launch_rms_norm(const NormArgs& a, cudaStream_t s);
 // The arguments of a caller's norm, checked, and the norm.
