@@ -17,14 +17,13 @@
 //              the tile through shared memory in whole lines.
 // Every wait is bounded in time and reports through a status word.
 #include <cuda.h>
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
 
 #include "device.cuh"
 #include "launch.cuh"
+#include "rows.cuh"
 #include "rows.h"
 #include "tc.cuh"
 
@@ -113,13 +112,8 @@ __device__ __forceinline__ float4 scales4(const float* sx, int b, int blocks, bo
   return v;
 }
 
-__device__ __forceinline__ uint32_t pack2(float a, float b, bool f16) {
-  if (f16) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *(const uint32_t*)&h;
-  }
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *(const uint32_t*)&h;
+__device__ __forceinline__ uint32_t pack16(float a, float b, bool f16) {
+  return f16 ? pack2<__half>(make_float2(a, b)) : pack2<__nv_bfloat16>(make_float2(a, b));
 }
 
 // A warp's 32 rows (a lane each) x CW columns to out, through 4 KB of shared
@@ -197,7 +191,7 @@ __device__ __forceinline__ void store_tile(const float2 (&acc)[CW / 2], uint8_t*
       for (int u = 0; u < CC / 8; ++u) {
         const float2* v = &acc[c / 2 + 4 * u];
         *(uint4*)(staging + lane * 128 + ((u ^ (lane & 7)) << 4)) =
-            make_uint4(pack2(v[0].x, v[0].y, f16), pack2(v[1].x, v[1].y, f16), pack2(v[2].x, v[2].y, f16), pack2(v[3].x, v[3].y, f16));
+            make_uint4(pack16(v[0].x, v[0].y, f16), pack16(v[1].x, v[1].y, f16), pack16(v[2].x, v[2].y, f16), pack16(v[3].x, v[3].y, f16));
       }
       chunk(col0 + c, CC / 8);
     }
@@ -254,13 +248,13 @@ __device__ __forceinline__ void join_parts(const uint8_t* part, const Fp8Args& a
     uint8_t* p = (uint8_t*)a.out + ((size_t)(row0 + r) * a.out_stride + at) * size;
     if (vec && at + 4 <= a.n) {
       if (f32) *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
-      else *(uint2*)p = make_uint2(pack2(v[0], v[1], f16), pack2(v[2], v[3], f16));
+      else *(uint2*)p = make_uint2(pack16(v[0], v[1], f16), pack16(v[2], v[3], f16));
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (at + j >= a.n) break;
         if (f32) ((float*)p)[j] = v[j];
-        else ((uint16_t*)p)[j] = (uint16_t)pack2(v[j], 0.0f, f16);
+        else ((uint16_t*)p)[j] = (uint16_t)pack16(v[j], 0.0f, f16);
       }
     }
   }

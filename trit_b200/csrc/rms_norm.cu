@@ -16,36 +16,27 @@
 // of a group (two runs of 8, so that a warp's loads are whole lines), 8 threads
 // share the group's maximum with shuffles, and the two quotients, the row's
 // root and the products are written with what is exact and cheap.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
 
 #include "device.cuh"
 #include "launch.cuh"
+#include "rows.cuh"
 #include "rows.h"
 
 namespace trit {
 namespace {
 
 template <class T>
-__device__ __forceinline__ float to_f32(T v);
-template <>
-__device__ __forceinline__ float to_f32<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <class T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ float from_f32<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
+__device__ __forceinline__ void unpack8(const uint32_t (&w)[4], float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = unpack2<T>(w[i]);
+    v[2 * i] = x.x;
+    v[2 * i + 1] = x.y;
+  }
+}
 // 8 values at p (16-byte aligned), or zeros.
 template <class T>
 __device__ __forceinline__ void load8(const T* p, int left, float (&v)[8]) {
@@ -58,9 +49,8 @@ __device__ __forceinline__ void load8(const T* p, int left, float (&v)[8]) {
     v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   } else {
     const uint4 a = *(const uint4*)p;
-    const T* h = (const T*)&a;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_f32(h[i]);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    unpack8<T>(w, v);
   }
 }
 template <class T>
@@ -70,11 +60,8 @@ __device__ __forceinline__ void store8(T* p, int left, const float (&v)[8]) {
     *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
     *(float4*)(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
   } else {
-    uint4 a;
-    T* h = (T*)&a;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = from_f32<T>(v[i]);
-    *(uint4*)p = a;
+    *(uint4*)p = make_uint4(pack2<T>(make_float2(v[0], v[1])), pack2<T>(make_float2(v[2], v[3])),
+                            pack2<T>(make_float2(v[4], v[5])), pack2<T>(make_float2(v[6], v[7])));
   }
 }
 
@@ -264,16 +251,15 @@ struct Loaded {
     if constexpr (PACKED) {
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        uint32_t* v = (uint32_t*)&x[g];
+        uint32_t v[4] = {x[g].x, x[g].y, x[g].z, x[g].w};
         if (a.residual) {
-          const uint32_t* w = (const uint32_t*)&r[g];
+          const uint32_t w[4] = {r[g].x, r[g].y, r[g].z, r[g].w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) v[i] = add_packed<T>(v[i], w[i]);
-          if ((g ? u.left1 : u.left0) > 0) *(uint4*)((T*)a.sum + row * a.sum_stride + u.at + g * 64) = x[g];
+          if ((g ? u.left1 : u.left0) > 0)
+            *(uint4*)((T*)a.sum + row * a.sum_stride + u.at + g * 64) = make_uint4(v[0], v[1], v[2], v[3]);
         }
-        const T* t = (const T*)v;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) h[g * 8 + i] = to_f32(t[i]);
+        unpack8<T>(v, *(float (*)[8])(h + g * 8));
       }
     } else {
       load16((const T*)a.x + row * a.x_stride, u, h);
