@@ -45,6 +45,7 @@ struct F8Shape {
   static constexpr int BUFS = BN * 4 * BLOCKS_ > 512 ? 2 : 4;
   static constexpr int COLS = BUFS * BN;                      // of TMEM
   static constexpr int STAGING = ROW_WARPS * COLUMN_WARPS * 4096;
+  static_assert(STAGE % 1024 == 0, "swizzled rows begin at whole kilobytes");
   static constexpr int TAIL = (128 - AR) * F8_K > STAGING ? (128 - AR) * F8_K : STAGING;  // behind the stages
   static constexpr int BLOCKS = BLOCKS_;                      // an SM holds
   static constexpr int ROOM = 226 * 1024 / BLOCKS - 2048 - 1024 - TAIL;  // (a block's own 1 KB, and its static memory)
@@ -116,60 +117,55 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, bool f16) {
   return f16 ? pack2<__half>(make_float2(a, b)) : pack2<__nv_bfloat16>(make_float2(a, b));
 }
 
-// A warp's 32 rows (a lane each) x CW columns to out, through 4 KB of shared
-// memory of its own: 16-byte unit u of row r lies at u ^ (r % 8).
+// A warp's 32 rows (a lane each) x CW columns to out, in chunks of 128 bytes a
+// row through 4 KB of shared memory of its own: 16-byte unit u of row r lies at
+// u ^ (r % 8), as the tensor copies' 128-byte swizzle has it. Where out's rows
+// are 16-byte aligned (a.tma), a chunk leaves by one tensor copy, which ends at
+// out's last row and column by itself, and the warp goes on meanwhile.
 template <int CW>
-__device__ __forceinline__ void store_tile(const float2 (&acc)[CW / 2], uint8_t* staging, const Fp8Args& a, int row0,
-                                           int col0, int lane) {
+__device__ __forceinline__ void store_tile(const float2 (&acc)[CW / 2], uint8_t* staging, const CUtensorMap& omap,
+                                           const Fp8Args& a, int row0, int col0, int lane) {
   const int rows = min(32, a.m - row0);
   const bool f32 = a.type == kRowF32, f16 = a.type == kRowF16;
   const int size = f32 ? 4 : 2;
-  const bool vec = (((uintptr_t)a.out | a.out_stride * size) & 15) == 0;
-  uint8_t* out = (uint8_t*)a.out + (size_t)row0 * a.out_stride * size;
-  // A chunk is up to 128 bytes of every row.
-  auto chunk = [&](int col, int units) {
+  uint8_t* const out = (uint8_t*)a.out + (size_t)row0 * a.out_stride * size;
+  // The chunk before has left the staging memory.
+  auto begin = [&]() {
+    if (a.tma && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     __syncwarp();
-    if (vec) {
-      const int u = lane % units, per = 32 / units, values = 16 / size;
-#pragma unroll 4
-      for (int r = lane / units; r < rows; r += per) {
-        const uint4 v = *(const uint4*)(staging + r * 128 + ((u ^ (r & 7)) << 4));
-        const int at = col + u * values;
-        uint8_t* p = out + ((size_t)r * a.out_stride + at) * size;
-        if (at + values <= a.n) {
-          *(uint4*)p = v;
-        } else {
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (f32 && i < 4 && at + i < a.n) ((uint32_t*)p)[i] = w[i & 3];
-            if (!f32 && at + i < a.n) ((uint16_t*)p)[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-          }
-        }
+  };
+  auto chunk = [&](int col) {
+    if (a.tma) {
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0 && col < a.n) {
+        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"((uint64_t)&omap),
+                     "r"(smem_u32(staging)), "r"(col), "r"(row0)
+                     : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
-    } else {
-      // Rows that start anywhere: a lane stores four bytes where they are
-      // aligned, so with an odd start of 16-bit rows a lane's two values begin
-      // one earlier, and lane 0 has the first and the last one alone.
-      const int live = min(units * 16 / size, a.n - col);
+      return;
+    }
+    __syncwarp();
+    const int live = min(128 / size, a.n - col);
 #pragma unroll 8
-      for (int r = 0; r < 32; ++r) {
-        if (r >= rows) break;
-        const uint8_t* from = staging + r * 128;
-        uint8_t* p = out + ((size_t)r * a.out_stride + col) * size;
-        if (f32) {
-          if (lane < live) ((uint32_t*)p)[lane] = *(const uint32_t*)(from + ((lane / 4 ^ (r & 7)) << 4) + (lane & 3) * 4);
-          continue;
-        }
-        const auto get = [&](int e) { return *(const uint16_t*)(from + ((e / 8 ^ (r & 7)) << 4) + (e & 7) * 2); };
-        const int odd = (int)((uintptr_t)p >> 1 & 1), e = 2 * lane - odd;
-        if (e >= 0 && e + 1 < live) {
-          *(uint32_t*)(p + 2 * e) = (uint32_t)get(e) | (uint32_t)get(e + 1) << 16;
-        } else {
-          if (e < 0 && live > 0) ((uint16_t*)p)[0] = get(0);
-          if (e >= 0 && e < live) ((uint16_t*)p)[e] = get(e);
-        }
-        if (odd && lane == 0 && live == 64) ((uint16_t*)p)[63] = get(63);
+    for (int r = 0; r < 32; ++r) {
+      if (r >= rows) break;
+      const uint32_t w = *(const uint32_t*)(staging + r * 128 + ((lane / 4 ^ (r & 7)) << 4) + (lane & 3) * 4);
+      uint8_t* p = out + ((size_t)r * a.out_stride + col) * size;
+      if (f32) {
+        if (lane < live) ((uint32_t*)p)[lane] = w;
+        continue;
+      }
+      // (A word of a row that starts on an odd place: see below.)
+      const int odd = (int)((uintptr_t)p >> 1 & 1), e = 2 * lane - odd;
+      if (e >= 0 && e + 1 < live) {
+        *(uint32_t*)(p + 2 * e) = w;
+      } else if (e >= 0) {
+        if (e < live) ((uint16_t*)p)[e] = (uint16_t)w;
+      } else {
+        if (live > 0) ((uint16_t*)p)[0] = (uint16_t)(w >> 16);
+        if (live == 64) ((uint16_t*)p)[63] = (uint16_t)w;
       }
     }
     __syncwarp();
@@ -177,23 +173,33 @@ __device__ __forceinline__ void store_tile(const float2 (&acc)[CW / 2], uint8_t*
   if (f32) {
 #pragma unroll
     for (int c = 0; c < CW; c += 32) {
+      begin();
 #pragma unroll
       for (int u = 0; u < 8; ++u)
         *(float4*)(staging + lane * 128 + ((u ^ (lane & 7)) << 4)) =
             make_float4(acc[c / 2 + 2 * u].x, acc[c / 2 + 2 * u].y, acc[c / 2 + 2 * u + 1].x, acc[c / 2 + 2 * u + 1].y);
-      chunk(col0 + c, 8);
+      chunk(col0 + c);
     }
   } else {
-    constexpr int CC = CW < 64 ? CW : 64;
 #pragma unroll
-    for (int c = 0; c < CW; c += CC) {
+    for (int c = 0; c < CW; c += 64) {
+      begin();
+      // A row that starts between two words has its values one half further
+      // on: word i holds values 2 i - 1 and 2 i, the first one the last value
+      // and value 0.
+      const bool odd = !a.tma && ((((uintptr_t)out >> 1) + (size_t)lane * a.out_stride + col0 + c) & 1);
 #pragma unroll
-      for (int u = 0; u < CC / 8; ++u) {
-        const float2* v = &acc[c / 2 + 4 * u];
-        *(uint4*)(staging + lane * 128 + ((u ^ (lane & 7)) << 4)) =
-            make_uint4(pack16(v[0].x, v[0].y, f16), pack16(v[1].x, v[1].y, f16), pack16(v[2].x, v[2].y, f16), pack16(v[3].x, v[3].y, f16));
+      for (int u = 0; u < 8; ++u) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 v = acc[c / 2 + 4 * u + i];
+          const float before = acc[c / 2 + (4 * u + i + 31) % 32].y;
+          w[i] = odd ? pack16(before, v.x, f16) : pack16(v.x, v.y, f16);
+        }
+        *(uint4*)(staging + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      chunk(col0 + c, CC / 8);
+      chunk(col0 + c);
     }
   }
 }
@@ -262,7 +268,7 @@ __device__ __forceinline__ void join_parts(const uint8_t* part, const Fp8Args& a
 
 template <int AR, int BN, int BLOCKS>
 __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
-    k_fp8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Fp8Args a) {
+    k_fp8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap omap, const __grid_constant__ Fp8Args a) {
   using S = F8Shape<AR, BN, BLOCKS>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -433,8 +439,10 @@ __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
           }
         }
         if (S::SPLITS && splits > 1) put_part<S::CW, BN>(acc, base, quarter * 32 + lane, part * S::CW);
-        else if (ok && row0 < a.m) store_tile<S::CW>(acc, staging, a, row0, col0, lane);
+        else if (ok && row0 < a.m) store_tile<S::CW>(acc, staging, omap, a, row0, col0, lane);
       }
+      // The last chunks have left shared memory before it is given back.
+      if (a.tma && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
   }
   fence_before();
@@ -454,7 +462,7 @@ __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
 }
 
 template <int AR, int BN, int BLOCKS>
-cudaError_t run(const TcMap& x, const Fp8Args& a, int splits, cudaStream_t s) {
+cudaError_t run(const TcMap& x, const TcMap& out, const Fp8Args& a, int splits, cudaStream_t s) {
   using S = F8Shape<AR, BN, BLOCKS>;
   static_assert(S::STAGES >= 3 && S::STAGES <= 12 && S::SMEM + (int)sizeof(F8Sync) <= 227 * 1024, "shared memory");
   static_assert(AR * BN * 4 <= S::STAGES * S::STAGE, "a split's sums");
@@ -478,7 +486,7 @@ cudaError_t run(const TcMap& x, const Fp8Args& a, int splits, cudaStream_t s) {
   // Blocks take tile after tile; those of a cluster have one.
   const long long grid = splits > 1 ? tiles * splits : std::min<long long>(tiles, current_sm_count() * BLOCKS);
   return launch_early(k_fp8<AR, BN, BLOCKS>, dim3((unsigned)grid), dim3(S::THREADS), S::SMEM, s, (unsigned)splits,
-                      *(const CUtensorMap*)&x, a);
+                      *(const CUtensorMap*)&x, *(const CUtensorMap*)&out, a);
 }
 
 // Rows of bytes to the units that k_fp8 reads: [n / 64][k / 128][64 rows][128
@@ -507,7 +515,7 @@ cudaError_t launch_fp8_pack(const uint8_t* codes, size_t n, size_t k, uint8_t* w
   return cudaGetLastError();
 }
 
-cudaError_t launch_fp8(const TcMap& x, const Fp8Args& a, cudaStream_t s) {
+cudaError_t launch_fp8(const TcMap& x, const TcMap& out, const Fp8Args& a, cudaStream_t s) {
   if (a.m <= 0) return cudaSuccess;
   const long long sms = current_sm_count();
   const auto tiles = [&](int bn) { return (a.m + 127LL) / 128 * ((a.n + bn - 1) / bn); };
@@ -518,11 +526,11 @@ cudaError_t launch_fp8(const TcMap& x, const Fp8Args& a, cudaStream_t s) {
     return z;
   };
   const int box = fp8_row_box(a.m);
-  if (box == 16) return run<16, 64, 2>(x, a, splits(tiles(64), 2 * sms), s);
-  if (box == 64) return run<64, 64, 2>(x, a, splits(tiles(64), 2 * sms), s);
+  if (box == 16) return run<16, 64, 2>(x, out, a, splits(tiles(64), 2 * sms), s);
+  if (box == 64) return run<64, 64, 2>(x, out, a, splits(tiles(64), 2 * sms), s);
   const auto waves = [&](int bn) { return (double)((tiles(bn) + sms - 1) / sms); };
-  if (waves(128) * 0.385 < waves(256) * 0.6) return run<128, 128, 1>(x, a, splits(tiles(128), sms), s);
-  return run<128, 256, 1>(x, a, 1, s);
+  if (waves(128) * 0.385 < waves(256) * 0.6) return run<128, 128, 1>(x, out, a, splits(tiles(128), sms), s);
+  return run<128, 256, 1>(x, out, a, 1, s);
 }
 
 }  // namespace trit

@@ -358,7 +358,9 @@ void DenseFp8::product(const void* codes, const float* scales, size_t m, void* o
   a.blocks = (int)((k_ + kFp8Group - 1) / kFp8Group);
   a.type = type;
   a.status = status_;
-  TRIT_CUDA(launch_fp8(map, a, s));
+  TcMap out_map{};
+  a.tma = make_fp8_out_map(&out_map, out, m, n_, out_stride, type) == cudaSuccess;
+  TRIT_CUDA(launch_fp8(map, out_map, a, s));
 }
 
 void DenseFp8::forward_codes(const void* codes, const float* scales, size_t m, void* out, size_t out_stride, int type,

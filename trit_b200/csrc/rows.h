@@ -121,16 +121,19 @@ struct Fp8Args {
   void* out = nullptr;
   size_t out_stride = 0;
   int m = 0, n = 0, blocks = 0;  // blocks of 128 values of k
-  int type = 0;
+  int type = 0, tma = 0;         // tma: out has a map (make_fp8_out_map)
   int* status = nullptr;
 };
 // A TMA map of 8-bit numbers [rows][k], row stride k, boxes of 128 values x
 // box_rows rows with the 128-byte swizzle; past either end reads zero.
 cudaError_t make_fp8_map(TcMap* out, const void* base, size_t rows, size_t k, int box_rows);
+// A TMA map of out, boxes of 128 bytes x 32 rows with the same swizzle; its rows
+// have to be 16-byte aligned.
+cudaError_t make_fp8_out_map(TcMap* out, void* base, size_t rows, size_t n, size_t stride, int type);
 int fp8_row_box(int m);  // its box rows for m rows
 // The weights [n][k] in the order that the product reads them.
 size_t fp8_packed_bytes(size_t n, size_t k);
 cudaError_t launch_fp8_pack(const uint8_t* codes, size_t n, size_t k, uint8_t* w, cudaStream_t s);
-cudaError_t launch_fp8(const TcMap& x, const Fp8Args& a, cudaStream_t s);
+cudaError_t launch_fp8(const TcMap& x, const TcMap& out, const Fp8Args& a, cudaStream_t s);
 
 }  // namespace trit
