@@ -260,28 +260,36 @@ void Rotary::apply(RotaryArgs a, size_t rows, cudaStream_t s) const {
 }
 
 // -------------------------------------------------------------- products
-namespace {
-// Scratch of calls that round their rows first. Memory of a pool comes and
-// goes in the order of the call's stream, so calls on several streams may
-// overlap; the pool keeps what it has across synchronisations.
-cudaMemPool_t scratch_pool(int device) {
-  static std::mutex mu;
-  static cudaMemPool_t pools[kMaxDevices] = {};
-  if (device < 0 || device >= kMaxDevices) throw Error("device index out of range");
-  std::lock_guard<std::mutex> lock(mu);
-  if (!pools[device]) {
+// Scratch of calls that round their rows first, shared by a device's layers and
+// given back with the last of them. Memory of a pool comes and goes in the
+// order of the call's stream, so calls on several streams may overlap; the pool
+// keeps what it has across synchronisations.
+struct ScratchPool {
+  cudaMemPool_t pool = nullptr;
+  explicit ScratchPool(int device) {
     cudaMemPoolProps props{};
     props.allocType = cudaMemAllocationTypePinned;
     props.location.type = cudaMemLocationTypeDevice;
     props.location.id = device;
-    cudaMemPool_t pool;
     TRIT_CUDA(cudaMemPoolCreate(&pool, &props));
     uint64_t keep = UINT64_MAX;
-    TRIT_CUDA(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep));
-    pools[device] = pool;
+    cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep);
   }
-  return pools[device];
-}
+  ~ScratchPool() { cudaMemPoolDestroy(pool); }
+  ScratchPool(const ScratchPool&) = delete;
+  ScratchPool& operator=(const ScratchPool&) = delete;
+  static std::shared_ptr<ScratchPool> of(int device) {
+    static std::mutex mu;
+    static std::weak_ptr<ScratchPool> pools[kMaxDevices];
+    if (device < 0 || device >= kMaxDevices) throw Error("device index out of range");
+    std::lock_guard<std::mutex> lock(mu);
+    std::shared_ptr<ScratchPool> p = pools[device].lock();
+    if (!p) pools[device] = p = std::make_shared<ScratchPool>(device);
+    return p;
+  }
+};
+
+namespace {
 bool is_capturing(cudaStream_t s) {
   cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
   TRIT_CUDA(cudaStreamIsCapturing(s, &st));
@@ -320,6 +328,9 @@ DenseFp8::~DenseFp8() {
   cudaGetDevice(&before);
   cudaSetDevice(device_);
   release();
+  scratch_.reset();
+  // What graphs that are gone had as scratch.
+  if (captured_) cudaDeviceGraphMemTrim(device_);
   cudaSetDevice(before);
 }
 void DenseFp8::release() {
@@ -383,8 +394,13 @@ void DenseFp8::forward_rows(const void* x, size_t x_stride, size_t m, void* out,
   const size_t codes = (m * k_ + 255) / 256 * 256, bytes = codes + m * ((k_ + kFp8Group - 1) / kFp8Group) * 4;
   uint8_t* scratch = nullptr;
   // A captured call's scratch belongs to its graph.
-  if (is_capturing(s)) TRIT_CUDA(cudaMallocAsync(&scratch, bytes, s));
-  else TRIT_CUDA(cudaMallocFromPoolAsync(&scratch, bytes, scratch_pool(device_), s));
+  if (is_capturing(s)) {
+    TRIT_CUDA(cudaMallocAsync(&scratch, bytes, s));
+    captured_ = true;
+  } else {
+    if (!scratch_) scratch_ = ScratchPool::of(device_);
+    TRIT_CUDA(cudaMallocFromPoolAsync(&scratch, bytes, scratch_->pool, s));
+  }
   NormArgs q;
   q.x = x;
   q.x_stride = x_stride;

@@ -84,6 +84,7 @@ struct Rotary {
 };
 
 // -------------------------------------------------------------- products
+struct ScratchPool;
 // A layer with e4m3 weights and an f32 scale for each block of 128 x 128.
 class DenseFp8 {
  public:
@@ -111,6 +112,8 @@ class DenseFp8 {
   uint8_t* codes_ = nullptr;  // packed (launch_fp8_pack)
   float* scales_ = nullptr;   // [ceil(n / 128)][ceil(k / 128)]
   cudaStream_t stream_ = nullptr;
+  std::shared_ptr<ScratchPool> scratch_;  // from the first call that rounds its rows
+  bool captured_ = false;
   int* status_ = nullptr;     // pinned: a wait inside a product ran out
 };
 
