@@ -99,9 +99,16 @@ __device__ __forceinline__ void store(T* p, const Pack<T, V>& r) {
 
 // A unit is V values, or V pairs of halves. Threads of a block: (unit of a head,
 // head, row); a thread has two heads.
+// All of it is passed by value: a call needs nothing on the device that outlives
+// it. PAIRS: 64 where they are enough, since a launch copies its parameters
+// (2 KB of them cost 3 us of the host's call).
+template <int PAIRS>
 struct RotaryWork {
   RotaryArgs a;
+  int head_dim, rotary_dim;
+  float factor;
   int turning, per_head;  // units of a head that turn, which come first, and all of them
+  double turns[PAIRS];    // of a whole circle a position
 };
 
 // cos and sin of t turns, times f: the nearest quarter turn, and the Taylor
@@ -136,13 +143,12 @@ __device__ __forceinline__ void read_angles(const float* from, float (&v)[PV]) {
   }
 }
 
-template <class T, int V, bool INTER, bool ALIGNED>
-__global__ void __launch_bounds__(kRotaryThreads, 4) k_rotary(const __grid_constant__ RotaryTable table,
-                                                           const __grid_constant__ RotaryWork w) {
+template <class T, int V, bool INTER, bool ALIGNED, int PAIRS>
+__global__ void __launch_bounds__(kRotaryThreads, 4) k_rotary(const __grid_constant__ RotaryWork<PAIRS> w) {
   constexpr int PV = INTER ? V / 2 : V;  // pairs of a unit
   extern __shared__ float4 angles[];     // [row][cos, sin][pair]
   const RotaryArgs& a = w.a;
-  const int hd = table.head_dim, rd = table.rotary_dim, pairs = rd / 2, slots = (w.turning * PV + 3) / 4 * 4;
+  const int hd = w.head_dim, rd = w.rotary_dim, pairs = rd / 2, slots = (w.turning * PV + 3) / 4 * 4;
   const int heads = a.q_heads + a.k_heads;
   const int row0 = blockIdx.x * blockDim.z, row = row0 + threadIdx.z;
   const int head0 = blockIdx.y * 2 * blockDim.y + threadIdx.y, head1 = head0 + blockDim.y;
@@ -178,7 +184,7 @@ __global__ void __launch_bounds__(kRotaryThreads, 4) k_rotary(const __grid_const
     float* to = (float*)angles + z * 2 * slots;
 #pragma unroll 1  // (the values on their way need the registers)
     for (int p = thread; p < pairs; p += threads) {
-      const float2 cs = turn((double)__ldg(a.positions + row0 + z) * table.turns[p], table.factor);
+      const float2 cs = turn((double)__ldg(a.positions + row0 + z) * w.turns[p], w.factor);
       to[p] = cs.x;
       to[slots + p] = cs.y;
     }
@@ -235,13 +241,18 @@ __global__ void __launch_bounds__(kRotaryThreads, 4) k_rotary(const __grid_const
   }
 }
 
-template <class T, int V, bool INTER, bool ALIGNED>
-cudaError_t run(const RotaryTable& t, const RotaryArgs& a, cudaStream_t s) {
+template <class T, int V, bool INTER, bool ALIGNED, int PAIRS>
+cudaError_t run_sized(const RotaryTable& t, const RotaryArgs& a, cudaStream_t s) {
   constexpr int PV = INTER ? V / 2 : V;
   const int pairs = t.rotary_dim / 2, heads = a.q_heads + a.k_heads;
   // In place, the values behind the pairs stay as they are.
   const bool still = a.q == a.q_out && a.k == a.k_out;
-  RotaryWork w{a};
+  RotaryWork<PAIRS> w;
+  w.a = a;
+  w.head_dim = t.head_dim;
+  w.rotary_dim = t.rotary_dim;
+  w.factor = t.factor;
+  std::copy(t.turns, t.turns + pairs, w.turns);
   w.turning = INTER ? (t.rotary_dim + V - 1) / V : pairs / V;
   w.per_head = still ? w.turning : INTER ? t.head_dim / V : w.turning + (t.head_dim - t.rotary_dim) / V;
   const int lanes = std::min(w.per_head, kRotaryThreads);
@@ -252,8 +263,13 @@ cudaError_t run(const RotaryTable& t, const RotaryArgs& a, cudaStream_t s) {
   int rows = std::min(std::max(1, teams / head_lanes), 8);
   if ((long long)a.rows * parts < 8LL * current_sm_count()) rows = 1;
   const size_t smem = (size_t)rows * 2 * ((w.turning * PV + 3) / 4 * 4) * sizeof(float);
-  return launch_early(k_rotary<T, V, INTER, ALIGNED>, dim3((a.rows + rows - 1) / rows, parts), dim3(lanes, head_lanes, rows),
-                      smem, s, 1, t, w);
+  return launch_early(k_rotary<T, V, INTER, ALIGNED, PAIRS>, dim3((a.rows + rows - 1) / rows, parts), dim3(lanes, head_lanes, rows),
+                      smem, s, 1, w);
+}
+template <class T, int V, bool INTER, bool ALIGNED>
+cudaError_t run(const RotaryTable& t, const RotaryArgs& a, cudaStream_t s) {
+  return t.rotary_dim <= 128 ? run_sized<T, V, INTER, ALIGNED, 64>(t, a, s)
+                             : run_sized<T, V, INTER, ALIGNED, kRotaryPairs>(t, a, s);
 }
 
 // The widest units that the sizes, strides and addresses allow.

@@ -60,7 +60,6 @@ void rms_norm(NormArgs a, size_t rows, size_t width, cudaStream_t s);
 
 // ---------------------------------------------------------------- rotary
 constexpr int kRotaryPairs = 256;
-// Passed by value: a call needs nothing on the device that outlives it.
 struct RotaryTable {
   int head_dim = 0, rotary_dim = 0, interleaved = 0;
   float factor = 1.0f;
