@@ -34,19 +34,23 @@ constexpr int F8_K = 128;  // values (bytes) of k a stage: one swizzle line, one
 constexpr int F8_UNIT = 64, F8_UNIT_BYTES = F8_UNIT * F8_K;  // rows of a unit of w
 
 // AR rows of x are loaded (the MMA's other rows read what lies behind them,
-// and nobody reads their sums); BN rows of w a tile.
+// and nobody reads their sums); BN rows of w a tile. Up to 64 rows take MMAs of
+// M = 64: under the power limit the arithmetic that nobody reads costs clocks
+// (151936 x 2048, three rows, seconds on end: 60 us with M = 128, 57 so).
 template <int AR, int BN, int BLOCKS_>
 struct F8Shape {
   static constexpr int STAGE = (AR + BN) * F8_K;
   static constexpr int COLUMN_WARPS = BN >= 128 ? 2 : 1;      // epilogue warps that share a tile's columns
   static constexpr int CW = BN / COLUMN_WARPS;                // columns of each
-  static constexpr int ROW_WARPS = (AR + 31) / 32;            // of the four TMEM quarters, those with rows
+  static constexpr int M = AR <= 64 ? 64 : 128;               // of the MMA
+  static constexpr int LANES = M / 4;                         // rows in a quarter of TMEM: its first lanes
+  static constexpr int ROW_WARPS = (AR + LANES - 1) / LANES;  // of the four quarters, those with rows
   static constexpr int THREADS = 128 + 128 * COLUMN_WARPS;
   static constexpr int BUFS = BN * 4 * BLOCKS_ > 512 ? 2 : 4;
   static constexpr int COLS = BUFS * BN;                      // of TMEM
   static constexpr int STAGING = ROW_WARPS * COLUMN_WARPS * 4096;
   static_assert(STAGE % 1024 == 0, "swizzled rows begin at whole kilobytes");
-  static constexpr int TAIL = (128 - AR) * F8_K > STAGING ? (128 - AR) * F8_K : STAGING;  // behind the stages
+  static constexpr int TAIL = (M - AR) * F8_K > STAGING ? (M - AR) * F8_K : STAGING;  // behind the stages
   static constexpr int BLOCKS = BLOCKS_;                      // an SM holds
   static constexpr int ROOM = 226 * 1024 / BLOCKS - 2048 - 1024 - TAIL;  // (a block's own 1 KB, and its static memory)
   static constexpr int STAGES = ROOM / STAGE < 12 ? ROOM / STAGE : 12;
@@ -117,15 +121,15 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, bool f16) {
   return f16 ? pack2<__half>(make_float2(a, b)) : pack2<__nv_bfloat16>(make_float2(a, b));
 }
 
-// A warp's 32 rows (a lane each) x CW columns to out, in chunks of 128 bytes a
+// A warp's rows (one in each of its first LANES lanes) x CW columns to out, in chunks of 128 bytes a
 // row through 4 KB of shared memory of its own: 16-byte unit u of row r lies at
 // u ^ (r % 8), as the tensor copies' 128-byte swizzle has it. Where out's rows
 // are 16-byte aligned (a.tma), a chunk leaves by one tensor copy, which ends at
 // out's last row and column by itself, and the warp goes on meanwhile.
-template <int CW>
+template <int CW, int LANES>
 __device__ __forceinline__ void store_tile(const float2 (&acc)[CW / 2], uint8_t* staging, const CUtensorMap& omap,
                                            const Fp8Args& a, int row0, int col0, int lane) {
-  const int rows = min(32, a.m - row0);
+  const int rows = min(LANES, a.m - row0);
   const bool f32 = a.type == kRowF32, f16 = a.type == kRowF16;
   const int size = f32 ? 4 : 2;
   uint8_t* const out = (uint8_t*)a.out + (size_t)row0 * a.out_stride * size;
@@ -149,7 +153,7 @@ __device__ __forceinline__ void store_tile(const float2 (&acc)[CW / 2], uint8_t*
     __syncwarp();
     const int live = min(128 / size, a.n - col);
 #pragma unroll 8
-    for (int r = 0; r < 32; ++r) {
+    for (int r = 0; r < LANES; ++r) {
       if (r >= rows) break;
       const uint32_t w = *(const uint32_t*)(staging + r * 128 + ((lane / 4 ^ (r & 7)) << 4) + (lane & 3) * 4);
       uint8_t* p = out + ((size_t)r * a.out_stride + col) * size;
@@ -367,7 +371,7 @@ __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
 #pragma unroll
           for (int j = 0; j < F8_K / 32; ++j)
             mma_f8(tmem + u * BN, smem_desc_sw128(s0 + i * S::STAGE + j * 32),
-                   smem_desc_sw128(s0 + i * S::STAGE + AR * F8_K + j * 32), idesc_f8(128, BN), j ? 1u : 0u);
+                   smem_desc_sw128(s0 + i * S::STAGE + AR * F8_K + j * 32), idesc_f8(S::M, BN), j ? 1u : 0u);
           mma_commit(&y->tfull[u]);
           mma_commit(&y->empty[i]);
         }
@@ -391,9 +395,9 @@ __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
       for (uint32_t t = first; t < tiles && ok; t += step) {
         int r, c;
         tile_place(t, row_tiles, col_tiles, &r, &c);
-        const int row0 = r * 128 + quarter * 32;  // m is at most 2^31 - 256
+        const int row0 = r * 128 + quarter * S::LANES;  // m is at most 2^31 - 256
         const int col0 = c * BN + part * S::CW;
-        const bool live = row0 + lane < a.m;
+        const bool live = lane < S::LANES && row0 + lane < a.m;
         const float* sx = a.x_scales + (size_t)(live ? row0 + lane : 0) * a.blocks;
         // Every 32 blocks a lane loads the scale of w of one of them. A warp's
         // columns lie in one block of w; past n they read the last block's.
@@ -438,8 +442,9 @@ __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
                                      acc[q * 16 + i]);
           }
         }
-        if (S::SPLITS && splits > 1) put_part<S::CW, BN>(acc, base, quarter * 32 + lane, part * S::CW);
-        else if (ok && row0 < a.m) store_tile<S::CW>(acc, staging, omap, a, row0, col0, lane);
+        if (S::SPLITS && splits > 1) {
+          if (lane < S::LANES) put_part<S::CW, BN>(acc, base, quarter * S::LANES + lane, part * S::CW);
+        } else if (ok && row0 < a.m) store_tile<S::CW, S::LANES>(acc, staging, omap, a, row0, col0, lane);
       }
       // The last chunks have left shared memory before it is given back.
       if (a.tma && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -507,6 +512,7 @@ __global__ void __launch_bounds__(256) k_fp8_pack(const uint8_t* codes, size_t n
 }  // namespace
 
 int fp8_row_box(int m) { return m <= 16 ? 16 : m <= 64 ? 64 : 128; }
+int fp8_out_box(int m) { return m <= 64 ? 16 : 32; }
 size_t fp8_packed_bytes(size_t n, size_t k) {
   return (n + F8_UNIT - 1) / F8_UNIT * ((k + F8_K - 1) / F8_K) * F8_UNIT_BYTES;
 }

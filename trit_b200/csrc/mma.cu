@@ -773,14 +773,14 @@ cudaError_t make_fp8_map(TcMap* out, const void* base, size_t rows, size_t k, in
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
-cudaError_t make_fp8_out_map(TcMap* out, void* base, size_t rows, size_t n, size_t stride, int type) {
+cudaError_t make_fp8_out_map(TcMap* out, void* base, size_t rows, size_t n, size_t stride, int type, int box_rows) {
   EncodeTiled enc = encoder();
   const size_t size = row_type_size(type);
   if (!enc) return cudaErrorNotSupported;
   if (!rows || !n || (((uintptr_t)base | stride * size) & 15)) return cudaErrorInvalidValue;
   cuuint64_t dims[2] = {n, rows};
   cuuint64_t strides[1] = {stride * size};
-  cuuint32_t box[2] = {(cuuint32_t)(128 / size), 32};
+  cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = enc((CUtensorMap*)out, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, base,
                    dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,

@@ -370,7 +370,7 @@ void DenseFp8::product(const void* codes, const float* scales, size_t m, void* o
   a.type = type;
   a.status = status_;
   TcMap out_map{};
-  a.tma = make_fp8_out_map(&out_map, out, m, n_, out_stride, type) == cudaSuccess;
+  a.tma = make_fp8_out_map(&out_map, out, m, n_, out_stride, type, fp8_out_box((int)m)) == cudaSuccess;
   TRIT_CUDA(launch_fp8(map, out_map, a, s));
 }
 

@@ -129,9 +129,10 @@ struct Fp8Args {
 // A TMA map of 8-bit numbers [rows][k], row stride k, boxes of 128 values x
 // box_rows rows with the 128-byte swizzle; past either end reads zero.
 cudaError_t make_fp8_map(TcMap* out, const void* base, size_t rows, size_t k, int box_rows);
-// A TMA map of out, boxes of 128 bytes x 32 rows with the same swizzle; its rows
+// A TMA map of out, boxes of 128 bytes x box_rows with the same swizzle; its rows
 // have to be 16-byte aligned.
-cudaError_t make_fp8_out_map(TcMap* out, void* base, size_t rows, size_t n, size_t stride, int type);
+cudaError_t make_fp8_out_map(TcMap* out, void* base, size_t rows, size_t n, size_t stride, int type, int box_rows);
+int fp8_out_box(int m);
 int fp8_row_box(int m);  // its box rows for m rows
 // The weights [n][k] in the order that the product reads them.
 size_t fp8_packed_bytes(size_t n, size_t k);
