@@ -93,6 +93,8 @@ def test_rotary_needs_an_object():
     (dict(q_out_stride=256), "q_out_stride without q_out"),
     (dict(q_out_ptr=P, q_out_stride=257), "one tensor with two strides"),
     (dict(k_ptr=P, k_heads=4, rows=0), "q_out and k_out are one tensor"),
+    (dict(q_out_ptr=2 * P, k_ptr=2 * P, k_heads=4, k_out_ptr=3 * P), "q_out and k are one tensor"),
+    (dict(q_out_ptr=2 * P, k_ptr=3 * P, k_heads=4, k_out_ptr=P), "k_out and q are one tensor"),
     (dict(dtype="f8"), "not one of"),
 ])
 def test_rotary_refusals(args, words):

@@ -66,6 +66,17 @@ def test_sizes(n, k, m):
     check(codes_call(dense, codes, scales, dtype), x, w)
 
 
+@pytest.mark.parametrize("n, stride", [(4, 0), (8, 0), (8, 24), (40, 48), (64, 72), (129, 136), (256, 264), (257, 258)])
+@pytest.mark.parametrize("m", [1, 16, 17, 64, 65, 150, 700])
+def test_places_of_the_output(n, stride, m):
+    """Rows of the output that tensor copies take (16-byte aligned), narrower than their boxes too, and rows that they do not;
+    what lies between and around them stays."""
+    dense, w = layer(n, 272, n)
+    codes, scales, x = rows(m, 272, m)
+    for dtype in ("f32", "f16", "bf16"):
+        check(codes_call(dense, codes, scales, dtype, out_stride=stride), x, w)
+
+
 @pytest.mark.parametrize("n, k, m", [(12288, 2048, 1), (4096, 4096, 5), (2048, 6144, 64), (32768, 256, 20), (5001, 2064, 333), (2560, 1024, 2100),
                                      (129, 128, 5000), (40, 16384, 3), (3000, 512, 1037), (256, 11008, 260)])
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])

@@ -15,7 +15,24 @@
 //   warp 1     issues four MMAs (K = 32) a stage into one of the TMEM buffers;
 //   warps 4..  epilogue: load a block's sums from TMEM, add them up, and write
 //              the tile through shared memory in whole lines.
-// Every wait is bounded in time and reports through a status word.
+// Every wait is bounded in time and reports through a status word. A block
+// takes tile after tile; where tiles are few, a cluster of up to eight blocks
+// shares one, each with a part of k, and adds the parts up in order through
+// distributed shared memory. Weights do not depend on the kernel in front, so a
+// block has its first stages of them on their way while that one still runs.
+//
+// Few rows are bound by the bytes of w: 151936 x 2048 and three rows 56 us (5.6
+// TB/s), 16384 x 4096 and 64 f32 rows 18.6 us with their rounding (3.9 TB/s),
+// 12288 x 2048 and one row 8.3 us, of which about 4 are a launch, the first copy
+// and the join. Many rows, 8000 of 12288 x 4096: 400 to 460 us with the clock
+// that the power limit leaves (1.75 to 2.0 PFLOP/s; 2.7 without the scaled
+// additions). What holds them up is the round trip of a TMEM buffer (MMA, commit,
+// load, release), of which 512 columns hold two of 256. Measured and left:
+// pairs of blocks with cta_group::2 (tiles of 256 x 256, half the bytes of w a
+// block, but a release crosses the blocks: 775 us), buffers of 128 columns
+// (the same), 16 epilogue warps (480 us, for want of registers), waits that
+// poll instead of suspending (510 us).
+
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -124,7 +141,7 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, bool f16) {
 // A warp's rows (one in each of its first LANES lanes) x CW columns to out, in chunks of 128 bytes a
 // row through 4 KB of shared memory of its own: 16-byte unit u of row r lies at
 // u ^ (r % 8), as the tensor copies' 128-byte swizzle has it. Where out's rows
-// are 16-byte aligned (a.tma), a chunk leaves by one tensor copy, which ends at
+// begin and end at whole 16 bytes (a.tma), a chunk leaves by one tensor copy, which ends at
 // out's last row and column by itself, and the warp goes on meanwhile.
 template <int CW, int LANES>
 __device__ __forceinline__ void store_tile(const float2 (&acc)[CW / 2], uint8_t* staging, const CUtensorMap& omap,
@@ -356,6 +373,7 @@ __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
           }
       }
     } else if (warp == 1 && elected()) {
+      after_kernel_before();  // however long that one takes, the limits of the waits run from its end
       const uint32_t s0 = smem_u32(base);
       uint32_t it = 0;
       bool ok = true;

@@ -777,7 +777,8 @@ cudaError_t make_fp8_out_map(TcMap* out, void* base, size_t rows, size_t n, size
   EncodeTiled enc = encoder();
   const size_t size = row_type_size(type);
   if (!enc) return cudaErrorNotSupported;
-  if (!rows || !n || (((uintptr_t)base | stride * size) & 15)) return cudaErrorInvalidValue;
+  // (A store ends at whole 16 bytes of a row: it would write behind another end.)
+  if (!rows || !n || (((uintptr_t)base | stride * size | n * size) & 15)) return cudaErrorInvalidValue;
   cuuint64_t dims[2] = {n, rows};
   cuuint64_t strides[1] = {stride * size};
   cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows};

@@ -253,6 +253,8 @@ void Rotary::apply(RotaryArgs a, size_t rows, cudaStream_t s) const {
   tensor(a.q, a.q_stride, a.q_out, a.q_out_stride, a.q_heads, "q");
   tensor(a.k, a.k_stride, a.k_out, a.k_out_stride, a.k_heads, "k");
   if (a.q_out && a.q_out == a.k_out) throw Error("q_out and k_out are one tensor");
+  if (a.q_out && a.q_out == a.k) throw Error("q_out and k are one tensor");
+  if (a.k_out && a.k_out == a.q) throw Error("k_out and q are one tensor");
   if (!rows) return;
   check_on_device(a.positions, 8, "positions", device);
   OnDevice on(device);

@@ -130,7 +130,7 @@ struct Fp8Args {
 // box_rows rows with the 128-byte swizzle; past either end reads zero.
 cudaError_t make_fp8_map(TcMap* out, const void* base, size_t rows, size_t k, int box_rows);
 // A TMA map of out, boxes of 128 bytes x box_rows with the same swizzle; its rows
-// have to be 16-byte aligned.
+// have to begin and end at whole 16 bytes.
 cudaError_t make_fp8_out_map(TcMap* out, void* base, size_t rows, size_t n, size_t stride, int type, int box_rows);
 int fp8_out_box(int m);
 int fp8_row_box(int m);  // its box rows for m rows
