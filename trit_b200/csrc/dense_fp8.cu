@@ -21,9 +21,9 @@
 // distributed shared memory. Weights do not depend on the kernel in front, so a
 // block has its first stages of them on their way while that one still runs.
 //
-// Few rows are bound by the bytes of w: 151936 x 2048 and three rows 56 us (5.6
+// Few rows are bound by the bytes of w: 151936 x 2048 and three rows 54 us (5.8
 // TB/s), 16384 x 4096 and 64 f32 rows 18.6 us with their rounding (3.9 TB/s),
-// 12288 x 2048 and one row 8.3 us, of which about 4 are a launch, the first copy
+// 12288 x 2048 and one row 7.8 us, of which about 4 are a launch, the first copy
 // and the join. Many rows, 8000 of 12288 x 4096: 400 to 460 us with the clock
 // that the power limit leaves (1.75 to 2.0 PFLOP/s; 2.7 without the scaled
 // additions). What holds them up is the round trip of a TMEM buffer (MMA, commit,
@@ -62,7 +62,11 @@ struct F8Shape {
   static constexpr int M = AR <= 64 ? 64 : 128;               // of the MMA
   static constexpr int LANES = M / 4;                         // rows in a quarter of TMEM: its first lanes
   static constexpr int ROW_WARPS = (AR + LANES - 1) / LANES;  // of the four quarters, those with rows
-  static constexpr int THREADS = 128 + 128 * COLUMN_WARPS;
+  // Epilogue warps read the quarter of TMEM that their number names; where one
+  // quarter has all rows, warp 0 is the epilogue beside the two others.
+  static constexpr bool LONE = ROW_WARPS == 1 && COLUMN_WARPS == 1;
+  static constexpr int THREADS = LONE ? 96 : 128 + 128 * COLUMN_WARPS;
+  static constexpr int LOADER = LONE ? 2 : 0, ISSUER = 1, EPILOGUE = LONE ? 0 : 4;
   static constexpr int BUFS = BN * 4 * BLOCKS_ > 512 ? 2 : 4;
   static constexpr int COLS = BUFS * BN;                      // of TMEM
   static constexpr int STAGING = ROW_WARPS * COLUMN_WARPS * 4096;
@@ -317,7 +321,7 @@ __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
     y->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) {
+  if (warp == S::ISSUER) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&y->tmem)), "r"(S::COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -328,9 +332,9 @@ __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
   const uint32_t tmem = y->tmem;
   let_next_start();
 
-  if (warp < 4) {
+  if (S::LONE ? warp != 0 : warp < 4) {
     if constexpr (S::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::REGS_FEW));
-    if (warp == 0 && elected()) {
+    if (warp == S::LOADER && elected()) {
       uint32_t it = 0;
       bool ok = true;
       // What does not depend on the kernel before, the first stages' weights,
@@ -372,7 +376,7 @@ __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
           while (!mbar_test(&y->full[z % S::STAGES], (z / S::STAGES) & 1) && now_ns() - t0 < TC_WAIT_NS) {
           }
       }
-    } else if (warp == 1 && elected()) {
+    } else if (warp == S::ISSUER && elected()) {
       after_kernel_before();  // however long that one takes, the limits of the waits run from its end
       const uint32_t s0 = smem_u32(base);
       uint32_t it = 0;
@@ -402,7 +406,7 @@ __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
     }
   } else {
     if constexpr (S::SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::REGS_MANY));
-    const int quarter = warp & 3, part = (warp - 4) >> 2;
+    const int quarter = warp & 3, part = (warp - S::EPILOGUE) >> 2;
     after_kernel_before();
     if (quarter < S::ROW_WARPS) {
       uint8_t* staging = base + S::STAGES * S::STAGE + (part * S::ROW_WARPS + quarter) * 4096;
@@ -477,7 +481,7 @@ __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
     join_parts<BN>(base, a, r * 128, min(AR, a.m - r * 128), c * BN, split, splits);
     cluster_sync();  // nobody leaves while others read its part
   }
-  if (warp == 1) {
+  if (warp == S::ISSUER) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
   }
@@ -543,17 +547,25 @@ cudaError_t launch_fp8(const TcMap& x, const TcMap& out, const Fp8Args& a, cudaS
   if (a.m <= 0) return cudaSuccess;
   const long long sms = current_sm_count();
   const auto tiles = [&](int bn) { return (a.m + 127LL) / 128 * ((a.n + bn - 1) / bn); };
-  // As many blocks of a cluster as there is room for beside each other.
+  // As many blocks of a cluster as there is room for beside each other, with at
+  // least two blocks of k, six where eight share (4096 x 4096, three rows: a
+  // cluster of 1 11.7 us, 2 8.6, 4 7.0, 8 7.8; 2048 x 6144: 16.2, 10.3, 7.2, 6.2;
+  // 12288 x 2048: 7.9, 7.8, 12.8, 19.3).
   const auto splits = [&](long long tiles, long long room) {
     int z = 1;
-    while (z < 8 && tiles * z * 2 <= room && a.blocks / (z * 2) >= (z < 4 ? 2 : 4)) z *= 2;
+    while (z < 8 && tiles * z * 2 <= room && a.blocks / (z * 2) >= (z < 4 ? 2 : 6)) z *= 2;
     return z;
   };
   const int box = fp8_row_box(a.m);
-  if (box == 16) return run<16, 64, 2>(x, out, a, splits(tiles(64), 2 * sms), s);
+  // Few rows: four blocks an SM, of three warps, so that the next call's blocks
+  // find room (two an SM: 151936 x 2048 57.1 us, 32768 x 8192 46.7; four: 53.6, 43.1).
+  if (box == 16) return run<16, 64, 4>(x, out, a, splits(tiles(64), 4 * sms), s);
   if (box == 64) return run<64, 64, 2>(x, out, a, splits(tiles(64), 2 * sms), s);
-  const auto waves = [&](int bn) { return (double)((tiles(bn) + sms - 1) / sms); };
-  if (waves(128) * 0.385 < waves(256) * 0.6) return run<128, 128, 1>(x, out, a, splits(tiles(128), sms), s);
+  // Tiles of 128 or 256 columns: whole turns of the SMs, at the measured time of
+  // a turn and block of k (0.385 and 0.6 us). 333 rows of 5001 x 2064: 128 columns
+  // 12.7 us, 256 columns 19.5; 1000 of 12288 x 4096: 81 and 55.
+  const auto turns = [&](int bn) { return (double)((tiles(bn) + sms - 1) / sms); };
+  if (turns(128) * 0.385 < turns(256) * 0.6) return run<128, 128, 1>(x, out, a, splits(tiles(128), sms), s);
   return run<128, 256, 1>(x, out, a, 1, s);
 }
 
