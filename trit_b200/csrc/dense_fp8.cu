@@ -50,13 +50,14 @@ namespace {
 constexpr int F8_K = 128;  // values (bytes) of k a stage: one swizzle line, one scale block
 constexpr int F8_UNIT = 64, F8_UNIT_BYTES = F8_UNIT * F8_K;  // rows of a unit of w
 
-// AR rows of x are loaded (the MMA's other rows read what lies behind them,
+// CTAS blocks a tile. AR rows of x are loaded a block (the MMA's other rows read what lies behind them,
 // and nobody reads their sums); BN rows of w a tile. Up to 64 rows take MMAs of
 // M = 64: under the power limit the arithmetic that nobody reads costs clocks
 // (151936 x 2048, three rows, seconds on end: 60 us with M = 128, 57 so).
-template <int AR, int BN, int BLOCKS_>
+template <int CTAS, int AR, int BN, int BLOCKS_>
 struct F8Shape {
-  static constexpr int STAGE = (AR + BN) * F8_K;
+  static constexpr int BR = BN / CTAS;  // rows of w a block holds
+  static constexpr int STAGE = (AR + BR) * F8_K;
   static constexpr int COLUMN_WARPS = BN >= 128 ? 2 : 1;      // epilogue warps that share a tile's columns
   static constexpr int CW = BN / COLUMN_WARPS;                // columns of each
   static constexpr int M = AR <= 64 ? 64 : 128;               // of the MMA
@@ -99,12 +100,46 @@ __device__ __forceinline__ bool elected() {
   return r != 0;
 }
 
+template <int CTAS>
 __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CTAS == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+// The MMAs issued so far arrive at *bar once they are done; of a pair, at both
+// blocks' (the same place in each).
+template <int CTAS>
+__device__ __forceinline__ void commit_f8(uint64_t* bar) {
+  if constexpr (CTAS == 1)
+    mma_commit(bar);
+  else
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                     smem_u32(bar)),
+                 "h"((uint16_t)3)
+                 : "memory");
+}
+// The address of the pair's first block's copy of a shared variable.
+__device__ __forceinline__ uint32_t first_of_pair(const void* p) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+  return r;
+}
+// A tensor copy whose bytes count at the first block's barrier.
+__device__ __forceinline__ void tma_load_pair(void* dst, const void* map, uint32_t bar, int x, int y) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"((uint64_t)map), "r"(bar), "r"(x), "r"(y)
+      : "memory");
 }
 // Instruction descriptor of kind::f8f6f4: D f32 (bits 4-5 = 1), A and B e4m3
 // (bits 7-9, 10-12 = 0), both K-major, N >> 3 at bit 17, M >> 4 at bit 24.
@@ -291,21 +326,23 @@ __device__ __forceinline__ void join_parts(const uint8_t* part, const Fp8Args& a
   }
 }
 
-template <int AR, int BN, int BLOCKS>
-__global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
-    k_fp8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap omap, const __grid_constant__ Fp8Args a) {
-  using S = F8Shape<AR, BN, BLOCKS>;
+template <int CTAS, int AR, int BN, int BLOCKS>
+__global__ void __launch_bounds__(F8Shape<CTAS, AR, BN, BLOCKS>::THREADS, BLOCKS)
+    k_fp8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
+          const __grid_constant__ CUtensorMap omap, const __grid_constant__ Fp8Args a) {
+  using S = F8Shape<CTAS, AR, BN, BLOCKS>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ F8Sync sync;
   F8Sync* y = &sync;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t row_tiles = ((uint32_t)a.m + 127) / 128, col_tiles = ((uint32_t)a.n + BN - 1) / BN, tiles = row_tiles * col_tiles;
+  const uint32_t row_tiles = ((uint32_t)a.m + CTAS * 128 - 1) / (CTAS * 128), col_tiles = ((uint32_t)a.n + BN - 1) / BN, tiles = row_tiles * col_tiles;
   // The blocks of a cluster share a tile, each with a part of k.
   const int splits = S::SPLITS ? cluster_size() : 1, split = S::SPLITS ? cluster_rank() : 0;
   const int lo = S::SPLITS ? (int)((long long)a.blocks * split / splits) : 0;
   const int hi = S::SPLITS ? (int)((long long)a.blocks * (split + 1) / splits) : a.blocks;
-  const uint32_t first = blockIdx.x / splits, step = gridDim.x / splits;
+  const int rank = CTAS == 2 ? cluster_rank() : 0;
+  const uint32_t first = blockIdx.x / (splits * CTAS), step = gridDim.x / (splits * CTAS);
   volatile int* abort = &y->abort;
 
   if (threadIdx.x == 0) {
@@ -315,19 +352,26 @@ __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
     }
     for (int i = 0; i < S::BUFS; ++i) {
       mbar_init(&y->tfull[i], 1);
-      mbar_init(&y->tempty[i], S::ROW_WARPS * S::COLUMN_WARPS);
+      mbar_init(&y->tempty[i], CTAS * S::ROW_WARPS * S::COLUMN_WARPS);
     }
     mbar_init(&y->drain, 1);
     y->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == S::ISSUER) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&y->tmem)), "r"(S::COLS)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (CTAS == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&y->tmem)), "r"(S::COLS)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&y->tmem)), "r"(S::COLS)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
   }
   fence_before();
   __syncthreads();
+  if constexpr (CTAS == 2) cluster_sync();
   fence_after();
   const uint32_t tmem = y->tmem;
   let_next_start();
@@ -343,13 +387,20 @@ __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
       for (uint32_t t = first; t < tiles && ok; t += step) {
         int r, c;
         tile_place(t, row_tiles, col_tiles, &r, &c);
-        const int units = min(BN / F8_UNIT, (a.n + F8_UNIT - 1) / F8_UNIT - c * (BN / F8_UNIT));
-        const uint8_t* w = a.w + (size_t)c * (BN / F8_UNIT) * a.blocks * F8_UNIT_BYTES;
+        // The tile's units of w; of a pair, each block has half of them.
+        const int left = (a.n + F8_UNIT - 1) / F8_UNIT - c * (BN / F8_UNIT);
+        const int all = min(BN / F8_UNIT, left), units = min(S::BR / F8_UNIT, left - rank * (S::BR / F8_UNIT));
+        const size_t unit0 = ((size_t)c * (BN / F8_UNIT) + rank * (S::BR / F8_UNIT)) * a.blocks;
         auto weights = [&](int b, uint32_t i) {
-          mbar_expect_tx(&y->full[i], AR * F8_K + units * F8_UNIT_BYTES);
-          for (int z = 0; z < units; ++z)
-            bulk_load(base + i * S::STAGE + AR * F8_K + z * F8_UNIT_BYTES, w + ((size_t)z * a.blocks + b) * F8_UNIT_BYTES,
-                      F8_UNIT_BYTES, &y->full[i]);
+          uint8_t* to = base + i * S::STAGE + AR * F8_K;
+          if (rank == 0) mbar_expect_tx(&y->full[i], CTAS * AR * F8_K + all * F8_UNIT_BYTES);
+          for (int z = 0; z < units; ++z) {
+            const size_t unit = unit0 + (size_t)z * a.blocks + b;
+            if constexpr (CTAS == 1)
+              bulk_load(to + z * F8_UNIT_BYTES, a.w + unit * F8_UNIT_BYTES, F8_UNIT_BYTES, &y->full[i]);
+            else
+              tma_load_pair(to + z * F8_UNIT_BYTES, &wmap, first_of_pair(&y->full[i]), 0, (int)unit * F8_UNIT);
+          }
         };
         if (it == 0) {
           for (; early < S::STAGES && lo + (int)early < hi; ++early) weights(lo + early, early);
@@ -364,19 +415,23 @@ __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
             }
             weights(b, i);
           }
-          tma_load_2d(base + i * S::STAGE, &xmap, &y->full[i], b * F8_K, r * 128);
+          if constexpr (CTAS == 1)
+            tma_load_2d(base + i * S::STAGE, &xmap, &y->full[i], b * F8_K, r * 128);
+          else
+            tma_load_pair(base + i * S::STAGE, &xmap, first_of_pair(&y->full[i]), b * F8_K, (r * 2 + rank) * 128);
         }
       }
       if (!ok) {
         // Let the copies in flight land before the block's memory is released
-        // (a stage whose rows were not asked for any more does not fill).
+        // (a stage whose rows were not asked for any more does not fill; a pair's
+        // second block has no barrier to ask: a copy waits for nothing, 20 ms are ample).
         const long long t0 = now_ns();
         const uint32_t end = max(it, early);
         for (uint32_t z = end > S::STAGES ? end - S::STAGES : 0; z < end; ++z)
-          while (!mbar_test(&y->full[z % S::STAGES], (z / S::STAGES) & 1) && now_ns() - t0 < TC_WAIT_NS) {
+          while ((rank || !mbar_test(&y->full[z % S::STAGES], (z / S::STAGES) & 1)) && now_ns() - t0 < (rank ? 20000000ll : TC_WAIT_NS)) {
           }
       }
-    } else if (warp == S::ISSUER && elected()) {
+    } else if (warp == S::ISSUER && rank == 0 && elected()) {
       after_kernel_before();  // however long that one takes, the limits of the waits run from its end
       const uint32_t s0 = smem_u32(base);
       uint32_t it = 0;
@@ -392,14 +447,14 @@ __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
           fence_after();
 #pragma unroll
           for (int j = 0; j < F8_K / 32; ++j)
-            mma_f8(tmem + u * BN, smem_desc_sw128(s0 + i * S::STAGE + j * 32),
-                   smem_desc_sw128(s0 + i * S::STAGE + AR * F8_K + j * 32), idesc_f8(S::M, BN), j ? 1u : 0u);
-          mma_commit(&y->tfull[u]);
-          mma_commit(&y->empty[i]);
+            mma_f8<CTAS>(tmem + u * BN, smem_desc_sw128(s0 + i * S::STAGE + j * 32),
+                   smem_desc_sw128(s0 + i * S::STAGE + AR * F8_K + j * 32), idesc_f8(CTAS * S::M, BN), j ? 1u : 0u);
+          commit_f8<CTAS>(&y->tfull[u]);
+          commit_f8<CTAS>(&y->empty[i]);
         }
       }
       // Every MMA issued has finished once `drain` completes.
-      mma_commit(&y->drain);
+      commit_f8<CTAS>(&y->drain);
       const long long t0 = now_ns();
       while (!mbar_test(&y->drain, 0) && now_ns() - t0 < TC_WAIT_NS) {
       }
@@ -417,7 +472,7 @@ __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
       for (uint32_t t = first; t < tiles && ok; t += step) {
         int r, c;
         tile_place(t, row_tiles, col_tiles, &r, &c);
-        const int row0 = r * 128 + quarter * S::LANES;  // m is at most 2^31 - 256
+        const int row0 = (r * CTAS + rank) * 128 + quarter * S::LANES;  // m is at most 2^31 - 256
         const int col0 = c * BN + part * S::CW;
         const bool live = lane < S::LANES && row0 + lane < a.m;
         const float* sx = a.x_scales + (size_t)(live ? row0 + lane : 0) * a.blocks;
@@ -456,7 +511,12 @@ __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
               tmem_ld<32>(from + (q + 1) * 32, v[(q + 1) & 1]);
             } else {
               fence_before();
-              if (lane == 0) mbar_arrive(&y->tempty[u]);
+              if (lane == 0) {
+                // (No memory is handed over, so the default scope will do across the
+                // pair too: an arrival with .release.cluster took it from 428 to 780 us.)
+                if constexpr (CTAS == 1) mbar_arrive(&y->tempty[u]);
+                else asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(first_of_pair(&y->tempty[u])) : "memory");
+              }
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i)
@@ -481,16 +541,21 @@ __global__ void __launch_bounds__(F8Shape<AR, BN, BLOCKS>::THREADS, BLOCKS)
     join_parts<BN>(base, a, r * 128, min(AR, a.m - r * 128), c * BN, split, splits);
     cluster_sync();  // nobody leaves while others read its part
   }
+  // A pair ends together: the first block's MMAs read the second's memory, and both arrive at its barriers.
+  if constexpr (CTAS == 2) cluster_sync();
   if (warp == S::ISSUER) {
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
+    if constexpr (CTAS == 1)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
   }
   if (threadIdx.x == 0 && y->abort) *(volatile int*)a.status = 1;
 }
 
-template <int AR, int BN, int BLOCKS>
-cudaError_t run(const TcMap& x, const TcMap& out, const Fp8Args& a, int splits, cudaStream_t s) {
-  using S = F8Shape<AR, BN, BLOCKS>;
+template <int CTAS, int AR, int BN, int BLOCKS>
+cudaError_t run(const TcMap& x, const TcMap& w, const TcMap& out, const Fp8Args& a, int splits, cudaStream_t s) {
+  using S = F8Shape<CTAS, AR, BN, BLOCKS>;
   static_assert(S::STAGES >= 3 && S::STAGES <= 12 && S::SMEM + (int)sizeof(F8Sync) <= 227 * 1024, "shared memory");
   static_assert(AR * BN * 4 <= S::STAGES * S::STAGE, "a split's sums");
   static_assert(S::COLS * S::BLOCKS <= 512 && (S::COLS & (S::COLS - 1)) == 0, "TMEM");
@@ -501,19 +566,19 @@ cudaError_t run(const TcMap& x, const TcMap& out, const Fp8Args& a, int splits, 
   static DeviceOnce once;
   e = once.run(dev, [] {
     cudaFuncAttributes f;
-    cudaError_t r = cudaFuncGetAttributes(&f, k_fp8<AR, BN, BLOCKS>);
+    cudaError_t r = cudaFuncGetAttributes(&f, k_fp8<CTAS, AR, BN, BLOCKS>);
     // A launch with fewer registers than the shares add up to would wait for them without end.
     if (r == cudaSuccess && S::SPLIT && f.numRegs != S::REGS) r = cudaErrorInvalidKernelImage;
     if (r != cudaSuccess) return r;
-    return cudaFuncSetAttribute(k_fp8<AR, BN, BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    return cudaFuncSetAttribute(k_fp8<CTAS, AR, BN, BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
   });
   if (e != cudaSuccess) return e;
-  const long long tiles = (a.m + 127LL) / 128 * ((a.n + BN - 1) / BN);
+  const long long tiles = (a.m + CTAS * 128 - 1LL) / (CTAS * 128) * ((a.n + BN - 1) / BN);
   if (tiles >> 30) return cudaErrorInvalidValue;  // an output of 2^42 values or more
   // Blocks take tile after tile; those of a cluster have one.
-  const long long grid = splits > 1 ? tiles * splits : std::min<long long>(tiles, current_sm_count() * BLOCKS);
-  return launch_early(k_fp8<AR, BN, BLOCKS>, dim3((unsigned)grid), dim3(S::THREADS), S::SMEM, s, (unsigned)splits,
-                      *(const CUtensorMap*)&x, *(const CUtensorMap*)&out, a);
+  const long long grid = splits > 1 ? tiles * splits : CTAS * std::min<long long>(tiles, current_sm_count() * BLOCKS / CTAS);
+  return launch_early(k_fp8<CTAS, AR, BN, BLOCKS>, dim3((unsigned)grid), dim3(S::THREADS), S::SMEM, s,
+                      (unsigned)(splits * CTAS), *(const CUtensorMap*)&x, *(const CUtensorMap*)&w, *(const CUtensorMap*)&out, a);
 }
 
 // Rows of bytes to the units that k_fp8 reads: [n / 64][k / 128][64 rows][128
@@ -543,7 +608,7 @@ cudaError_t launch_fp8_pack(const uint8_t* codes, size_t n, size_t k, uint8_t* w
   return cudaGetLastError();
 }
 
-cudaError_t launch_fp8(const TcMap& x, const TcMap& out, const Fp8Args& a, cudaStream_t s) {
+cudaError_t launch_fp8(const TcMap& x, const TcMap& w, const TcMap& out, const Fp8Args& a, cudaStream_t s) {
   if (a.m <= 0) return cudaSuccess;
   const long long sms = current_sm_count();
   const auto tiles = [&](int bn) { return (a.m + 127LL) / 128 * ((a.n + bn - 1) / bn); };
@@ -559,14 +624,14 @@ cudaError_t launch_fp8(const TcMap& x, const TcMap& out, const Fp8Args& a, cudaS
   const int box = fp8_row_box(a.m);
   // Few rows: four blocks an SM, of three warps, so that the next call's blocks
   // find room (two an SM: 151936 x 2048 57.1 us, 32768 x 8192 46.7; four: 53.6, 43.1).
-  if (box == 16) return run<16, 64, 4>(x, out, a, splits(tiles(64), 4 * sms), s);
-  if (box == 64) return run<64, 64, 2>(x, out, a, splits(tiles(64), 2 * sms), s);
+  if (box == 16) return run<1, 16, 64, 4>(x, w, out, a, splits(tiles(64), 4 * sms), s);
+  if (box == 64) return run<1, 64, 64, 2>(x, w, out, a, splits(tiles(64), 2 * sms), s);
   // Tiles of 128 or 256 columns: whole turns of the SMs, at the measured time of
   // a turn and block of k (0.385 and 0.6 us). 333 rows of 5001 x 2064: 128 columns
   // 12.7 us, 256 columns 19.5; 1000 of 12288 x 4096: 81 and 55.
   const auto turns = [&](int bn) { return (double)((tiles(bn) + sms - 1) / sms); };
-  if (turns(128) * 0.385 < turns(256) * 0.6) return run<128, 128, 1>(x, out, a, splits(tiles(128), sms), s);
-  return run<128, 256, 1>(x, out, a, 1, s);
+  if (turns(128) * 0.385 < turns(256) * 0.6) return run<1, 128, 128, 1>(x, w, out, a, splits(tiles(128), sms), s);
+  return run<2, 128, 256, 1>(x, w, out, a, 1, s);
 }
 
 }  // namespace trit

@@ -773,6 +773,19 @@ cudaError_t make_fp8_map(TcMap* out, const void* base, size_t rows, size_t k, in
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
+cudaError_t make_fp8_packed_map(TcMap* out, const void* base, size_t bytes) {
+  EncodeTiled enc = encoder();
+  if (!enc) return cudaErrorNotSupported;
+  if (!bytes || bytes % 8192 || bytes / 128 > (size_t)INT32_MAX || ((uintptr_t)base & 15)) return cudaErrorInvalidValue;
+  cuuint64_t dims[2] = {128, bytes / 128};
+  cuuint64_t strides[1] = {128};
+  cuuint32_t box[2] = {128, 64};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc((CUtensorMap*)out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box,
+                   estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
 cudaError_t make_fp8_out_map(TcMap* out, void* base, size_t rows, size_t n, size_t stride, int type, int box_rows) {
   EncodeTiled enc = encoder();
   const size_t size = row_type_size(type);

@@ -320,6 +320,7 @@ DenseFp8::DenseFp8(const void* codes, const float* scales, size_t n, size_t k, i
     if (e == cudaSuccess) e = cudaStreamSynchronize(stream_);
     cudaFree(raw);
     TRIT_CUDA(e);
+    TRIT_CUDA(make_fp8_packed_map(&map_, codes_, fp8_packed_bytes(n, k)));
   } catch (...) {
     release();
     throw;
@@ -373,7 +374,7 @@ void DenseFp8::product(const void* codes, const float* scales, size_t m, void* o
   a.status = status_;
   TcMap out_map{};
   a.tma = make_fp8_out_map(&out_map, out, m, n_, out_stride, type, fp8_out_box((int)m)) == cudaSuccess;
-  TRIT_CUDA(launch_fp8(map, out_map, a, s));
+  TRIT_CUDA(launch_fp8(map, map_, out_map, a, s));
 }
 
 void DenseFp8::forward_codes(const void* codes, const float* scales, size_t m, void* out, size_t out_stride, int type,

@@ -113,6 +113,7 @@ class DenseFp8 {
   cudaStream_t stream_ = nullptr;
   std::shared_ptr<ScratchPool> scratch_;  // from the first call that rounds its rows
   bool captured_ = false;
+  TcMap map_;                 // of the packed weights
   int* status_ = nullptr;     // pinned: a wait inside a product ran out
 };
 
@@ -137,6 +138,8 @@ int fp8_row_box(int m);  // its box rows for m rows
 // The weights [n][k] in the order that the product reads them.
 size_t fp8_packed_bytes(size_t n, size_t k);
 cudaError_t launch_fp8_pack(const uint8_t* codes, size_t n, size_t k, uint8_t* w, cudaStream_t s);
-cudaError_t launch_fp8(const TcMap& x, const TcMap& out, const Fp8Args& a, cudaStream_t s);
+cudaError_t launch_fp8(const TcMap& x, const TcMap& w, const TcMap& out, const Fp8Args& a, cudaStream_t s);
+// A TMA map of the packed weights: rows of 128 bytes, boxes of a unit's 64.
+cudaError_t make_fp8_packed_map(TcMap* out, const void* base, size_t bytes);
 
 }  // namespace trit
