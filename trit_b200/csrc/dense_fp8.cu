@@ -21,17 +21,22 @@
 // distributed shared memory. Weights do not depend on the kernel in front, so a
 // block has its first stages of them on their way while that one still runs.
 //
-// Few rows are bound by the bytes of w: 151936 x 2048 and three rows 54 us (5.8
-// TB/s), 16384 x 4096 and 64 f32 rows 18.6 us with their rounding (3.9 TB/s),
-// 12288 x 2048 and one row 7.8 us, of which about 4 are a launch, the first copy
-// and the join. Many rows, 8000 of 12288 x 4096: 400 to 460 us with the clock
-// that the power limit leaves (1.75 to 2.0 PFLOP/s; 2.7 without the scaled
-// additions). What holds them up is the round trip of a TMEM buffer (MMA, commit,
-// load, release), of which 512 columns hold two of 256. Measured and left:
-// pairs of blocks with cta_group::2 (tiles of 256 x 256, half the bytes of w a
-// block, but a release crosses the blocks: 775 us), buffers of 128 columns
-// (the same), 16 epilogue warps (480 us, for want of registers), waits that
-// poll instead of suspending (510 us).
+// With CTAS = 2 a pair of blocks shares a tile of 256 x 256: each holds its own
+// 128 rows of x and half of the tile's rows of w, and the first one's MMAs
+// (cta_group::2) read both. An SM takes 64 bytes a clock from L2, 48 KB a block of
+// k of a tile of 128 x 256 and 32 KB of the pair's.
+//
+// Few rows are bound by the bytes of w: 151936 x 2048 and three rows 53 us (5.9
+// TB/s), 16384 x 4096 and 64 f32 rows 18.7 us with their rounding (3.9 TB/s),
+// 12288 x 2048 and one row 7.7 us, of which about 4 are a launch, the first copy
+// and the join. Many rows: 1000 of 12288 x 4096 53 us (1.9 PFLOP/s, the tensor pipe
+// busy half of the time), 8000 of them 380 to 460 us with the clocks that the
+// power limit leaves (2.9 PFLOP/s with neither loads from TMEM nor additions).
+// What holds them up is an epilogue warp's chain (wait, load, load, add) and the
+// round trip of a TMEM buffer, of which 512 columns hold two of 256. Measured and
+// left: tiles of 128 x 256 a block (55 us for the 1000 rows), MMAs and buffers of
+// half the columns (68), 16 epilogue warps (64, for want of registers), the next
+// block's first load ahead of the last additions (60), waits that poll (61).
 
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -626,11 +631,13 @@ cudaError_t launch_fp8(const TcMap& x, const TcMap& w, const TcMap& out, const F
   // find room (two an SM: 151936 x 2048 57.1 us, 32768 x 8192 46.7; four: 53.6, 43.1).
   if (box == 16) return run<1, 16, 64, 4>(x, w, out, a, splits(tiles(64), 4 * sms), s);
   if (box == 64) return run<1, 64, 64, 2>(x, w, out, a, splits(tiles(64), 2 * sms), s);
-  // Tiles of 128 or 256 columns: whole turns of the SMs, at the measured time of
-  // a turn and block of k (0.385 and 0.6 us). 333 rows of 5001 x 2064: 128 columns
-  // 12.7 us, 256 columns 19.5; 1000 of 12288 x 4096: 81 and 55.
-  const auto turns = [&](int bn) { return (double)((tiles(bn) + sms - 1) / sms); };
-  if (turns(128) * 0.385 < turns(256) * 0.6) return run<1, 128, 128, 1>(x, w, out, a, splits(tiles(128), sms), s);
+  // Tiles of 128 x 128 by a block or of 256 x 256 by a pair: whole turns of the SMs,
+  // at the measured time of a turn and block of k (0.385 and 0.5 us). 333 rows of
+  // 5001 x 2064: 12.7 us by blocks, 19.5 by tiles of 256 columns; 1000 of 12288 x
+  // 4096: 81 and 53.
+  const long long pairs = (a.m + 255LL) / 256 * ((a.n + 255LL) / 256), teams = std::max(1LL, sms / 2);
+  const long long small = (tiles(128) + sms - 1) / sms, large = (pairs + teams - 1) / teams;
+  if (small * 0.385 < large * 0.5) return run<1, 128, 128, 1>(x, w, out, a, splits(tiles(128), sms), s);
   return run<2, 128, 256, 1>(x, w, out, a, 1, s);
 }
 
