@@ -324,9 +324,10 @@ TritDense *trit_dense_q4_0(const void *blocks, size_t n, size_t k, int table, in
  * ceil(n / 128) x ceil(k / 128), row-major), both in host memory. A weight is
  * code * scale. k is a multiple of 16 up to 2^24, n at most 2^31 - 256. Rows of
  * x are 8-bit rows: e4m3 numbers with an f32 scale for each 128 of a row, which
- * trit_cuda_rms_norm writes; rows of values are rounded to such first. Each
- * block's products are summed on the tensor cores, the blocks in f32. Calls use
- * no memory of the layer's but its weights, so they may overlap and be captured.
+ * trit_cuda_rms_norm writes; rows of values are rounded to such first, in memory
+ * that a call takes and gives back in its stream's order (a captured one has its
+ * graph's). Each block's products are summed on the tensor cores, the blocks in
+ * f32. Calls share no memory but the weights, so they may overlap and be captured.
  * NULL on failure. (No counterpart in the reference.) */
 TritDense *trit_dense_fp8(const void *codes, const float *scales, size_t n, size_t k, int device);
 
@@ -528,10 +529,11 @@ void trit_cuda_rotary_free(TritRotary *rotary);
 int64_t trit_cuda_rotary_frequencies(const TritRotary *rotary, double *out, size_t cap, double *factor);
 
 /* Turns the pairs of q (rows x q_heads x head_dim) and k (rows x k_heads x
- * head_dim; 0 heads and NULL: no such tensor) by position * frequency, which is
- * formed in 64 bits (positions up to 2^53 either way; a negative one turns
- * back). `positions` has one number a row. q_out and k_out: NULL for in place.
- * Values of a head behind rotary_dim stay as they are. Returns 0, or -1. */
+ * head_dim; 0 heads and NULL: no such tensor; at most 65535 heads each) by
+ * position * frequency, which is formed in 64 bits (positions up to 2^53 either
+ * way; a negative one turns back). `positions` has one number a row. q_out and
+ * k_out: NULL for in place. Values of a head behind rotary_dim stay as they are.
+ * Returns 0, or -1. */
 int trit_cuda_rotary_apply(const TritRotary *rotary, const int64_t *positions, size_t rows, const void *q, size_t q_stride,
                            int32_t q_heads, void *q_out, size_t q_out_stride, const void *k, size_t k_stride,
                            int32_t k_heads, void *k_out, size_t k_out_stride, int type, void *cuda_stream);

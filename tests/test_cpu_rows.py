@@ -85,6 +85,8 @@ def test_rotary_needs_an_object():
 
 @pytest.mark.parametrize("args, words", [
     (dict(q_heads=-1), "heads are from 0"),
+    (dict(q_heads=65536), "heads are from 0 to 65535"),
+    (dict(k_ptr=2 * P, k_heads=65536), "heads are from 0 to 65535"),
     (dict(q_heads=0, k_ptr=2 * P, k_heads=2), "q is given with no heads"),
     (dict(q_ptr=None, q_heads=0), "neither q nor k"),
     (dict(k_ptr=P), "k is given with no heads"),

@@ -62,6 +62,19 @@ def test_heads(hd, rd, layout, dtype):
         assert torch.equal(p, qo[:-1]) and torch.equal(r, ko[:-1])
 
 
+def test_most_heads():
+    """As many heads as a call takes, one value a turn: each head as a call of few heads turns it."""
+    rotary = Rotary(512)
+    flat = torch.randn(2 * 65535 * 512 + 1, device="cuda").to(torch.bfloat16)
+    want, at = flat.clone(), torch.tensor([77], device="cuda")
+    q, k = flat[1:].view(2, 1, 65535, 512)
+    call(rotary, at, q, k, "bf16")
+    for i in range(0, 65535 * 2, 6555):
+        part = want[1 + i * 512:1 + min(i + 6555, 65535 * 2) * 512]
+        call(rotary, at, part.view(1, -1, 512), None, "bf16")
+    assert torch.equal(flat, want)
+
+
 @pytest.mark.parametrize("rows, heads, kv", [(1, 32, 8), (2, 64, 1), (64, 32, 8), (500, 16, 16), (4001, 8, 1)])
 @pytest.mark.parametrize("layout", ["halves", "interleaved"])
 def test_rows(rows, heads, kv, layout):

@@ -225,7 +225,8 @@ std::unique_ptr<Rotary> Rotary::parse(const char* text) {
 void Rotary::apply(RotaryArgs a, size_t rows, cudaStream_t s) const {
   check_type(a.type);
   a.rows = check_rows(rows);
-  if (a.q_heads < 0 || a.k_heads < 0 || a.q_heads > 65536 || a.k_heads > 65536) throw Error("heads are from 0 to 65536");
+  // (Two heads a thread and as little as a team a block: 65535 blocks in y.)
+  if (a.q_heads < 0 || a.k_heads < 0 || a.q_heads > 65535 || a.k_heads > 65535) throw Error("heads are from 0 to 65535");
   if (!a.q_heads && !a.k_heads) throw Error("neither q nor k has heads");
   int device = -1;
   const size_t size = row_type_size(a.type);
