@@ -1928,8 +1928,11 @@ std::unique_ptr<DenseOp> dense_q8_0(const void* blocks, size_t n, size_t k, int 
   }
   size_t co = 0, so = (n * k + 255) / 256 * 256;
   TRIT_CUDA(cudaMalloc(&op->mem, so + scales.size()));
-  TRIT_CUDA(cudaMemcpy(op->mem, codes.data(), codes.size(), cudaMemcpyHostToDevice));
-  TRIT_CUDA(cudaMemcpy((char*)op->mem + so, scales.data(), scales.size(), cudaMemcpyHostToDevice));
+  // On the layer's stream: a plain cudaMemcpy may return before its last bytes
+  // are there, and that stream does not wait for it.
+  TRIT_CUDA(cudaMemcpyAsync(op->mem, codes.data(), codes.size(), cudaMemcpyHostToDevice, op->stream));
+  TRIT_CUDA(cudaMemcpyAsync((char*)op->mem + so, scales.data(), scales.size(), cudaMemcpyHostToDevice, op->stream));
+  TRIT_CUDA(cudaStreamSynchronize(op->stream));
   if (table) {
     op->tab.n = (int)n; op->tab.k = (int)k; op->tab.scale_f16 = 1;
     op->tab.codes = (const int8_t*)op->mem + co;
@@ -1973,7 +1976,7 @@ std::unique_ptr<DenseOp> dense_q4_0(const void* blocks, size_t n, size_t k, int 
   op->w4.scales = (char*)op->mem + so;
   void* raw = nullptr;
   TRIT_CUDA(cudaMalloc(&raw, n * (k / 32) * 18));
-  cudaError_t e = cudaMemcpy(raw, blocks, n * (k / 32) * 18, cudaMemcpyHostToDevice);
+  cudaError_t e = cudaMemcpyAsync(raw, blocks, n * (k / 32) * 18, cudaMemcpyHostToDevice, op->stream);
   if (e == cudaSuccess) e = launch_q4_pack(raw, op->w4, op->mem, (char*)op->mem + so, op->stream);
   if (e == cudaSuccess) e = cudaStreamSynchronize(op->stream);
   cudaFree(raw);
