@@ -88,6 +88,18 @@ def test_larger(n, k, m, dtype):
     assert torch.equal(got, codes_call(dense, codes, scales, dtype)), "two calls differ"
 
 
+@pytest.mark.parametrize("n, k, m", [(357, 2112, 225), (20001, 400, 333), (3825, 672, 621), (3824, 672, 621), (2049, 4112, 389), (2064, 4112, 389),
+                                     (110, 1360, 83), (257, 8208, 1131), (2561, 528, 6400)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_rows(n, k, m, dtype):
+    """Tiles of one block or two an SM and of pairs, k split or not, whole 16 bytes or odd rows to write."""
+    dense, w = layer(n, k, 3)
+    codes, scales, x = rows(m, k, 4)
+    got = codes_call(dense, codes, scales, dtype)
+    check(got, x, w)
+    assert torch.equal(got, codes_call(dense, codes, scales, dtype)), "two calls differ"
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("n, k, m", [(96, 272, 5), (700, 1024, 70), (1024, 2048, 600)])
 def test_rows_of_values(n, k, m, dtype):

@@ -24,7 +24,10 @@
 // With CTAS = 2 a pair of blocks shares a tile of 256 x 256: each holds its own
 // 128 rows of x and half of the tile's rows of w, and the first one's MMAs
 // (cta_group::2) read both. An SM takes 64 bytes a clock from L2, 48 KB a block of
-// k of a tile of 128 x 256 and 32 KB of the pair's.
+// k of a tile of 128 x 256 and 32 KB of the pair's. Where such tiles leave many
+// rows or SMs unused, two blocks an SM take tiles of 128 x 128, one each: one
+// copies and starts while the other ends (600 rows of 4096 x 4096: 28.2 us with
+// one block an SM, 21.1 with two).
 //
 // Few rows are bound by the bytes of w: 151936 x 2048 and three rows 53 us (5.9
 // TB/s), 16384 x 4096 and 64 f32 rows 18.7 us with their rounding (3.9 TB/s),
@@ -36,7 +39,8 @@
 // round trip of a TMEM buffer, of which 512 columns hold two of 256. Measured and
 // left: tiles of 128 x 256 a block (55 us for the 1000 rows), MMAs and buffers of
 // half the columns (68), 16 epilogue warps (64, for want of registers), the next
-// block's first load ahead of the last additions (60), waits that poll (61).
+// block's first load ahead of the last additions (60), waits that poll (61), pairs of
+// 256 x 128 two an SM (61; 8000 rows 424 beside 365).
 
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -63,7 +67,7 @@ template <int CTAS, int AR, int BN, int BLOCKS_>
 struct F8Shape {
   static constexpr int BR = BN / CTAS;  // rows of w a block holds
   static constexpr int STAGE = (AR + BR) * F8_K;
-  static constexpr int COLUMN_WARPS = BN >= 128 ? 2 : 1;      // epilogue warps that share a tile's columns
+  static constexpr int COLUMN_WARPS = BN >= 128 && BLOCKS_ == 1 ? 2 : 1;  // epilogue warps that share a tile's columns
   static constexpr int CW = BN / COLUMN_WARPS;                // columns of each
   static constexpr int M = AR <= 64 ? 64 : 128;               // of the MMA
   static constexpr int LANES = M / 4;                         // rows in a quarter of TMEM: its first lanes
@@ -75,20 +79,24 @@ struct F8Shape {
   static constexpr int LOADER = LONE ? 2 : 0, ISSUER = 1, EPILOGUE = LONE ? 0 : 4;
   static constexpr int BUFS = BN * 4 * BLOCKS_ > 512 ? 2 : 4;
   static constexpr int COLS = BUFS * BN;                      // of TMEM
-  static constexpr int STAGING = ROW_WARPS * COLUMN_WARPS * 4096;
+  // Two blocks of 128 x 128 an SM: each takes one tile, so that its rows leave
+  // through the stages' memory, which is free by then.
+  static constexpr bool ONE_TILE = BN >= 128 && BLOCKS_ == 2;
+  static constexpr int STAGING = ONE_TILE ? 0 : ROW_WARPS * COLUMN_WARPS * 4096;
   static_assert(STAGE % 1024 == 0, "swizzled rows begin at whole kilobytes");
   static constexpr int TAIL = (M - AR) * F8_K > STAGING ? (M - AR) * F8_K : STAGING;  // behind the stages
   static constexpr int BLOCKS = BLOCKS_;                      // an SM holds
   static constexpr int ROOM = 226 * 1024 / BLOCKS - 2048 - 1024 - TAIL;  // (a block's own 1 KB, and its static memory)
   static constexpr int STAGES = ROOM / STAGE < 12 ? ROOM / STAGE : 12;
   static constexpr int SMEM = 1024 + STAGES * STAGE + TAIL;
-  // 128 sums and two loads of 32 a thread do not fit the block's even share of
-  // the registers: the epilogue takes what the other roles do not need. The
-  // shares add up to the launch's 384 threads x 168.
-  static constexpr bool SPLITS = BN < 256;  // k may be split over a cluster
+  // 128 sums and two loads a thread do not fit the block's even share of the
+  // registers: the epilogue takes what the other roles do not need. The shares
+  // add up to the launch's 384 threads x 168, or 256 x 128.
+  static constexpr bool SPLITS = BLOCKS_ > 1;  // k may be split over a cluster
+  static constexpr int LOAD = ONE_TILE ? 16 : 32;  // columns a load from TMEM
   static constexpr bool SPLIT = CW == 128;
-  static constexpr int REGS = 168, REGS_FEW = 56, REGS_MANY = 224;
-  static_assert(!SPLIT || (THREADS == 384 && 128 * REGS_FEW + 256 * REGS_MANY == THREADS * REGS), "register shares");
+  static constexpr int REGS = ONE_TILE ? 128 : 168, REGS_FEW = ONE_TILE ? 48 : 40, REGS_MANY = ONE_TILE ? 208 : 232;
+  static_assert(!SPLIT || 128 * REGS_FEW + (THREADS - 128) * REGS_MANY == THREADS * REGS, "register shares");
 };
 struct F8Sync {
   uint64_t full[12], empty[12], tfull[4], tempty[4], drain;
@@ -212,26 +220,32 @@ __device__ __forceinline__ void store_tile(const float2 (&acc)[CW / 2], uint8_t*
       return;
     }
     __syncwarp();
+    // Plain stores, a row's word from each lane; eight rows' words are read
+    // before the first is stored, and only whole words are (a branch a row for
+    // what a word leaves over took 3 us more of 333 rows of 5001 x 2064 in f16).
     const int live = min(128 / size, a.n - col);
-#pragma unroll 8
-    for (int r = 0; r < LANES; ++r) {
-      if (r >= rows) break;
-      const uint32_t w = *(const uint32_t*)(staging + r * 128 + ((lane / 4 ^ (r & 7)) << 4) + (lane & 3) * 4);
-      uint8_t* p = out + ((size_t)r * a.out_stride + col) * size;
-      if (f32) {
-        if (lane < live) ((uint32_t*)p)[lane] = w;
-        continue;
+    const size_t pitch = a.out_stride * size;
+    uint8_t* p = out + (size_t)col * size;
+    const int odd0 = (int)((uintptr_t)p >> 1 & 1), odd_step = f32 ? 0 : (int)(a.out_stride & 1);
+#pragma unroll 1
+    for (int r0 = 0; r0 < rows; r0 += 8) {
+      uint32_t w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = *(const uint32_t*)(staging + (r0 + j) * 128 + ((lane / 4 ^ j) << 4) + (lane & 3) * 4);
+#pragma unroll
+      for (int j = 0; j < 8; ++j, p += pitch) {
+        // (A word of a row that starts on an odd place: see below.)
+        const int e = f32 ? lane : 2 * lane - (odd0 ^ (odd_step & j));
+        if (r0 + j < rows && e >= 0 && (f32 ? e : e + 1) < live) *(uint32_t*)(p + e * size) = w[j];
       }
-      // (A word of a row that starts on an odd place: see below.)
-      const int odd = (int)((uintptr_t)p >> 1 & 1), e = 2 * lane - odd;
-      if (e >= 0 && e + 1 < live) {
-        *(uint32_t*)(p + 2 * e) = w;
-      } else if (e >= 0) {
-        if (e < live) ((uint16_t*)p)[e] = (uint16_t)w;
-      } else {
-        if (live > 0) ((uint16_t*)p)[0] = (uint16_t)(w >> 16);
-        if (live == 64) ((uint16_t*)p)[63] = (uint16_t)w;
-      }
+    }
+    // What whole words leave over of its row stores each lane.
+    if (!f32 && lane < rows && live > 0) {
+      const int odd = odd0 ^ (odd_step & lane);
+      uint16_t* q = (uint16_t*)(out + ((size_t)lane * a.out_stride + col) * size);
+      const auto word = [&](int i) { return *(const uint32_t*)(staging + lane * 128 + ((i / 4 ^ (lane & 7)) << 4) + (i & 3) * 4); };
+      if (odd) q[0] = (uint16_t)(word(0) >> 16);
+      if ((live ^ odd) & 1 && live > odd) q[live - 1] = (uint16_t)word(odd ? live / 2 % 32 : live / 2);
     }
     __syncwarp();
   };
@@ -469,7 +483,7 @@ __global__ void __launch_bounds__(F8Shape<CTAS, AR, BN, BLOCKS>::THREADS, BLOCKS
     const int quarter = warp & 3, part = (warp - S::EPILOGUE) >> 2;
     after_kernel_before();
     if (quarter < S::ROW_WARPS) {
-      uint8_t* staging = base + S::STAGES * S::STAGE + (part * S::ROW_WARPS + quarter) * 4096;
+      uint8_t* staging = base + (S::ONE_TILE ? 0 : S::STAGES * S::STAGE) + (part * S::ROW_WARPS + quarter) * 4096;
       const uint32_t tl = tmem + ((uint32_t)(quarter * 32) << 16) + part * S::CW;
       const bool vec = a.blocks % 4 == 0 && ((uintptr_t)a.x_scales & 15) == 0;
       uint32_t it = 0;
@@ -507,13 +521,13 @@ __global__ void __launch_bounds__(F8Shape<CTAS, AR, BN, BLOCKS>::THREADS, BLOCKS
           fence_after();
           // 32 columns a load; the next ones are on the way while these are added.
           const uint32_t from = tl + u * BN;
-          uint32_t v[2][32];
-          tmem_ld<32>(from, v[0]);
+          uint32_t v[2][S::LOAD];
+          tmem_ld<S::LOAD>(from, v[0]);
 #pragma unroll
-          for (int q = 0; q < S::CW / 32; ++q) {
+          for (int q = 0; q < S::CW / S::LOAD; ++q) {
             tmem_wait_ld();
-            if (q + 1 < S::CW / 32) {
-              tmem_ld<32>(from + (q + 1) * 32, v[(q + 1) & 1]);
+            if (q + 1 < S::CW / S::LOAD) {
+              tmem_ld<S::LOAD>(from + (q + 1) * S::LOAD, v[(q + 1) & 1]);
             } else {
               fence_before();
               if (lane == 0) {
@@ -524,9 +538,10 @@ __global__ void __launch_bounds__(F8Shape<CTAS, AR, BN, BLOCKS>::THREADS, BLOCKS
               }
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              acc[q * 16 + i] = fma2(make_float2(__uint_as_float(v[q & 1][2 * i]), __uint_as_float(v[q & 1][2 * i + 1])), s2,
-                                     acc[q * 16 + i]);
+            for (int i = 0; i < S::LOAD / 2; ++i) {
+              float2& sum = acc[q * (S::LOAD / 2) + i];
+              sum = fma2(make_float2(__uint_as_float(v[q & 1][2 * i]), __uint_as_float(v[q & 1][2 * i + 1])), s2, sum);
+            }
           }
         }
         if (S::SPLITS && splits > 1) {
@@ -581,7 +596,7 @@ cudaError_t run(const TcMap& x, const TcMap& w, const TcMap& out, const Fp8Args&
   const long long tiles = (a.m + CTAS * 128 - 1LL) / (CTAS * 128) * ((a.n + BN - 1) / BN);
   if (tiles >> 30) return cudaErrorInvalidValue;  // an output of 2^42 values or more
   // Blocks take tile after tile; those of a cluster have one.
-  const long long grid = splits > 1 ? tiles * splits : CTAS * std::min<long long>(tiles, current_sm_count() * BLOCKS / CTAS);
+  const long long grid = splits > 1 || S::ONE_TILE ? tiles * splits : CTAS * std::min<long long>(tiles, current_sm_count() * BLOCKS / CTAS);
   return launch_early(k_fp8<CTAS, AR, BN, BLOCKS>, dim3((unsigned)grid), dim3(S::THREADS), S::SMEM, s,
                       (unsigned)(splits * CTAS), *(const CUtensorMap*)&x, *(const CUtensorMap*)&w, *(const CUtensorMap*)&out, a);
 }
@@ -631,13 +646,23 @@ cudaError_t launch_fp8(const TcMap& x, const TcMap& w, const TcMap& out, const F
   // find room (two an SM: 151936 x 2048 57.1 us, 32768 x 8192 46.7; four: 53.6, 43.1).
   if (box == 16) return run<1, 16, 64, 4>(x, w, out, a, splits(tiles(64), 4 * sms), s);
   if (box == 64) return run<1, 64, 64, 2>(x, w, out, a, splits(tiles(64), 2 * sms), s);
-  // Tiles of 128 x 128 by a block or of 256 x 256 by a pair: whole turns of the SMs,
-  // at the measured time of a turn and block of k (0.385 and 0.5 us). 333 rows of
-  // 5001 x 2064: 12.7 us by blocks, 19.5 by tiles of 256 columns; 1000 of 12288 x
-  // 4096: 81 and 53.
-  const long long pairs = (a.m + 255LL) / 256 * ((a.n + 255LL) / 256), teams = std::max(1LL, sms / 2);
-  const long long small = (tiles(128) + sms - 1) / sms, large = (pairs + teams - 1) / teams;
-  if (small * 0.385 < large * 0.5) return run<1, 128, 128, 1>(x, w, out, a, splits(tiles(128), sms), s);
+  // More rows: tiles of 128 x 128, one block or two an SM (these have fewer warps
+  // and stages each; one copies while the other ends), or of 256 x 256 by pairs.
+  // What each takes, in us: a call, whole turns of the SMs, and a turn's blocks of
+  // k, as measured. us by one, two and pairs: 333 rows of 5001 x 2064 11.0, 13.7,
+  // 15.2; 128 of 12288 x 2048 10.0, 11.3, 13.2; 512 of 2048 x 6144 -, 15.0 (k in
+  // four), 26; 300 of 20000 x 4096 51, 39, 53; 4000 of 1024 x 2048 16.4, 12.8,
+  // 13.8; 1140 of 14746 x 528 31, 32, 26; 1000 of 12288 x 4096 76, 61, 54; 8000
+  // of them -, 441, 372.
+  const auto us = [&](double call, double turn, double block, int blocks, long long work, long long room) {
+    return call + (turn + block * blocks) * (double)((work + room - 1) / room);
+  };
+  const int z = splits(tiles(128), 2 * sms);
+  const double one = us(3.0, 1.0, 0.385, a.blocks, tiles(128), sms);
+  const double two = us(z > 1 ? 4.0 : 1.0, 3.0, 0.58, (a.blocks + z - 1) / z, tiles(128) * z, 2 * sms);
+  const double pairs = us(4.0, 1.5, 0.545, a.blocks, (a.m + 255LL) / 256 * ((a.n + 255LL) / 256), std::max(1LL, sms / 2));
+  if (one <= two && one <= pairs) return run<1, 128, 128, 1>(x, w, out, a, 1, s);
+  if (two <= pairs) return run<1, 128, 128, 2>(x, w, out, a, z, s);
   return run<2, 128, 256, 1>(x, w, out, a, 1, s);
 }
 
