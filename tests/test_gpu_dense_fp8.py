@@ -89,7 +89,8 @@ def test_larger(n, k, m, dtype):
 
 
 @pytest.mark.parametrize("n, k, m", [(357, 2112, 225), (20001, 400, 333), (3825, 672, 621), (3824, 672, 621), (2049, 4112, 389), (2064, 4112, 389),
-                                     (110, 1360, 83), (257, 8208, 1131), (2561, 528, 6400)])
+                                     (110, 1360, 83), (257, 8208, 1131), (2561, 528, 6400), (20001, 400, 50),
+                                     (23001, 2064, 50), (5001, 4112, 33), (1000, 8208, 64), (9417, 5200, 35)])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_many_rows(n, k, m, dtype):
     """Tiles of one block or two an SM and of pairs, k split or not, whole 16 bytes or odd rows to write."""

@@ -30,7 +30,7 @@
 // one block an SM, 21.1 with two).
 //
 // Few rows are bound by the bytes of w: 151936 x 2048 and three rows 53 us (5.9
-// TB/s), 16384 x 4096 and 64 f32 rows 18.7 us with their rounding (3.9 TB/s),
+// TB/s), 16384 x 4096 and 64 f32 rows 18.0 us with their rounding (4.0 TB/s),
 // 12288 x 2048 and one row 7.7 us, of which about 4 are a launch, the first copy
 // and the join. Many rows: 1000 of 12288 x 4096 53 us (1.9 PFLOP/s, the tensor pipe
 // busy half of the time), 8000 of them 380 to 460 us with the clocks that the
@@ -635,31 +635,39 @@ cudaError_t launch_fp8(const TcMap& x, const TcMap& w, const TcMap& out, const F
   // As many blocks of a cluster as there is room for beside each other, with at
   // least two blocks of k, six where eight share (4096 x 4096, three rows: a
   // cluster of 1 11.7 us, 2 8.6, 4 7.0, 8 7.8; 2048 x 6144: 16.2, 10.3, 7.2, 6.2;
-  // 12288 x 2048: 7.9, 7.8, 12.8, 19.3).
+  // 12288 x 2048: 7.9, 7.8, 12.8, 19.3). The parts of the chip that a cluster stays
+  // within hold no whole number of large ones: of 296 blocks 70 clusters of four
+  // and 33 of eight (k = 6400, 40 rows: 70 tiles in four 15.1 us, 72 23.3).
   const auto splits = [&](long long tiles, long long room) {
     int z = 1;
-    while (z < 8 && tiles * z * 2 <= room && a.blocks / (z * 2) >= (z < 4 ? 2 : 6)) z *= 2;
+    while (z < 8 && tiles * z * 2 <= room * (z == 1 ? 16 : z == 2 ? 15 : 14) / 16 && a.blocks / (z * 2) >= (z < 4 ? 2 : 6)) z *= 2;
     return z;
   };
   const int box = fp8_row_box(a.m);
   // Few rows: four blocks an SM, of three warps, so that the next call's blocks
   // find room (two an SM: 151936 x 2048 57.1 us, 32768 x 8192 46.7; four: 53.6, 43.1).
   if (box == 16) return run<1, 16, 64, 4>(x, w, out, a, splits(tiles(64), 4 * sms), s);
-  if (box == 64) return run<1, 64, 64, 2>(x, w, out, a, splits(tiles(64), 2 * sms), s);
-  // More rows: tiles of 128 x 128, one block or two an SM (these have fewer warps
-  // and stages each; one copies while the other ends), or of 256 x 256 by pairs.
+  // More rows: 128 columns, one block or two an SM (these have fewer warps and
+  // stages each; one copies while the other ends), or tiles of 256 x 256 by pairs.
   // What each takes, in us: a call, whole turns of the SMs, and a turn's blocks of
-  // k, as measured. us by one, two and pairs: 333 rows of 5001 x 2064 11.0, 13.7,
-  // 15.2; 128 of 12288 x 2048 10.0, 11.3, 13.2; 512 of 2048 x 6144 -, 15.0 (k in
-  // four), 26; 300 of 20000 x 4096 51, 39, 53; 4000 of 1024 x 2048 16.4, 12.8,
-  // 13.8; 1140 of 14746 x 528 31, 32, 26; 1000 of 12288 x 4096 76, 61, 54; 8000
-  // of them -, 441, 372.
+  // k, as measured. us by one, two and pairs, up to 64 rows: 16384 x 4096 15.1,
+  // 16.4; 151936 x 2048 58, 61; 32768 x 8192 48, 44; 8192 x 4096 13.2, 10.1 (k in
+  // four). More: 333 rows of 5001 x 2064 11.0, 13.7, 15.2; 128 of 12288 x 2048 10.0,
+  // 11.3, 13.2; 512 of 2048 x 6144 -, 15.0 (k in four), 26; 300 of 20000 x 4096 51,
+  // 39, 53; 4000 of 1024 x 2048 16.4, 12.8, 13.8; 1140 of 14746 x 528 31, 32, 26;
+  // 1000 of 12288 x 4096 76, 61, 54; 8000 of them -, 441, 372.
   const auto us = [&](double call, double turn, double block, int blocks, long long work, long long room) {
     return call + (turn + block * blocks) * (double)((work + room - 1) / room);
   };
-  const int z = splits(tiles(128), 2 * sms);
+  const int z = splits(tiles(128), 2 * sms), part = (a.blocks + z - 1) / z;
+  if (box == 64) {
+    const double one = us(2.3, 0.0, 0.40, a.blocks, tiles(128), sms);
+    const double two = us(z > 1 ? 2.2 : 1.0, 3.0, 0.62, part, tiles(128) * z, 2 * sms);
+    if (one <= two) return run<1, 64, 128, 1>(x, w, out, a, 1, s);
+    return run<1, 64, 128, 2>(x, w, out, a, z, s);
+  }
   const double one = us(3.0, 1.0, 0.385, a.blocks, tiles(128), sms);
-  const double two = us(z > 1 ? 4.0 : 1.0, 3.0, 0.58, (a.blocks + z - 1) / z, tiles(128) * z, 2 * sms);
+  const double two = us(z > 1 ? 4.0 : 1.0, 3.0, 0.58, part, tiles(128) * z, 2 * sms);
   const double pairs = us(4.0, 1.5, 0.545, a.blocks, (a.m + 255LL) / 256 * ((a.n + 255LL) / 256), std::max(1LL, sms / 2));
   if (one <= two && one <= pairs) return run<1, 128, 128, 1>(x, w, out, a, 1, s);
   if (two <= pairs) return run<1, 128, 128, 2>(x, w, out, a, z, s);
