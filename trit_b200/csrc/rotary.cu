@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kRotaryThreads, 4) k_rotary(const __grid_const
     float* to = (float*)angles + z * 2 * slots;
 #pragma unroll 1  // (the values on their way need the registers)
     for (int p = thread; p < pairs; p += threads) {
-      const float2 cs = turn((double)__ldg(a.positions + row0 + z) * w.turns[p], w.factor);
+      const float2 cs = turn((double)a.positions[row0 + z] * w.turns[p], w.factor);
       to[p] = cs.x;
       to[slots + p] = cs.y;
     }
