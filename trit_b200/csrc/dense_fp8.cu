@@ -30,9 +30,9 @@
 // one block an SM, 21.1 with two).
 //
 // Few rows are bound by the bytes of w: 151936 x 2048 and three rows 53 us (5.9
-// TB/s), 16384 x 4096 and 64 f32 rows 18.0 us with their rounding (4.0 TB/s),
+// TB/s), 16384 x 4096 and 64 f32 rows 17.1 us with their rounding (4.2 TB/s),
 // 12288 x 2048 and one row 7.7 us, of which about 4 are a launch, the first copy
-// and the join. Many rows: 1000 of 12288 x 4096 53 us (1.9 PFLOP/s, the tensor pipe
+// and the join. Many rows: 1000 of 12288 x 4096 52 us (1.9 PFLOP/s, the tensor pipe
 // busy half of the time), 8000 of them 380 to 460 us with the clocks that the
 // power limit leaves (2.9 PFLOP/s with neither loads from TMEM nor additions).
 // What holds them up is an epilogue warp's chain (wait, load, load, add) and the
@@ -86,14 +86,16 @@ struct F8Shape {
   static_assert(STAGE % 1024 == 0, "swizzled rows begin at whole kilobytes");
   static constexpr int TAIL = (M - AR) * F8_K > STAGING ? (M - AR) * F8_K : STAGING;  // behind the stages
   static constexpr int BLOCKS = BLOCKS_;                      // an SM holds
-  static constexpr int ROOM = 226 * 1024 / BLOCKS - 2048 - 1024 - TAIL;  // (a block's own 1 KB, and its static memory)
+  static constexpr int EPILOGUE_THREADS = LONE ? 32 : THREADS - 128;
+  static constexpr int SCALES = LONE ? 0 : 2 * 16 * EPILOGUE_THREADS;  // of x, eight of each thread's row
+  static constexpr int ROOM = 226 * 1024 / BLOCKS - 2048 - 1024 - TAIL - SCALES;  // (a block's own 1 KB, and its static memory)
   static constexpr int STAGES = ROOM / STAGE < 12 ? ROOM / STAGE : 12;
-  static constexpr int SMEM = 1024 + STAGES * STAGE + TAIL;
+  static constexpr int SMEM = 1024 + STAGES * STAGE + TAIL + SCALES;
   // 128 sums and two loads a thread do not fit the block's even share of the
   // registers: the epilogue takes what the other roles do not need. The shares
   // add up to the launch's 384 threads x 168, or 256 x 128.
   static constexpr bool SPLITS = BLOCKS_ > 1;  // k may be split over a cluster
-  static constexpr int LOAD = ONE_TILE ? 16 : 32;  // columns a load from TMEM
+  static constexpr int LOAD = ONE_TILE || CTAS == 2 ? 16 : 32;  // columns a load from TMEM (as registers allow)
   static constexpr bool SPLIT = CW == 128;
   static constexpr int REGS = ONE_TILE ? 128 : 168, REGS_FEW = ONE_TILE ? 48 : 40, REGS_MANY = ONE_TILE ? 208 : 232;
   static_assert(!SPLIT || 128 * REGS_FEW + (THREADS - 128) * REGS_MANY == THREADS * REGS, "register shares");
@@ -174,16 +176,36 @@ __device__ __forceinline__ void tile_place(uint32_t t, uint32_t row_tiles, uint3
   *c = (int)(at / rows);
 }
 
-// The scales of x of four blocks of a row; those past the end are not used.
+// The scales of x of a row's blocks b to b + 3; those past the end are not used.
+// (Not through the read-only path: the kernel before may write them while this
+// one waits.)
 __device__ __forceinline__ float4 scales4(const float* sx, int b, int blocks, bool live, bool vec) {
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (!live || b >= blocks) return v;
-  if (vec) return __ldg((const float4*)(sx + b));
-  v.x = __ldg(sx + b);
-  if (b + 1 < blocks) v.y = __ldg(sx + b + 1);
-  if (b + 2 < blocks) v.z = __ldg(sx + b + 2);
-  if (b + 3 < blocks) v.w = __ldg(sx + b + 3);
+  if (vec) return *(const float4*)(sx + b);
+  v.x = sx[b];
+  if (b + 1 < blocks) v.y = sx[b + 1];
+  if (b + 2 < blocks) v.z = sx[b + 2];
+  if (b + 3 < blocks) v.w = sx[b + 3];
   return v;
+}
+// The same on their way to shared memory. Loads to registers four blocks ahead
+// hold up a warp with many other loads all the same (64 rows of 16384 x 4096 15.3
+// us, 14.6 so); the one warp of up to 16 rows is faster with them (three rows of
+// 151936 x 2048 52.2 us, 53.8 so).
+__device__ __forceinline__ void fetch_scales(float4* to, const float* sx, int b, int blocks, bool live, bool vec) {
+  if (vec) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(live && b < blocks ? sx + b : sx),
+                 "r"(live && b < blocks ? 16 : 0)
+                 : "memory");
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(to) + 4 * j),
+                   "l"(live && b + j < blocks ? sx + b + j : sx), "r"(live && b + j < blocks ? 4 : 0)
+                   : "memory");
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
 __device__ __forceinline__ uint32_t pack16(float a, float b, bool f16) {
@@ -485,6 +507,7 @@ __global__ void __launch_bounds__(F8Shape<CTAS, AR, BN, BLOCKS>::THREADS, BLOCKS
     if (quarter < S::ROW_WARPS) {
       uint8_t* staging = base + (S::ONE_TILE ? 0 : S::STAGES * S::STAGE) + (part * S::ROW_WARPS + quarter) * 4096;
       const uint32_t tl = tmem + ((uint32_t)(quarter * 32) << 16) + part * S::CW;
+      float4* scales = (float4*)(base + S::STAGES * S::STAGE + S::TAIL) + (threadIdx.x - S::EPILOGUE * 32);
       const bool vec = a.blocks % 4 == 0 && ((uintptr_t)a.x_scales & 15) == 0;
       uint32_t it = 0;
       bool ok = true;
@@ -501,17 +524,30 @@ __global__ void __launch_bounds__(F8Shape<CTAS, AR, BN, BLOCKS>::THREADS, BLOCKS
         float2 acc[S::CW / 2];
 #pragma unroll
         for (int i = 0; i < S::CW / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
-        float4 now = make_float4(0.0f, 0.0f, 0.0f, 0.0f), next = scales4(sx, lo & ~3, hi, live, vec);
+        float4 now = make_float4(0.0f, 0.0f, 0.0f, 0.0f), next = now;
+        if constexpr (S::LONE) next = scales4(sx, lo & ~3, hi, live, vec);
+        else fetch_scales(scales + (lo >> 2 & 1) * S::EPILOGUE_THREADS, sx, lo & ~3, hi, live, vec);
         float sws = lo + lane < hi ? __ldg(sw + lo + lane) : 0.0f;
         for (int b = lo; b < hi; ++b, ++it) {
           if ((b & 3) == 0 || b == lo) {
-            now = next;
-            for (int i = 0; S::SPLITS && i < (b & 3); ++i) now = make_float4(now.y, now.z, now.w, 0.0f);
-            next = scales4(sx, (b & ~3) + 4, hi, live, vec);
+            if constexpr (S::LONE) {
+              now = next;
+              for (int i = 0; i < (b & 3); ++i) now = make_float4(now.y, now.z, now.w, 0.0f);
+              next = scales4(sx, (b & ~3) + 4, hi, live, vec);
+            } else {
+              asm volatile("cp.async.wait_group 0;" ::: "memory");
+              if ((b & ~3) + 4 < hi) fetch_scales(scales + ((b >> 2 & 1) ^ 1) * S::EPILOGUE_THREADS, sx, (b & ~3) + 4, hi, live, vec);
+            }
           }
           if (b > lo && ((b - lo) & 31) == 0) sws = b + lane < hi ? __ldg(sw + b + lane) : 0.0f;
-          const float scale = now.x * __shfl_sync(0xffffffffu, sws, (b - lo) & 31);
-          now = make_float4(now.y, now.z, now.w, 0.0f);
+          float scale;
+          if constexpr (S::LONE) {
+            scale = now.x;
+            now = make_float4(now.y, now.z, now.w, 0.0f);
+          } else {
+            scale = ((const float*)(scales + (b >> 2 & 1) * S::EPILOGUE_THREADS))[b & 3];
+          }
+          scale *= __shfl_sync(0xffffffffu, sws, (b - lo) & 31);
           const float2 s2 = make_float2(scale, scale);
           const uint32_t u = it % S::BUFS;
           if (!__all_sync(0xffffffffu, mbar_wait(&y->tfull[u], (it / S::BUFS) & 1, abort))) {
@@ -519,7 +555,7 @@ __global__ void __launch_bounds__(F8Shape<CTAS, AR, BN, BLOCKS>::THREADS, BLOCKS
             break;
           }
           fence_after();
-          // 32 columns a load; the next ones are on the way while these are added.
+          // The next columns are on the way while these are added.
           const uint32_t from = tl + u * BN;
           uint32_t v[2][S::LOAD];
           tmem_ld<S::LOAD>(from, v[0]);
@@ -548,7 +584,8 @@ __global__ void __launch_bounds__(F8Shape<CTAS, AR, BN, BLOCKS>::THREADS, BLOCKS
           if (lane < S::LANES) put_part<S::CW, BN>(acc, base, quarter * S::LANES + lane, part * S::CW);
         } else if (ok && row0 < a.m) store_tile<S::CW, S::LANES>(acc, staging, omap, a, row0, col0, lane);
       }
-      // The last chunks have left shared memory before it is given back.
+      // Copies to and from shared memory have ended before it is given back.
+      asm volatile("cp.async.wait_all;" ::: "memory");
       if (a.tma && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
   }
