@@ -27,13 +27,13 @@
 // k of a tile of 128 x 256 and 32 KB of the pair's. Where such tiles leave many
 // rows or SMs unused, two blocks an SM take tiles of 128 x 128, one each: one
 // copies and starts while the other ends (600 rows of 4096 x 4096: 28.2 us with
-// one block an SM, 21.1 with two).
+// one block an SM, 20.3 with two).
 //
 // Few rows are bound by the bytes of w: 151936 x 2048 and three rows 53 us (5.9
 // TB/s), 16384 x 4096 and 64 f32 rows 17.1 us with their rounding (4.2 TB/s),
-// 12288 x 2048 and one row 7.7 us, of which about 4 are a launch, the first copy
+// 12288 x 2048 and one row 7.6 us, of which about 4 are a launch, the first copy
 // and the join. Many rows: 1000 of 12288 x 4096 52 us (1.9 PFLOP/s, the tensor pipe
-// busy half of the time), 8000 of them 380 to 460 us with the clocks that the
+// busy half of the time), 8000 of them 370 to 450 us with the clocks that the
 // power limit leaves (2.9 PFLOP/s with neither loads from TMEM nor additions).
 // What holds them up is an epilogue warp's chain (wait, load, load, add) and the
 // round trip of a TMEM buffer, of which 512 columns hold two of 256. Measured and
