@@ -472,6 +472,17 @@ __global__ void __launch_bounds__(F8Shape<CTAS, AR, BN, BLOCKS>::THREADS, BLOCKS
           while ((rank || !mbar_test(&y->full[z % S::STAGES], (z / S::STAGES) & 1)) && now_ns() - t0 < (rank ? 20000000ll : TC_WAIT_NS)) {
           }
       }
+      if constexpr (CTAS == 2) {
+        // The first block's MMAs arrive at both blocks' barriers. A barrier of this
+        // block says nothing about the other's copy, so each block sees its own
+        // last arrivals before it ends: one that is still on its way would land in
+        // memory that belongs to the next block by then.
+        for (uint32_t z = it > S::STAGES ? it - S::STAGES : 0; z < it && ok; ++z)
+          ok = mbar_wait(&y->empty[z % S::STAGES], (z / S::STAGES) & 1, abort);
+        const long long t0 = now_ns();
+        while (!mbar_test(&y->drain, 0) && now_ns() - t0 < TC_WAIT_NS) {
+        }
+      }
     } else if (warp == S::ISSUER && rank == 0 && elected()) {
       after_kernel_before();  // however long that one takes, the limits of the waits run from its end
       const uint32_t s0 = smem_u32(base);
@@ -598,7 +609,7 @@ __global__ void __launch_bounds__(F8Shape<CTAS, AR, BN, BLOCKS>::THREADS, BLOCKS
     join_parts<BN>(base, a, r * 128, min(AR, a.m - r * 128), c * BN, split, splits);
     cluster_sync();  // nobody leaves while others read its part
   }
-  // A pair ends together: the first block's MMAs read the second's memory, and both arrive at its barriers.
+  // A pair ends together: the first block's MMAs read the second's memory, whose epilogue arrives at the first's barriers.
   if constexpr (CTAS == 2) cluster_sync();
   if (warp == S::ISSUER) {
     fence_after();
