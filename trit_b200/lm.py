@@ -379,6 +379,17 @@ class CausalLm:
                 "launches": launches.value}
 
 
+def _e4m3_bytes(codes) -> np.ndarray:
+    """The bytes of e4m3 numbers: those of a one-byte type as they lie in memory (a conversion to integers would take
+    the numbers' values), or integers of a wider one that are bytes."""
+    a = np.asarray(codes)
+    if a.dtype.itemsize == 1 and (a.dtype.kind in "ui" or a.dtype.name == "float8_e4m3fn"):
+        return np.ascontiguousarray(a).view(np.uint8)
+    if a.dtype.kind in "ui" and (not a.size or (a.min() >= 0 and a.max() <= 255)):
+        return np.ascontiguousarray(a, dtype=np.uint8)
+    raise TritError(f"codes of {a.dtype} are neither bytes nor e4m3 numbers")
+
+
 class Dense:
     """One product layer from ggml Q8_0 blocks (Dense, src/cpu/gemm.rs:14-24), from Q4_0 blocks, or of 8-bit
     floating point with block scales."""
@@ -410,9 +421,10 @@ class Dense:
 
     @classmethod
     def fp8(cls, codes: np.ndarray, scales: np.ndarray, n: int, k: int, device: int = 0) -> "Dense":
-        """A layer of e4m3 weights (codes: n x k bytes) with an f32 scale for each block of 128 x 128
-        (ceil(n / 128) x ceil(k / 128)) (trit_dense_fp8). Rows of x are e4m3 with a scale for each 128 of a row."""
-        b = np.ascontiguousarray(codes, dtype=np.uint8)
+        """A layer of e4m3 weights (codes: n x k, as bytes or as numbers of a float8_e4m3fn type) with an f32 scale for
+        each block of 128 x 128 (ceil(n / 128) x ceil(k / 128)) (trit_dense_fp8). Rows of x are e4m3 with a scale for
+        each 128 of a row."""
+        b = _e4m3_bytes(codes)
         s = np.ascontiguousarray(scales, dtype=np.float32)
         if b.size != n * k:
             raise TritError(f"{b.size} bytes are not the numbers of a {n}x{k} matrix")
