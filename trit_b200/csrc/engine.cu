@@ -148,9 +148,18 @@ void Lm::map_slot(int slot, const PrefixState* prefix) {
 
 namespace {
 
+// Host memory to the device, there for kernels of `s` when it returns. A plain
+// cudaMemcpy of pageable memory may return before its last bytes are there, and
+// a non-blocking stream does not wait for it.
+void upload(void* to, const void* from, size_t bytes, cudaStream_t s) {
+  TRIT_CUDA(cudaMemcpyAsync(to, from, bytes, cudaMemcpyHostToDevice, s));
+  TRIT_CUDA(cudaStreamSynchronize(s));
+}
+
 // Two passes over the weights: the first sizes the arena, the second
 // copies every tensor into it.
 struct Arena {
+  cudaStream_t stream = nullptr;
   char* base = nullptr;
   size_t used = 0;
   bool fill = false;
@@ -160,7 +169,7 @@ struct Arena {
     return at;
   }
   void put(size_t at, const void* src, size_t n) {
-    if (fill) TRIT_CUDA(cudaMemcpy(base + at, src, n, cudaMemcpyHostToDevice));
+    if (fill) upload(base + at, src, n, stream);
   }
   const void* ptr(size_t at) const { return base ? base + at : nullptr; }
 };
@@ -701,6 +710,7 @@ void Lm::load(const std::string& dir) {
   std::string cache_file;
   for (int pass = 0; pass < 2; ++pass) {
     Arena A;
+    A.stream = stream_;
     A.fill = pass == 1 && !from_cache;
     A.base = (char*)arena_;
     layers_.assign(cfg_.layers, DLayer{});
@@ -744,7 +754,7 @@ void Lm::load(const std::string& dir) {
   cache_file_ = opt_.weight_cache ? cache_file : "";
   if (opt_.weight_cache && !from_cache) write_weight_cache(cache_file, arena_, arena_bytes_, stream_);
   TRIT_CUDA(cudaMalloc(&d_layers_, sizeof(DLayer) * cfg_.layers));
-  TRIT_CUDA(cudaMemcpy(d_layers_, layers_.data(), sizeof(DLayer) * cfg_.layers, cudaMemcpyHostToDevice));
+  upload(d_layers_, layers_.data(), sizeof(DLayer) * cfg_.layers, stream_);
 
   // Rotary::halves (layers.rs:276-300): inv_freq = base^(-2i/hd) in f32, and
   // (position * f).sin_cos() in f32, here once per position: [pos][sin | cos].
@@ -758,7 +768,7 @@ void Lm::load(const std::string& dir) {
       table[(size_t)p * hd + hd / 2 + i] = cosf(a);
     }
   TRIT_CUDA(cudaMalloc(&rope_, table.size() * 4));
-  TRIT_CUDA(cudaMemcpy(rope_, table.data(), table.size() * 4, cudaMemcpyHostToDevice));
+  upload(rope_, table.data(), table.size() * 4, stream_);
 }
 
 void Lm::alloc_buffers() {
@@ -790,7 +800,7 @@ void Lm::alloc_buffers() {
     TRIT_CUDA(cudaMalloc(&pool_, pool_pages_ * page_bytes_));
     // Zeroed: positions past a stream's end are read (and masked) by the
     // tensor-core prompt attention, which must see finite values there.
-    TRIT_CUDA(cudaMemset(pool_, 0, pool_pages_ * page_bytes_));
+    TRIT_CUDA(cudaMemsetAsync(pool_, 0, pool_pages_ * page_bytes_, stream_));
   }
   cache_.pool = pool_;
   table_host_.resize(pages);
@@ -798,7 +808,7 @@ void Lm::alloc_buffers() {
   prefix_free_.clear();
   for (int i = prefix_pages_total_ - 1; i >= 0; --i) prefix_free_.push_back((int)pages + i);
   TRIT_CUDA(cudaMalloc(&page_table_, pages * sizeof(int)));
-  TRIT_CUDA(cudaMemcpy(page_table_, table_host_.data(), pages * sizeof(int), cudaMemcpyHostToDevice));
+  upload(page_table_, table_host_.data(), pages * sizeof(int), stream_);
   cache_.page_table = page_table_;
 
   rows_cap_ = std::max(opt_.prefill_rows, opt_.max_streams);
@@ -1073,10 +1083,10 @@ void Lm::set_ffn_scales(const float* scales) {
   wait();
   if (scales) {
     if (!ffn_scales_) TRIT_CUDA(cudaMalloc(&ffn_scales_, (size_t)cfg_.layers * cfg_.d * 4));
-    TRIT_CUDA(cudaMemcpy(ffn_scales_, scales, (size_t)cfg_.layers * cfg_.d * 4, cudaMemcpyHostToDevice));
+    upload(ffn_scales_, scales, (size_t)cfg_.layers * cfg_.d * 4, stream_);
   }
   for (int l = 0; l < cfg_.layers; ++l) layers_[l].ffn_scale = scales ? ffn_scales_ + (size_t)l * cfg_.d : nullptr;
-  TRIT_CUDA(cudaMemcpy(d_layers_, layers_.data(), sizeof(DLayer) * cfg_.layers, cudaMemcpyHostToDevice));
+  upload(d_layers_, layers_.data(), sizeof(DLayer) * cfg_.layers, stream_);
 }
 
 // CausalLm::generate_additive (causal_lm.rs:317-345), Voxtral Realtime's
@@ -1286,7 +1296,7 @@ void Lm::setup_tensor_cores() {
   }
   TRIT_CUDA(cudaMalloc(&gu_, (size_t)rows_cap_ * 2 * cfg_.ffn * 4));
   TRIT_CUDA(cudaMalloc(&tc_status_, 4));
-  TRIT_CUDA(cudaMemset(tc_status_, 0, 4));
+  TRIT_CUDA(cudaMemsetAsync(tc_status_, 0, 4, stream_));
   // "exact": false: prompt attention on the tensor cores (f16 cache, pages
   // of a multiple of 64 positions), over a TMA view of the whole pool.
   if (opt_.tc_attention && attention_tc_supported(cfg_, cache_)) {
@@ -1305,7 +1315,7 @@ void Lm::check_tc_status() {
   int st = 0;
   TRIT_CUDA(cudaMemcpy(&st, tc_status_, 4, cudaMemcpyDeviceToHost));
   if (st) {
-    cudaMemset(tc_status_, 0, 4);
+    cudaMemsetAsync(tc_status_, 0, 4, stream_);
     throw Error("a tensor-core product gave up waiting for its pipeline (status " + std::to_string(st) + ")");
   }
 }
@@ -1928,11 +1938,8 @@ std::unique_ptr<DenseOp> dense_q8_0(const void* blocks, size_t n, size_t k, int 
   }
   size_t co = 0, so = (n * k + 255) / 256 * 256;
   TRIT_CUDA(cudaMalloc(&op->mem, so + scales.size()));
-  // On the layer's stream: a plain cudaMemcpy may return before its last bytes
-  // are there, and that stream does not wait for it.
-  TRIT_CUDA(cudaMemcpyAsync(op->mem, codes.data(), codes.size(), cudaMemcpyHostToDevice, op->stream));
-  TRIT_CUDA(cudaMemcpyAsync((char*)op->mem + so, scales.data(), scales.size(), cudaMemcpyHostToDevice, op->stream));
-  TRIT_CUDA(cudaStreamSynchronize(op->stream));
+  upload(op->mem, codes.data(), codes.size(), op->stream);
+  upload((char*)op->mem + so, scales.data(), scales.size(), op->stream);
   if (table) {
     op->tab.n = (int)n; op->tab.k = (int)k; op->tab.scale_f16 = 1;
     op->tab.codes = (const int8_t*)op->mem + co;
@@ -1947,7 +1954,8 @@ std::unique_ptr<DenseOp> dense_q8_0(const void* blocks, size_t n, size_t k, int 
     TRIT_CUDA(cudaDeviceGetAttribute(&op->sm_count, cudaDevAttrMultiProcessorCount, device));
     if (major == 10 && k % 128 == 0 && make_tc_weight_map(&op->tc_w, op->mat, op->mat.codes) == cudaSuccess) {
       TRIT_CUDA(cudaMalloc(&op->tc_status, 4));
-      TRIT_CUDA(cudaMemset(op->tc_status, 0, 4));
+      TRIT_CUDA(cudaMemsetAsync(op->tc_status, 0, 4, op->stream));
+      TRIT_CUDA(cudaStreamSynchronize(op->stream));
       op->tc_ok = true;
     }
   }
