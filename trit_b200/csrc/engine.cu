@@ -1085,6 +1085,11 @@ void Lm::set_ffn_scales(const float* scales) {
     if (!ffn_scales_) TRIT_CUDA(cudaMalloc(&ffn_scales_, (size_t)cfg_.layers * cfg_.d * 4));
     upload(ffn_scales_, scales, (size_t)cfg_.layers * cfg_.d * 4, stream_);
   }
+  // A recorded batch step holds whether there are scales.
+  if (batch_graph_ && (layers_[0].ffn_scale != nullptr) != (scales != nullptr)) {
+    cudaGraphExecDestroy(batch_graph_);
+    batch_graph_ = nullptr;
+  }
   for (int l = 0; l < cfg_.layers; ++l) layers_[l].ffn_scale = scales ? ffn_scales_ + (size_t)l * cfg_.d : nullptr;
   upload(d_layers_, layers_.data(), sizeof(DLayer) * cfg_.layers, stream_);
 }
