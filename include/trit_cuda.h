@@ -530,8 +530,9 @@ int64_t trit_cuda_rotary_frequencies(const TritRotary *rotary, double *out, size
 
 /* Turns the pairs of q (rows x q_heads x head_dim) and k (rows x k_heads x
  * head_dim; 0 heads and NULL: no such tensor; at most 65535 heads each) by
- * position * frequency, which is formed in 64 bits (positions up to 2^53 either
- * way; a negative one turns back). `positions` has one number a row. q_out and
+ * position * frequency, the exact product of the two 64-bit numbers (positions
+ * up to 2^53 either way; a negative one turns back; angles of up to 2^80 radians
+ * are right to 2^-24). `positions` has one number a row. q_out and
  * k_out: NULL for in place. Values of a head behind rotary_dim stay as they are.
  * Returns 0, or -1. */
 int trit_cuda_rotary_apply(const TritRotary *rotary, const int64_t *positions, size_t rows, const void *q, size_t q_stride,

@@ -1,13 +1,14 @@
 // Rotary positions of queries and keys in one pass: pair i of a head at
-// position p turns by the angle 2 pi p t_i, t_i in turns a position,
+// position p turns by the angle p f_i,
 //   (a, b) -> f (a cos - b sin, b cos + a sin),
 // pairs (i, i + d / 2) or (2 i, 2 i + 1) of the head's first d values; values
 // behind them are copied, bit for bit.
 //
-// p t_i is formed in 64 bits and brought to an eighth of a turn around a
-// quarter turn before anything is rounded to f32, so positions of any size
-// lose nothing. A block computes the angles of its rows once for all heads,
-// while its values load. Bound by bytes, each read and written once.
+// p f_i is formed exactly, in two 64-bit numbers, and brought to an eighth of a
+// turn around a quarter turn before anything is rounded to f32: an angle of A
+// radians is off by 2^-49 + A 2^-104, so positions of up to 2^53 lose nothing. A
+// block computes the angles of its rows once for all heads, while its values
+// load. Bound by bytes, each read and written once.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -108,14 +109,22 @@ struct RotaryWork {
   int head_dim, rotary_dim;
   float factor;
   int turning, per_head;  // units of a head that turn, which come first, and all of them
-  double turns[PAIRS];    // of a whole circle a position
+  double frequency[PAIRS];  // radians a position
 };
 
-// cos and sin of t turns, times f: the nearest quarter turn, and the Taylor
-// series of what is left, up to an eighth of a turn (|x| <= pi / 4: the first
-// terms left out are x^11 / 11! < 2e-9 and x^12 / 12! < 2e-10). Short, so that
-// it keeps few registers from the values on their way.
-__device__ __forceinline__ float2 turn(double t, float f) {
+// cos and sin of p w radians, times f: in turns, the nearest quarter turn, and
+// the Taylor series of what is left, up to an eighth of a turn (|x| <= pi / 4: the
+// first terms left out are x^11 / 11! < 2e-9 and x^12 / 12! < 2e-10). Short, so
+// that it keeps few registers from the values on their way.
+__device__ __forceinline__ float2 turn(double p, double w, float f) {
+  // 1 / (2 pi) is kTurn + kTurnRest, and p w is u + (the rest) exactly; whole
+  // turns leave the product with kTurn before it is rounded. (u is not to be
+  // fused with what is subtracted from it.)
+  constexpr double kTurn = 0x1.45f306dc9c883p-3, kTurnRest = -0x1.6b01ec5417056p-57;
+  const double u = __dmul_rn(p, w);
+  double t = fma(u, kTurn, -rint(__dmul_rn(u, kTurn)));
+  t = fma(u, kTurnRest, t);
+  t = fma(fma(p, w, -u), kTurn, t);
   t -= rint(t);                     // [-1/2, 1/2]
   const double q = rint(4.0 * t);   // the quarter turn
   const float x = (float)(fma(-0.25, q, t) * 6.283185307179586), z = x * x;
@@ -184,7 +193,7 @@ __global__ void __launch_bounds__(kRotaryThreads, 4) k_rotary(const __grid_const
     float* to = (float*)angles + z * 2 * slots;
 #pragma unroll 1  // (the values on their way need the registers)
     for (int p = thread; p < pairs; p += threads) {
-      const float2 cs = turn((double)a.positions[row0 + z] * w.turns[p], w.factor);
+      const float2 cs = turn((double)a.positions[row0 + z], w.frequency[p], w.factor);
       to[p] = cs.x;
       to[slots + p] = cs.y;
     }
@@ -252,7 +261,7 @@ cudaError_t run_sized(const RotaryTable& t, const RotaryArgs& a, cudaStream_t s)
   w.head_dim = t.head_dim;
   w.rotary_dim = t.rotary_dim;
   w.factor = t.factor;
-  std::copy(t.turns, t.turns + pairs, w.turns);
+  std::copy(t.frequency, t.frequency + pairs, w.frequency);
   w.turning = INTER ? (t.rotary_dim + V - 1) / V : pairs / V;
   w.per_head = still ? w.turning : INTER ? t.head_dim / V : w.turning + (t.head_dim - t.rotary_dim) / V;
   const int lanes = std::min(w.per_head, kRotaryThreads);

@@ -218,7 +218,7 @@ std::unique_ptr<Rotary> Rotary::parse(const char* text) {
     if (yarn && factor < 1) t.factor = 1.0f;
   }
   if (attention > 0) t.factor = (float)attention;
-  for (int i = 0; i < pairs; ++i) t.turns[i] = r->frequencies[i] / (2 * kPi);
+  std::copy(r->frequencies.begin(), r->frequencies.end(), t.frequency);
   return r;
 }
 

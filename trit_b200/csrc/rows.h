@@ -63,7 +63,7 @@ constexpr int kRotaryPairs = 256;
 struct RotaryTable {
   int head_dim = 0, rotary_dim = 0, interleaved = 0;
   float factor = 1.0f;
-  double turns[kRotaryPairs];  // of a whole circle a position, per pair
+  double frequency[kRotaryPairs];  // radians a position, per pair
 };
 struct RotaryArgs {
   const int64_t* positions = nullptr;
