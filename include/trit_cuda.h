@@ -327,7 +327,10 @@ TritDense *trit_dense_q4_0(const void *blocks, size_t n, size_t k, int table, in
  * trit_cuda_rms_norm writes; rows of values are rounded to such first, in memory
  * that a call takes and gives back in its stream's order (a captured one has its
  * graph's). Each block's products are summed on the tensor cores, the blocks in
- * f32. Calls share no memory but the weights, so they may overlap and be captured.
+ * f32, each by f32(scale of x * scale of w): where that is no normal number of f32
+ * (below 2^-126 and not 0, or 2^128 and more), a block loses bits, or is infinite
+ * or NaN, also if its part of the result would be in range. Calls share no memory
+ * but the weights, so they may overlap and be captured.
  * NULL on failure. (No counterpart in the reference.) */
 TritDense *trit_dense_fp8(const void *codes, const float *scales, size_t n, size_t k, int device);
 

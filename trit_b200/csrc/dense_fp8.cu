@@ -7,7 +7,10 @@
 //
 // Rows of x are the MMA's M (a TMEM lane each), so a thread's scale of x is one
 // register a block and that of w the same for all its columns: one packed
-// multiply-add for two sums. Warp roles:
+// multiply-add for two sums. The two scales' product is an f32 of its own and has
+// to be in range (looking at it, to take it apart where it is not, is a vote in
+// the epilogue's chain: 13.5 -> 14.1 us for 64 rows of 16384 x 4096, 52.3 -> 53.7 for
+// 1000 of 12288 x 4096). Warp roles:
 //   warp 0     producer: a stage is 128 values of k of the tile's rows of x (a
 //              tensor copy) and w (bulk copies: w is kept in units of 64 rows x
 //              128 values as the MMA reads them, a unit's next ones behind it,
