@@ -355,6 +355,14 @@ int trit_dense_forward(TritDense *layer, const float *x, size_t rows, float *out
  * cudaStream_t, or NULL for the layer's own stream); does not wait. */
 int trit_dense_forward_device(TritDense *layer, const float *x, size_t rows, float *out, void *cuda_stream);
 
+/* Whether the layer's products that have ended are whole: every wait inside a
+ * tensor-core product is bounded in time, and one that ran out leaves outputs that
+ * are not. Returns 0, or -1 if that has happened since it was last reported: here,
+ * or as the failure of a call of the layer (trit_dense_forward, and any further
+ * product of a trit_dense_fp8 layer). A caller of the calls that do not wait asks
+ * after synchronising its stream, and after replays of a recorded graph. */
+int trit_dense_check(TritDense *layer);
+
 /* Frees a layer. NULL is a no-op. */
 void trit_dense_free(TritDense *layer);
 

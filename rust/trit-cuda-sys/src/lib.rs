@@ -177,6 +177,7 @@ pub mod ffi {
             q_heads: i32, q_out: *mut c_void, q_out_stride: usize, k: *const c_void, k_stride: usize, k_heads: i32,
             k_out: *mut c_void, k_out_stride: usize, kind: c_int, cuda_stream: *mut c_void,
         ) -> c_int;
+        pub fn trit_dense_check(layer: *mut TritDense) -> c_int;
         pub fn trit_dense_free(layer: *mut TritDense);
         pub fn trit_dense_q8_0_forward_static(
             codes: *const c_void, scales: *const c_void, n: usize, k: usize, x: *const f32, rows: usize,

@@ -522,6 +522,26 @@ int trit_dense_forward_device(TritDense* layer, const float* x, size_t rows, flo
   });
 }
 
+int trit_dense_check(TritDense* layer) {
+  return guard<int>(-1, [&]() {
+    need(layer, "layer");
+    std::lock_guard<std::mutex> lock(layer->mu);
+    if (layer->fp8) {
+      layer->fp8->check_status();
+      return 0;
+    }
+    trit::DenseOp& op = *layer->op;
+    if (!op.tc_status) return 0;
+    TRIT_CUDA(cudaSetDevice(op.device));
+    int st = 0;
+    TRIT_CUDA(cudaMemcpyAsync(&st, op.tc_status, 4, cudaMemcpyDeviceToHost, op.stream));
+    TRIT_CUDA(cudaMemsetAsync(op.tc_status, 0, 4, op.stream));
+    TRIT_CUDA(cudaStreamSynchronize(op.stream));
+    if (st) throw trit::Error("the tensor-core product gave up waiting for its pipeline");
+    return 0;
+  });
+}
+
 void trit_dense_free(TritDense* layer) { delete layer; }
 
 TritKv* trit_cuda_kv_new(const char* options_json) {

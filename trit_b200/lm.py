@@ -117,6 +117,7 @@ def library() -> ctypes.CDLL:
         "trit_cuda_rotary_apply": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, _size, ctypes.c_void_p, _size, ctypes.c_int32,
                                                   ctypes.c_void_p, _size, ctypes.c_void_p, _size, ctypes.c_int32,
                                                   ctypes.c_void_p, _size, ctypes.c_int, ctypes.c_void_p]),
+        "trit_dense_check": (ctypes.c_int, [ctypes.c_void_p]),
         "trit_dense_forward": (ctypes.c_int, [ctypes.c_void_p, _f32p, _size, _f32p]),
         "trit_dense_forward_device": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, _size, ctypes.c_void_p,
                                                      ctypes.c_void_p]),
@@ -459,6 +460,12 @@ class Dense:
                      stream: int | None = None) -> None:
         """forward_codes of rows of `dtype`, rounded to 8-bit rows first."""
         if library().trit_dense_forward_rows(self._handle, x_ptr, x_stride, rows, out_ptr, out_stride, _type(dtype), stream) != 0:
+            raise _error()
+
+    def check(self) -> None:
+        """Raises if a product of the layer that has ended since the last report gave up waiting inside, so that its
+        output is not whole (trit_dense_check). For after a synchronisation, or replays of a recorded graph."""
+        if library().trit_dense_check(self._handle) != 0:
             raise _error()
 
     def close(self) -> None:
