@@ -522,8 +522,9 @@ int trit_cuda_rms_norm(const void *x, size_t x_stride, const void *residual, siz
  *   "linear":  f / factor
  *   "ntk":     that of theta * factor^(d / (d - 2)), d = rotary_dim
  *   "yarn":    between the pairs that turn `fast` (32) and `slow` (1) times
- *              over `trained` positions, rounded outwards, a straight line from
- *              f to f / factor; rotated values times 0.1 ln(factor) + 1
+ *              over `trained` positions, rounded outwards and to pairs that there
+ *              are, a straight line from f to f / factor; rotated values times
+ *              0.1 ln(factor) + 1 (1 for factors below 1)
  *   "bands":   f for wavelengths below trained / high (4), f / factor for those
  *              above trained / low (1), a straight line over f between
  * "frequencies" gives them instead (rotary_dim / 2 numbers), and

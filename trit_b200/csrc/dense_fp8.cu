@@ -29,12 +29,12 @@
 // (cta_group::2) read both. An SM takes 64 bytes a clock from L2, 48 KB a block of
 // k of a tile of 128 x 256 and 32 KB of the pair's. Where such tiles leave many
 // rows or SMs unused, two blocks an SM take tiles of 128 x 128, one each: one
-// copies and starts while the other ends (600 rows of 4096 x 4096: 28.2 us with
-// one block an SM, 20.3 with two).
+// copies and starts while the other ends (600 rows of 4096 x 4096: 23.4 us with
+// one block an SM, 19.9 with two).
 //
 // Few rows are bound by the bytes of w: 151936 x 2048 and three rows 53 us (5.9
 // TB/s), 16384 x 4096 and 64 f32 rows 17.1 us with their rounding (4.2 TB/s),
-// 12288 x 2048 and one row 7.6 us, of which about 4 are a launch, the first copy
+// 12288 x 2048 and one row 7.4 us, of which about 4 are a launch, the first copy
 // and the join. Many rows: 1000 of 12288 x 4096 52 us (1.9 PFLOP/s, the tensor pipe
 // busy half of the time), 8000 of them 370 to 450 us with the clocks that the
 // power limit leaves (2.9 PFLOP/s with neither loads from TMEM nor additions).
@@ -685,8 +685,8 @@ cudaError_t launch_fp8(const TcMap& x, const TcMap& w, const TcMap& out, const F
   const auto tiles = [&](int bn) { return (a.m + 127LL) / 128 * ((a.n + bn - 1) / bn); };
   // As many blocks of a cluster as there is room for beside each other, with at
   // least two blocks of k, six where eight share (4096 x 4096, three rows: a
-  // cluster of 1 11.7 us, 2 8.6, 4 7.0, 8 7.8; 2048 x 6144: 16.2, 10.3, 7.2, 6.2;
-  // 12288 x 2048: 7.9, 7.8, 12.8, 19.3). The parts of the chip that a cluster stays
+  // cluster of 1 12.7 us, 2 8.9, 4 6.8, 8 7.7; 2048 x 6144: 16.8, 10.7, 7.3, 5.8;
+  // 12288 x 2048: 7.6, 7.4, 12.5, 19.2). The parts of the chip that a cluster stays
   // within hold no whole number of large ones: of 296 blocks 70 clusters of four
   // and 33 of eight (k = 6400, 40 rows: 70 tiles in four 15.1 us, 72 23.3).
   const auto splits = [&](long long tiles, long long room) {
@@ -701,12 +701,15 @@ cudaError_t launch_fp8(const TcMap& x, const TcMap& w, const TcMap& out, const F
   // More rows: 128 columns, one block or two an SM (these have fewer warps and
   // stages each; one copies while the other ends), or tiles of 256 x 256 by pairs.
   // What each takes, in us: a call, whole turns of the SMs, and a turn's blocks of
-  // k, as measured. us by one, two and pairs, up to 64 rows: 16384 x 4096 15.1,
-  // 16.4; 151936 x 2048 58, 61; 32768 x 8192 48, 44; 8192 x 4096 13.2, 10.1 (k in
-  // four). More: 333 rows of 5001 x 2064 11.0, 13.7, 15.2; 128 of 12288 x 2048 10.0,
-  // 11.3, 13.2; 512 of 2048 x 6144 -, 15.0 (k in four), 26; 300 of 20000 x 4096 51,
-  // 39, 53; 4000 of 1024 x 2048 16.4, 12.8, 13.8; 1140 of 14746 x 528 31, 32, 26;
-  // 1000 of 12288 x 4096 76, 61, 54; 8000 of them -, 441, 372.
+  // k, as measured. us by one, two and pairs (8-bit rows, bf16 out, replays of a
+  // recorded graph), 64 rows: 16384 x 4096 13.4, 15.9; 151936 x 2048 56, 60; 32768 x
+  // 8192 46, 44; 8192 x 4096 12.1, 10.6 (k in four). More: 333 rows of 5001 x 2064
+  // 9.4, 13.5, 13.3; 128 of 12288 x 2048 9.0, 12.4, 11.9; 512 of 2048 x 6144 17.5,
+  // 14.0 (k in four), 24.7; 300 of 20000 x 4096 44, 40, 49; 1140 of 14746 x 528 27,
+  // 31, 25; 1000 of 12288 x 4096 69, 61, 52 to 57; 8000 of them 549, 474, 385. The
+  // constants are from before the scales of x went through shared memory, which
+  // took up to 15 % off one and pairs; two are chosen a little too often since (600
+  // of 4096 x 4096 23.4, 19.9, 18.7; 129 of 16384 x 4096 23.7, 21.2, 19.5).
   const auto us = [&](double call, double turn, double block, int blocks, long long work, long long room) {
     return call + (turn + block * blocks) * (double)((work + room - 1) / room);
   };

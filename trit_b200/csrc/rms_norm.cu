@@ -5,9 +5,10 @@
 //   out = y rounded to the rows' type;  a group of 128 of y as e4m3 numbers:
 //   scale = max(f32(max |y| / 448), 2^-126) (1 for zeros),
 //   code = e4m3(f32(y * f32(1 / scale)))
-// The sum of squares is 64 bits wide, so that s, and with it every code, does
-// not depend on the order of the sum (an order's error of 1e-16 moves an f32
-// s once in 1e8 rows), and rows of any size of values have an answer. The
+// The sum of squares is 64 bits wide, so that s, and with it every code, all but
+// never depends on the order of the sum (an order's error of 1e-16 moves an f32
+// s once in 1e8 rows; the order goes by the width and the alignment, not by the
+// rows beside), and rows of any size of values have an answer. The
 // floor of the scale keeps 1 / scale finite. A group with a NaN or an infinity
 // gets the scale NaN.
 //
